@@ -340,6 +340,139 @@ int pkx_quantize(int gtype, const float* src_dev, void* dst_dev, int64_t n_rows,
 int pkx_quantize_gguf(const char* in_path, const char* out_path, int gtype, int* n_quantized, int* n_kept,
                       int* n_skipped);
 
+/* ---- attention decoder operators -------------------------------------------------
+ * No counterpart in the reference, whose decoders are CTC and transducers: what an
+ * attention decoder under beam search runs per token on an encoder's output.
+ * Buffers are the caller's, on the current device (as the stream is, or the call
+ * fails); a call starts kernels on the stream and nothing else: no allocation, no
+ * copy, no synchronisation, so it may be captured into a graph.  Lengths, slots and
+ * parents are device arrays; the kernels keep within the buffers whatever they hold.
+ * A workspace (its size from the call's _workspace function, 16-byte aligned; none
+ * needed: 0 bytes, NULL) belongs to one call at a time: calls that may overlap, and
+ * graphs that may run at once, need one each.  Calls with none of the shared buffers
+ * written may overlap freely.  Sizes of zero are calls that do nothing. */
+
+/* Cross attention: for every item b, query row i < q_len[b] and head h
+ *   out[b,i,h] = sum over t of softmax_t(scale * q[b,i,h] . k[b,t,h / (n_heads / n_kv_heads)]) v[b,t,.]
+ * over the keys t < k_len[b] with k_mask[b][t] != 0; zeros where there is none.
+ * Rows i >= q_len[b] of out are left as they were, and what k and v hold at keys left
+ * out does not matter.  The rows of an item share its keys, so W beams of one item
+ * are W query rows.  f16: f16 operands, softmax and sums in f32, weights rounded to f16
+ * for the second product; f32: f32 throughout.
+ * Strides are in elements (item, row, head; the d_head elements are adjacent), those of
+ * k and v not negative and below 2^24 between rows.  d_head: a multiple of 8 up to 128;
+ * buffers 16-byte aligned, strides multiples of 16 bytes; n_heads a multiple of
+ * n_kv_heads.  out overlaps no input. */
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of q, k, v and out */
+    int n_items, n_q, n_k;
+    int n_heads, n_kv_heads, d_head;
+    float scale;
+    const void* q;   int64_t q_item, q_row, q_head;
+    const void* k;   int64_t k_item, k_row, k_head;
+    const void* v;   int64_t v_item, v_row, v_head;
+    void* out;       int64_t out_item, out_row, out_head;
+    const int32_t* q_len;                /* dev [n_items], or NULL: n_q (values are clamped to 0..n_q) */
+    const int32_t* k_len;                /* dev [n_items], or NULL: n_k (clamped to 0..n_k) */
+    const uint8_t* k_mask;               /* dev [n_items][n_k], or NULL: every key */
+    int64_t k_mask_item;                 /* bytes between items of k_mask */
+} pkx_cross_attn;
+int pkx_cross_attention_workspace(const pkx_cross_attn* a, size_t* bytes);
+int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void* stream);
+
+/* A key/value cache in 8 bits: n_slots sequences of up to `capacity` tokens (a multiple
+ * of PKX_CACHE8_BLOCK).  A block of PKX_CACHE8_BLOCK tokens of one slot and head has one
+ * scale; an element is k * k_scale.  d_head: a multiple of 16 up to 128; 16-byte aligned. */
+#define PKX_CACHE8_BLOCK 32
+typedef struct {
+    int n_slots, n_kv_heads, d_head, capacity;
+    int8_t *k, *v;                       /* dev [n_slots][n_kv_heads][capacity][d_head] */
+    float *k_scale, *v_scale;            /* dev [n_slots][n_kv_heads][capacity / PKX_CACHE8_BLOCK] */
+} pkx_cache8;
+
+/* Append: tokens 0..count[r] of row r become positions start[r].. of its slot.  With s the
+ * block's scale (0 where the block starts with a new token), s' = max(s, max|x| / 127) over the
+ * block's new elements x of that head, a new element is held as round(x / s') within +-127 and an
+ * earlier one, q, becomes round(q * (s / s')): each step one f32 operation, ties to even.  NaN is
+ * held as 0, an infinity as +-127, and neither counts in max|x|.  What follows the new tokens in
+ * their last block is left as it was and is expected to be appended next.  Tokens past the capacity
+ * are dropped; a row with a start or slot out of range is skipped; of rows that name the same slot
+ * only the first is appended.  table: see pkx_cache8_attention; entries start[r].. of row r are set
+ * to its slot.  Strides in elements, multiples of 16 bytes. */
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of k and v */
+    int n_rows, n_new;
+    const void* k;   int64_t k_row, k_tok, k_head;
+    const void* v;   int64_t v_row, v_tok, v_head;
+    const int32_t* slot;                 /* dev [n_rows], or NULL: row r is slot r */
+    const int32_t* start;                /* dev [n_rows] */
+    const int32_t* count;                /* dev [n_rows], or NULL: n_new (clamped to 0..n_new) */
+    int32_t* table;  int64_t table_row;  /* dev [n_rows][>= capacity], or NULL */
+} pkx_cache8_tokens;
+int pkx_cache8_append(const pkx_cache8* c, const pkx_cache8_tokens* t, void* stream);
+
+/* The values of tokens start[r] .. start[r] + n of row r's slot: k_out, v_out [n_rows][n][n_kv_heads]
+ * [d_head] f32 (either may be NULL); zeros at positions outside 0..capacity and for slots out of range. */
+int pkx_cache8_read(const pkx_cache8* c, int n_rows, int n, const int32_t* slot, const int32_t* start,
+                    float* k_out, float* v_out, void* stream);
+
+/* Attention of n_q query rows per cache row over the cache: as pkx_cross_attention over positions
+ * t < len[r] (clamped to the capacity) of row r's slot.  causal: the last of the row's q_len[r] queries
+ * is token len[r] - 1, so query i sees positions t <= len[r] - q_len[r] + i; a query that sees none gives
+ * zeros.  table: position t of row r is read from slot table[r][t] instead (an entry out of range: the
+ * position is left out).  Beams share their histories that way: every beam appends to a slot of its own
+ * with the table, and after a selection the table's rows, not the cache, are reordered by parent.
+ * A slot out of range (without table) has no positions.  f16: int8 keys and values exact in f16,
+ * queries as given, weights rounded to f16; f32: queries and weights as two f16 terms, 22 bits. */
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of q and out */
+    int n_rows, n_q, n_heads, causal;
+    float scale;
+    const void* q;   int64_t q_row, q_tok, q_head;
+    void* out;       int64_t out_row, out_tok, out_head;
+    const int32_t* slot;                 /* dev [n_rows], or NULL: row r is slot r */
+    const int32_t* len;                  /* dev [n_rows] */
+    const int32_t* q_len;                /* dev [n_rows], or NULL: n_q */
+    const int32_t* table;  int64_t table_row;  /* dev [n_rows][>= max len], or NULL */
+    int max_len;                         /* no len[r] is above it (0: the capacity); longer ones are cut to it */
+} pkx_cache8_attn;
+int pkx_cache8_attention_workspace(const pkx_cache8* c, const pkx_cache8_attn* a, size_t* bytes);
+int pkx_cache8_attention(const pkx_cache8* c, const pkx_cache8_attn* a, void* ws, size_t ws_bytes, void* stream);
+
+/* Beam selection: for every item the n_beams best of its n_beams x vocab candidates (w, v), of score
+ * scores[w] + log_softmax(logits[w])[v] (64-bit sums), ties to the lowest w * vocab + v, within a beam
+ * after the order of the logits.  A finished beam (done[w] != 0) has the one candidate (w, end_id) of score
+ * scores[w].  A beam with a NaN or +inf among its logits, or with no finite one, or whose score is NaN or
+ * +inf, has candidates of score -inf only.  Outputs per item, best first: parent beam, token, score and
+ * whether the beam is finished (its parent was, or the token is end_id).  n_beams: 1 to 32;
+ * outputs overlap no input. */
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of logits */
+    int n_items, n_beams, vocab;
+    int end_id;                          /* in 0..vocab-1, or -1: none (done NULL) */
+    const void* logits;  int64_t logits_row;  /* dev [n_items * n_beams][vocab], elements between rows */
+    const float* scores;                 /* dev [n_items][n_beams] */
+    const uint8_t* done;                 /* dev [n_items][n_beams], or NULL: none */
+    int32_t *parent, *token;             /* dev [n_items][n_beams] */
+    float* new_scores;                   /* dev [n_items][n_beams] */
+    uint8_t* new_done;                   /* dev [n_items][n_beams], or NULL */
+} pkx_beam_select_args;
+int pkx_beam_select_workspace(const pkx_beam_select_args* a, size_t* bytes);
+int pkx_beam_select(const pkx_beam_select_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/* Reordering: row b * n_beams + w of every dst = row b * n_beams + parent[b][w] of its src, `bytes` of it
+ * (prediction-network states, cache tables, ...); rows whose parent is out of range are left as they were.
+ * states: host array of at most PKX_BEAM_MAX_STATES; row strides in bytes, at least `bytes` (src: or 0).
+ * No src, from its first row to its last, overlaps a dst. */
+#define PKX_BEAM_MAX_STATES 32
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t src_row, dst_row, bytes;
+} pkx_beam_state;
+int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_beam_state* states, int n_states,
+                     void* stream);
+
 /* ---- profiling ----------------------------------------------------------------
  * No counterpart in the reference (its benchmarks time whole calls).
  * family_mask selects kernel families by bit (bit i = family i in the order

@@ -6,6 +6,7 @@
 #include <string>
 
 #include "../../include/pkx.h"
+#include "decoder.hpp"
 #include "mel.hpp"
 #include "model.hpp"
 #include "quantize.hpp"
@@ -132,6 +133,135 @@ pkx_config to_public(const pkx::ModelConfig& m) {
     c.stream_valid_out_len = m.stream_valid_out_len;
     c.stream_drop_extra = m.stream_drop_extra;
     return c;
+}
+
+// A stream of another device than the current one: the launch would go astray.
+void need_device(hipStream_t s) {
+    if (!s) return;
+    int cur = 0;
+    hipDevice_t dev = 0;
+    PKX_HIP(hipGetDevice(&cur));
+    PKX_HIP(hipStreamGetDevice(s, &dev));
+    need(dev == cur, "the stream belongs to another device than the current one");
+}
+
+bool is_f32(int type, const char* what) {
+    need(type == PKX_TYPE_F32 || type == PKX_TYPE_F16, what);
+    return type == PKX_TYPE_F32;
+}
+
+// A strided operand read or written in 16-byte pieces.
+void need_view(const void* p, int64_t a, int64_t b, int64_t c, bool f32, const char* what) {
+    const int64_t unit = f32 ? 4 : 8;
+    need(p != nullptr && (uintptr_t)p % 16 == 0, what);
+    need(a >= 0 && b >= 0 && c >= 0 && a % unit == 0 && b % unit == 0 && c % unit == 0, what);
+}
+
+pkx::DecAttnParams cross_params(const pkx_cross_attn* a) {
+    need(a, "null argument");
+    const bool f32 = is_f32(a->type, "cross attention: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(a->n_items >= 0 && a->n_q >= 0 && a->n_k >= 0, "cross attention: negative size");
+    need(a->n_heads >= 1 && a->n_kv_heads >= 1 && a->n_heads % a->n_kv_heads == 0,
+         "cross attention: n_heads must be a multiple of n_kv_heads");
+    need(a->d_head >= 8 && a->d_head <= 128 && a->d_head % 8 == 0, "cross attention: d_head must be a multiple of 8 up to 128");
+    pkx::DecAttnParams p;
+    p.kv = f32 ? pkx::KV_F32 : pkx::KV_F16;
+    p.q_f32 = f32;
+    p.B = a->n_items;
+    p.n_q = a->n_q;
+    p.n_k = a->n_k;
+    p.Hkv = a->n_kv_heads;
+    p.G = a->n_heads / a->n_kv_heads;
+    p.dk = a->d_head;
+    p.scale = a->scale;
+    p.q = a->q; p.q_item = a->q_item; p.q_row = a->q_row; p.q_head = a->q_head;
+    p.k = a->k; p.k_item = a->k_item; p.k_row = a->k_row; p.k_head = a->k_head;
+    p.v = a->v; p.v_item = a->v_item; p.v_row = a->v_row; p.v_head = a->v_head;
+    p.out = a->out; p.o_item = a->out_item; p.o_row = a->out_row; p.o_head = a->out_head;
+    p.q_len = a->q_len;
+    p.k_len = a->k_len;
+    p.mask = a->k_mask;
+    p.mask_item = a->k_mask_item;
+    return p;
+}
+
+pkx::Cache8 cache_params(const pkx_cache8* c) {
+    need(c, "null argument");
+    need(c->n_slots >= 1 && c->n_kv_heads >= 1, "8-bit cache: no slots or heads");
+    need(c->d_head >= 16 && c->d_head <= 128 && c->d_head % 16 == 0, "8-bit cache: d_head must be a multiple of 16 up to 128");
+    need(c->capacity >= PKX_CACHE8_BLOCK && c->capacity % PKX_CACHE8_BLOCK == 0,
+         "8-bit cache: capacity must be a multiple of PKX_CACHE8_BLOCK");
+    need(c->k && c->v && c->k_scale && c->v_scale, "8-bit cache: null buffer");
+    need(((uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0 && ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 4 == 0,
+         "8-bit cache: k and v must be 16-byte aligned");
+    pkx::Cache8 o;
+    o.n_slots = c->n_slots;
+    o.Hkv = c->n_kv_heads;
+    o.dk = c->d_head;
+    o.cap = c->capacity;
+    o.k = c->k;
+    o.v = c->v;
+    o.k_scale = c->k_scale;
+    o.v_scale = c->v_scale;
+    return o;
+}
+
+pkx::DecAttnParams cache_attn_params(const pkx_cache8* c, const pkx_cache8_attn* a) {
+    const pkx::Cache8 o = cache_params(c);
+    need(a, "null argument");
+    pkx::DecAttnParams p;
+    p.kv = pkx::KV_I8;
+    p.q_f32 = is_f32(a->type, "cache attention: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(a->n_rows >= 0 && a->n_q >= 0, "cache attention: negative size");
+    need(a->n_heads >= 1 && a->n_heads % o.Hkv == 0, "cache attention: n_heads must be a multiple of the cache's heads");
+    need(a->max_len >= 0, "cache attention: negative max_len");
+    p.B = a->n_rows;
+    p.n_q = a->n_q;
+    p.n_k = a->max_len > 0 && a->max_len < o.cap ? a->max_len : o.cap;
+    p.Hkv = o.Hkv;
+    p.G = a->n_heads / o.Hkv;
+    p.dk = o.dk;
+    p.scale = a->scale;
+    p.causal = a->causal != 0;
+    p.q = a->q; p.q_item = a->q_row; p.q_row = a->q_tok; p.q_head = a->q_head;
+    p.out = a->out; p.o_item = a->out_row; p.o_row = a->out_tok; p.o_head = a->out_head;
+    p.k = o.k;
+    p.v = o.v;
+    p.k_item = p.v_item = (int64_t)o.Hkv * o.cap * o.dk;
+    p.k_head = p.v_head = (int64_t)o.cap * o.dk;
+    p.k_row = p.v_row = o.dk;
+    p.k_scale = o.k_scale;
+    p.v_scale = o.v_scale;
+    p.n_slots = o.n_slots;
+    p.n_blocks = o.cap / PKX_CACHE8_BLOCK;
+    p.slot = a->slot;
+    p.table = a->table;
+    p.table_ld = a->table_row;
+    p.k_len = a->len;
+    p.q_len = a->q_len;
+    return p;
+}
+
+pkx::BeamSelectParams beam_params(const pkx_beam_select_args* a) {
+    need(a, "null argument");
+    pkx::BeamSelectParams p;
+    p.f32 = is_f32(a->type, "beam select: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(a->n_items >= 0 && a->n_beams >= 1 && a->n_beams <= pkx::kMaxBeams, "beam select: n_beams must be 1 to 32");
+    need(a->vocab >= 1 && a->end_id >= -1 && a->end_id < a->vocab, "beam select: end_id must be -1 or a word of the vocabulary");
+    need(!a->done || a->end_id >= 0, "beam select: finished beams need an end_id");
+    p.B = a->n_items;
+    p.W = a->n_beams;
+    p.V = a->vocab;
+    p.end_id = a->end_id;
+    p.logits = a->logits;
+    p.row = a->logits_row;
+    p.scores = a->scores;
+    p.done = a->done;
+    p.parent = a->parent;
+    p.token = a->token;
+    p.new_scores = a->new_scores;
+    p.new_done = a->new_done;
+    return p;
 }
 }  // namespace
 
@@ -573,6 +703,136 @@ int pkx_quantize_gguf(const char* in_path, const char* out_path, int gtype, int*
         if (n_quantized) *n_quantized = c.quantized;
         if (n_kept) *n_kept = c.kept;
         if (n_skipped) *n_skipped = c.skipped;
+    });
+}
+
+int pkx_cross_attention_workspace(const pkx_cross_attn* a, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = pkx::dec_attention_workspace(cross_params(a));
+    });
+}
+int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void* s) {
+    return guarded([&] {
+        const pkx::DecAttnParams p = cross_params(a);
+        if (p.B == 0 || p.n_q == 0) return;
+        need_view(p.q, p.q_item, p.q_row, p.q_head, p.q_f32, "cross attention: q must be 16-byte aligned with strides of whole 16 bytes");
+        need_view(p.out, p.o_item, p.o_row, p.o_head, p.q_f32, "cross attention: out must be 16-byte aligned with strides of whole 16 bytes");
+        if (p.n_k > 0) {
+            need_view(p.k, p.k_item, p.k_row, p.k_head, p.q_f32, "cross attention: k must be 16-byte aligned with strides of whole 16 bytes");
+            need_view(p.v, p.v_item, p.v_row, p.v_head, p.q_f32, "cross attention: v must be 16-byte aligned with strides of whole 16 bytes");
+            need(p.k_row < (1 << 24) && p.v_row < (1 << 24), "cross attention: key rows must be less than 2^24 elements apart");
+        }
+        need_device(st(s));
+        pkx::launch_dec_attention(p, ws, ws_bytes, st(s));
+    });
+}
+
+int pkx_cache8_append(const pkx_cache8* c, const pkx_cache8_tokens* t, void* s) {
+    return guarded([&] {
+        pkx::CacheAppendParams p;
+        p.c = cache_params(c);
+        need(t, "null argument");
+        p.f32 = is_f32(t->type, "cache append: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+        need(t->n_rows >= 0 && t->n_new >= 0, "cache append: negative size");
+        if (t->n_rows == 0 || t->n_new == 0) return;
+        need_view(t->k, t->k_row, t->k_tok, t->k_head, p.f32, "cache append: k must be 16-byte aligned with strides of whole 16 bytes");
+        need_view(t->v, t->v_row, t->v_tok, t->v_head, p.f32, "cache append: v must be 16-byte aligned with strides of whole 16 bytes");
+        need(t->start, "cache append: null start");
+        need(t->slot || t->n_rows <= c->n_slots, "cache append: more rows than slots");
+        need(!t->table || t->table_row >= c->capacity, "cache append: table rows are shorter than the capacity");
+        p.k = t->k; p.k_row = t->k_row; p.k_tok = t->k_tok; p.k_head = t->k_head;
+        p.v = t->v; p.v_row = t->v_row; p.v_tok = t->v_tok; p.v_head = t->v_head;
+        p.slot = t->slot;
+        p.start = t->start;
+        p.count = t->count;
+        p.table = t->table;
+        p.table_ld = t->table_row;
+        p.R = t->n_rows;
+        p.n_new = t->n_new;
+        need_device(st(s));
+        pkx::launch_cache8_append(p, st(s));
+    });
+}
+int pkx_cache8_read(const pkx_cache8* c, int n_rows, int n, const int32_t* slot, const int32_t* start, float* k_out,
+                    float* v_out, void* s) {
+    return guarded([&] {
+        pkx::CacheReadParams p;
+        p.c = cache_params(c);
+        need(n_rows >= 0 && n >= 0, "cache read: negative size");
+        if (n_rows == 0 || n == 0) return;
+        need(start && ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0, "cache read: null start, or outputs not 16-byte aligned");
+        p.slot = slot;
+        p.start = start;
+        p.k = k_out;
+        p.v = v_out;
+        p.R = n_rows;
+        p.n = n;
+        need_device(st(s));
+        pkx::launch_cache8_read(p, st(s));
+    });
+}
+int pkx_cache8_attention_workspace(const pkx_cache8* c, const pkx_cache8_attn* a, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = pkx::dec_attention_workspace(cache_attn_params(c, a));
+    });
+}
+int pkx_cache8_attention(const pkx_cache8* c, const pkx_cache8_attn* a, void* ws, size_t ws_bytes, void* s) {
+    return guarded([&] {
+        const pkx::DecAttnParams p = cache_attn_params(c, a);
+        if (p.B == 0 || p.n_q == 0) return;
+        need_view(p.q, p.q_item, p.q_row, p.q_head, p.q_f32, "cache attention: q must be 16-byte aligned with strides of whole 16 bytes");
+        need_view(p.out, p.o_item, p.o_row, p.o_head, p.q_f32, "cache attention: out must be 16-byte aligned with strides of whole 16 bytes");
+        need(p.k_len, "cache attention: null len");
+        need(p.slot || p.table || p.B <= p.n_slots, "cache attention: more rows than slots");
+        need(!p.table || p.table_ld >= p.n_k, "cache attention: table rows are shorter than max_len");
+        need_device(st(s));
+        pkx::launch_dec_attention(p, ws, ws_bytes, st(s));
+    });
+}
+
+int pkx_beam_select_workspace(const pkx_beam_select_args* a, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        *bytes = pkx::beam_select_workspace(beam_params(a));
+    });
+}
+int pkx_beam_select(const pkx_beam_select_args* a, void* ws, size_t ws_bytes, void* s) {
+    return guarded([&] {
+        const pkx::BeamSelectParams p = beam_params(a);
+        if (p.B == 0) return;
+        need(p.logits && p.scores && p.parent && p.token && p.new_scores, "beam select: null buffer");
+        need((uintptr_t)p.logits % (p.f32 ? 4 : 2) == 0 && p.row >= 0, "beam select: misaligned logits or a negative row stride");
+        need((uintptr_t)ws % 16 == 0, "beam select: the workspace must be 16-byte aligned");
+        need_device(st(s));
+        pkx::launch_beam_select(p, ws, ws_bytes, st(s));
+    });
+}
+int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_beam_state* states, int n_states, void* s) {
+    return guarded([&] {
+        need(n_items >= 0 && n_beams >= 1, "beam reorder: bad size");
+        need(n_states >= 0 && n_states <= pkx::kMaxBeamStates, "beam reorder: at most PKX_BEAM_MAX_STATES states");
+        if (n_items == 0 || n_states == 0) return;
+        need(parent && states, "null argument");
+        pkx::BeamState p[pkx::kMaxBeamStates];
+        const int64_t rows = (int64_t)n_items * n_beams;
+        for (int i = 0; i < n_states; ++i) {
+            const pkx_beam_state& x = states[i];
+            need(x.bytes >= 0 && (x.src_row >= x.bytes || x.src_row == 0) && x.dst_row >= x.bytes,
+                 "beam reorder: row strides must be at least the row's bytes");
+            if (x.bytes > 0) {
+                need(x.src && x.dst, "beam reorder: null state");
+                const uintptr_t b = (uintptr_t)x.dst, be = b + (rows - 1) * x.dst_row + x.bytes;
+                for (int j = 0; j < n_states; ++j) {
+                    const uintptr_t a = (uintptr_t)states[j].src, ae = a + (rows - 1) * states[j].src_row + states[j].bytes;
+                    need(states[j].bytes <= 0 || ae <= b || be <= a, "beam reorder: a source overlaps a destination");
+                }
+            }
+            p[i] = pkx::BeamState{(const uint8_t*)x.src, (uint8_t*)x.dst, x.src_row, x.dst_row, x.bytes};
+        }
+        need_device(st(s));
+        pkx::launch_beam_reorder(parent, n_items, n_beams, p, n_states, st(s));
     });
 }
 

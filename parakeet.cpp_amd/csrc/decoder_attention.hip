@@ -1,0 +1,687 @@
+// Attention of a decoder's queries to keys of another length: encoder states
+// in f16 or f32, or an 8-bit cache (int8 with a scale for each 32 tokens and
+// head).  One pass over the keys with the running maximum m and sum l of the
+// softmax: for a tile of keys, m' = max(m, max s), a = 2^(m - m'),
+// p = 2^(s - m'), l = a l + sum p, O = a O + p V; out = O / l, zeros where no
+// key was attended (l = 0).  s is in log2 units (log2 e folded into the scale).
+//
+// Everything stays in registers.  Both products are formed transposed on
+// 16-row matrix instructions, so that a lane's column is one query:
+// S^T = K Q^T leaves lane (c, g) (c = lane % 16, g = lane / 16) the scores of
+// query c with keys 4g + e and 16 + 4g + e of a 32-key tile, which is already
+// the B operand of O^T = V^T P^T when that product's contraction index (g, i)
+// stands for key 4g + i (i < 4) or 16 + 4g + i - 4.  Its A operand wants eight
+// keys of one dimension per lane while V is stored by key, so each lane loads
+// dimensions [c D/16, (c+1) D/16) of its eight keys (the 16 lanes of a group
+// read one whole row) and pairs of rows are interleaved with v_perm: row c of
+// the j-th product is dimension c D/16 + j, and a lane ends with runs of D/16
+// consecutive output dimensions.  No LDS but for joining waves.
+//
+// A workgroup is WM x WK waves: WM tiles of 16 QT query rows, WK shares of the
+// keys (joined in LDS at the end).  Where a call has few rows the keys are
+// also split over workgroups, each writing its unnormalised O and (m, l), and
+// dec_join_kernel joins them.
+//
+// 8-bit keys: the int8 go through v_perm into f16 mantissas
+// (0x6400 | (b ^ 0x80) = 1024 + b + 128, minus 1152: exact), the scale of a
+// block multiplies the scores and the tile's P V product in f32.  With f32
+// queries, q and p are split into two f16 terms of 22 bits together, so the
+// int8 products keep f32's accuracy at twice the matrix instructions.
+#include "decoder.hpp"
+
+namespace pkx {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoMax = -3.0e38f;   // below every score: m - m' is finite from the start
+
+__device__ __forceinline__ float xgroup_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float xgroup_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// int8 pairs spread to the low bytes of two halves -> f16
+__device__ __forceinline__ uint32_t i8_pair_f16(uint32_t spread) {
+    const half2v h = __builtin_bit_cast(half2v, spread ^ 0x64806480u) + (half2v){(f16)-1152.0f, (f16)-1152.0f};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+template <int N> __device__ __forceinline__ void load_words(uint32_t (&d)[N], const uint8_t* p) {
+    if constexpr (N == 1) {
+        d[0] = *(const uint32_t*)p;
+    } else if constexpr (N == 2) {
+        const int2v t = *(const int2v*)p;
+        d[0] = t[0]; d[1] = t[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const int4v t = *(const int4v*)(p + 4 * i);
+            d[i] = t[0]; d[i + 1] = t[1]; d[i + 2] = t[2]; d[i + 3] = t[3];
+        }
+    }
+}
+
+// Registers of a 32-key tile: key tiles kt = 0, 1 of 16 keys (lane c's row),
+// and the lane's eight value rows.
+template <int KV, int D> struct Tile {
+    static constexpr int ES = KV == KV_F16 ? 2 : KV == KV_F32 ? 4 : 1;
+    static constexpr int NK = D * ES / 16;                        // dwords of a lane's quarter of a key row
+    static constexpr int NV = D * ES / 64 > 0 ? D * ES / 64 : 1;  // dwords of its sixteenth of a value row
+    uint32_t k[2][NK];
+    uint32_t v[8][NV];
+    float ks, vs;    // scales of the block, or (table) of key lane % 32
+    int ok;          // key lane % 32 is attended
+};
+
+// byte offset in a key row of the n-th 16-byte (or narrower) piece of group g
+template <int KV, int D> __device__ __forceinline__ int key_piece(int n, int g) {
+    if constexpr (KV == KV_I8 && D == 32) return 8 * g;
+    return 64 * n + 16 * g;
+}
+// dimension of element x of group g's fragment of contraction step s (32 deep)
+template <int KV, int D> __device__ __forceinline__ int key_dim(int s, int g) {
+    if constexpr (KV == KV_I8 && D > 32) return 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+    return 32 * s + 8 * g;
+}
+
+struct KeySource {
+    const uint8_t *k, *v;        // item and head
+    int64_t k_slot, v_slot;      // table: bytes between slots
+    uint32_t k_row, v_row;       // bytes between keys
+    const float *ks, *vs;
+    int64_t s_slot;
+    const uint8_t* mask;
+    const int* table;
+    int T, n_slots, k_bytes, v_off;
+};
+
+template <int KV, int D, bool TABLE>
+__device__ __forceinline__ void load_tile(Tile<KV, D>& t, const KeySource& s, int t0, int slot, int lane) {
+    using TL = Tile<KV, D>;
+    const int c = lane & 15, g = lane >> 4, last = s.T - 1;
+    const int tb = t0 < last ? t0 : last;                 // tiles past the end read the last key again
+    const int left = last - tb;
+    const int mine = lane & 31;
+    bool ok = t0 + mine < s.T;
+    if (s.mask) ok = ok && s.mask[tb + (mine < left ? mine : left)] != 0;
+    if constexpr (TABLE) {
+        ok = ok && (unsigned)slot < (unsigned)s.n_slots;
+        slot = (unsigned)slot < (unsigned)s.n_slots ? slot : 0;
+        t.ks = s.ks[slot * s.s_slot + tb / kCacheBlock];
+        t.vs = s.vs[slot * s.s_slot + tb / kCacheBlock];
+    } else if constexpr (KV == KV_I8) {
+        t.ks = s.ks[tb / kCacheBlock];
+        t.vs = s.vs[tb / kCacheBlock];
+    }
+    t.ok = ok;
+    const uint8_t* kb = s.k + (int64_t)tb * s.k_row;
+    const uint8_t* vb = s.v + (int64_t)tb * s.v_row;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        const int r = 16 * kt + c, rr = r < left ? r : left;
+        const uint8_t* p = kb + (uint32_t)rr * s.k_row;
+        if constexpr (TABLE) p += __shfl(slot, r, 64) * s.k_slot;
+        if constexpr (TL::NK == 2) {
+            uint32_t d[2];
+            const int o = key_piece<KV, D>(0, g);
+            load_words(d, p + (o < s.k_bytes ? o : 0));
+            t.k[kt][0] = d[0]; t.k[kt][1] = d[1];
+        } else {
+#pragma unroll
+            for (int n = 0; n < TL::NK / 4; ++n) {
+                // pieces past the head's dimensions read its first again; their queries are zero
+                const int o = key_piece<KV, D>(n, g);
+                uint32_t d[4];
+                load_words(d, p + (o < s.k_bytes ? o : 0));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) t.k[kt][4 * n + i] = d[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = (i < 4 ? 0 : 12) + 4 * g + i, rr = r < left ? r : left;
+        const uint8_t* p = vb + (uint32_t)rr * s.v_row + s.v_off;
+        if constexpr (TABLE) p += __shfl(slot, r, 64) * s.v_slot;
+        if constexpr (KV == KV_I8 && D == 32) t.v[i][0] = *(const uint16_t*)p;
+        else load_words(t.v[i], p);
+    }
+}
+
+// scores of a 16-key tile (c: keys 4g + e of query lane % 16)
+template <int KV, int D, bool QF32, int NQ>
+__device__ __forceinline__ float4v tile_scores(const uint32_t (&k)[Tile<KV, D>::NK], const uint32_t (&q)[NQ]) {
+    float4v acc = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (KV == KV_F32) {
+#pragma unroll
+        for (int i = 0; i < D / 4; ++i)
+            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i]), __uint_as_float(q[i]), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+            int4v a;
+            if constexpr (KV == KV_F16) {
+                a = (int4v){(int)k[4 * s], (int)k[4 * s + 1], (int)k[4 * s + 2], (int)k[4 * s + 3]};
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    a[2 * h] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c010c00));
+                    a[2 * h + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c030c02));
+                }
+            }
+            const half8v af = __builtin_bit_cast(half8v, a);
+            const int4v b = {(int)q[4 * s], (int)q[4 * s + 1], (int)q[4 * s + 2], (int)q[4 * s + 3]};
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, __builtin_bit_cast(half8v, b), acc, 0, 0, 0);
+            if constexpr (KV == KV_I8 && QF32) {
+                const int o = D / 8 + 4 * s;
+                const int4v bl = {(int)q[o], (int)q[o + 1], (int)q[o + 2], (int)q[o + 3]};
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, __builtin_bit_cast(half8v, bl), acc, 0, 0, 0);
+            }
+        }
+    }
+    return acc;
+}
+
+// A operand of the j-th value product: eight keys of dimension c D/16 + j
+template <int KV, int D> __device__ __forceinline__ half8v value_frag(const uint32_t (&v)[8][Tile<KV, D>::NV], int j) {
+    int4v a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (KV == KV_F16) {
+            a[i] = __builtin_amdgcn_perm(v[2 * i + 1][j >> 1], v[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+        } else {
+            const uint32_t b = j & 3;
+            a[i] = i8_pair_f16(__builtin_amdgcn_perm(v[2 * i + 1][j >> 2], v[2 * i][j >> 2], 0x0c040c00u | b | (b << 16)));
+        }
+    }
+    return __builtin_bit_cast(half8v, a);
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const half2v h = {(f16)a, (f16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+template <int KV, bool QF32, int D, int QT, int WM, int WK, bool TABLE>
+__global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p) {
+    using TL = Tile<KV, D>;
+    static_assert(WK == 1 || (QT == 1 && WM == 1 && WK == 4), "joined waves: one row tile, four key shares");
+    constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
+    constexpr int NQ = KV == KV_F32 ? D / 4 : SPLIT ? D / 4 : D / 8;
+    constexpr int NJ = D / 16, ROWS = 16 * QT * WM;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int wm = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
+    const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
+    int id = xcd_tile(blockIdx.x, gridDim.x);              // row tiles of one item and head share an XCD's L2
+    const int mtile = id % mt;
+    id /= mt;
+    const int split = id % p.splits;
+    id /= p.splits;
+    const int kh = id % p.Hkv, b = id / p.Hkv;
+
+    int T = p.k_len ? p.k_len[b] : p.n_k;
+    T = T < 0 ? 0 : T > p.n_k ? p.n_k : T;
+    int cnt = p.q_len ? p.q_len[b] : p.n_q;
+    cnt = cnt < 0 ? 0 : cnt > p.n_q ? p.n_q : cnt;
+    if (mtile * ROWS / p.G >= cnt) return;                 // no row of this tile is asked for
+    const int m0 = mtile * ROWS + wm * 16 * QT;
+    KeySource s = {};
+    if constexpr (KV == KV_I8) {
+        const int sl = p.slot ? p.slot[b] : b;
+        s.n_slots = p.n_slots;
+        s.s_slot = (int64_t)p.Hkv * p.n_blocks;
+        s.k_slot = p.k_item;
+        s.v_slot = p.v_item;
+        int64_t at = 0;
+        if constexpr (TABLE) s.table = p.table + b * p.table_ld;
+        else if ((unsigned)sl >= (unsigned)p.n_slots) T = 0;
+        else at = sl;
+        s.k = (const uint8_t*)p.k + at * p.k_item + kh * p.k_head;
+        s.v = (const uint8_t*)p.v + at * p.v_item + kh * p.v_head;
+        s.ks = p.k_scale + at * s.s_slot + (int64_t)kh * p.n_blocks;
+        s.vs = p.v_scale + at * s.s_slot + (int64_t)kh * p.n_blocks;
+    } else {
+        s.k = (const uint8_t*)p.k + (b * p.k_item + kh * p.k_head) * TL::ES;
+        s.v = (const uint8_t*)p.v + (b * p.v_item + kh * p.v_head) * TL::ES;
+        s.mask = p.mask ? p.mask + b * p.mask_item : nullptr;
+    }
+    s.T = T;
+    s.k_row = (uint32_t)p.k_row * TL::ES;
+    s.v_row = (uint32_t)p.v_row * TL::ES;
+    s.k_bytes = p.dk * TL::ES;
+    s.v_off = (c * NJ < p.dk ? c * NJ : 0) * TL::ES;       // rows past the head's dimensions are not stored
+
+    // queries: B operand, column c = row m0 + 16 qt + c
+    uint32_t q[QT][NQ];
+    float qf[QT];        // factor of the scores
+    int lim[QT];         // keys below it are seen
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int m = m0 + 16 * qt + c, i = m / p.G, h = kh * p.G + (m - i * p.G);
+        const bool live = i < cnt;
+        const int64_t at = b * p.q_item + (live ? i * p.q_row + h * p.q_head : 0);
+        lim[qt] = p.causal ? T - cnt + i + 1 : T;
+        qf[qt] = p.scale;
+        if constexpr (KV == KV_F32) {
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) {
+                const int d = 16 * n + 4 * g;
+                float4v x = {0.f, 0.f, 0.f, 0.f};
+                if (live && d < p.dk) x = *(const float4v*)((const float*)p.q + at + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[qt][4 * n + e] = __float_as_uint(x[e]);
+            }
+        } else if constexpr (!QF32) {
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                const int d = key_dim<KV, D>(n, g);
+                int4v x = {0, 0, 0, 0};
+                if (live && d < p.dk) x = *(const int4v*)((const f16*)p.q + at + d);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[qt][4 * n + e] = x[e];
+            }
+        } else {
+            // q = (hi + lo) / f with f the power of two that takes the row's
+            // largest value to [2^13, 2^14): hi has 11 bits, lo the next 11,
+            // and what both drop is below 2^-37 of the largest
+            float x[D / 32][8], top = 0.f;
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                const int d = key_dim<KV, D>(n, g);
+                const bool in = live && d < p.dk;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[n][e] = in ? ((const float*)p.q + at)[d + e] : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[n][e]));
+            }
+            top = xgroup_max(top);
+            int ex = 0;
+            (void)frexpf(top, &ex);                        // top = [1/2, 1) 2^ex
+            ex = ex < -100 ? -100 : ex;
+            const float f = ldexpf(1.0f, 14 - ex);
+            qf[qt] *= ldexpf(1.0f, ex - 14);
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = x[n][2 * e] * f, bq = x[n][2 * e + 1] * f;
+                    const f16 ah = (f16)a, bh = (f16)bq;
+                    q[qt][4 * n + e] = pack_f16((float)ah, (float)bh);
+                    q[qt][D / 8 + 4 * n + e] = pack_f16(a - (float)ah, bq - (float)bh);
+                }
+        }
+    }
+
+    float4v o[QT][NJ];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = kNoMax;
+        l[qt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[qt][j] = (float4v){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // keys of this wave: every WK-th tile of the workgroup's share, up to the
+    // last that one of its rows sees
+    int hi = T;
+    if (p.causal) {
+        const int mi = (m0 + 16 * QT - 1) / p.G, il = mi < cnt ? mi : cnt - 1;
+        hi = T - cnt + il + 1 < T ? T - cnt + il + 1 : T;
+    }
+    const int k0 = split * p.split_keys;
+    const int64_t ke = (int64_t)k0 + p.split_keys;
+    const int k1 = ke < hi ? (int)ke : hi;
+    constexpr int STEP = 32 * WK;
+
+    auto compute = [&](Tile<KV, D>& t, int t0) {
+        const uint32_t keep = (uint32_t)__ballot(t.ok);
+        if (keep == 0) return;
+        const bool whole = keep == 0xffffffffu;
+        if (!whole) {      // what stands in the value rows of keys left out may be anything
+            const uint32_t bits = ((keep >> (4 * g)) & 0xF) | (((keep >> (16 + 4 * g)) & 0xF) << 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int w = 0; w < TL::NV; ++w) t.v[i][w] = (bits >> i) & 1 ? t.v[i][w] : 0;
+        }
+        float ks8[8], vs8[8];
+        if constexpr (TABLE) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = (i < 4 ? 0 : 12) + 4 * g + i;
+                ks8[i] = __shfl(t.ks, r, 64);
+                vs8[i] = __shfl(t.vs, r, 64);
+            }
+        }
+        float alpha[QT], vf[QT];
+        uint32_t ph[QT][4], pl[QT][4];
+        float pf[QT][8];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            const float4v s0 = tile_scores<KV, D, QF32, NQ>(t.k[0], q[qt]);
+            const float4v s1 = tile_scores<KV, D, QF32, NQ>(t.k[1], q[qt]);
+            float f = qf[qt];
+            if constexpr (KV == KV_I8 && !TABLE) f *= t.ks;
+            float sc[8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                sc[e] = s0[e] * f;
+                sc[4 + e] = s1[e] * f;
+                if constexpr (TABLE) {
+                    sc[e] *= ks8[e];
+                    sc[4 + e] *= ks8[4 + e];
+                }
+            }
+            if (!whole || p.causal) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int r = (e < 4 ? 0 : 12) + 4 * g + e;
+                    if (!((keep >> r) & 1) || t0 + r >= lim[qt]) sc[e] = -INFINITY;
+                }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
+            mx = fmaxf(m[qt], xgroup_max(mx));
+            alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mx);
+            m[qt] = mx;
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                pf[qt][e] = __builtin_amdgcn_exp2f(sc[e] - mx);
+                sum += pf[qt][e];
+            }
+            l[qt] = l[qt] * alpha[qt] + sum;
+            vf[qt] = 1.0f;
+            if constexpr (KV == KV_I8) {
+                if constexpr (TABLE) {
+                    // weights p vs of keys with different scales: divided by
+                    // their largest, so that f16 keeps it whatever the scales
+                    float top = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        pf[qt][e] *= vs8[e];
+                        top = fmaxf(top, pf[qt][e]);
+                    }
+                    top = xgroup_max(top);
+                    const float inv = top > 0.f ? 1.0f / top : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) pf[qt][e] *= inv;
+                    vf[qt] = top;
+                } else {
+                    vf[qt] = t.vs;
+                }
+            }
+            if constexpr (SPLIT) {
+                vf[qt] *= 0x1p-14f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = pf[qt][2 * e] * 0x1p14f, bq = pf[qt][2 * e + 1] * 0x1p14f;
+                    const f16 ah = (f16)a, bh = (f16)bq;
+                    ph[qt][e] = pack_f16((float)ah, (float)bh);
+                    pl[qt][e] = pack_f16(a - (float)ah, bq - (float)bh);
+                }
+            } else if constexpr (KV != KV_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ph[qt][e] = pack_f16(pf[qt][2 * e], pf[qt][2 * e + 1]);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if constexpr (KV == KV_F32) {
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    float4v acc = o[qt][j] * alpha[qt];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.v[i][j]), pf[qt][i], acc, 0, 0, 0);
+                    o[qt][j] = acc;
+                }
+            } else {
+                const half8v a = value_frag<KV, D>(t.v, j);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    const int4v bi = {(int)ph[qt][0], (int)ph[qt][1], (int)ph[qt][2], (int)ph[qt][3]};
+                    float4v acc = o[qt][j] * alpha[qt];
+                    if constexpr (KV == KV_F16) {
+                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi), acc, 0, 0, 0);
+                    } else {
+                        float4v blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi),
+                                                                            (float4v){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                        if constexpr (SPLIT) {
+                            const int4v bl = {(int)pl[qt][0], (int)pl[qt][1], (int)pl[qt][2], (int)pl[qt][3]};
+                            blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), blk, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[e] = fmaf(vf[qt], blk[e], acc[e]);
+                    }
+                    o[qt][j] = acc;
+                }
+            }
+        }
+    };
+
+    if (k0 + 32 * wk < k1) {
+        auto entry = [&](int t0) -> int {
+            if constexpr (TABLE) {
+                const int at = t0 + (lane & 31);
+                return s.table[at < T ? at : T - 1];
+            } else {
+                return 0;
+            }
+        };
+        int t0 = k0 + 32 * wk;
+        if constexpr (KV == KV_F32) {
+            for (; t0 < k1; t0 += STEP) {
+                Tile<KV, D> a;
+                load_tile<KV, D, TABLE>(a, s, t0, 0, lane);
+                compute(a, t0);
+            }
+        } else {
+            // the next tile's loads are in flight while a tile is computed,
+            // the table's entries one tile further ahead
+            Tile<KV, D> a, bt;
+            int e0 = entry(t0);
+            int e1 = entry(t0 + STEP);
+            load_tile<KV, D, TABLE>(a, s, t0, e0, lane);
+            while (true) {
+                e0 = entry(t0 + 2 * STEP);
+                load_tile<KV, D, TABLE>(bt, s, t0 + STEP, e1, lane);
+                compute(a, t0);
+                t0 += STEP;
+                if (t0 >= k1) break;
+                e1 = entry(t0 + 2 * STEP);
+                load_tile<KV, D, TABLE>(a, s, t0 + STEP, e0, lane);
+                compute(bt, t0);
+                t0 += STEP;
+                if (t0 >= k1) break;
+            }
+        }
+    }
+
+    // a lane's sums cover its own keys: join the four groups
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) l[qt] = xgroup_sum(l[qt]);
+
+    // lane (c, g) stores row c, dimensions (4g + e) NJ .. + NJ
+    auto store = [&](int qt, int e, const float* x, float ml, float ll) {
+        const int mr = m0 + 16 * qt + c, i = mr / p.G, h = kh * p.G + (mr - i * p.G), d = (4 * g + e) * NJ;
+        if (i >= cnt || d >= p.dk) return;
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
+            if (d == 0) p.part_ml[at] = float2{ml, ll};
+            if (ll != 0.f) {
+                float* y = p.part_o + at * p.dk + d;
+#pragma unroll
+                for (int j = 0; j < NJ; j += 2) *(float2v*)(y + j) = (float2v){x[j], x[j + 1]};
+            }
+            return;
+        }
+        const float inv = ll != 0.f ? 1.0f / ll : 0.f;
+        const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + d;
+        if constexpr (QF32) {
+            float* y = (float*)p.out + at;
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) *(float2v*)(y + j) = (float2v){x[j] * inv, x[j + 1] * inv};
+        } else {
+            uint32_t w[NJ / 2];
+#pragma unroll
+            for (int j = 0; j < NJ; j += 2) w[j / 2] = pack_f16(x[j] * inv, x[j + 1] * inv);
+            f16* y = (f16*)p.out + at;
+            if constexpr (NJ == 8) *(int4v*)y = (int4v){(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+            else if constexpr (NJ == 4) *(int2v*)y = (int2v){(int)w[0], (int)w[1]};
+            else *(uint32_t*)y = w[0];
+        }
+    };
+    if constexpr (WK == 1) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float x[NJ];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) x[j] = o[qt][j][e];
+                store(qt, e, x, m[qt], l[qt]);
+            }
+    } else {
+        // four key shares: brought to a common maximum, wave e adds and stores
+        // accumulator register e of every wave, in wave order
+        __shared__ float sml[2][WK][16];
+        __shared__ float so[WK][4][NJ][64];
+        if (g == 0) {
+            sml[0][wk][c] = m[0];
+            sml[1][wk][c] = l[0];
+        }
+        __syncthreads();
+        float mm = sml[0][0][c], ll = 0.f;
+#pragma unroll
+        for (int w = 1; w < WK; ++w) mm = fmaxf(mm, sml[0][w][c]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) ll += sml[1][w][c] * __builtin_amdgcn_exp2f(sml[0][w][c] - mm);
+        const float fw = __builtin_amdgcn_exp2f(m[0] - mm);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) so[wk][e][j][lane] = o[0][j][e] * fw;
+        __syncthreads();
+        float x[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            x[j] = so[0][wk][j][lane];
+#pragma unroll
+            for (int w = 1; w < WK; ++w) x[j] += so[w][wk][j][lane];
+        }
+        store(0, wk, x, mm, ll);
+    }
+}
+
+// One wave per row: joins the splits' (m, l, O) in split order.
+template <bool F32> __global__ __launch_bounds__(256) void dec_join_kernel(DecAttnParams p) {
+    const int lane = threadIdx.x & 63, M = p.n_q * p.G;
+    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= (int64_t)p.B * p.Hkv * M) return;
+    const int mr = (int)(row % M), kh = (int)(row / M % p.Hkv), b = (int)(row / M / p.Hkv);
+    const int i = mr / p.G, h = kh * p.G + (mr - i * p.G);
+    int cnt = p.q_len ? p.q_len[b] : p.n_q;
+    if (i >= cnt) return;
+    const float2* ml = p.part_ml + row * p.splits;
+    float mm = kNoMax;
+    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[s].x);
+    mm = wave_max(mm);
+    float l = 0.f, x0 = 0.f, x1 = 0.f;
+    const int d = 2 * lane;
+    for (int s = 0; s < p.splits; ++s) {
+        const float2 v = ml[s];
+        if (v.y == 0.f) continue;      // no key of this split is attended: its O is not written
+        const float f = __builtin_amdgcn_exp2f(v.x - mm);
+        l += v.y * f;
+        if (d < p.dk) {
+            const float2v o = *(const float2v*)(p.part_o + (row * p.splits + s) * p.dk + d);
+            x0 += o[0] * f;
+            x1 += o[1] * f;
+        }
+    }
+    if (d >= p.dk) return;
+    const float inv = l != 0.f ? 1.0f / l : 0.f;
+    const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + d;
+    if constexpr (F32) *(float2v*)((float*)p.out + at) = (float2v){x0 * inv, x1 * inv};
+    else *(uint32_t*)((f16*)p.out + at) = pack_f16(x0 * inv, x1 * inv);
+}
+
+// Rows a workgroup takes and how many ways the keys are split over workgroups.
+struct Shape { bool wide; int rows, mt, splits, keys; };
+Shape attn_shape(const DecAttnParams& p) {
+    Shape s;
+    const int64_t M = (int64_t)p.n_q * p.G, units = (int64_t)p.B * p.Hkv;
+    s.wide = M >= 64;
+    s.rows = s.wide ? 128 : 16;
+    s.mt = cdiv(M, s.rows);
+    const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
+    const int64_t wgs = units * s.mt;
+    int64_t want = wgs >= 512 ? 1 : 512 / wgs;             // about two workgroups per CU
+    const int least = s.wide ? 8 : 8;                      // tiles a split is worth
+    const int64_t most = tiles / least > 0 ? tiles / least : 1;
+    if (want > most) want = most;
+    if (want > 64) want = 64;
+    const int per = cdiv(tiles, want);
+    s.splits = cdiv(tiles, per);
+    s.keys = per * 32;
+    return s;
+}
+
+template <int KV, bool QF32, int D, bool TABLE> void launch_shape(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * sh.mt * sh.splits));
+    if (sh.wide) launch(dec_attn_kernel<KV, QF32, D, 2, 4, 1, TABLE>, grid, dim3(256), 0, s, p);
+    else launch(dec_attn_kernel<KV, QF32, D, 1, 1, 4, TABLE>, grid, dim3(256), 0, s, p);
+}
+template <int KV, bool QF32, bool TABLE> void launch_width(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
+    if (p.dk <= 32) launch_shape<KV, QF32, 32, TABLE>(p, sh, s);
+    else if (p.dk <= 64) launch_shape<KV, QF32, 64, TABLE>(p, sh, s);
+    else launch_shape<KV, QF32, 128, TABLE>(p, sh, s);
+}
+
+}  // namespace
+
+size_t dec_attention_workspace(const DecAttnParams& p) {
+    if (p.B == 0 || p.n_q == 0) return 0;
+    const Shape sh = attn_shape(p);
+    if (sh.splits == 1) return 0;
+    const size_t parts = (size_t)p.B * p.Hkv * p.n_q * p.G * sh.splits;
+    return parts * (sizeof(float2) + (size_t)p.dk * sizeof(float));
+}
+
+void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_t s) {
+    if (p.B == 0 || p.n_q == 0) return;
+    const Shape sh = attn_shape(p);
+    require((int64_t)p.B * p.Hkv * sh.mt * sh.splits < (1 << 23) && (int64_t)p.B * p.Hkv * p.n_q * p.G < (1 << 30),
+            "attention: too many rows for one call");
+    const size_t need = dec_attention_workspace(p);
+    require(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need),
+            "attention: the workspace is smaller than its size query says, or not 16-byte aligned");
+    p.scale *= kLog2e;
+    p.splits = sh.splits;
+    p.split_keys = sh.keys;
+    if (need) {
+        const size_t parts = (size_t)p.B * p.Hkv * p.n_q * p.G * sh.splits;
+        p.part_ml = (float2*)ws;
+        p.part_o = (float*)((char*)ws + parts * sizeof(float2));
+    }
+    if (p.kv == KV_F16) launch_width<KV_F16, false, false>(p, sh, s);
+    else if (p.kv == KV_F32) launch_width<KV_F32, true, false>(p, sh, s);
+    else if (p.q_f32) p.table ? launch_width<KV_I8, true, true>(p, sh, s) : launch_width<KV_I8, true, false>(p, sh, s);
+    else p.table ? launch_width<KV_I8, false, true>(p, sh, s) : launch_width<KV_I8, false, false>(p, sh, s);
+    if (sh.splits > 1) {
+        const int64_t rows = (int64_t)p.B * p.Hkv * p.n_q * p.G;
+        if (p.q_f32) launch(dec_join_kernel<true>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+        else launch(dec_join_kernel<false>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+    }
+}
+
+}  // namespace pkx

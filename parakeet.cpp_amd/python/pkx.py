@@ -44,6 +44,47 @@ class Config(C.Structure):
                                         "stream_valid_out_len", "stream_drop_extra")]
 
 
+_i32, _i64, _sz = C.c_int, C.c_int64, C.c_size_t
+TYPE_F32, TYPE_F16 = 0, 1
+CACHE8_BLOCK, BEAM_MAX_STATES = 32, 32
+
+
+class CrossAttnArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_items", "n_q", "n_k", "n_heads", "n_kv_heads", "d_head")] +
+                [("scale", C.c_float)] +
+                [f for n in ("q", "k", "v", "out")
+                 for f in [(n, _vp), (n + "_item", _i64), (n + "_row", _i64), (n + "_head", _i64)]] +
+                [("q_len", _vp), ("k_len", _vp), ("k_mask", _vp), ("k_mask_item", _i64)])
+
+
+class Cache8Args(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("n_slots", "n_kv_heads", "d_head", "capacity")] +
+                [(n, _vp) for n in ("k", "v", "k_scale", "v_scale")])
+
+
+class Cache8Tokens(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_rows", "n_new")] +
+                [f for n in ("k", "v") for f in [(n, _vp), (n + "_row", _i64), (n + "_tok", _i64), (n + "_head", _i64)]] +
+                [("slot", _vp), ("start", _vp), ("count", _vp), ("table", _vp), ("table_row", _i64)])
+
+
+class Cache8AttnArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_rows", "n_q", "n_heads", "causal")] + [("scale", C.c_float)] +
+                [f for n in ("q", "out") for f in [(n, _vp), (n + "_row", _i64), (n + "_tok", _i64), (n + "_head", _i64)]] +
+                [("slot", _vp), ("len", _vp), ("q_len", _vp), ("table", _vp), ("table_row", _i64), ("max_len", _i32)])
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_items", "n_beams", "vocab", "end_id")] +
+                [("logits", _vp), ("logits_row", _i64)] +
+                [(n, _vp) for n in ("scores", "done", "parent", "token", "new_scores", "new_done")])
+
+
+class BeamState(C.Structure):
+    _fields_ = [("src", _vp), ("dst", _vp), ("src_row", _i64), ("dst_row", _i64), ("bytes", _i64)]
+
+
+_P = C.POINTER
 SIGS = {
     "pkx_abi_version": ([], C.c_int),
     "pkx_last_error": ([], C.c_char_p),
@@ -106,6 +147,15 @@ SIGS = {
     "pkx_streaming_info": ([_vp, _ip, _ip, _ip, _ip, _ip], C.c_int),
     "pkx_streaming_chunk_len": ([_vp, C.c_int], C.c_int),
     "pkx_streaming_step": ([_vp, _vp, C.c_int, C.c_int, _vp, _ip, _vp], C.c_int),
+    "pkx_cross_attention_workspace": ([_P(CrossAttnArgs), _P(_sz)], C.c_int),
+    "pkx_cross_attention": ([_P(CrossAttnArgs), _vp, _sz, _vp], C.c_int),
+    "pkx_cache8_append": ([_P(Cache8Args), _P(Cache8Tokens), _vp], C.c_int),
+    "pkx_cache8_read": ([_P(Cache8Args), _i32, _i32, _vp, _vp, _vp, _vp, _vp], C.c_int),
+    "pkx_cache8_attention_workspace": ([_P(Cache8Args), _P(Cache8AttnArgs), _P(_sz)], C.c_int),
+    "pkx_cache8_attention": ([_P(Cache8Args), _P(Cache8AttnArgs), _vp, _sz, _vp], C.c_int),
+    "pkx_beam_select_workspace": ([_P(BeamSelectArgs), _P(_sz)], C.c_int),
+    "pkx_beam_select": ([_P(BeamSelectArgs), _vp, _sz, _vp], C.c_int),
+    "pkx_beam_reorder": ([_vp, _i32, _i32, _P(BeamState), _i32, _vp], C.c_int),
     "pkx_model_set_profiling": ([_vp, C.c_uint, C.c_int], C.c_int),
     "pkx_model_profile_read": ([_vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)], C.c_int),
 }
@@ -549,3 +599,169 @@ def quantize_gguf(in_path, out_path, qtype: str):
     check(lib().pkx_quantize_gguf(str(in_path).encode(), str(out_path).encode(), gt, C.byref(nq), C.byref(nk),
                                   C.byref(ns)))
     return nq.value, nk.value, ns.value
+
+
+# ---- attention decoder operators ------------------------------------------------
+# Each object binds its buffers once (a decode loop calls the same ones every step)
+# and keeps them and its workspace alive; calling it starts the kernels on `stream`.
+# An object's calls share its workspace: they must not overlap.  Arrays are
+# DeviceArrays or anything with .ptr, .shape and .dtype.
+def _type(a):
+    t = {"float32": TYPE_F32, "float16": TYPE_F16}.get(np.dtype(a.dtype).name)
+    if t is None:
+        raise PkxError(f"float16 or float32 arrays are wanted, got {a.dtype}")
+    return t
+
+
+def _ptr(a):
+    return None if a is None else a.ptr
+
+
+def _expect(a, shape, dtype, what):
+    if a is not None and (tuple(a.shape) != tuple(shape) or np.dtype(a.dtype) != np.dtype(dtype)):
+        raise PkxError(f"{what}: {np.dtype(dtype).name} {list(shape)} is wanted, got {np.dtype(a.dtype).name} {list(a.shape)}")
+
+
+def _strides(a):
+    """Elements between items, rows and heads of a packed [item][row][head][dim] array, or the array's own .strides."""
+    own = getattr(a, "strides", None)
+    if own is not None:
+        return tuple(own)[:3]
+    _, t, h, d = a.shape
+    return t * h * d, h * d, d
+
+
+class _Bound:
+    """A call with its arguments bound: fn(*args, stream)."""
+
+    def _bind(self, fn, args, keep, size_fn=None):
+        self._fn, self._keep, self.workspace = getattr(lib(), fn), keep, None
+        if size_fn is not None:
+            n = C.c_size_t()
+            check(getattr(lib(), size_fn)(*args, C.byref(n)))
+            if n.value:
+                self.workspace = DeviceArray((n.value,), np.uint8)
+            args = args + (_ptr(self.workspace), n.value)
+        self._args = args
+
+    def __call__(self, stream=None):
+        if self._fn(*self._args, stream.handle if stream is not None else None):
+            raise PkxError(lib().pkx_last_error().decode())
+
+
+class CrossAttention(_Bound):
+    """pkx_cross_attention: q, out [B][n_q][H][d], k, v [B][n_k][Hkv][d]; k_mask [B][n_k] uint8."""
+
+    def __init__(self, q, k, v, out, q_len=None, k_len=None, k_mask=None, scale=None):
+        (B, nq, H, d), (_, nk, Hkv, _) = q.shape, k.shape
+        for a, n, dt in ((k, (B, nk, Hkv, d), q.dtype), (v, (B, nk, Hkv, d), q.dtype), (out, q.shape, q.dtype),
+                         (q_len, (B,), np.int32), (k_len, (B,), np.int32), (k_mask, (B, nk), np.uint8)):
+            _expect(a, n, dt, "cross attention")
+        a = CrossAttnArgs(_type(q), B, nq, nk, H, Hkv, d, d ** -0.5 if scale is None else scale, q.ptr, *_strides(q),
+                          k.ptr, *_strides(k), v.ptr, *_strides(v), out.ptr, *_strides(out), _ptr(q_len), _ptr(k_len),
+                          _ptr(k_mask), nk)
+        self._bind("pkx_cross_attention", (C.byref(a),), (a, q, k, v, out, q_len, k_len, k_mask),
+                   "pkx_cross_attention_workspace")
+
+
+class Cache8:
+    """A key/value cache in 8 bits (pkx_cache8): k, v int8 [S][Hkv][capacity][d], scales f32 [S][Hkv][capacity / 32]."""
+
+    def __init__(self, n_slots, n_kv_heads, d_head, capacity):
+        n = (n_slots, n_kv_heads, capacity)
+        self._set(*(DeviceArray(n + (d_head,), np.int8) for _ in range(2)),
+                  *(DeviceArray(n[:2] + (capacity // CACHE8_BLOCK,), np.float32) for _ in range(2)))
+
+    @classmethod
+    def wrap(cls, k, v, k_scale, v_scale):
+        """A cache in the caller's buffers."""
+        c = cls.__new__(cls)
+        c._set(k, v, k_scale, v_scale)
+        return c
+
+    def _set(self, k, v, k_scale, v_scale):
+        S, H, cap, d = k.shape
+        for a, n, dt in ((k, k.shape, np.int8), (v, k.shape, np.int8), (k_scale, (S, H, cap // CACHE8_BLOCK), np.float32),
+                         (v_scale, (S, H, cap // CACHE8_BLOCK), np.float32)):
+            _expect(a, n, dt, "8-bit cache")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.n_slots, self.n_kv_heads, self.capacity, self.d_head = S, H, cap, d
+        self.args = Cache8Args(S, H, d, cap, k.ptr, v.ptr, k_scale.ptr, v_scale.ptr)
+
+
+def _table_row(table, rows):
+    if table is None:
+        return 0
+    if len(table.shape) != 2 or table.shape[0] != rows or np.dtype(table.dtype) != np.int32:
+        raise PkxError(f"cache table: int32 [{rows}][positions] is wanted, got {table.dtype} {list(table.shape)}")
+    return table.shape[1]
+
+
+class CacheAppend(_Bound):
+    """pkx_cache8_append: k, v [R][n_new][Hkv][d]; start, slot, count [R] int32; table [R][capacity] int32."""
+
+    def __init__(self, cache, k, v, start, slot=None, count=None, table=None):
+        R, n, H, d = k.shape
+        for a, m, dt in ((k, (R, n, cache.n_kv_heads, cache.d_head), k.dtype), (v, k.shape, k.dtype),
+                         (start, (R,), np.int32), (slot, (R,), np.int32), (count, (R,), np.int32)):
+            _expect(a, m, dt, "cache append")
+        a = Cache8Tokens(_type(k), R, n, k.ptr, *_strides(k), v.ptr, *_strides(v), _ptr(slot), start.ptr, _ptr(count),
+                         _ptr(table), _table_row(table, R))
+        self._bind("pkx_cache8_append", (C.byref(cache.args), C.byref(a)), (cache, a, k, v, start, slot, count, table))
+
+
+class CacheRead(_Bound):
+    """pkx_cache8_read: k_out, v_out f32 [R][n][Hkv][d]."""
+
+    def __init__(self, cache, k_out, v_out, start, slot=None):
+        R, n = (k_out if k_out is not None else v_out).shape[:2]
+        for a, m, dt in ((k_out, (R, n, cache.n_kv_heads, cache.d_head), np.float32),
+                         (v_out, (R, n, cache.n_kv_heads, cache.d_head), np.float32), (start, (R,), np.int32),
+                         (slot, (R,), np.int32)):
+            _expect(a, m, dt, "cache read")
+        self._bind("pkx_cache8_read", (C.byref(cache.args), R, n, _ptr(slot), start.ptr, _ptr(k_out), _ptr(v_out)),
+                   (cache, k_out, v_out, start, slot))
+
+
+class CacheAttention(_Bound):
+    """pkx_cache8_attention: q, out [R][n_q][H][d]; length, slot, q_len [R] int32; table [R][positions] int32."""
+
+    def __init__(self, cache, q, out, length, slot=None, q_len=None, table=None, causal=True, scale=None, max_len=0):
+        R, n, H, d = q.shape
+        for a, m, dt in ((q, (R, n, H, cache.d_head), q.dtype), (out, q.shape, q.dtype), (length, (R,), np.int32),
+                         (slot, (R,), np.int32), (q_len, (R,), np.int32)):
+            _expect(a, m, dt, "cache attention")
+        a = Cache8AttnArgs(_type(q), R, n, H, int(causal), d ** -0.5 if scale is None else scale, q.ptr, *_strides(q),
+                           out.ptr, *_strides(out), _ptr(slot), length.ptr, _ptr(q_len), _ptr(table),
+                           _table_row(table, R), max_len)
+        self._bind("pkx_cache8_attention", (C.byref(cache.args), C.byref(a)),
+                   (cache, a, q, out, length, slot, q_len, table), "pkx_cache8_attention_workspace")
+
+
+class BeamSelect(_Bound):
+    """pkx_beam_select: logits [B][W][V] -> parent, token int32, new_scores f32, new_done uint8, all [B][W]."""
+
+    def __init__(self, logits, scores, parent, token, new_scores, done=None, new_done=None, end_id=-1):
+        B, W, V = logits.shape
+        for a, dt in ((scores, np.float32), (parent, np.int32), (token, np.int32), (new_scores, np.float32),
+                      (done, np.uint8), (new_done, np.uint8)):
+            _expect(a, (B, W), dt, "beam select")
+        a = BeamSelectArgs(_type(logits), B, W, V, end_id, logits.ptr, V, scores.ptr, _ptr(done), parent.ptr, token.ptr,
+                           new_scores.ptr, _ptr(new_done))
+        self._bind("pkx_beam_select", (C.byref(a),), (a, logits, scores, parent, token, new_scores, done, new_done),
+                   "pkx_beam_select_workspace")
+
+
+class BeamReorder(_Bound):
+    """pkx_beam_reorder: for every (src, dst) pair of [B * W][...] arrays, row b W + w of dst = row b W + parent[b][w] of src."""
+
+    def __init__(self, parent, states):
+        B, W = parent.shape
+        _expect(parent, (B, W), np.int32, "beam reorder")
+        a = (BeamState * max(len(states), 1))()
+        for i, (s, d) in enumerate(states):
+            if tuple(s.shape) != tuple(d.shape) or np.dtype(s.dtype) != np.dtype(d.dtype) or s.shape[0] != B * W:
+                raise PkxError(f"beam reorder: states are pairs of the same [{B * W}][...], got {list(s.shape)} and {list(d.shape)}")
+            n = int(np.prod(s.shape[1:])) * np.dtype(s.dtype).itemsize
+            a[i] = BeamState(s.ptr, d.ptr, n, n, n)
+        self._bind("pkx_beam_reorder", (parent.ptr, B, W, a, len(states)), (parent, a, states))
