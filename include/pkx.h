@@ -444,8 +444,8 @@ int pkx_cache8_attention(const pkx_cache8* c, const pkx_cache8_attn* a, void* ws
  * after the order of the logits.  A finished beam (done[w] != 0) has the one candidate (w, end_id) of score
  * scores[w].  A beam with a NaN or +inf among its logits, or with no finite one, or whose score is NaN or
  * +inf, has candidates of score -inf only.  Outputs per item, best first: parent beam, token, score and
- * whether the beam is finished (its parent was, or the token is end_id).  n_beams: 1 to 32;
- * outputs overlap no input. */
+ * whether the beam is finished (its parent was, or the token is end_id).  n_beams: 1 to 32,
+ * vocab up to 2^22; outputs overlap no input. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of logits */
     int n_items, n_beams, vocab;

@@ -247,6 +247,7 @@ pkx::BeamSelectParams beam_params(const pkx_beam_select_args* a) {
     pkx::BeamSelectParams p;
     p.f32 = is_f32(a->type, "beam select: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
     need(a->n_items >= 0 && a->n_beams >= 1 && a->n_beams <= pkx::kMaxBeams, "beam select: n_beams must be 1 to 32");
+    need(a->vocab <= (1 << 22), "beam select: a vocabulary of at most 2^22 words");
     need(a->vocab >= 1 && a->end_id >= -1 && a->end_id < a->vocab, "beam select: end_id must be -1 or a word of the vocabulary");
     need(!a->done || a->end_id >= 0, "beam select: finished beams need an end_id");
     p.B = a->n_items;

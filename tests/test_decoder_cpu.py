@@ -116,10 +116,10 @@ def test_beam_refusals():
         for kw in (dict(type=8), dict(n_beams=0), dict(n_beams=33), dict(vocab=0), dict(end_id=100), dict(end_id=-2),
                    dict(done=A, end_id=-1), dict(logits=None), dict(token=None), dict(logits=A + 1), dict(logits_row=-1)):
             said(L.pkx_beam_select(beam(**kw), A, 1 << 30, None))
-        n = C.c_size_t()
-        said(L.pkx_beam_select_workspace(beam(), C.byref(n)))
-        said(L.pkx_beam_select(beam(), A, n.value - 1, None))
-        said(L.pkx_beam_select(beam(), None, 0, None))
+        n, many = C.c_size_t(), beam(vocab=100000, logits_row=100000)
+        said(L.pkx_beam_select_workspace(many, C.byref(n)))
+        said(L.pkx_beam_select(many, A, n.value - 1, None))
+        said(L.pkx_beam_select(many, None, 0, None))
         said(L.pkx_beam_select(beam(n_items=0), None, 0, None))
         S = pkx.BeamState
         def order(states, B=2, W=2, n=None):
