@@ -360,7 +360,7 @@ int pkx_quantize_gguf(const char* in_path, const char* out_path, int gtype, int*
  * are W query rows.  f16: f16 operands, softmax and sums in f32, weights rounded to f16
  * for the second product; f32: f32 throughout.
  * Strides are in elements (item, row, head; the d_head elements are adjacent), those of
- * k and v not negative and below 2^24 between rows.  d_head: a multiple of 8 up to 128;
+ * k and v not negative and below 2^22 between rows.  d_head: a multiple of 8 up to 128;
  * buffers 16-byte aligned, strides multiples of 16 bytes; n_heads a multiple of
  * n_kv_heads.  out overlaps no input. */
 typedef struct {

@@ -722,7 +722,7 @@ int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void
         if (p.n_k > 0) {
             need_view(p.k, p.k_item, p.k_row, p.k_head, p.q_f32, "cross attention: k must be 16-byte aligned with strides of whole 16 bytes");
             need_view(p.v, p.v_item, p.v_row, p.v_head, p.q_f32, "cross attention: v must be 16-byte aligned with strides of whole 16 bytes");
-            need(p.k_row < (1 << 24) && p.v_row < (1 << 24), "cross attention: key rows must be less than 2^24 elements apart");
+            need(p.k_row < (1 << 22) && p.v_row < (1 << 22), "cross attention: key rows must be less than 2^22 elements apart");
         }
         need_device(st(s));
         pkx::launch_dec_attention(p, ws, ws_bytes, st(s));

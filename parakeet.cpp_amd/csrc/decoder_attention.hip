@@ -48,6 +48,9 @@ __device__ __forceinline__ float xgroup_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// x / d for scalars below 2^22
+__device__ __forceinline__ int uniform_div(int x, int d) { return __builtin_amdgcn_readfirstlane(udiv_small(x, d)); }
+
 // int8 pairs spread to the low bytes of two halves -> f16
 __device__ __forceinline__ uint32_t i8_pair_f16(uint32_t spread) {
     const half2v h = __builtin_bit_cast(half2v, spread ^ 0x64806480u) + (half2v){(f16)-1152.0f, (f16)-1152.0f};
@@ -156,6 +159,84 @@ __device__ __forceinline__ void load_tile(Tile<KV, D>& t, const KeySource& s, in
     }
 }
 
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    const half2v h = {(f16)a, (f16)b};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// Row m of an item and key head as lane group g's fragments (LAYOUT: the kind
+// of keys whose order of dimensions they meet); returns its query index.  Rows past the queries are zeros.
+template <int KV, bool QF32, int D, int LAYOUT, int NQ>
+__device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, int kh, int cnt, int g, uint32_t (&q)[NQ], float& qf) {
+    const int i = udiv_small(m, p.G), h = kh * p.G + (m - i * p.G);
+    const bool live = i < cnt;
+    // rows past the queries and pieces past the head's dimensions read another
+    // row's or piece instead and become zeros: the loads wait on no branch
+    const int64_t at = b * p.q_item + (live ? i * p.q_row : 0) + h * p.q_head;
+    qf = p.scale;
+    if constexpr (KV == KV_F32) {
+        float4v x[D / 16];
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            const int d = 16 * n + 4 * g;
+            x[n] = *(const float4v*)((const float*)p.q + at + (d < p.dk ? d : 0));
+        }
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[4 * n + e] = live && 16 * n + 4 * g < p.dk ? __float_as_uint(x[n][e]) : 0u;
+    } else if constexpr (!QF32) {
+        int4v x[D / 32];
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const int d = key_dim<LAYOUT, D>(n, g);
+            x[n] = *(const int4v*)((const f16*)p.q + at + (d < p.dk ? d : 0));
+        }
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[4 * n + e] = live && key_dim<LAYOUT, D>(n, g) < p.dk ? x[n][e] : 0;
+    } else {
+        // q = (hi + lo) / f with f the power of two that takes the row's
+        // largest value to [2^13, 2^14): hi has 11 bits, lo the next 11,
+        // and what both drop is below 2^-37 of the largest
+        float4v y[D / 32][2];
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const int d = key_dim<LAYOUT, D>(n, g);
+            const float* src = (const float*)p.q + at + (d < p.dk ? d : 0);
+            y[n][0] = *(const float4v*)src;
+            y[n][1] = *(const float4v*)(src + 4);
+        }
+        float x[D / 32][8], top = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n) {
+            const bool in = live && key_dim<LAYOUT, D>(n, g) < p.dk;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[n][e] = in ? y[n][e >> 2][e & 3] : 0.f;
+                top = fmaxf(top, fabsf(x[n][e]));
+            }
+        }
+        top = xgroup_max(top);
+        int ex = 0;
+        (void)frexpf(top, &ex);                        // top = [1/2, 1) 2^ex
+        ex = ex < -100 ? -100 : ex;
+        const float f = ldexpf(1.0f, 14 - ex);
+        qf *= ldexpf(1.0f, ex - 14);
+#pragma unroll
+        for (int n = 0; n < D / 32; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float a = x[n][2 * e] * f, bq = x[n][2 * e + 1] * f;
+                const f16 ah = (f16)a, bh = (f16)bq;
+                q[4 * n + e] = pack_f16((float)ah, (float)bh);
+                q[D / 8 + 4 * n + e] = pack_f16(a - (float)ah, bq - (float)bh);
+            }
+    }
+    return i;
+}
+
 // scores of a 16-key tile (c: keys 4g + e of query lane % 16)
 template <int KV, int D, bool QF32, int NQ>
 __device__ __forceinline__ float4v tile_scores(const uint32_t (&k)[Tile<KV, D>::NK], const uint32_t (&q)[NQ]) {
@@ -205,11 +286,6 @@ template <int KV, int D> __device__ __forceinline__ half8v value_frag(const uint
     return __builtin_bit_cast(half8v, a);
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    const half2v h = {(f16)a, (f16)b};
-    return __builtin_bit_cast(uint32_t, h);
-}
-
 template <int KV, bool QF32, int D, int QT, int WM, int WK, bool TABLE>
 __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p) {
     using TL = Tile<KV, D>;
@@ -217,21 +293,19 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
     constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
     constexpr int NQ = KV == KV_F32 ? D / 4 : SPLIT ? D / 4 : D / 8;
     constexpr int NJ = D / 16, ROWS = 16 * QT * WM;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int wm = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
     const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
-    int id = xcd_tile(blockIdx.x, gridDim.x);              // row tiles of one item and head share an XCD's L2
-    const int mtile = id % mt;
-    id /= mt;
-    const int split = id % p.splits;
-    id /= p.splits;
-    const int kh = id % p.Hkv, b = id / p.Hkv;
+    // row tiles of one item and head share an XCD's L2
+    const int id = xcd_tile(blockIdx.x, gridDim.x), id1 = uniform_div(id, mt), mtile = id - id1 * mt;
+    const int id2 = uniform_div(id1, p.splits), split = id1 - id2 * p.splits;
+    const int b = uniform_div(id2, p.Hkv), kh = id2 - b * p.Hkv;
 
     int T = p.k_len ? p.k_len[b] : p.n_k;
     T = T < 0 ? 0 : T > p.n_k ? p.n_k : T;
     int cnt = p.q_len ? p.q_len[b] : p.n_q;
     cnt = cnt < 0 ? 0 : cnt > p.n_q ? p.n_q : cnt;
-    if (mtile * ROWS / p.G >= cnt) return;                 // no row of this tile is asked for
+    if (uniform_div(mtile * ROWS, p.G) >= cnt) return;                 // no row of this tile is asked for
     const int m0 = mtile * ROWS + wm * 16 * QT;
     KeySource s = {};
     if constexpr (KV == KV_I8) {
@@ -265,59 +339,8 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
     int lim[QT];         // keys below it are seen
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        const int m = m0 + 16 * qt + c, i = m / p.G, h = kh * p.G + (m - i * p.G);
-        const bool live = i < cnt;
-        const int64_t at = b * p.q_item + (live ? i * p.q_row + h * p.q_head : 0);
+        const int i = load_query<KV, QF32, D, KV>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt]);
         lim[qt] = p.causal ? T - cnt + i + 1 : T;
-        qf[qt] = p.scale;
-        if constexpr (KV == KV_F32) {
-#pragma unroll
-            for (int n = 0; n < D / 16; ++n) {
-                const int d = 16 * n + 4 * g;
-                float4v x = {0.f, 0.f, 0.f, 0.f};
-                if (live && d < p.dk) x = *(const float4v*)((const float*)p.q + at + d);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[qt][4 * n + e] = __float_as_uint(x[e]);
-            }
-        } else if constexpr (!QF32) {
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                const int d = key_dim<KV, D>(n, g);
-                int4v x = {0, 0, 0, 0};
-                if (live && d < p.dk) x = *(const int4v*)((const f16*)p.q + at + d);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) q[qt][4 * n + e] = x[e];
-            }
-        } else {
-            // q = (hi + lo) / f with f the power of two that takes the row's
-            // largest value to [2^13, 2^14): hi has 11 bits, lo the next 11,
-            // and what both drop is below 2^-37 of the largest
-            float x[D / 32][8], top = 0.f;
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                const int d = key_dim<KV, D>(n, g);
-                const bool in = live && d < p.dk;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[n][e] = in ? ((const float*)p.q + at)[d + e] : 0.f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[n][e]));
-            }
-            top = xgroup_max(top);
-            int ex = 0;
-            (void)frexpf(top, &ex);                        // top = [1/2, 1) 2^ex
-            ex = ex < -100 ? -100 : ex;
-            const float f = ldexpf(1.0f, 14 - ex);
-            qf[qt] *= ldexpf(1.0f, ex - 14);
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = x[n][2 * e] * f, bq = x[n][2 * e + 1] * f;
-                    const f16 ah = (f16)a, bh = (f16)bq;
-                    q[qt][4 * n + e] = pack_f16((float)ah, (float)bh);
-                    q[qt][D / 8 + 4 * n + e] = pack_f16(a - (float)ah, bq - (float)bh);
-                }
-        }
     }
 
     float4v o[QT][NJ];
@@ -334,7 +357,7 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
     // last that one of its rows sees
     int hi = T;
     if (p.causal) {
-        const int mi = (m0 + 16 * QT - 1) / p.G, il = mi < cnt ? mi : cnt - 1;
+        const int mi = uniform_div(m0 + 16 * QT - 1, p.G), il = mi < cnt ? mi : cnt - 1;
         hi = T - cnt + il + 1 < T ? T - cnt + il + 1 : T;
     }
     const int k0 = split * p.split_keys;
@@ -382,10 +405,12 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
                 }
             }
             if (!whole || p.causal) {
+                const uint32_t bits = keep >> (4 * g);
+                const int below = lim[qt] - t0 - 4 * g;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int r = (e < 4 ? 0 : 12) + 4 * g + e;
-                    if (!((keep >> r) & 1) || t0 + r >= lim[qt]) sc[e] = -INFINITY;
+                    const int r = e < 4 ? e : 12 + e;
+                    if (!(bits & (1u << r)) || r >= below) sc[e] = -INFINITY;
                 }
             }
             float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
@@ -512,7 +537,7 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
 
     // lane (c, g) stores row c, dimensions (4g + e) NJ .. + NJ
     auto store = [&](int qt, int e, const float* x, float ml, float ll) {
-        const int mr = m0 + 16 * qt + c, i = mr / p.G, h = kh * p.G + (mr - i * p.G), d = (4 * g + e) * NJ;
+        const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G), d = (4 * g + e) * NJ;
         if (i >= cnt || d >= p.dk) return;
         if (p.splits > 1) {
             const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
@@ -582,33 +607,390 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
     }
 }
 
-// One wave per row: joins the splits' (m, l, O) in split order.
-template <bool F32> __global__ __launch_bounds__(256) void dec_join_kernel(DecAttnParams p) {
-    const int lane = threadIdx.x & 63, M = p.n_q * p.G;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= (int64_t)p.B * p.Hkv * M) return;
-    const int mr = (int)(row % M), kh = (int)(row / M % p.Hkv), b = (int)(row / M / p.Hkv);
-    const int i = mr / p.G, h = kh * p.G + (mr - i * p.G);
+// A buffer resource of one step's rows, built from scalars.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const uint8_t* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, 0x00020000);
+}
+
+// Many query rows against the same keys: 128 rows a workgroup, 32 a wave, the
+// keys in steps of 64 through LDS, where every wave reads them.  8-bit keys
+// become f16 on the way in, once for the workgroup.  The value rows are turned
+// there too: a thread loads 8 keys x D/32 dimensions and writes, per dimension,
+// its 8 keys as one 16-byte piece, in the order in which the value product's
+// operand wants them.  The next step's rows are loaded to registers while a
+// step is computed.  LDS rows of 16-byte pieces are permuted (piece ^ row) so
+// that neither the writes nor the operand reads meet in a bank.
+//
+// Weights go to f16 as 2^14 p r, r = (value scale of the block) / (largest so
+// far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
+// different scales add up in one accumulator, which is rescaled when v grows.
+// Both ride in the exponent: 2^(s - m + 14 + log2 r).
+template <int KV, bool QF32, int D, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
+    constexpr int QT = 2, NW = 4, ROWS = 16 * QT * NW, KT = 64;
+    constexpr bool SPLIT = KV == KV_I8 && QF32;
+    constexpr int ES = KV == KV_F16 ? 2 : 1, NQ = SPLIT ? D / 4 : D / 8, NJ = D / 16;
+    constexpr int PIECES = D * ES / 16, KP = KT * PIECES / 256;     // 16-byte pieces of a key row; of a thread
+    constexpr int NKP = KP > 0 ? KP : 1;
+    constexpr int DV = D / 32;                                      // value dimensions of a thread
+    constexpr int KC = D / 8;                                       // 16-byte pieces of a key row in LDS
+    __shared__ __align__(16) f16 sk[KT * D];
+    __shared__ __align__(16) f16 sv[D * KT];
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), c = lane & 15, g = lane >> 4;
+    const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
+    // row tiles of one item and head share an XCD's L2
+    const int id = xcd_tile(blockIdx.x, gridDim.x), id1 = uniform_div(id, mt), mtile = id - id1 * mt;
+    const int id2 = uniform_div(id1, p.splits), split = id1 - id2 * p.splits;
+    const int b = uniform_div(id2, p.Hkv), kh = id2 - b * p.Hkv;
+    int T = p.k_len ? p.k_len[b] : p.n_k;
+    T = T < 0 ? 0 : T > p.n_k ? p.n_k : T;
     int cnt = p.q_len ? p.q_len[b] : p.n_q;
-    if (i >= cnt) return;
-    const float2* ml = p.part_ml + row * p.splits;
-    float mm = kNoMax;
-    for (int s = lane; s < p.splits; s += 64) mm = fmaxf(mm, ml[s].x);
-    mm = wave_max(mm);
-    float l = 0.f, x0 = 0.f, x1 = 0.f;
-    const int d = 2 * lane;
-    for (int s = 0; s < p.splits; ++s) {
-        const float2 v = ml[s];
-        if (v.y == 0.f) continue;      // no key of this split is attended: its O is not written
-        const float f = __builtin_amdgcn_exp2f(v.x - mm);
-        l += v.y * f;
-        if (d < p.dk) {
-            const float2v o = *(const float2v*)(p.part_o + (row * p.splits + s) * p.dk + d);
-            x0 += o[0] * f;
-            x1 += o[1] * f;
+    cnt = cnt < 0 ? 0 : cnt > p.n_q ? p.n_q : cnt;
+    if (uniform_div(mtile * ROWS, p.G) >= cnt) return;                 // no row of this tile is asked for
+    const int m0 = mtile * ROWS + wave * 16 * QT;
+    const uint8_t *kb, *vb;
+    const float *ksc = nullptr, *vsc = nullptr;
+    const uint8_t* mask = nullptr;
+    if constexpr (KV == KV_I8) {
+        int sl = p.slot ? p.slot[b] : b;
+        if ((unsigned)sl >= (unsigned)p.n_slots) {
+            sl = 0;
+            T = 0;
+        }
+        kb = (const uint8_t*)p.k + sl * p.k_item + kh * p.k_head;
+        vb = (const uint8_t*)p.v + sl * p.v_item + kh * p.v_head;
+        ksc = p.k_scale + ((int64_t)sl * p.Hkv + kh) * p.n_blocks;
+        vsc = p.v_scale + ((int64_t)sl * p.Hkv + kh) * p.n_blocks;
+    } else {
+        kb = (const uint8_t*)p.k + (b * p.k_item + kh * p.k_head) * ES;
+        vb = (const uint8_t*)p.v + (b * p.v_item + kh * p.v_head) * ES;
+        mask = p.mask ? p.mask + b * p.mask_item : nullptr;
+    }
+    const uint32_t k_row = (uint32_t)p.k_row * ES, v_row = (uint32_t)p.v_row * ES;
+
+    uint32_t q[QT][NQ];
+    float qf[QT];
+    int lim[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const int i = load_query<KV, QF32, D, KV_F16>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt]);
+        lim[qt] = CAUSAL ? T - cnt + i + 1 : T;
+        if (p.scale < 0.f) {       // the factor is not negative: maxima are taken before it
+            qf[qt] = -qf[qt];
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) q[qt][n] ^= 0x80008000u;
         }
     }
-    if (d >= p.dk) return;
+    // keys that one of the rows of the workgroup, of the wave sees; keys that all of the wave's see
+    auto seen = [&](int m) {
+        const int i = uniform_div(m, p.G);
+        return CAUSAL ? T - cnt + (i < cnt ? i : cnt - 1) + 1 : T;
+    };
+    const int hi = seen(mtile * ROWS + ROWS - 1), hi_wave = seen(m0 + 16 * QT - 1), all_wave = seen(m0);
+    const int k0 = split * p.split_keys;
+    const int64_t ke = (int64_t)k0 + p.split_keys;
+    const int k1 = ke < hi ? (int)ke : hi;
+
+    float4v o[QT][NJ];
+    float m[QT], l[QT], vref = 0.f;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        m[qt] = kNoMax;
+        l[qt] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[qt][j] = (float4v){0.f, 0.f, 0.f, 0.f};
+    }
+
+    // the step in flight
+    uint32_t kr[NKP][4], vr[8][DV * ES / 4 > 0 ? DV * ES / 4 : 1];
+    uint32_t mr8 = 1;
+    float ksr[2] = {1.f, 1.f}, vsr[2] = {1.f, 1.f};
+    const int oct = t >> 5, d0 = (t & 31) * DV;            // value work: keys of octet oct, dimensions d0 .. d0 + DV
+    const int v_key = 32 * (oct >> 2) + 4 * (oct & 3);
+    const uint32_t v_at = (uint32_t)v_key * v_row + (d0 < p.dk ? d0 : 0) * ES;
+    constexpr int KSTEP = 256 / PIECES;                    // key work: piece k_ch of keys k_key + n KSTEP
+    const int k_key = t / PIECES % KT, k_ch = t % PIECES;
+    const uint32_t k_at = (uint32_t)k_key * k_row + (16 * k_ch < p.dk * ES ? 16 * k_ch : 0);
+    // LDS addresses that differ in more than a constant (see stage for the permutation)
+    const int kx = KC >= 8 ? c & 7 : (c >> 1) & 3;
+    int ka[2], va[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        ka[i] = c * D + 8 * ((4 * i + g) ^ kx);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) va[h][i] = c * KT + 8 * ((4 * h + g) ^ (c & 7) ^ (c >> 3) ^ (2 * i));
+    }
+    auto load = [&](int t0) {
+        const int left = T - 1 - t0;                       // t0 < T
+        if (mask) mr8 = mask[t0 + (lane < left ? lane : left)];
+        if constexpr (KV == KV_I8) {
+            const int blk = t0 / kCacheBlock, last = (T - 1) / kCacheBlock;
+            ksr[0] = ksc[blk];
+            vsr[0] = vsc[blk];
+            ksr[1] = ksc[blk < last ? blk + 1 : blk];
+            vsr[1] = vsc[blk < last ? blk + 1 : blk];
+        }
+        // rows past the last key are out of the resources' range: zeros
+        const int rows = left < KT - 1 ? left : KT - 1;
+        const auto kt = step_rsrc(kb + (int64_t)t0 * k_row, rows * k_row + p.dk * ES);
+        const auto vt = step_rsrc(vb + (int64_t)t0 * v_row, rows * v_row + p.dk * ES);
+#pragma unroll
+        for (int n = 0; n < NKP; ++n) {
+            const int4v x = __builtin_amdgcn_raw_buffer_load_b128(kt, k_at, n * KSTEP * k_row, 0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kr[n][e] = x[e];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t so = (i < 4 ? i : 12 + i) * v_row;
+            if constexpr (DV * ES == 1) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b8(vt, v_at, so, 0);
+            else if constexpr (DV * ES == 2) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b16(vt, v_at, so, 0);
+            else if constexpr (DV * ES == 4) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(vt, v_at, so, 0);
+            else {
+                const int2v x = __builtin_amdgcn_raw_buffer_load_b64(vt, v_at, so, 0);
+                vr[i][0] = x[0];
+                vr[i][1] = x[1];
+            }
+        }
+    };
+    auto stage = [&](uint64_t keep) {
+        if (KP > 0 || t < KT * PIECES) {
+#pragma unroll
+            for (int n = 0; n < NKP; ++n) {
+                const int key = k_key + n * KSTEP, ch = k_ch, x = KC >= 8 ? k_key & 7 : (k_key >> 1) & 3;    // KSTEP % 8 = 0
+                f16* row = sk + key * D;
+                if constexpr (KV == KV_F16) {
+                    *(int4v*)(row + 8 * (ch ^ x)) = (int4v){(int)kr[n][0], (int)kr[n][1], (int)kr[n][2], (int)kr[n][3]};
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        int4v w;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            w[2 * e] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c010c00));
+                            w[2 * e + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c030c02));
+                        }
+                        *(int4v*)(row + 8 * ((2 * ch + h) ^ x)) = w;
+                    }
+                }
+            }
+        }
+        if (keep != ~0ull) {       // what stands in the value rows of keys left out may be anything
+            const uint32_t half = (uint32_t)(keep >> (32 * (oct >> 2))), at = 4 * (oct & 3);
+            const uint32_t bits = ((half >> at) & 0xF) | (((half >> (16 + at)) & 0xF) << 4);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (uint32_t& w : vr[i]) w = (bits >> i) & 1 ? w : 0;
+        }
+#pragma unroll
+        for (int j = 0; j < DV; ++j) {
+            const int d = d0 + j, f = (d & 7) ^ ((d >> 3) & 3);
+            int4v w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (KV == KV_F16) {
+                    w[i] = __builtin_amdgcn_perm(vr[2 * i + 1][j >> 1], vr[2 * i][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+                } else {
+                    const uint32_t e = j & 3;
+                    w[i] = i8_pair_f16(__builtin_amdgcn_perm(vr[2 * i + 1][j >> 2], vr[2 * i][j >> 2], 0x0c040c00u | e | (e << 16)));
+                }
+            }
+            *(int4v*)(sv + d * KT + 8 * (oct ^ f)) = w;
+        }
+    };
+    auto compute = [&](int t0, uint64_t keep, const float (&ks)[2], const float (&vs)[2]) {
+        float4v s[QT][4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+            for (int n = 0; n < D / 32; ++n) {
+                const half8v a = *(const half8v*)(sk + ka[n & 1] + 16 * kt * D + 64 * (n >> 1));
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    const int4v bh = {(int)q[qt][4 * n], (int)q[qt][4 * n + 1], (int)q[qt][4 * n + 2], (int)q[qt][4 * n + 3]};
+                    const float4v from = n == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : s[qt][kt];
+                    s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bh), from, 0, 0, 0);
+                    if constexpr (SPLIT) {
+                        const int o = D / 8 + 4 * n;
+                        const int4v bl = {(int)q[qt][o], (int)q[qt][o + 1], (int)q[qt][o + 2], (int)q[qt][o + 3]};
+                        s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), s[qt][kt], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        const bool cut = keep != ~0ull || t0 + KT > all_wave;
+        float rv[2] = {1.f, 1.f}, grow = 1.f;
+        if constexpr (KV == KV_I8) {
+            const float top = fmaxf(vref, fmaxf(vs[0], vs[1]));
+            if (top > vref) {
+                grow = vref / top;
+                vref = top;
+            }
+            rv[0] = vref > 0.f ? vs[0] / vref : 1.f;
+            rv[1] = vref > 0.f ? vs[1] / vref : 1.f;
+        }
+        uint32_t ph[QT][2][4], pl[QT][2][4];
+        float alpha[QT];
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) {
+            // (not zero, as for a block of zeros: -inf stays -inf)
+            const float f[2] = {fmaxf(KV == KV_I8 ? qf[qt] * ks[0] : qf[qt], 1e-37f),
+                                fmaxf(KV == KV_I8 ? qf[qt] * ks[1] : qf[qt], 1e-37f)};
+            if (cut) {
+                const uint32_t bits[2] = {(uint32_t)keep >> (4 * g), (uint32_t)(keep >> 32) >> (4 * g)};
+                const int below = lim[qt] - t0 - 4 * g;
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!(bits[kt >> 1] & (1u << (16 * (kt & 1) + e))) || 16 * kt + e >= below) s[qt][kt][e] = -INFINITY;
+            }
+            float mx = m[qt];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4v x = s[qt][2 * h], y = s[qt][2 * h + 1];
+                const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+                mx = fmaxf(mx, top * f[h]);
+            }
+            mx = fmaxf(m[qt], xgroup_max(mx));
+            alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mx) * grow;
+            l[qt] *= __builtin_amdgcn_exp2f(m[qt] - mx);
+            m[qt] = mx;
+            const float off = 14.0f - mx;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float pf[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float x = s[qt][2 * h + (e >> 2)][e & 3];
+                    pf[e] = __builtin_amdgcn_exp2f(fmaf(x, f[h], off));
+                }
+                l[qt] += ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float a = KV == KV_I8 ? pf[2 * e] * rv[h] : pf[2 * e], bq = KV == KV_I8 ? pf[2 * e + 1] * rv[h] : pf[2 * e + 1];
+                    if constexpr (SPLIT) {
+                        const f16 ah = (f16)a, bh = (f16)bq;
+                        ph[qt][h][e] = pack_f16((float)ah, (float)bh);
+                        pl[qt][h][e] = pack_f16(a - (float)ah, bq - (float)bh);
+                    } else {
+                        ph[qt][h][e] = pack_f16(a, bq);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[qt][j] *= alpha[qt];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const half8v a = *(const half8v*)(sv + va[h][j & 1] + 16 * j * KT);
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    const int4v bh = {(int)ph[qt][h][0], (int)ph[qt][h][1], (int)ph[qt][h][2], (int)ph[qt][h][3]};
+                    o[qt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bh), o[qt][j], 0, 0, 0);
+                    if constexpr (SPLIT) {
+                        const int4v bl = {(int)pl[qt][h][0], (int)pl[qt][h][1], (int)pl[qt][h][2], (int)pl[qt][h][3]};
+                        o[qt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), o[qt][j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    };
+
+    if (k0 < k1) load(k0);
+    for (int t0 = k0; t0 < k1; t0 += KT) {
+        const uint64_t keep = __ballot(t0 + lane < T && mr8 != 0);     // the same in every wave
+        const float ks[2] = {ksr[0], ksr[1]}, vs[2] = {vsr[0], vsr[1]};
+        stage(keep);
+        __syncthreads();
+        if (t0 + KT < k1) load(t0 + KT);
+        if (!CAUSAL || t0 < hi_wave) compute(t0, keep, ks, vs);
+        __syncthreads();
+    }
+
+    // lane (c, g) has row c's dimensions 16 j + 4 g .. + 4
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+        const float ll = xgroup_sum(l[qt]);
+        const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
+        if (i >= cnt) continue;
+        const float unit = KV == KV_I8 ? vref : 1.0f;
+        if (p.splits > 1) {
+            const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
+            if (g == 0) p.part_ml[at] = float2{m[qt], ll};
+            if (ll == 0.f) continue;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                if (16 * j + 4 * g < p.dk) *(float4v*)(p.part_o + at * p.dk + 16 * j + 4 * g) = o[qt][j] * unit;
+            continue;
+        }
+        const float f = ll != 0.f ? unit / ll : 0.f;
+        const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + 4 * g;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if (16 * j + 4 * g >= p.dk) continue;
+            const float4v x = o[qt][j] * f;
+            if constexpr (QF32) *(float4v*)((float*)p.out + at + 16 * j) = x;
+            else *(int2v*)((f16*)p.out + at + 16 * j) = (int2v){(int)pack_f16(x[0], x[1]), (int)pack_f16(x[2], x[3])};
+        }
+    }
+}
+
+// Joins the splits' (m, l, O), at most 64 of them, WPR waves a row (four where
+// rows are few).  Lane s of a wave has split s's factor 2^(m_s - max m); the
+// wave adds splits w, w + WPR, ... in that order, two dimensions a lane, and the
+// waves' sums are added in wave order.
+template <bool F32, int WPR> __global__ __launch_bounds__(256) void dec_join_kernel(DecAttnParams p) {
+    __shared__ float so[4][128];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, M = p.n_q * p.G, d = 2 * lane;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR, rows = (int64_t)p.B * p.Hkv * M;
+    const int64_t rc = row < rows ? row : rows - 1;
+    const int unit = (int)(rc / M), mr = (int)(rc - (int64_t)unit * M), w = wave % WPR;
+    const int b = unit / p.Hkv, kh = unit - b * p.Hkv, i = mr / p.G, h = kh * p.G + (mr - i * p.G);
+    const bool live = row < rows && i < (p.q_len ? p.q_len[b] : p.n_q);
+    const float2 ml = live && lane < p.splits ? p.part_ml[rc * p.splits + lane] : float2{kNoMax, 0.f};
+    const float mm = wave_max(ml.x);
+    // a split without a key (l = 0) has not written its O
+    const float f = ml.y != 0.f ? __builtin_amdgcn_exp2f(ml.x - mm) : 0.f;
+    const float l = wave_sum(ml.y * f);
+    float x0 = 0.f, x1 = 0.f;
+    if (live && d < p.dk) {
+        const float* src = p.part_o + rc * p.splits * p.dk + d;
+        for (int s0 = w; s0 < p.splits; s0 += 4 * WPR) {
+            float2v o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int s = s0 + k * WPR, at = s < p.splits ? s : s0;
+                o[k] = *(const float2v*)(src + (int64_t)at * p.dk);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int s = s0 + k * WPR;
+                const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s < p.splits ? s : 63));
+                const bool add = s < p.splits && fs != 0.f;
+                x0 += add ? o[k][0] * fs : 0.f;
+                x1 += add ? o[k][1] * fs : 0.f;
+            }
+        }
+    }
+    if constexpr (WPR > 1) {
+        so[wave][d] = x0;
+        so[wave][d + 1] = x1;
+        __syncthreads();
+        if (w != 0) return;
+        x0 = x1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < WPR; ++k) {
+            x0 += so[wave + k][d];
+            x1 += so[wave + k][d + 1];
+        }
+    }
+    if (!live || d >= p.dk) return;
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + d;
     if constexpr (F32) *(float2v*)((float*)p.out + at) = (float2v){x0 * inv, x1 * inv};
@@ -620,7 +1002,7 @@ struct Shape { bool wide; int rows, mt, splits, keys; };
 Shape attn_shape(const DecAttnParams& p) {
     Shape s;
     const int64_t M = (int64_t)p.n_q * p.G, units = (int64_t)p.B * p.Hkv;
-    s.wide = M >= 64;
+    s.wide = M >= 64 && !p.table;
     s.rows = s.wide ? 128 : 16;
     s.mt = cdiv(M, s.rows);
     const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
@@ -630,7 +1012,8 @@ Shape attn_shape(const DecAttnParams& p) {
     const int64_t most = tiles / least > 0 ? tiles / least : 1;
     if (want > most) want = most;
     if (want > 64) want = 64;
-    const int per = cdiv(tiles, want);
+    int per = cdiv(tiles, want);
+    if (s.wide) per += per & 1;                            // whole steps of dec_tile_kernel
     s.splits = cdiv(tiles, per);
     s.keys = per * 32;
     return s;
@@ -638,8 +1021,11 @@ Shape attn_shape(const DecAttnParams& p) {
 
 template <int KV, bool QF32, int D, bool TABLE> void launch_shape(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * sh.mt * sh.splits));
-    if (sh.wide) launch(dec_attn_kernel<KV, QF32, D, 2, 4, 1, TABLE>, grid, dim3(256), 0, s, p);
-    else launch(dec_attn_kernel<KV, QF32, D, 1, 1, 4, TABLE>, grid, dim3(256), 0, s, p);
+    if (sh.wide) {
+        if constexpr (KV == KV_F32) launch(dec_attn_kernel<KV, QF32, D, 2, 4, 1, false>, grid, dim3(256), 0, s, p);
+        else if (p.causal && KV == KV_I8) launch(dec_tile_kernel<KV, QF32, D, KV == KV_I8>, grid, dim3(256), 0, s, p);
+        else launch(dec_tile_kernel<KV, QF32, D, false>, grid, dim3(256), 0, s, p);
+    } else launch(dec_attn_kernel<KV, QF32, D, 1, 1, 4, TABLE>, grid, dim3(256), 0, s, p);
 }
 template <int KV, bool QF32, bool TABLE> void launch_width(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     if (p.dk <= 32) launch_shape<KV, QF32, 32, TABLE>(p, sh, s);
@@ -660,7 +1046,7 @@ size_t dec_attention_workspace(const DecAttnParams& p) {
 void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_t s) {
     if (p.B == 0 || p.n_q == 0) return;
     const Shape sh = attn_shape(p);
-    require((int64_t)p.B * p.Hkv * sh.mt * sh.splits < (1 << 23) && (int64_t)p.B * p.Hkv * p.n_q * p.G < (1 << 30),
+    require((int64_t)p.B * p.Hkv * sh.mt * sh.splits < (1 << 22) && (int64_t)p.B * p.Hkv * p.n_q * p.G < (1 << 22),
             "attention: too many rows for one call");
     const size_t need = dec_attention_workspace(p);
     require(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need),
@@ -679,8 +1065,10 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     else p.table ? launch_width<KV_I8, false, true>(p, sh, s) : launch_width<KV_I8, false, false>(p, sh, s);
     if (sh.splits > 1) {
         const int64_t rows = (int64_t)p.B * p.Hkv * p.n_q * p.G;
-        if (p.q_f32) launch(dec_join_kernel<true>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
-        else launch(dec_join_kernel<false>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p);
+        const bool few = rows <= 1024;             // a wave a row leaves the chip short of waves
+        auto* k = p.q_f32 ? (few ? dec_join_kernel<true, 4> : dec_join_kernel<true, 1>)
+                          : (few ? dec_join_kernel<false, 4> : dec_join_kernel<false, 1>);
+        launch(k, dim3((unsigned)(few ? rows : (rows + 3) / 4)), dim3(256), 0, s, p);
     }
 }
 

@@ -63,7 +63,7 @@ def beam(**kw):
 def test_cross_attention_refusals():
     out = _run("""
         for kw in (dict(type=8), dict(n_items=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(d_head=60), dict(d_head=136),
-                   dict(q=None), dict(k=A + 8), dict(v_row=132), dict(out_head=-64), dict(k_row=1 << 24), dict(type=0, q_head=66)):
+                   dict(q=None), dict(k=A + 8), dict(v_row=132), dict(out_head=-64), dict(k_row=1 << 22), dict(type=0, q_head=66)):
             said(L.pkx_cross_attention(cross(**kw), None, 0, None))
         said(L.pkx_cross_attention(None, None, 0, None))
         said(L.pkx_cross_attention_workspace(cross(), None))
@@ -75,7 +75,7 @@ def test_cross_attention_refusals():
         for kw in (dict(n_items=0), dict(n_q=0, q=None), dict(n_items=0, k=None)):
             said(L.pkx_cross_attention(cross(**kw), None, 0, None))
     """)
-    words = ["type", "negative", "n_heads", "n_heads", "d_head", "d_head", "q must", "k must", "v must", "out must", "2^24", "q must",
+    words = ["type", "negative", "n_heads", "n_heads", "d_head", "d_head", "q must", "k must", "v must", "out must", "2^22", "q must",
              "null", "null"]
     for line, w in zip(out[:14], words):
         assert line.startswith("1 ") and w in line, (line, w)
