@@ -113,34 +113,37 @@ template <bool F32> __global__ __launch_bounds__(256) void cache8_append_kernel(
     }
 }
 
-// Eight values per thread: tokens start[r] .. + n of row r's slot as q * scale.
-__global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p) {
-    const int n8 = p.c.dk / 8;
-    const int64_t per = (int64_t)p.n * p.c.Hkv * n8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= per * p.R) return;
-    const int r = (int)(id / per);
-    const int64_t in = id - r * per;
-    const int d = 8 * (int)(in % n8), kh = (int)(in / n8 % p.c.Hkv), i = (int)(in / n8 / p.c.Hkv);
-    const int64_t at = (int64_t)p.start[r] + i;
+// Eight values of K and V per thread: tokens start[r] .. + n of row r's slot as q * scale.
+__global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int per) {
+    const int n8 = p.c.dk / 8, r = blockIdx.y;
+    const unsigned in = blockIdx.x * 256 + threadIdx.x;
+    if (in >= (unsigned)per) return;
+    const unsigned hk = in / n8, i = hk / p.c.Hkv;
+    const int d = 8 * (in - hk * n8), kh = hk - i * p.c.Hkv;
+    const int64_t at = (int64_t)p.start[r] + i, out = ((int64_t)r * per + in) * 8;
     const int slot = p.slot ? p.slot[r] : r;
     const bool live = at >= 0 && at < p.c.cap && (unsigned)slot < (unsigned)p.c.n_slots;
     const int64_t head = live ? (int64_t)slot * p.c.Hkv + kh : 0, tk = live ? at : 0;
+    int2v w[2] = {};
+    float s[2] = {};
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+        if (live && (z ? p.v : p.k)) {
+            w[z] = *(const int2v*)((z ? p.c.v : p.c.k) + (head * p.c.cap + tk) * p.c.dk + d);
+            s[z] = (z ? p.c.v_scale : p.c.k_scale)[head * (p.c.cap / kCacheBlock) + tk / kCacheBlock];
+        }
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-        float* out = z ? p.v : p.k;
-        if (!out) continue;
-        float4v a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        if (live) {
-            const int2v w = *(const int2v*)((z ? p.c.v : p.c.k) + (head * p.c.cap + tk) * p.c.dk + d);
-            const float s = (z ? p.c.v_scale : p.c.k_scale)[head * (p.c.cap / kCacheBlock) + tk / kCacheBlock];
+        float* y = z ? p.v : p.k;
+        if (!y) continue;
+        float4v a, b;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                a[e] = (float)(int8_t)(w[0] >> (8 * e)) * s;
-                b[e] = (float)(int8_t)(w[1] >> (8 * e)) * s;
-            }
+        for (int e = 0; e < 4; ++e) {
+            a[e] = live ? (float)(int8_t)(w[z][0] >> (8 * e)) * s[z] : 0.f;
+            b[e] = live ? (float)(int8_t)(w[z][1] >> (8 * e)) * s[z] : 0.f;
         }
-        *(float4v*)(out + id * 8) = a;
-        *(float4v*)(out + id * 8 + 4) = b;
+        *(float4v*)(y + out) = a;
+        *(float4v*)(y + out + 4) = b;
     }
 }
 
@@ -156,10 +159,10 @@ void launch_cache8_append(const CacheAppendParams& p, hipStream_t s) {
 }
 
 void launch_cache8_read(const CacheReadParams& p, hipStream_t s) {
-    const int64_t n = (int64_t)p.R * p.n * p.c.Hkv * (p.c.dk / 8);
-    if (n == 0) return;
-    require(n < ((int64_t)1 << 31), "cache read: too many values for one call");
-    launch(cache8_read_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p);
+    const int64_t per = (int64_t)p.n * p.c.Hkv * (p.c.dk / 8);
+    if (p.R == 0 || per == 0 || (!p.k && !p.v)) return;
+    require(p.R <= 65535 && per < ((int64_t)1 << 31), "cache read: at most 65535 rows and 2^34 values of one in a call");
+    launch(cache8_read_kernel, dim3((unsigned)((per + 255) / 256), p.R), dim3(256), 0, s, p, (int)per);
 }
 
 }  // namespace pkx

@@ -48,6 +48,17 @@ __device__ __forceinline__ float xgroup_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// v_max3_f32 as it is: the compiler puts a canonicalising v_max before every
+// fmaxf of a matrix product's result
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// bits 0 .. n - 1
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+
 // x / d for scalars below 2^22
 __device__ __forceinline__ int uniform_div(int x, int d) { return __builtin_amdgcn_readfirstlane(udiv_small(x, d)); }
 
@@ -286,8 +297,34 @@ template <int KV, int D> __device__ __forceinline__ half8v value_frag(const uint
     return __builtin_bit_cast(half8v, a);
 }
 
+// Block -> work.  Block n runs on XCD n % 8.  The blocks of one split of an item
+// (its key heads, whose rows lie side by side in encoder states, and their row
+// tiles, which read the same keys) stay on one XCD; eight neighbouring items go to
+// the eight XCDs, each eight turned by one against the last, so that no XCD gets
+// all of a long item or of a split that most items do not reach.  The last items,
+// where they are no multiple of 8, are spread over the XCDs.  With a table
+// neighbouring items share keys, and each XCD takes a range of them.
+template <bool TABLE>
+__device__ __forceinline__ void work_of(int bid, const DecAttnParams& p, int mt, int& b, int& kh, int& split, int& mtile) {
+    const int per = p.Hkv * mt, items = p.B * p.splits, even = (items >> 3) * 8 * per;
+    int u, in;
+    if (TABLE || bid >= even) {
+        const int at = TABLE ? xcd_tile(bid, items * per) : bid;
+        u = uniform_div(at, per);
+        in = at - u * per;
+    } else {
+        const int loc = bid >> 3, r = uniform_div(loc, per);
+        u = r * 8 + ((bid + r) & 7);
+        in = loc - r * per;
+    }
+    kh = uniform_div(in, mt);
+    mtile = in - kh * mt;
+    split = uniform_div(u, p.B);
+    b = u - split * p.B;
+}
+
 template <int KV, bool QF32, int D, int QT, int WM, int WK, bool TABLE>
-__global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p) {
+__global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn_kernel(DecAttnParams p) {
     using TL = Tile<KV, D>;
     static_assert(WK == 1 || (QT == 1 && WM == 1 && WK == 4), "joined waves: one row tile, four key shares");
     constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
@@ -296,10 +333,8 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int wm = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
     const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
-    // row tiles of one item and head share an XCD's L2
-    const int id = xcd_tile(blockIdx.x, gridDim.x), id1 = uniform_div(id, mt), mtile = id - id1 * mt;
-    const int id2 = uniform_div(id1, p.splits), split = id1 - id2 * p.splits;
-    const int b = uniform_div(id2, p.Hkv), kh = id2 - b * p.Hkv;
+    int b, kh, split, mtile;
+    work_of<TABLE>(blockIdx.x, p, mt, b, kh, split, mtile);
 
     int T = p.k_len ? p.k_len[b] : p.n_k;
     T = T < 0 ? 0 : T > p.n_k ? p.n_k : T;
@@ -405,13 +440,10 @@ __global__ __launch_bounds__(64 * WM * WK) void dec_attn_kernel(DecAttnParams p)
                 }
             }
             if (!whole || p.causal) {
-                const uint32_t bits = keep >> (4 * g);
-                const int below = lim[qt] - t0 - 4 * g;
+                const uint32_t see = keep >> (4 * g) & low_bits(lim[qt] - t0 - 4 * g);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const int r = e < 4 ? e : 12 + e;
-                    if (!(bits & (1u << r)) || r >= below) sc[e] = -INFINITY;
-                }
+                for (int e = 0; e < 8; ++e)
+                    if (!(see & (1u << (e < 4 ? e : 12 + e)))) sc[e] = -INFINITY;
             }
             float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
             mx = fmaxf(m[qt], xgroup_max(mx));
@@ -634,14 +666,13 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     constexpr int NKP = KP > 0 ? KP : 1;
     constexpr int DV = D / 32;                                      // value dimensions of a thread
     constexpr int KC = D / 8;                                       // 16-byte pieces of a key row in LDS
+    constexpr int JB = NJ < 4 ? NJ : 4;                             // value products in flight
     __shared__ __align__(16) f16 sk[KT * D];
     __shared__ __align__(16) f16 sv[D * KT];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), c = lane & 15, g = lane >> 4;
     const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
-    // row tiles of one item and head share an XCD's L2
-    const int id = xcd_tile(blockIdx.x, gridDim.x), id1 = uniform_div(id, mt), mtile = id - id1 * mt;
-    const int id2 = uniform_div(id1, p.splits), split = id1 - id2 * p.splits;
-    const int b = uniform_div(id2, p.Hkv), kh = id2 - b * p.Hkv;
+    int b, kh, split, mtile;
+    work_of<false>(blockIdx.x, p, mt, b, kh, split, mtile);
     int T = p.k_len ? p.k_len[b] : p.n_k;
     T = T < 0 ? 0 : T > p.n_k ? p.n_k : T;
     int cnt = p.q_len ? p.q_len[b] : p.n_q;
@@ -801,34 +832,39 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     };
     auto compute = [&](int t0, uint64_t keep, const float (&ks)[2], const float (&vs)[2]) {
         float4v s[QT][4];
+        // consecutive products go to different accumulators
 #pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
+        for (int n = 0; n < D / 32; ++n) {
+            half8v a[4];
 #pragma unroll
-            for (int n = 0; n < D / 32; ++n) {
-                const half8v a = *(const half8v*)(sk + ka[n & 1] + 16 * kt * D + 64 * (n >> 1));
+            for (int kt = 0; kt < 4; ++kt) a[kt] = *(const half8v*)(sk + ka[n & 1] + 16 * kt * D + 64 * (n >> 1));
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    const int4v bh = {(int)q[qt][4 * n], (int)q[qt][4 * n + 1], (int)q[qt][4 * n + 2], (int)q[qt][4 * n + 3]};
-                    const float4v from = n == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : s[qt][kt];
-                    s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bh), from, 0, 0, 0);
-                    if constexpr (SPLIT) {
-                        const int o = D / 8 + 4 * n;
-                        const int4v bl = {(int)q[qt][o], (int)q[qt][o + 1], (int)q[qt][o + 2], (int)q[qt][o + 3]};
-                        s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), s[qt][kt], 0, 0, 0);
+            for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt) {
+                        const int o = part * (D / 8) + 4 * n;
+                        const int4v bq = {(int)q[qt][o], (int)q[qt][o + 1], (int)q[qt][o + 2], (int)q[qt][o + 3]};
+                        const float4v from = n == 0 && part == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : s[qt][kt];
+                        s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kt], __builtin_bit_cast(half8v, bq), from, 0, 0, 0);
                     }
-                }
-            }
         }
         const bool cut = keep != ~0ull || t0 + KT > all_wave;
-        float rv[2] = {1.f, 1.f}, grow = 1.f;
+        float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f;
         if constexpr (KV == KV_I8) {
             const float top = fmaxf(vref, fmaxf(vs[0], vs[1]));
             if (top > vref) {
                 grow = vref / top;
                 vref = top;
             }
-            rv[0] = vref > 0.f ? vs[0] / vref : 1.f;
-            rv[1] = vref > 0.f ? vs[1] / vref : 1.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // (a block of zeros: any factor, so that the weights' sum survives)
+                rv[h] = vref > 0.f ? fmaxf(vs[h] / vref, 0x1p-60f) : 1.f;
+                ri[h] = 1.0f / rv[h];
+                rl[h] = __builtin_amdgcn_logf(rv[h]);
+            }
         }
         uint32_t ph[QT][2][4], pl[QT][2][4];
         float alpha[QT];
@@ -838,38 +874,43 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
             const float f[2] = {fmaxf(KV == KV_I8 ? qf[qt] * ks[0] : qf[qt], 1e-37f),
                                 fmaxf(KV == KV_I8 ? qf[qt] * ks[1] : qf[qt], 1e-37f)};
             if (cut) {
-                const uint32_t bits[2] = {(uint32_t)keep >> (4 * g), (uint32_t)(keep >> 32) >> (4 * g)};
                 const int below = lim[qt] - t0 - 4 * g;
+                const uint32_t see[2] = {(uint32_t)keep >> (4 * g) & low_bits(below), (uint32_t)(keep >> 32) >> (4 * g) & low_bits(below - 32)};
 #pragma unroll
                 for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (!(bits[kt >> 1] & (1u << (16 * (kt & 1) + e))) || 16 * kt + e >= below) s[qt][kt][e] = -INFINITY;
+                        if (!(see[kt >> 1] & (1u << (16 * (kt & 1) + e)))) s[qt][kt][e] = -INFINITY;
             }
             float mx = m[qt];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float4v x = s[qt][2 * h], y = s[qt][2 * h + 1];
-                const float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
-                mx = fmaxf(mx, top * f[h]);
+                mx = fmaxf(mx, max3(max3(x[0], x[1], x[2]), max3(x[3], y[0], y[1]), max3(y[2], y[3], y[3])) * f[h]);
             }
             mx = fmaxf(m[qt], xgroup_max(mx));
             alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mx) * grow;
             l[qt] *= __builtin_amdgcn_exp2f(m[qt] - mx);
             m[qt] = mx;
-            const float off = 14.0f - mx;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                // where p goes to f16 alone the factor r rides in the exponent
+                constexpr bool RIDES = KV == KV_I8 && !SPLIT;
+                const float off = 14.0f - mx + (RIDES ? rl[h] : 0.f);
                 float pf[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float x = s[qt][2 * h + (e >> 2)][e & 3];
                     pf[e] = __builtin_amdgcn_exp2f(fmaf(x, f[h], off));
                 }
-                l[qt] += ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7]));
+                const float sum = ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7]));
+                l[qt] = RIDES ? fmaf(sum, ri[h], l[qt]) : l[qt] + sum;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float a = KV == KV_I8 ? pf[2 * e] * rv[h] : pf[2 * e], bq = KV == KV_I8 ? pf[2 * e + 1] * rv[h] : pf[2 * e + 1];
+                    float a = SPLIT ? pf[2 * e] * rv[h] : pf[2 * e], bq = SPLIT ? pf[2 * e + 1] * rv[h] : pf[2 * e + 1];
+                    // the products as rounded here: fused into the conversions, the two
+                    // uses of hi below could differ by one of its steps
+                    if constexpr (SPLIT) asm("" : "+v"(a), "+v"(bq));
                     if constexpr (SPLIT) {
                         const f16 ah = (f16)a, bh = (f16)bq;
                         ph[qt][h][e] = pack_f16((float)ah, (float)bh);
@@ -885,21 +926,23 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j) o[qt][j] *= alpha[qt];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const half8v a = *(const half8v*)(sv + va[h][j & 1] + 16 * j * KT);
+            for (int j0 = 0; j0 < NJ; j0 += JB) {
+                half8v a[JB];
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    const int4v bh = {(int)ph[qt][h][0], (int)ph[qt][h][1], (int)ph[qt][h][2], (int)ph[qt][h][3]};
-                    o[qt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bh), o[qt][j], 0, 0, 0);
-                    if constexpr (SPLIT) {
-                        const int4v bl = {(int)pl[qt][h][0], (int)pl[qt][h][1], (int)pl[qt][h][2], (int)pl[qt][h][3]};
-                        o[qt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), o[qt][j], 0, 0, 0);
-                    }
-                }
+                for (int j = 0; j < JB; ++j) a[j] = *(const half8v*)(sv + va[h][(j0 + j) & 1] + 16 * (j0 + j) * KT);
+#pragma unroll
+                for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
+#pragma unroll
+                    for (int j = 0; j < JB; ++j)
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt) {
+                            const uint32_t(&w)[4] = part ? pl[qt][h] : ph[qt][h];
+                            const int4v bp = {(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+                            o[qt][j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], __builtin_bit_cast(half8v, bp), o[qt][j0 + j], 0, 0, 0);
+                        }
             }
-        }
     };
 
     if (k0 < k1) load(k0);
@@ -1008,12 +1051,11 @@ Shape attn_shape(const DecAttnParams& p) {
     const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
     const int64_t wgs = units * s.mt;
     int64_t want = wgs >= 512 ? 1 : 512 / wgs;             // about two workgroups per CU
-    const int least = s.wide ? 8 : 8;                      // tiles a split is worth
-    const int64_t most = tiles / least > 0 ? tiles / least : 1;
-    if (want > most) want = most;
     if (want > 64) want = 64;
-    int per = cdiv(tiles, want);
-    if (s.wide) per += per & 1;                            // whole steps of dec_tile_kernel
+    // whole rounds of the four key shares, or steps of dec_tile_kernel, and at
+    // least four rounds: a split costs its partial sums and the join's launch
+    int per = (cdiv(tiles, want) + 3) / 4 * 4;
+    if (per < 16) per = 16;
     s.splits = cdiv(tiles, per);
     s.keys = per * 32;
     return s;

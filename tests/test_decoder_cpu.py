@@ -90,7 +90,7 @@ def test_cache_refusals():
         for c, t in ((cache(n_slots=0), toks()), (cache(d_head=72), toks()), (cache(d_head=144), toks()), (cache(capacity=100), toks()),
                      (cache(capacity=0), toks()), (cache(k=None), toks()), (cache(v=A + 4), toks()), (cache(), toks(type=2)),
                      (cache(), toks(n_new=-1)), (cache(), toks(k_tok=130)), (cache(), toks(start=None)), (cache(), toks(n_rows=4)),
-                     (cache(), toks(table=A, table_row=95)), (cache(), toks(n_rows=40000, slot=A))):
+                     (cache(), toks(table=A, table_row=95)), (cache(), toks(n_rows=70000, slot=A))):
             said(L.pkx_cache8_append(c, t, None))
         for a in (attn(type=3), attn(n_heads=3), attn(n_q=-1), attn(max_len=-1), attn(len=None), attn(n_rows=4), attn(q=None),
                   attn(out_tok=100), attn(table=A, table_row=95)):

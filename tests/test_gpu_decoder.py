@@ -192,6 +192,8 @@ CACHE = [
     ("f16", 3, 7, 4, 2, 80, 65, True, False), ("f16", 2, 70, 2, 2, 64, 200, True, False), ("f16", 1, 1, 2, 1, 32, 5000, True, False),
     ("f16", 2, 8, 2, 2, 16, 333, False, False), ("f16", 2, 40, 4, 2, 128, 90, False, True), ("f16", 1, 2, 16, 1, 48, 1, True, False),
     ("f32", 1, 1, 8, 8, 64, 18, True, False), ("f32", 6, 1, 4, 4, 128, 100, True, True), ("f32", 2, 70, 2, 1, 64, 200, True, False),
+    # many rows over few keys: a weight's two f16 terms that do not add up to it are seen
+    ("f32", 4, 128, 8, 8, 64, 48, False, False),
     ("f32", 1, 3, 2, 1, 32, 3000, True, False), ("f32", 3, 5, 2, 2, 16, 64, False, False), ("f32", 2, 80, 2, 2, 80, 111, True, True),
 ]
 
