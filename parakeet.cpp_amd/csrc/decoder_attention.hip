@@ -108,65 +108,120 @@ template <int KV, int D> __device__ __forceinline__ int key_dim(int s, int g) {
 
 struct KeySource {
     const uint8_t *k, *v;        // item and head
-    int64_t k_slot, v_slot;      // table: bytes between slots
     uint32_t k_row, v_row;       // bytes between keys
     const float *ks, *vs;
-    int64_t s_slot;
     const uint8_t* mask;
+    int T, k_bytes;
+    uint32_t v_at;               // the lane's first value row and dimension, from a tile's first row
+    uint32_t k_at[8];            // its pieces of key row c
+    // table
     const int* table;
-    int T, n_slots, k_bytes, v_off;
+    int n_slots;
+    int64_t k_slot, s_slot;      // bytes and scales between slots (keys and values alike)
+    bool far;                    // a slot's offset may not fit 32 bits
 };
 
-template <int KV, int D, bool TABLE>
-__device__ __forceinline__ void load_tile(Tile<KV, D>& t, const KeySource& s, int t0, int slot, int lane) {
+// A buffer resource of one step's rows, built from scalars.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const uint8_t* base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, 0x00020000);
+}
+
+// n dwords at a byte offset.  All of it goes into the per-lane offset, which is
+// what the range check compares with the resource's size (a scalar offset is
+// subtracted from the size first, and a larger one would wrap).
+template <int N, typename R> __device__ __forceinline__ void buffer_words(uint32_t (&d)[N], R r, uint32_t at) {
+    if constexpr (N == 1) {
+        d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0);
+    } else if constexpr (N == 2) {
+        const int2v x = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, 0);
+        d[0] = x[0]; d[1] = x[1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const int4v x = __builtin_amdgcn_raw_buffer_load_b128(r, at + 4 * i, 0, 0);
+            d[i] = x[0]; d[i + 1] = x[1]; d[i + 2] = x[2]; d[i + 3] = x[3];
+        }
+    }
+}
+
+// The rows of a tile come through a buffer resource of exactly the tile's valid
+// rows, built from scalars: offsets are the same in every tile, and rows past the
+// last key read as zeros.
+template <int KV, int D>
+__device__ __forceinline__ void load_tile(Tile<KV, D>& t, const KeySource& s, int t0, int lane) {
     using TL = Tile<KV, D>;
-    const int c = lane & 15, g = lane >> 4, last = s.T - 1;
-    const int tb = t0 < last ? t0 : last;                 // tiles past the end read the last key again
-    const int left = last - tb;
-    const int mine = lane & 31;
+    const int last = s.T - 1, tb = t0 < last ? t0 : last;          // tiles past the end read the last key again
+    const int left = last - tb, rows = left < 31 ? left : 31, mine = lane & 31;
     bool ok = t0 + mine < s.T;
     if (s.mask) ok = ok && s.mask[tb + (mine < left ? mine : left)] != 0;
-    if constexpr (TABLE) {
-        ok = ok && (unsigned)slot < (unsigned)s.n_slots;
-        slot = (unsigned)slot < (unsigned)s.n_slots ? slot : 0;
-        t.ks = s.ks[slot * s.s_slot + tb / kCacheBlock];
-        t.vs = s.vs[slot * s.s_slot + tb / kCacheBlock];
-    } else if constexpr (KV == KV_I8) {
+    t.ok = ok;
+    if constexpr (KV == KV_I8) {
         t.ks = s.ks[tb / kCacheBlock];
         t.vs = s.vs[tb / kCacheBlock];
     }
-    t.ok = ok;
-    const uint8_t* kb = s.k + (int64_t)tb * s.k_row;
-    const uint8_t* vb = s.v + (int64_t)tb * s.v_row;
+    const auto kr = step_rsrc(s.k + (int64_t)tb * s.k_row, rows * s.k_row + s.k_bytes);
+    const auto vr = step_rsrc(s.v + (int64_t)tb * s.v_row, rows * s.v_row + s.k_bytes);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-        const int r = 16 * kt + c, rr = r < left ? r : left;
-        const uint8_t* p = kb + (uint32_t)rr * s.k_row;
-        if constexpr (TABLE) p += __shfl(slot, r, 64) * s.k_slot;
-        if constexpr (TL::NK == 2) {
-            uint32_t d[2];
-            const int o = key_piece<KV, D>(0, g);
-            load_words(d, p + (o < s.k_bytes ? o : 0));
-            t.k[kt][0] = d[0]; t.k[kt][1] = d[1];
-        } else {
+        constexpr int N = TL::NK == 2 ? 2 : 4;
 #pragma unroll
-            for (int n = 0; n < TL::NK / 4; ++n) {
-                // pieces past the head's dimensions read its first again; their queries are zero
-                const int o = key_piece<KV, D>(n, g);
-                uint32_t d[4];
-                load_words(d, p + (o < s.k_bytes ? o : 0));
+        for (int n = 0; n < TL::NK / N; ++n) {
+            uint32_t d[N];
+            buffer_words(d, kr, s.k_at[n] + 16 * kt * s.k_row);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) t.k[kt][4 * n + i] = d[i];
-            }
+            for (int i = 0; i < N; ++i) t.k[kt][N * n + i] = d[i];
         }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const int r = (i < 4 ? 0 : 12) + 4 * g + i, rr = r < left ? r : left;
-        const uint8_t* p = vb + (uint32_t)rr * s.v_row + s.v_off;
-        if constexpr (TABLE) p += __shfl(slot, r, 64) * s.v_slot;
-        if constexpr (KV == KV_I8 && D == 32) t.v[i][0] = *(const uint16_t*)p;
-        else load_words(t.v[i], p);
+        const uint32_t at = s.v_at + (i < 4 ? i : 12 + i) * s.v_row;
+        if constexpr (KV == KV_I8 && D == 32) t.v[i][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, at, 0, 0);
+        else buffer_words(t.v[i], vr, at);
+    }
+}
+
+// The same with every key's slot from the table: lane l (mod 32) forms key l's
+// offset, the lanes that read its row fetch it from there.
+template <int D> __device__ __forceinline__ void load_tile_by_table(Tile<KV_I8, D>& t, const KeySource& s, int t0, int slot, int lane) {
+    using TL = Tile<KV_I8, D>;
+    const int c = lane & 15, g = lane >> 4, last = s.T - 1, tb = t0 < last ? t0 : last;
+    const int left = last - tb, mine = lane & 31, row = mine < left ? mine : left;
+    const bool in = (unsigned)slot < (unsigned)s.n_slots;
+    t.ok = t0 + mine < s.T && in;
+    slot = in ? slot : 0;
+    t.ks = s.ks[slot * s.s_slot + tb / kCacheBlock];
+    t.vs = s.vs[slot * s.s_slot + tb / kCacheBlock];
+    const uint8_t* kb = s.k + (int64_t)tb * s.k_row;
+    const uint8_t* vb = s.v + (int64_t)tb * s.v_row;
+    auto fetch = [&](auto&& at_k, auto&& at_v) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            constexpr int N = TL::NK == 2 ? 2 : 4;
+#pragma unroll
+            for (int n = 0; n < TL::NK / N; ++n) {
+                uint32_t d[N];
+                load_words(d, at_k(16 * kt + c, s.k_at[n]));
+#pragma unroll
+                for (int i = 0; i < N; ++i) t.k[kt][N * n + i] = d[i];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint8_t* x = at_v((i < 4 ? 0 : 12) + 4 * g + i, s.v_at);
+            if constexpr (D == 32) t.v[i][0] = *(const uint16_t*)x;
+            else load_words(t.v[i], x);
+        }
+    };
+    if (!s.far) {
+        const uint32_t mine_at = (uint32_t)slot * (uint32_t)s.k_slot + row * s.k_row;
+        fetch([&](int r, uint32_t d) { return kb + ((uint32_t)__shfl((int)mine_at, r, 64) + d); },
+              [&](int r, uint32_t d) { return vb + ((uint32_t)__shfl((int)mine_at, r, 64) + d); });
+    } else {
+        const int64_t mine_at = slot * s.k_slot + row * s.k_row;
+        auto from = [&](int r) {
+            return (int64_t)((uint64_t)(uint32_t)__shfl((int)(mine_at >> 32), r, 64) << 32 | (uint32_t)__shfl((int)mine_at, r, 64));
+        };
+        fetch([&](int r, uint32_t d) { return kb + (from(r) + d); }, [&](int r, uint32_t d) { return vb + (from(r) + d); });
     }
 }
 
@@ -343,30 +398,40 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
     if (uniform_div(mtile * ROWS, p.G) >= cnt) return;                 // no row of this tile is asked for
     const int m0 = mtile * ROWS + wm * 16 * QT;
     KeySource s = {};
+    s.k_row = (uint32_t)p.k_row * TL::ES;
+    s.v_row = (uint32_t)p.v_row * TL::ES;
+    s.k_bytes = p.dk * TL::ES;
     if constexpr (KV == KV_I8) {
-        const int sl = p.slot ? p.slot[b] : b;
-        s.n_slots = p.n_slots;
+        int sl = TABLE ? 0 : p.slot ? p.slot[b] : b;
+        if ((unsigned)sl >= (unsigned)p.n_slots) {
+            sl = 0;
+            T = 0;
+        }
         s.s_slot = (int64_t)p.Hkv * p.n_blocks;
-        s.k_slot = p.k_item;
-        s.v_slot = p.v_item;
-        int64_t at = 0;
-        if constexpr (TABLE) s.table = p.table + b * p.table_ld;
-        else if ((unsigned)sl >= (unsigned)p.n_slots) T = 0;
-        else at = sl;
-        s.k = (const uint8_t*)p.k + at * p.k_item + kh * p.k_head;
-        s.v = (const uint8_t*)p.v + at * p.v_item + kh * p.v_head;
-        s.ks = p.k_scale + at * s.s_slot + (int64_t)kh * p.n_blocks;
-        s.vs = p.v_scale + at * s.s_slot + (int64_t)kh * p.n_blocks;
+        s.k = (const uint8_t*)p.k + sl * p.k_item + kh * p.k_head;
+        s.v = (const uint8_t*)p.v + sl * p.v_item + kh * p.v_head;
+        s.ks = p.k_scale + sl * s.s_slot + (int64_t)kh * p.n_blocks;
+        s.vs = p.v_scale + sl * s.s_slot + (int64_t)kh * p.n_blocks;
+        if constexpr (TABLE) {
+            s.table = p.table + b * p.table_ld;
+            s.n_slots = p.n_slots;
+            s.k_slot = p.k_item;
+            s.far = p.n_slots * p.k_item > 0x7fffffffll;
+        }
     } else {
         s.k = (const uint8_t*)p.k + (b * p.k_item + kh * p.k_head) * TL::ES;
         s.v = (const uint8_t*)p.v + (b * p.v_item + kh * p.v_head) * TL::ES;
         s.mask = p.mask ? p.mask + b * p.mask_item : nullptr;
     }
     s.T = T;
-    s.k_row = (uint32_t)p.k_row * TL::ES;
-    s.v_row = (uint32_t)p.v_row * TL::ES;
-    s.k_bytes = p.dk * TL::ES;
-    s.v_off = (c * NJ < p.dk ? c * NJ : 0) * TL::ES;       // rows past the head's dimensions are not stored
+    // pieces past the head's dimensions read its first again (their queries are
+    // zero; their output is not stored); with the table the row comes separately
+#pragma unroll
+    for (int n = 0; n < (TL::NK + 3) / 4; ++n) {
+        const int o = key_piece<KV, D>(n, g);
+        s.k_at[n] = (TABLE ? 0 : c * s.k_row) + (o < s.k_bytes ? o : 0);
+    }
+    s.v_at = (TABLE ? 0 : 4 * g * s.v_row) + (c * NJ < p.dk ? c * NJ : 0) * TL::ES;
 
     // queries: B operand, column c = row m0 + 16 qt + c
     uint32_t q[QT][NQ];
@@ -390,10 +455,11 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
 
     // keys of this wave: every WK-th tile of the workgroup's share, up to the
     // last that one of its rows sees
-    int hi = T;
+    int hi = T, all = T;         // (all: keys that every row sees)
     if (p.causal) {
         const int mi = uniform_div(m0 + 16 * QT - 1, p.G), il = mi < cnt ? mi : cnt - 1;
         hi = T - cnt + il + 1 < T ? T - cnt + il + 1 : T;
+        all = T - cnt + uniform_div(m0, p.G) + 1;
     }
     const int k0 = split * p.split_keys;
     const int64_t ke = (int64_t)k0 + p.split_keys;
@@ -439,7 +505,7 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
                     sc[4 + e] *= ks8[4 + e];
                 }
             }
-            if (!whole || p.causal) {
+            if (!whole || t0 + 32 > all) {
                 const uint32_t see = keep >> (4 * g) & low_bits(lim[qt] - t0 - 4 * g);
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -526,36 +592,38 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
     };
 
     if (k0 + 32 * wk < k1) {
-        auto entry = [&](int t0) -> int {
-            if constexpr (TABLE) {
-                const int at = t0 + (lane & 31);
-                return s.table[at < T ? at : T - 1];
-            } else {
-                return 0;
-            }
-        };
         int t0 = k0 + 32 * wk;
         if constexpr (KV == KV_F32) {
             for (; t0 < k1; t0 += STEP) {
                 Tile<KV, D> a;
-                load_tile<KV, D, TABLE>(a, s, t0, 0, lane);
+                load_tile<KV, D>(a, s, t0, lane);
                 compute(a, t0);
             }
         } else {
             // the next tile's loads are in flight while a tile is computed,
             // the table's entries one tile further ahead
             Tile<KV, D> a, bt;
-            int e0 = entry(t0);
-            int e1 = entry(t0 + STEP);
-            load_tile<KV, D, TABLE>(a, s, t0, e0, lane);
+            int e = 0;
+            auto load = [&](Tile<KV, D>& t, int at) {
+                if constexpr (TABLE) {
+                    const int slot = e, next = at + STEP + (lane & 31);
+                    e = s.table[next < T ? next : T - 1];
+                    load_tile_by_table<D>(t, s, at, slot, lane);
+                } else {
+                    load_tile<KV, D>(t, s, at, lane);
+                }
+            };
+            if constexpr (TABLE) {
+                const int at = t0 + (lane & 31);
+                e = s.table[at < T ? at : T - 1];
+            }
+            load(a, t0);
             while (true) {
-                e0 = entry(t0 + 2 * STEP);
-                load_tile<KV, D, TABLE>(bt, s, t0 + STEP, e1, lane);
+                load(bt, t0 + STEP);
                 compute(a, t0);
                 t0 += STEP;
                 if (t0 >= k1) break;
-                e1 = entry(t0 + 2 * STEP);
-                load_tile<KV, D, TABLE>(a, s, t0 + STEP, e0, lane);
+                load(a, t0 + STEP);
                 compute(bt, t0);
                 t0 += STEP;
                 if (t0 >= k1) break;
@@ -637,11 +705,6 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
         }
         store(0, wk, x, mm, ll);
     }
-}
-
-// A buffer resource of one step's rows, built from scalars.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const uint8_t* base, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, (int)bytes, 0x00020000);
 }
 
 // Many query rows against the same keys: 128 rows a workgroup, 32 a wave, the
@@ -766,22 +829,13 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const auto kt = step_rsrc(kb + (int64_t)t0 * k_row, rows * k_row + p.dk * ES);
         const auto vt = step_rsrc(vb + (int64_t)t0 * v_row, rows * v_row + p.dk * ES);
 #pragma unroll
-        for (int n = 0; n < NKP; ++n) {
-            const int4v x = __builtin_amdgcn_raw_buffer_load_b128(kt, k_at, n * KSTEP * k_row, 0);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) kr[n][e] = x[e];
-        }
+        for (int n = 0; n < NKP; ++n) buffer_words(kr[n], kt, k_at + n * KSTEP * k_row);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t so = (i < 4 ? i : 12 + i) * v_row;
-            if constexpr (DV * ES == 1) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b8(vt, v_at, so, 0);
-            else if constexpr (DV * ES == 2) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b16(vt, v_at, so, 0);
-            else if constexpr (DV * ES == 4) vr[i][0] = __builtin_amdgcn_raw_buffer_load_b32(vt, v_at, so, 0);
-            else {
-                const int2v x = __builtin_amdgcn_raw_buffer_load_b64(vt, v_at, so, 0);
-                vr[i][0] = x[0];
-                vr[i][1] = x[1];
-            }
+            const uint32_t at = v_at + (i < 4 ? i : 12 + i) * v_row;
+            if constexpr (DV * ES == 1) vr[i][0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vt, at, 0, 0);
+            else if constexpr (DV * ES == 2) vr[i][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vt, at, 0, 0);
+            else buffer_words(vr[i], vt, at);
         }
     };
     auto stage = [&](uint64_t keep) {
