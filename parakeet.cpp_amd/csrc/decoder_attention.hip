@@ -593,7 +593,7 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
 
     if (k0 + 32 * wk < k1) {
         int t0 = k0 + 32 * wk;
-        if constexpr (KV == KV_F32) {
+        if constexpr (KV == KV_F32) {      // (a second tile in flight gained nothing: the matrix pipe is what these wait for)
             for (; t0 < k1; t0 += STEP) {
                 Tile<KV, D> a;
                 load_tile<KV, D>(a, s, t0, lane);
@@ -1038,60 +1038,88 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     }
 }
 
-// Joins the splits' (m, l, O), at most 64 of them, WPR waves a row (four where
-// rows are few).  Lane s of a wave has split s's factor 2^(m_s - max m); the
-// wave adds splits w, w + WPR, ... in that order, two dimensions a lane, and the
-// waves' sums are added in wave order.
-template <bool F32, int WPR> __global__ __launch_bounds__(256) void dec_join_kernel(DecAttnParams p) {
+// Joins the splits' (m, l, O), at most 64 of them.  Few rows: a workgroup a row,
+// lane s of every wave with split s's factor 2^(m_s - max m); wave w adds splits
+// w, w + 4, ... in that order, two dimensions a lane, and the four sums are added
+// in wave order.
+template <bool F32> __global__ __launch_bounds__(256) void dec_join_kernel(DecAttnParams p) {
     __shared__ float so[4][128];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, M = p.n_q * p.G, d = 2 * lane;
-    const int64_t row = (int64_t)blockIdx.x * (4 / WPR) + wave / WPR, rows = (int64_t)p.B * p.Hkv * M;
-    const int64_t rc = row < rows ? row : rows - 1;
-    const int unit = (int)(rc / M), mr = (int)(rc - (int64_t)unit * M), w = wave % WPR;
-    const int b = unit / p.Hkv, kh = unit - b * p.Hkv, i = mr / p.G, h = kh * p.G + (mr - i * p.G);
-    const bool live = row < rows && i < (p.q_len ? p.q_len[b] : p.n_q);
-    const float2 ml = live && lane < p.splits ? p.part_ml[rc * p.splits + lane] : float2{kNoMax, 0.f};
+    const int row = blockIdx.x, unit = uniform_div(row, M), mr = row - unit * M;
+    const int b = uniform_div(unit, p.Hkv), kh = unit - b * p.Hkv, i = uniform_div(mr, p.G), h = kh * p.G + (mr - i * p.G);
+    const float2 ml = lane < p.splits ? p.part_ml[(int64_t)row * p.splits + lane] : float2{kNoMax, 0.f};
+    if (i >= (p.q_len ? p.q_len[b] : p.n_q)) return;
     const float mm = wave_max(ml.x);
     // a split without a key (l = 0) has not written its O
     const float f = ml.y != 0.f ? __builtin_amdgcn_exp2f(ml.x - mm) : 0.f;
     const float l = wave_sum(ml.y * f);
     float x0 = 0.f, x1 = 0.f;
-    if (live && d < p.dk) {
-        const float* src = p.part_o + rc * p.splits * p.dk + d;
-        for (int s0 = w; s0 < p.splits; s0 += 4 * WPR) {
+    if (d < p.dk) {
+        const float* src = p.part_o + (int64_t)row * p.splits * p.dk + d;
+        for (int s0 = wave; s0 < p.splits; s0 += 16) {
             float2v o[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int s = s0 + k * WPR, at = s < p.splits ? s : s0;
-                o[k] = *(const float2v*)(src + (int64_t)at * p.dk);
+                const int s = s0 + 4 * k;
+                o[k] = *(const float2v*)(src + (int64_t)(s < p.splits ? s : s0) * p.dk);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int s = s0 + k * WPR;
-                const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s < p.splits ? s : 63));
+                const int s = s0 + 4 * k;
+                const float fs = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s & 63));
                 const bool add = s < p.splits && fs != 0.f;
                 x0 += add ? o[k][0] * fs : 0.f;
                 x1 += add ? o[k][1] * fs : 0.f;
             }
         }
     }
-    if constexpr (WPR > 1) {
-        so[wave][d] = x0;
-        so[wave][d + 1] = x1;
-        __syncthreads();
-        if (w != 0) return;
-        x0 = x1 = 0.f;
-#pragma unroll
-        for (int k = 0; k < WPR; ++k) {
-            x0 += so[wave + k][d];
-            x1 += so[wave + k][d + 1];
-        }
-    }
-    if (!live || d >= p.dk) return;
+    so[wave][d] = x0;
+    so[wave][d + 1] = x1;
+    __syncthreads();
+    if (wave != 0 || d >= p.dk) return;
+    x0 = (so[0][d] + so[1][d]) + (so[2][d] + so[3][d]);
+    x1 = (so[0][d + 1] + so[1][d + 1]) + (so[2][d + 1] + so[3][d + 1]);
     const float inv = l != 0.f ? 1.0f / l : 0.f;
     const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + d;
     if constexpr (F32) *(float2v*)((float*)p.out + at) = (float2v){x0 * inv, x1 * inv};
     else *(uint32_t*)((f16*)p.out + at) = pack_f16(x0 * inv, x1 * inv);
+}
+
+// Many rows (and so few splits): four dimensions a thread, dk / 4 threads a row,
+// the splits in order, four at a time.
+template <bool F32> __global__ __launch_bounds__(256) void dec_join_rows_kernel(DecAttnParams p, int rows) {
+    const int per = p.dk >> 2, M = p.n_q * p.G, tr = udiv_small(threadIdx.x, per), d = 4 * (threadIdx.x - tr * per);
+    const int rpb = uniform_div(256, per), row = blockIdx.x * rpb + tr;
+    if (tr >= rpb || row >= rows) return;
+    const int unit = udiv_small(row, M), mr = row - unit * M, b = udiv_small(unit, p.Hkv), kh = unit - b * p.Hkv;
+    const int i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
+    if (i >= (p.q_len ? p.q_len[b] : p.n_q)) return;
+    const float2* ml = p.part_ml + (int64_t)row * p.splits;
+    const float* src = p.part_o + (int64_t)row * p.splits * p.dk + d;
+    float m = kNoMax, l = 0.f;
+    float4v x = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < p.splits; s0 += 4) {
+        float2 v[4];
+        float4v o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int s = s0 + k < p.splits ? s0 + k : s0;
+            v[k] = ml[s];
+            o[k] = *(const float4v*)(src + (int64_t)s * p.dk);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (s0 + k >= p.splits || v[k].y == 0.f) continue;     // (O of a split without a key is not written)
+            const float hi = fmaxf(m, v[k].x), fo = __builtin_amdgcn_exp2f(m - hi), fn = __builtin_amdgcn_exp2f(v[k].x - hi);
+            m = hi;
+            l = l * fo + v[k].y * fn;
+            x = x * fo + o[k] * fn;
+        }
+    }
+    x *= l != 0.f ? 1.0f / l : 0.f;
+    const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + d;
+    if constexpr (F32) *(float4v*)((float*)p.out + at) = x;
+    else *(int2v*)((f16*)p.out + at) = (int2v){(int)pack_f16(x[0], x[1]), (int)pack_f16(x[2], x[3])};
 }
 
 // Rows a workgroup takes and how many ways the keys are split over workgroups.
@@ -1161,10 +1189,14 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     else p.table ? launch_width<KV_I8, false, true>(p, sh, s) : launch_width<KV_I8, false, false>(p, sh, s);
     if (sh.splits > 1) {
         const int64_t rows = (int64_t)p.B * p.Hkv * p.n_q * p.G;
-        const bool few = rows <= 1024;             // a wave a row leaves the chip short of waves
-        auto* k = p.q_f32 ? (few ? dec_join_kernel<true, 4> : dec_join_kernel<true, 1>)
-                          : (few ? dec_join_kernel<false, 4> : dec_join_kernel<false, 1>);
-        launch(k, dim3((unsigned)(few ? rows : (rows + 3) / 4)), dim3(256), 0, s, p);
+        if (rows <= 1024) {                        // threads by the row leave the chip short of them
+            auto* k = p.q_f32 ? dec_join_kernel<true> : dec_join_kernel<false>;
+            launch(k, dim3((unsigned)rows), dim3(256), 0, s, p);
+        } else {
+            const int rpb = 256 / (p.dk / 4);
+            auto* k = p.q_f32 ? dec_join_rows_kernel<true> : dec_join_rows_kernel<false>;
+            launch(k, dim3((unsigned)((rows + rpb - 1) / rpb)), dim3(256), 0, s, p, (int)rows);
+        }
     }
 }
 
