@@ -362,7 +362,7 @@ int pkx_quantize_gguf(const char* in_path, const char* out_path, int gtype, int*
  * Strides are in elements (item, row, head; the d_head elements are adjacent), those of
  * k and v not negative and below 2^22 between rows.  d_head: a multiple of 8 up to 128;
  * buffers 16-byte aligned, strides multiples of 16 bytes; n_heads a multiple of
- * n_kv_heads.  out overlaps no input. */
+ * n_kv_heads; n_k at most 2^30, n_items x n_q x n_heads below 2^22.  out overlaps no input. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of q, k, v and out */
     int n_items, n_q, n_k;
@@ -396,8 +396,8 @@ typedef struct {
  * earlier one, q, becomes round(q * (s / s')): each step one f32 operation, ties to even.  NaN is
  * held as 0, an infinity as +-127, and neither counts in max|x|.  What follows the new tokens in
  * their last block is left as it was and is expected to be appended next.  Tokens past the capacity
- * are dropped; a row with a start or slot out of range is skipped; of rows that name the same slot
- * only the first is appended.  table: see pkx_cache8_attention; entries start[r].. of row r are set
+ * are dropped; a row with a start or slot out of range is skipped, and so is one whose slot an earlier
+ * row names.  table: see pkx_cache8_attention; entries start[r].. of row r are set
  * to its slot.  Strides in elements, multiples of 16 bytes. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of k and v */

@@ -585,6 +585,7 @@ size_t beam_select_workspace(const BeamSelectParams& p) {
 void launch_beam_select(const BeamSelectParams& p, void* ws, size_t ws_bytes, hipStream_t s) {
     if (p.B == 0) return;
     const int wide = p.f32 ? 4 : 8;
+    require(p.B < (1 << 22), "beam select: at most 2^22 items in one call");
     if (const int per = small_waves(p)) {
         const bool one = p.V < per * 64 * wide;
         auto* k = p.f32 ? (one ? select_small_kernel<true, 1> : select_small_kernel<true, 4>)

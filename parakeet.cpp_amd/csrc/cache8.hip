@@ -18,15 +18,15 @@ namespace {
 // holds dimensions [8 (t % n8), +8) of the block's tokens t / n8 + k * (256 / n8),
 // n8 = dk / 8: at most 32 values, read once, kept in registers between the
 // maximum and the quantisation.
-template <bool F32> __global__ __launch_bounds__(256) void cache8_append_kernel(CacheAppendParams p) {
-    const int t = threadIdx.x, kh = blockIdx.y % p.c.Hkv, r = blockIdx.y / p.c.Hkv;
+template <bool F32> __global__ __launch_bounds__(256) void cache8_append_kernel(CacheAppendParams p, int blocks) {
+    const int t = threadIdx.x, kh = blockIdx.y, r = udiv_small(blockIdx.x, blocks), bi = blockIdx.x - r * blocks;
     const bool values = blockIdx.z != 0;
     const int start = p.start[r], slot = p.slot ? p.slot[r] : r;
     int n = p.count ? p.count[r] : p.n_new;
     n = n < 0 ? 0 : n > p.n_new ? p.n_new : n;
     if (start < 0 || start >= p.c.cap || (unsigned)slot >= (unsigned)p.c.n_slots) return;
     const int end = n < p.c.cap - start ? start + n : p.c.cap;     // tokens past the capacity are dropped
-    const int blk = start / kCacheBlock + blockIdx.x, t0 = blk * kCacheBlock;
+    const int blk = start / kCacheBlock + bi, t0 = blk * kCacheBlock;
     const int lo = start > t0 ? start : t0, hi = end < t0 + kCacheBlock ? end : t0 + kCacheBlock;
     if (lo >= hi) return;
     __shared__ float part[4];
@@ -114,9 +114,9 @@ template <bool F32> __global__ __launch_bounds__(256) void cache8_append_kernel(
 }
 
 // Eight values of K and V per thread: tokens start[r] .. + n of row r's slot as q * scale.
-__global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int per) {
-    const int n8 = p.c.dk / 8, r = blockIdx.y;
-    const unsigned in = blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int per, int chunks) {
+    const int n8 = p.c.dk / 8, r = udiv_small(blockIdx.x, chunks);
+    const unsigned in = (blockIdx.x - r * chunks) * 256 + threadIdx.x;
     if (in >= (unsigned)per) return;
     const unsigned hk = in / n8, i = hk / p.c.Hkv;
     const int d = 8 * (in - hk * n8), kh = hk - i * p.c.Hkv;
@@ -152,17 +152,19 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int
 void launch_cache8_append(const CacheAppendParams& p, hipStream_t s) {
     if (p.R == 0 || p.n_new == 0) return;
     const int blocks = (p.n_new + kCacheBlock - 2) / kCacheBlock + 1;     // wherever the first token falls in its block
-    require((int64_t)p.R * p.c.Hkv <= 65535, "cache append: at most 65535 rows x heads in one call");
-    const dim3 grid(blocks, p.R * p.c.Hkv, 2);
-    if (p.f32) launch(cache8_append_kernel<true>, grid, dim3(256), 0, s, p);
-    else launch(cache8_append_kernel<false>, grid, dim3(256), 0, s, p);
+    const int64_t x = (int64_t)p.R * blocks;
+    require(x < (1 << 22) && p.c.Hkv <= 65535, "cache append: at most 2^22 blocks of 32 tokens in one call");
+    const dim3 grid((unsigned)x, p.c.Hkv, 2);
+    if (p.f32) launch(cache8_append_kernel<true>, grid, dim3(256), 0, s, p, blocks);
+    else launch(cache8_append_kernel<false>, grid, dim3(256), 0, s, p, blocks);
 }
 
 void launch_cache8_read(const CacheReadParams& p, hipStream_t s) {
     const int64_t per = (int64_t)p.n * p.c.Hkv * (p.c.dk / 8);
     if (p.R == 0 || per == 0 || (!p.k && !p.v)) return;
-    require(p.R <= 65535 && per < ((int64_t)1 << 31), "cache read: at most 65535 rows and 2^34 values of one in a call");
-    launch(cache8_read_kernel, dim3((unsigned)((per + 255) / 256), p.R), dim3(256), 0, s, p, (int)per);
+    const int64_t chunks = (per + 255) / 256;
+    require(p.R * chunks < (1 << 22), "cache read: at most 2^33 values in one call");
+    launch(cache8_read_kernel, dim3((unsigned)(p.R * chunks)), dim3(256), 0, s, p, (int)per, (int)chunks);
 }
 
 }  // namespace pkx

@@ -150,6 +150,11 @@ bool is_f32(int type, const char* what) {
     return type == PKX_TYPE_F32;
 }
 
+// Rows of an output that do not run into each other.
+void need_apart(int64_t a, int64_t na, int64_t b, int64_t nb, int64_t c, int64_t nc, int64_t row, const char* what) {
+    need((na <= 1 || a >= row) && (nb <= 1 || b >= row) && (nc <= 1 || c >= row), what);
+}
+
 // A strided operand read or written in 16-byte pieces.
 void need_view(const void* p, int64_t a, int64_t b, int64_t c, bool f32, const char* what) {
     const int64_t unit = f32 ? 4 : 8;
@@ -161,6 +166,7 @@ pkx::DecAttnParams cross_params(const pkx_cross_attn* a) {
     need(a, "null argument");
     const bool f32 = is_f32(a->type, "cross attention: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
     need(a->n_items >= 0 && a->n_q >= 0 && a->n_k >= 0, "cross attention: negative size");
+    need(a->n_k <= (1 << 30), "cross attention: more than 2^30 keys");
     need(a->n_heads >= 1 && a->n_kv_heads >= 1 && a->n_heads % a->n_kv_heads == 0,
          "cross attention: n_heads must be a multiple of n_kv_heads");
     need(a->d_head >= 8 && a->d_head <= 128 && a->d_head % 8 == 0, "cross attention: d_head must be a multiple of 8 up to 128");
@@ -189,8 +195,8 @@ pkx::Cache8 cache_params(const pkx_cache8* c) {
     need(c, "null argument");
     need(c->n_slots >= 1 && c->n_kv_heads >= 1, "8-bit cache: no slots or heads");
     need(c->d_head >= 16 && c->d_head <= 128 && c->d_head % 16 == 0, "8-bit cache: d_head must be a multiple of 16 up to 128");
-    need(c->capacity >= PKX_CACHE8_BLOCK && c->capacity % PKX_CACHE8_BLOCK == 0,
-         "8-bit cache: capacity must be a multiple of PKX_CACHE8_BLOCK");
+    need(c->capacity >= PKX_CACHE8_BLOCK && c->capacity % PKX_CACHE8_BLOCK == 0 && c->capacity <= (1 << 30),
+         "8-bit cache: capacity must be a multiple of PKX_CACHE8_BLOCK up to 2^30");
     need(c->k && c->v && c->k_scale && c->v_scale, "8-bit cache: null buffer");
     need(((uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0 && ((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 4 == 0,
          "8-bit cache: k and v must be 16-byte aligned");
@@ -719,6 +725,7 @@ int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void
         if (p.B == 0 || p.n_q == 0) return;
         need_view(p.q, p.q_item, p.q_row, p.q_head, p.q_f32, "cross attention: q must be 16-byte aligned with strides of whole 16 bytes");
         need_view(p.out, p.o_item, p.o_row, p.o_head, p.q_f32, "cross attention: out must be 16-byte aligned with strides of whole 16 bytes");
+        need_apart(p.o_item, p.B, p.o_row, p.n_q, p.o_head, a->n_heads, p.dk, "cross attention: rows of out overlap");
         if (p.n_k > 0) {
             need_view(p.k, p.k_item, p.k_row, p.k_head, p.q_f32, "cross attention: k must be 16-byte aligned with strides of whole 16 bytes");
             need_view(p.v, p.v_item, p.v_row, p.v_head, p.q_f32, "cross attention: v must be 16-byte aligned with strides of whole 16 bytes");
@@ -785,6 +792,7 @@ int pkx_cache8_attention(const pkx_cache8* c, const pkx_cache8_attn* a, void* ws
         if (p.B == 0 || p.n_q == 0) return;
         need_view(p.q, p.q_item, p.q_row, p.q_head, p.q_f32, "cache attention: q must be 16-byte aligned with strides of whole 16 bytes");
         need_view(p.out, p.o_item, p.o_row, p.o_head, p.q_f32, "cache attention: out must be 16-byte aligned with strides of whole 16 bytes");
+        need_apart(p.o_item, p.B, p.o_row, p.n_q, p.o_head, a->n_heads, p.dk, "cache attention: rows of out overlap");
         need(p.k_len, "cache attention: null len");
         need(p.slot || p.table || p.B <= p.n_slots, "cache attention: more rows than slots");
         need(!p.table || p.table_ld >= p.n_k, "cache attention: table rows are shorter than max_len");

@@ -885,6 +885,8 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         }
     };
     auto compute = [&](int t0, uint64_t keep, const float (&ks)[2], const float (&vs)[2]) {
+        // (a wave that feeds the matrix pipe goes before one at its softmax: 2 to 5% in f16)
+        if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(1);
         float4v s[QT][4];
         // consecutive products go to different accumulators
 #pragma unroll
@@ -904,6 +906,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                         s[qt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[kt], __builtin_bit_cast(half8v, bq), from, 0, 0, 0);
                     }
         }
+        if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(0);
         const bool cut = keep != ~0ull || t0 + KT > all_wave;
         float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f;
         if constexpr (KV == KV_I8) {
@@ -979,6 +982,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) o[qt][j] *= alpha[qt];
+        if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -997,6 +1001,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                             o[qt][j0 + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[j], __builtin_bit_cast(half8v, bp), o[qt][j0 + j], 0, 0, 0);
                         }
             }
+        if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(0);
     };
 
     if (k0 < k1) load(k0);
@@ -1010,10 +1015,12 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         __syncthreads();
     }
 
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) l[qt] = xgroup_sum(l[qt]);
     // lane (c, g) has row c's dimensions 16 j + 4 g .. + 4
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        const float ll = xgroup_sum(l[qt]);
+        const float ll = l[qt];
         const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
         if (i >= cnt) continue;
         const float unit = KV == KV_I8 ? vref : 1.0f;
@@ -1134,10 +1141,13 @@ Shape attn_shape(const DecAttnParams& p) {
     const int64_t wgs = units * s.mt;
     int64_t want = wgs >= 512 ? 1 : 512 / wgs;             // about two workgroups per CU
     if (want > 64) want = 64;
-    // whole rounds of the four key shares, or steps of dec_tile_kernel, and at
-    // least four rounds: a split costs its partial sums and the join's launch
+    // whole rounds of the four key shares, or steps of dec_tile_kernel.  A split
+    // costs its partial sums and the join's launch, so it takes at least four
+    // rounds (of about 0.5 us; f32 heads above 64 one round, of 2 us) or eight steps
+    // (1 us), four where there are few rows to join
     int per = (cdiv(tiles, want) + 3) / 4 * 4;
-    if (per < 16) per = 16;
+    const int least = p.kv == KV_F32 && p.dk > 64 ? 4 : s.wide && units * M <= 1024 ? 8 : 16;
+    if (per < least) per = least;
     s.splits = cdiv(tiles, per);
     s.keys = per * 32;
     return s;
@@ -1171,7 +1181,7 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     if (p.B == 0 || p.n_q == 0) return;
     const Shape sh = attn_shape(p);
     require((int64_t)p.B * p.Hkv * sh.mt * sh.splits < (1 << 22) && (int64_t)p.B * p.Hkv * p.n_q * p.G < (1 << 22),
-            "attention: too many rows for one call");
+            "attention: at most 2^22 rows x heads in one call");
     const size_t need = dec_attention_workspace(p);
     require(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need),
             "attention: the workspace is smaller than its size query says, or not 16-byte aligned");

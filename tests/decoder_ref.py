@@ -46,9 +46,10 @@ def append(ints, scales, x, slot, start, count):
     for r in range(x.shape[0]):
         s0, sl = int(start[r]), int(slot[r])
         n = min(max(int(count[r]), 0), x.shape[1])
-        if not (0 <= s0 < cap and 0 <= sl < ints.shape[0]) or sl in seen:
-            continue
+        first = sl not in seen
         seen.add(sl)
+        if not (0 <= s0 < cap and 0 <= sl < ints.shape[0] and first):
+            continue
         end = min(s0 + n, cap)
         for b in range(s0 // BLOCK, (end + BLOCK - 1) // BLOCK if end > s0 else 0):
             lo, hi = max(s0, b * BLOCK), min(end, (b + 1) * BLOCK)

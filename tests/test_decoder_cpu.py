@@ -63,7 +63,7 @@ def beam(**kw):
 def test_cross_attention_refusals():
     out = _run("""
         for kw in (dict(type=8), dict(n_items=-1), dict(n_heads=3), dict(n_kv_heads=0), dict(d_head=60), dict(d_head=136),
-                   dict(q=None), dict(k=A + 8), dict(v_row=132), dict(out_head=-64), dict(k_row=1 << 22), dict(type=0, q_head=66)):
+                   dict(n_k=(1 << 30) + 1), dict(out_row=56), dict(out_head=0), dict(q=None), dict(k=A + 8), dict(v_row=132), dict(out_head=-64), dict(k_row=1 << 22), dict(type=0, q_head=66)):
             said(L.pkx_cross_attention(cross(**kw), None, 0, None))
         said(L.pkx_cross_attention(None, None, 0, None))
         said(L.pkx_cross_attention_workspace(cross(), None))
@@ -75,14 +75,14 @@ def test_cross_attention_refusals():
         for kw in (dict(n_items=0), dict(n_q=0, q=None), dict(n_items=0, k=None)):
             said(L.pkx_cross_attention(cross(**kw), None, 0, None))
     """)
-    words = ["type", "negative", "n_heads", "n_heads", "d_head", "d_head", "q must", "k must", "v must", "out must", "2^22", "q must",
+    words = ["type", "negative", "n_heads", "n_heads", "d_head", "d_head", "2^30", "overlap", "overlap", "q must", "k must", "v must", "out must", "2^22", "q must",
              "null", "null"]
-    for line, w in zip(out[:14], words):
+    for line, w in zip(out[:17], words):
         assert line.startswith("1 ") and w in line, (line, w)
-    assert out[14].strip() == "0"
-    for line, w in zip(out[15:18], ("workspace", "aligned", "too many")):
+    assert out[17].strip() == "0"
+    for line, w in zip(out[18:21], ("workspace", "aligned", "at most")):
         assert line.startswith("1 ") and w in line, (line, w)
-    assert [x.strip() for x in out[18:]] == ["0"] * 3
+    assert [x.strip() for x in out[21:]] == ["0"] * 3
 
 
 def test_cache_refusals():
@@ -90,7 +90,7 @@ def test_cache_refusals():
         for c, t in ((cache(n_slots=0), toks()), (cache(d_head=72), toks()), (cache(d_head=144), toks()), (cache(capacity=100), toks()),
                      (cache(capacity=0), toks()), (cache(k=None), toks()), (cache(v=A + 4), toks()), (cache(), toks(type=2)),
                      (cache(), toks(n_new=-1)), (cache(), toks(k_tok=130)), (cache(), toks(start=None)), (cache(), toks(n_rows=4)),
-                     (cache(), toks(table=A, table_row=95)), (cache(), toks(n_rows=70000, slot=A))):
+                     (cache(), toks(table=A, table_row=95)), (cache(), toks(n_rows=3 << 20, slot=A))):
             said(L.pkx_cache8_append(c, t, None))
         for a in (attn(type=3), attn(n_heads=3), attn(n_q=-1), attn(max_len=-1), attn(len=None), attn(n_rows=4), attn(q=None),
                   attn(out_tok=100), attn(table=A, table_row=95)):
@@ -104,7 +104,7 @@ def test_cache_refusals():
         said(L.pkx_cache8_read(cache(), 1, 0, None, None, None, None, None))
     """)
     words = ["no slots", "d_head", "d_head", "capacity", "capacity", "null", "aligned", "type", "negative", "k must", "null start",
-             "more rows", "shorter", "65535", "type", "n_heads", "negative", "max_len", "null len", "more rows", "q must", "out must",
+             "more rows", "shorter", "2^22", "type", "n_heads", "negative", "max_len", "null len", "more rows", "q must", "out must",
              "shorter", "null start", "aligned"]
     for line, w in zip(out[:25], words):
         assert line.startswith("1 ") and w in line, (line, w)

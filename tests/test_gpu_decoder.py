@@ -42,7 +42,9 @@ CROSS = [
     ("f16", 2, 17, 70, 2, 2, 80), ("f16", 1, 2, 3001, 2, 1, 64), ("f16", 1, 1, 4096, 1, 1, 128), ("f16", 2, 130, 97, 2, 2, 64),
     ("f16", 1, 65, 300, 4, 1, 128), ("f16", 1, 64, 1, 1, 1, 24), ("f16", 2, 300, 515, 1, 1, 32), ("f16", 1, 200, 130, 2, 2, 128),
     ("f32", 1, 1, 125, 8, 8, 64), ("f32", 3, 4, 33, 4, 2, 128), ("f32", 2, 5, 7, 3, 3, 8), ("f32", 2, 37, 211, 2, 2, 64),
-    ("f32", 1, 2, 2048, 2, 1, 32), ("f32", 2, 130, 97, 2, 2, 80), ("f32", 1, 70, 64, 4, 1, 128),
+    # no keys at all
+    ("f16", 2, 3, 0, 2, 1, 64), ("f16", 1, 70, 0, 1, 1, 64), ("f32", 2, 3, 0, 2, 1, 64), ("f32", 1, 70, 0, 1, 1, 32),
+    ("f32", 1, 2, 2048, 2, 1, 32), ("f32", 1, 3, 900, 2, 2, 128), ("f32", 2, 130, 97, 2, 2, 80), ("f32", 1, 70, 64, 4, 1, 128),
 ]
 
 
@@ -109,6 +111,22 @@ def test_cross_attention_strides_and_streams(gpu, stream):
         for h in range(H):
             want = ref.attention(q[b, h, :nq, 8:8 + d], kv[b, :, 0, h], kv[b, :, 1, h], d ** -0.5, np.ones((nq, nk), bool))
             check_attention(got[0][b, h, :, 8:8 + d], want, True, d, f"strides b{b} h{h}")
+
+
+@pytest.mark.parametrize("type,nq,d", [("f16", 5, 64), ("f16", 80, 64), ("f32", 5, 64), ("f32", 80, 128)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+def test_cross_attention_scales(gpu, stream, type, nq, d, scale):
+    """Any factor: negative, zero (the mean of the kept values), large, with keys left out."""
+    rng = np.random.default_rng(nq)
+    dt = np.float16 if type == "f16" else np.float32
+    q, k, v = (rng.standard_normal((1, n, 2, d)).astype(dt) for n in (nq, 75, 75))
+    mask = (rng.random((1, 75)) < 0.7).astype(np.uint8)
+    out = gpu.DeviceArray(q.shape, dt)
+    gpu.CrossAttention(*(dev(gpu, x, stream) for x in (q, k, v)), out, k_mask=dev(gpu, mask, stream), scale=scale)(stream)
+    got = out.numpy(stream)
+    for h in range(2):
+        want = ref.attention(q[0, :, h], k[0, :, h], v[0, :, h], scale, np.broadcast_to(mask[0] != 0, (nq, 75)))
+        check_attention(got[0, :, h], want, type == "f16", d, f"scale {scale} h{h}")
 
 
 def test_cross_attention_far_items(gpu, stream):
