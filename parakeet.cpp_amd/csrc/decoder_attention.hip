@@ -381,7 +381,7 @@ __device__ __forceinline__ void work_of(int bid, const DecAttnParams& p, int mt,
 template <int KV, bool QF32, int D, int QT, int WM, int WK, bool TABLE>
 __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn_kernel(DecAttnParams p) {
     using TL = Tile<KV, D>;
-    static_assert(WK == 1 || (QT == 1 && WM == 1 && WK == 4), "joined waves: one row tile, four key shares");
+    static_assert(WK == 1 || (QT == 1 && WM == 1 && (WK == 4 || WK == 8)), "joined waves: one row tile, four or eight key shares");
     constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
     constexpr int NQ = KV == KV_F32 ? D / 4 : SPLIT ? D / 4 : D / 8;
     constexpr int NJ = D / 16, ROWS = 16 * QT * WM;
@@ -676,10 +676,11 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
                 store(qt, e, x, m[qt], l[qt]);
             }
     } else {
-        // four key shares: brought to a common maximum, wave e adds and stores
-        // accumulator register e of every wave, in wave order
+        // the key shares, brought to a common maximum; of eight, four first add
+        // the others' to theirs; then wave e adds and stores accumulator register
+        // e of all four, in wave order
         __shared__ float sml[2][WK][16];
-        __shared__ float so[WK][4][NJ][64];
+        __shared__ float so[4][4][NJ][64];
         if (g == 0) {
             sml[0][wk][c] = m[0];
             sml[1][wk][c] = l[0];
@@ -692,16 +693,33 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
         for (int w = 0; w < WK; ++w) ll += sml[1][w][c] * __builtin_amdgcn_exp2f(sml[0][w][c] - mm);
         const float fw = __builtin_amdgcn_exp2f(m[0] - mm);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int j = 0; j < NJ; ++j) o[0][j] *= fw;
+        auto put = [&](int at) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) so[wk][e][j][lane] = o[0][j][e] * fw;
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) so[at][e][j][lane] = o[0][j][e];
+        };
+        if constexpr (WK == 8) {
+            if (wk >= 4) put(wk - 4);
+            __syncthreads();
+            if (wk < 4) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[0][j][e] += so[wk][e][j][lane];
+            }
+            __syncthreads();
+        }
+        if (wk < 4) put(wk);
         __syncthreads();
+        if (wk >= 4) return;
         float x[NJ];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             x[j] = so[0][wk][j][lane];
 #pragma unroll
-            for (int w = 1; w < WK; ++w) x[j] += so[w][wk][j][lane];
+            for (int w = 1; w < 4; ++w) x[j] += so[w][wk][j][lane];
         }
         store(0, wk, x, mm, ll);
     }
@@ -713,8 +731,10 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
 // there too: a thread loads 8 keys x D/32 dimensions and writes, per dimension,
 // its 8 keys as one 16-byte piece, in the order in which the value product's
 // operand wants them.  The next step's rows are loaded to registers while a
-// step is computed.  LDS rows of 16-byte pieces are permuted (piece ^ row) so
-// that neither the writes nor the operand reads meet in a bank.
+// step is computed.  LDS rows of 16-byte pieces are permuted (piece ^ a number
+// from the row) so that the 16 rows of an operand read fall on different banks
+// (64 of 4 bytes here: with a permutation that repeats after 8 rows the reads of
+// 256-byte rows took twice as long).
 //
 // Weights go to f16 as 2^14 p r, r = (value scale of the block) / (largest so
 // far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
@@ -806,11 +826,12 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     const int k_key = t / PIECES % KT, k_ch = t % PIECES;
     const uint32_t k_at = (uint32_t)k_key * k_row + (16 * k_ch < p.dk * ES ? 16 * k_ch : 0);
     // LDS addresses that differ in more than a constant (see stage for the permutation)
-    const int kx = KC >= 8 ? c & 7 : (c >> 1) & 3;
-    int ka[2], va[2][2];
+    auto key_turn = [](int key) { return KC == 16 ? key & 15 : KC == 8 ? (key >> 1) & 7 : (key >> 2) & 3; };
+    int ka[D / 32], va[2][2];
+#pragma unroll
+    for (int n = 0; n < D / 32; ++n) ka[n] = c * D + 8 * ((4 * n + g) ^ key_turn(c));
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        ka[i] = c * D + 8 * ((4 * i + g) ^ kx);
 #pragma unroll
         for (int h = 0; h < 2; ++h) va[h][i] = c * KT + 8 * ((4 * h + g) ^ (c & 7) ^ (c >> 3) ^ (2 * i));
     }
@@ -842,7 +863,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         if (KP > 0 || t < KT * PIECES) {
 #pragma unroll
             for (int n = 0; n < NKP; ++n) {
-                const int key = k_key + n * KSTEP, ch = k_ch, x = KC >= 8 ? k_key & 7 : (k_key >> 1) & 3;    // KSTEP % 8 = 0
+                const int key = k_key + n * KSTEP, ch = k_ch, x = key_turn(k_key);    // KSTEP % 16 = 0
                 f16* row = sk + key * D;
                 if constexpr (KV == KV_F16) {
                     *(int4v*)(row + 8 * (ch ^ x)) = (int4v){(int)kr[n][0], (int)kr[n][1], (int)kr[n][2], (int)kr[n][3]};
@@ -893,7 +914,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         for (int n = 0; n < D / 32; ++n) {
             half8v a[4];
 #pragma unroll
-            for (int kt = 0; kt < 4; ++kt) a[kt] = *(const half8v*)(sk + ka[n & 1] + 16 * kt * D + 64 * (n >> 1));
+            for (int kt = 0; kt < 4; ++kt) a[kt] = *(const half8v*)(sk + ka[n] + 16 * kt * D);
 #pragma unroll
             for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
