@@ -17,10 +17,9 @@
 // the j-th product is dimension c D/16 + j, and a lane ends with runs of D/16
 // consecutive output dimensions.  No LDS but for joining waves.
 //
-// A workgroup is WM x WK waves: WM tiles of 16 QT query rows, WK shares of the
-// keys (joined in LDS at the end).  Where a call has few rows the keys are
-// also split over workgroups, each writing its unnormalised O and (m, l), and
-// dec_join_kernel joins them.
+// A workgroup is four waves with a share of the keys each, joined in LDS at the
+// end.  Where a call has few rows the keys are also split over workgroups, each
+// writing its unnormalised O and (m, l), and dec_join_kernel joins them.
 //
 // 8-bit keys: the int8 go through v_perm into f16 mantissas
 // (0x6400 | (b ^ 0x80) = 1024 + b + 128, minus 1152: exact), the scale of a
@@ -378,15 +377,13 @@ __device__ __forceinline__ void work_of(int bid, const DecAttnParams& p, int mt,
     b = u - split * p.B;
 }
 
-template <int KV, bool QF32, int D, int QT, int WM, int WK, bool TABLE>
-__global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn_kernel(DecAttnParams p) {
+template <int KV, bool QF32, int D, bool TABLE>
+__global__ __launch_bounds__(256, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn_kernel(DecAttnParams p) {
     using TL = Tile<KV, D>;
-    static_assert(WK == 1 || (QT == 1 && WM == 1 && (WK == 4 || WK == 8)), "joined waves: one row tile, four or eight key shares");
     constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
     constexpr int NQ = KV == KV_F32 ? D / 4 : SPLIT ? D / 4 : D / 8;
-    constexpr int NJ = D / 16, ROWS = 16 * QT * WM;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int wm = WK == 1 ? wave : 0, wk = WK == 1 ? 0 : wave;
+    constexpr int NJ = D / 16, WK = 4, ROWS = 16;
+    const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int M = p.n_q * p.G, mt = (M + ROWS - 1) / ROWS;
     int b, kh, split, mtile;
     work_of<TABLE>(blockIdx.x, p, mt, b, kh, split, mtile);
@@ -396,7 +393,7 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
     int cnt = p.q_len ? p.q_len[b] : p.n_q;
     cnt = cnt < 0 ? 0 : cnt > p.n_q ? p.n_q : cnt;
     if (uniform_div(mtile * ROWS, p.G) >= cnt) return;                 // no row of this tile is asked for
-    const int m0 = mtile * ROWS + wm * 16 * QT;
+    const int m0 = mtile * ROWS;
     KeySource s = {};
     s.k_row = (uint32_t)p.k_row * TL::ES;
     s.v_row = (uint32_t)p.v_row * TL::ES;
@@ -433,31 +430,22 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
     }
     s.v_at = (TABLE ? 0 : 4 * g * s.v_row) + (c * NJ < p.dk ? c * NJ : 0) * TL::ES;
 
-    // queries: B operand, column c = row m0 + 16 qt + c
-    uint32_t q[QT][NQ];
-    float qf[QT];        // factor of the scores
-    int lim[QT];         // keys below it are seen
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        const int i = load_query<KV, QF32, D, KV>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt]);
-        lim[qt] = p.causal ? T - cnt + i + 1 : T;
-    }
+    // queries: B operand, column c = row m0 + c
+    uint32_t q[NQ];
+    float qf;            // factor of the scores
+    const int qi = load_query<KV, QF32, D, KV>(p, m0 + c, b, kh, cnt, g, q, qf);
+    const int lim = p.causal ? T - cnt + qi + 1 : T;       // keys below it are seen
 
-    float4v o[QT][NJ];
-    float m[QT], l[QT];
+    float4v o[NJ];
+    float m = kNoMax, l = 0.f;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) {
-        m[qt] = kNoMax;
-        l[qt] = 0.f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) o[qt][j] = (float4v){0.f, 0.f, 0.f, 0.f};
-    }
+    for (int j = 0; j < NJ; ++j) o[j] = (float4v){0.f, 0.f, 0.f, 0.f};
 
     // keys of this wave: every WK-th tile of the workgroup's share, up to the
     // last that one of its rows sees
     int hi = T, all = T;         // (all: keys that every row sees)
     if (p.causal) {
-        const int mi = uniform_div(m0 + 16 * QT - 1, p.G), il = mi < cnt ? mi : cnt - 1;
+        const int mi = uniform_div(m0 + ROWS - 1, p.G), il = mi < cnt ? mi : cnt - 1;
         hi = T - cnt + il + 1 < T ? T - cnt + il + 1 : T;
         all = T - cnt + uniform_div(m0, p.G) + 1;
     }
@@ -486,107 +474,95 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
                 vs8[i] = __shfl(t.vs, r, 64);
             }
         }
-        float alpha[QT], vf[QT];
-        uint32_t ph[QT][4], pl[QT][4];
-        float pf[QT][8];
+        float vf = 1.0f, pf[8];
+        uint32_t ph[4], pl[4];
+        const float4v s0 = tile_scores<KV, D, QF32, NQ>(t.k[0], q);
+        const float4v s1 = tile_scores<KV, D, QF32, NQ>(t.k[1], q);
+        float f = qf;
+        if constexpr (KV == KV_I8 && !TABLE) f *= t.ks;
+        float sc[8];
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            const float4v s0 = tile_scores<KV, D, QF32, NQ>(t.k[0], q[qt]);
-            const float4v s1 = tile_scores<KV, D, QF32, NQ>(t.k[1], q[qt]);
-            float f = qf[qt];
-            if constexpr (KV == KV_I8 && !TABLE) f *= t.ks;
-            float sc[8];
+        for (int e = 0; e < 4; ++e) {
+            sc[e] = s0[e] * f;
+            sc[4 + e] = s1[e] * f;
+            if constexpr (TABLE) {
+                sc[e] *= ks8[e];
+                sc[4 + e] *= ks8[4 + e];
+            }
+        }
+        if (!whole || t0 + 32 > all) {
+            const uint32_t see = keep >> (4 * g) & low_bits(lim - t0 - 4 * g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (!(see & (1u << (e < 4 ? e : 12 + e)))) sc[e] = -INFINITY;
+        }
+        const float mx = fmaxf(m, xgroup_max(max3(max3(sc[0], sc[1], sc[2]), max3(sc[3], sc[4], sc[5]), fmaxf(sc[6], sc[7]))));
+        const float alpha = __builtin_amdgcn_exp2f(m - mx);
+        m = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            pf[e] = __builtin_amdgcn_exp2f(sc[e] - mx);
+            sum += pf[e];
+        }
+        l = l * alpha + sum;
+        if constexpr (KV == KV_I8) {
+            if constexpr (TABLE) {
+                // weights p vs of keys with different scales: divided by
+                // their largest, so that f16 keeps it whatever the scales
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    pf[e] *= vs8[e];
+                    top = fmaxf(top, pf[e]);
+                }
+                top = xgroup_max(top);
+                const float inv = top > 0.f ? 1.0f / top : 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) pf[e] *= inv;
+                vf = top;
+            } else {
+                vf = t.vs;
+            }
+        }
+        if constexpr (SPLIT) {
+            vf *= 0x1p-14f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                sc[e] = s0[e] * f;
-                sc[4 + e] = s1[e] * f;
-                if constexpr (TABLE) {
-                    sc[e] *= ks8[e];
-                    sc[4 + e] *= ks8[4 + e];
-                }
+                const float a = pf[2 * e] * 0x1p14f, bq = pf[2 * e + 1] * 0x1p14f;
+                const f16 ah = (f16)a, bh = (f16)bq;
+                ph[e] = pack_f16((float)ah, (float)bh);
+                pl[e] = pack_f16(a - (float)ah, bq - (float)bh);
             }
-            if (!whole || t0 + 32 > all) {
-                const uint32_t see = keep >> (4 * g) & low_bits(lim[qt] - t0 - 4 * g);
+        } else if constexpr (KV != KV_F32) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!(see & (1u << (e < 4 ? e : 12 + e)))) sc[e] = -INFINITY;
-            }
-            float mx = fmaxf(fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3])), fmaxf(fmaxf(sc[4], sc[5]), fmaxf(sc[6], sc[7])));
-            mx = fmaxf(m[qt], xgroup_max(mx));
-            alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mx);
-            m[qt] = mx;
-            float sum = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                pf[qt][e] = __builtin_amdgcn_exp2f(sc[e] - mx);
-                sum += pf[qt][e];
-            }
-            l[qt] = l[qt] * alpha[qt] + sum;
-            vf[qt] = 1.0f;
-            if constexpr (KV == KV_I8) {
-                if constexpr (TABLE) {
-                    // weights p vs of keys with different scales: divided by
-                    // their largest, so that f16 keeps it whatever the scales
-                    float top = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        pf[qt][e] *= vs8[e];
-                        top = fmaxf(top, pf[qt][e]);
-                    }
-                    top = xgroup_max(top);
-                    const float inv = top > 0.f ? 1.0f / top : 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) pf[qt][e] *= inv;
-                    vf[qt] = top;
-                } else {
-                    vf[qt] = t.vs;
-                }
-            }
-            if constexpr (SPLIT) {
-                vf[qt] *= 0x1p-14f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float a = pf[qt][2 * e] * 0x1p14f, bq = pf[qt][2 * e + 1] * 0x1p14f;
-                    const f16 ah = (f16)a, bh = (f16)bq;
-                    ph[qt][e] = pack_f16((float)ah, (float)bh);
-                    pl[qt][e] = pack_f16(a - (float)ah, bq - (float)bh);
-                }
-            } else if constexpr (KV != KV_F32) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) ph[qt][e] = pack_f16(pf[qt][2 * e], pf[qt][2 * e + 1]);
-            }
+            for (int e = 0; e < 4; ++e) ph[e] = pack_f16(pf[2 * e], pf[2 * e + 1]);
         }
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if constexpr (KV == KV_F32) {
+                float4v acc = o[j] * alpha;
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    float4v acc = o[qt][j] * alpha[qt];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.v[i][j]), pf[qt][i], acc, 0, 0, 0);
-                    o[qt][j] = acc;
-                }
+                for (int i = 0; i < 8; ++i)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(t.v[i][j]), pf[i], acc, 0, 0, 0);
+                o[j] = acc;
             } else {
                 const half8v a = value_frag<KV, D>(t.v, j);
-#pragma unroll
-                for (int qt = 0; qt < QT; ++qt) {
-                    const int4v bi = {(int)ph[qt][0], (int)ph[qt][1], (int)ph[qt][2], (int)ph[qt][3]};
-                    float4v acc = o[qt][j] * alpha[qt];
-                    if constexpr (KV == KV_F16) {
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi), acc, 0, 0, 0);
-                    } else {
-                        float4v blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi),
-                                                                            (float4v){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                        if constexpr (SPLIT) {
-                            const int4v bl = {(int)pl[qt][0], (int)pl[qt][1], (int)pl[qt][2], (int)pl[qt][3]};
-                            blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), blk, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[e] = fmaf(vf[qt], blk[e], acc[e]);
+                const int4v bi = {(int)ph[0], (int)ph[1], (int)ph[2], (int)ph[3]};
+                float4v acc = o[j] * alpha;
+                if constexpr (KV == KV_F16) {
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi), acc, 0, 0, 0);
+                } else {
+                    float4v blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bi),
+                                                                        (float4v){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    if constexpr (SPLIT) {
+                        const int4v bl = {(int)pl[0], (int)pl[1], (int)pl[2], (int)pl[3]};
+                        blk = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, __builtin_bit_cast(half8v, bl), blk, 0, 0, 0);
                     }
-                    o[qt][j] = acc;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[e] = fmaf(vf, blk[e], acc[e]);
                 }
+                o[j] = acc;
             }
         }
     };
@@ -631,13 +607,11 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
         }
     }
 
-    // a lane's sums cover its own keys: join the four groups
-#pragma unroll
-    for (int qt = 0; qt < QT; ++qt) l[qt] = xgroup_sum(l[qt]);
+    l = xgroup_sum(l);       // a lane's sum covers its own keys
 
     // lane (c, g) stores row c, dimensions (4g + e) NJ .. + NJ
-    auto store = [&](int qt, int e, const float* x, float ml, float ll) {
-        const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G), d = (4 * g + e) * NJ;
+    auto store = [&](int e, const float* x, float ml, float ll) {
+        const int mr = m0 + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G), d = (4 * g + e) * NJ;
         if (i >= cnt || d >= p.dk) return;
         if (p.splits > 1) {
             const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
@@ -665,64 +639,34 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
             else *(uint32_t*)y = w[0];
         }
     };
-    if constexpr (WK == 1) {
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float x[NJ];
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) x[j] = o[qt][j][e];
-                store(qt, e, x, m[qt], l[qt]);
-            }
-    } else {
-        // the key shares, brought to a common maximum; of eight, four first add
-        // the others' to theirs; then wave e adds and stores accumulator register
-        // e of all four, in wave order
-        __shared__ float sml[2][WK][16];
-        __shared__ float so[4][4][NJ][64];
-        if (g == 0) {
-            sml[0][wk][c] = m[0];
-            sml[1][wk][c] = l[0];
-        }
-        __syncthreads();
-        float mm = sml[0][0][c], ll = 0.f;
-#pragma unroll
-        for (int w = 1; w < WK; ++w) mm = fmaxf(mm, sml[0][w][c]);
-#pragma unroll
-        for (int w = 0; w < WK; ++w) ll += sml[1][w][c] * __builtin_amdgcn_exp2f(sml[0][w][c] - mm);
-        const float fw = __builtin_amdgcn_exp2f(m[0] - mm);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) o[0][j] *= fw;
-        auto put = [&](int at) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) so[at][e][j][lane] = o[0][j][e];
-        };
-        if constexpr (WK == 8) {
-            if (wk >= 4) put(wk - 4);
-            __syncthreads();
-            if (wk < 4) {
-#pragma unroll
-                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[0][j][e] += so[wk][e][j][lane];
-            }
-            __syncthreads();
-        }
-        if (wk < 4) put(wk);
-        __syncthreads();
-        if (wk >= 4) return;
-        float x[NJ];
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            x[j] = so[0][wk][j][lane];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) x[j] += so[w][wk][j][lane];
-        }
-        store(0, wk, x, mm, ll);
+    // the key shares, brought to a common maximum: wave e adds and stores
+    // accumulator register e of all four, in wave order
+    __shared__ float sml[2][WK][16];
+    __shared__ float so[WK][4][NJ][64];
+    if (g == 0) {
+        sml[0][wk][c] = m;
+        sml[1][wk][c] = l;
     }
+    __syncthreads();
+    float mm = sml[0][0][c], ll = 0.f;
+#pragma unroll
+    for (int w = 1; w < WK; ++w) mm = fmaxf(mm, sml[0][w][c]);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) ll += sml[1][w][c] * __builtin_amdgcn_exp2f(sml[0][w][c] - mm);
+    const float fw = __builtin_amdgcn_exp2f(m - mm);
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) so[wk][e][j][lane] = o[j][e] * fw;
+    __syncthreads();
+    float x[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        x[j] = so[0][wk][j][lane];
+#pragma unroll
+        for (int w = 1; w < WK; ++w) x[j] += so[w][wk][j][lane];
+    }
+    store(wk, x, mm, ll);
 }
 
 // Many query rows against the same keys: 128 rows a workgroup, 32 a wave, the
@@ -739,7 +683,7 @@ __global__ __launch_bounds__(64 * WM * WK, KV != KV_F32 && D <= 64 ? 4 : 1) void
 // Weights go to f16 as 2^14 p r, r = (value scale of the block) / (largest so
 // far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
 // different scales add up in one accumulator, which is rescaled when v grows.
-// Both ride in the exponent: 2^(s - m + 14 + log2 r).
+// 2^14 rides in the exponent, and r too where f16's 11 bits are what is kept.
 template <int KV, bool QF32, int D, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     constexpr int QT = 2, NW = 4, ROWS = 16 * QT * NW, KT = 64;
@@ -1155,10 +1099,16 @@ struct Shape { bool wide; int rows, mt, splits, keys; };
 Shape attn_shape(const DecAttnParams& p) {
     Shape s;
     const int64_t M = (int64_t)p.n_q * p.G, units = (int64_t)p.B * p.Hkv;
-    s.wide = M >= 64 && !p.table;
+    const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
+    // dec_tile_kernel's rows share what they read and convert, but it needs the
+    // chip full of 128-row tiles: by tiles of 16 rows x 32 keys, 512 x 12 run in
+    // 8.7 us on dec_attn_kernel and 11.9 on it, 896 x 12 in 14.2 and 12.3, 512 x 118
+    // in 80 and 40; 8-bit, where lengths differ and rows see part of the keys,
+    // 832 x 34 in 18.3 and 22.8
+    const int64_t work = units * cdiv(M, 16) * tiles;
+    s.wide = p.kv != KV_F32 && !p.table && M >= 64 && work >= (p.kv == KV_F16 ? 10000 : 32000);
     s.rows = s.wide ? 128 : 16;
     s.mt = cdiv(M, s.rows);
-    const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
     const int64_t wgs = units * s.mt;
     int64_t want = wgs >= 512 ? 1 : 512 / wgs;             // about two workgroups per CU
     if (want > 64) want = 64;
@@ -1176,11 +1126,13 @@ Shape attn_shape(const DecAttnParams& p) {
 
 template <int KV, bool QF32, int D, bool TABLE> void launch_shape(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * sh.mt * sh.splits));
-    if (sh.wide) {
-        if constexpr (KV == KV_F32) launch(dec_attn_kernel<KV, QF32, D, 2, 4, 1, false>, grid, dim3(256), 0, s, p);
-        else if (p.causal && KV == KV_I8) launch(dec_tile_kernel<KV, QF32, D, KV == KV_I8>, grid, dim3(256), 0, s, p);
-        else launch(dec_tile_kernel<KV, QF32, D, false>, grid, dim3(256), 0, s, p);
-    } else launch(dec_attn_kernel<KV, QF32, D, 1, 1, 4, TABLE>, grid, dim3(256), 0, s, p);
+    if constexpr (KV != KV_F32 && !TABLE)
+        if (sh.wide) {
+            if (p.causal && KV == KV_I8) launch(dec_tile_kernel<KV, QF32, D, KV == KV_I8>, grid, dim3(256), 0, s, p);
+            else launch(dec_tile_kernel<KV, QF32, D, false>, grid, dim3(256), 0, s, p);
+            return;
+        }
+    launch(dec_attn_kernel<KV, QF32, D, TABLE>, grid, dim3(256), 0, s, p);
 }
 template <int KV, bool QF32, bool TABLE> void launch_width(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     if (p.dk <= 32) launch_shape<KV, QF32, 32, TABLE>(p, sh, s);

@@ -42,6 +42,9 @@ CROSS = [
     ("f16", 2, 17, 70, 2, 2, 80), ("f16", 1, 2, 3001, 2, 1, 64), ("f16", 1, 1, 4096, 1, 1, 128), ("f16", 2, 130, 97, 2, 2, 64),
     ("f16", 1, 65, 300, 4, 1, 128), ("f16", 1, 64, 1, 1, 1, 24), ("f16", 2, 300, 515, 1, 1, 32), ("f16", 1, 200, 130, 2, 2, 128),
     ("f32", 1, 1, 125, 8, 8, 64), ("f32", 3, 4, 33, 4, 2, 128), ("f32", 2, 5, 7, 3, 3, 8), ("f32", 2, 37, 211, 2, 2, 64),
+    # enough rows and keys for the many-row kernel, every head width, rows and keys that end inside a tile
+    ("f16", 3, 130, 300, 48, 24, 64), ("f16", 2, 200, 515, 32, 32, 32), ("f16", 1, 257, 700, 32, 8, 128), ("f16", 2, 150, 430, 40, 40, 80),
+    ("f16", 1, 200, 3000, 16, 2, 40),
     # no keys at all
     ("f16", 2, 3, 0, 2, 1, 64), ("f16", 1, 70, 0, 1, 1, 64), ("f32", 2, 3, 0, 2, 1, 64), ("f32", 1, 70, 0, 1, 1, 32),
     ("f32", 1, 2, 2048, 2, 1, 32), ("f32", 1, 3, 900, 2, 2, 128), ("f32", 2, 130, 97, 2, 2, 80), ("f32", 1, 70, 64, 4, 1, 128),
@@ -113,19 +116,19 @@ def test_cross_attention_strides_and_streams(gpu, stream):
             check_attention(got[0][b, h, :, 8:8 + d], want, True, d, f"strides b{b} h{h}")
 
 
-@pytest.mark.parametrize("type,nq,d", [("f16", 5, 64), ("f16", 80, 64), ("f32", 5, 64), ("f32", 80, 128)])
+@pytest.mark.parametrize("type,H,nq,nk,d", [("f16", 2, 5, 75, 64), ("f16", 64, 330, 250, 64), ("f32", 2, 5, 75, 64), ("f32", 2, 80, 75, 128)])
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
-def test_cross_attention_scales(gpu, stream, type, nq, d, scale):
+def test_cross_attention_scales(gpu, stream, type, H, nq, nk, d, scale):
     """Any factor: negative, zero (the mean of the kept values), large, with keys left out."""
     rng = np.random.default_rng(nq)
     dt = np.float16 if type == "f16" else np.float32
-    q, k, v = (rng.standard_normal((1, n, 2, d)).astype(dt) for n in (nq, 75, 75))
-    mask = (rng.random((1, 75)) < 0.7).astype(np.uint8)
+    q, k, v = (rng.standard_normal((1, n, H, d)).astype(dt) for n in (nq, nk, nk))
+    mask = (rng.random((1, nk)) < 0.7).astype(np.uint8)
     out = gpu.DeviceArray(q.shape, dt)
     gpu.CrossAttention(*(dev(gpu, x, stream) for x in (q, k, v)), out, k_mask=dev(gpu, mask, stream), scale=scale)(stream)
     got = out.numpy(stream)
-    for h in range(2):
-        want = ref.attention(q[0, :, h], k[0, :, h], v[0, :, h], scale, np.broadcast_to(mask[0] != 0, (nq, 75)))
+    for h in (0, H - 1):
+        want = ref.attention(q[0, :, h], k[0, :, h], v[0, :, h], scale, np.broadcast_to(mask[0] != 0, (nq, nk)))
         check_attention(got[0, :, h], want, type == "f16", d, f"scale {scale} h{h}")
 
 
@@ -212,6 +215,10 @@ CACHE = [
     ("f32", 1, 1, 8, 8, 64, 18, True, False), ("f32", 6, 1, 4, 4, 128, 100, True, True), ("f32", 2, 70, 2, 1, 64, 200, True, False),
     # many rows over few keys: a weight's two f16 terms that do not add up to it are seen
     ("f32", 4, 128, 8, 8, 64, 48, False, False),
+    # the many-row kernel: causal and not, every head width, keys split and whole
+    ("f16", 6, 200, 16, 16, 64, 900, True, False), ("f16", 6, 257, 16, 16, 32, 650, False, False), ("f16", 6, 150, 32, 16, 128, 715, True, False),
+    ("f16", 6, 130, 32, 8, 80, 1000, False, False), ("f32", 6, 200, 16, 16, 64, 900, True, False), ("f32", 6, 257, 16, 16, 32, 650, True, False),
+    ("f32", 6, 150, 32, 16, 128, 715, False, False), ("f32", 6, 600, 16, 16, 16, 333, True, False),
     ("f32", 1, 3, 2, 1, 32, 3000, True, False), ("f32", 3, 5, 2, 2, 16, 64, False, False), ("f32", 2, 80, 2, 2, 80, 111, True, True),
 ]
 
