@@ -362,7 +362,8 @@ int pkx_quantize_gguf(const char* in_path, const char* out_path, int gtype, int*
  * Strides are in elements (item, row, head; the d_head elements are adjacent), those of
  * k and v not negative and below 2^22 between rows.  d_head: a multiple of 8 up to 128;
  * buffers 16-byte aligned, strides multiples of 16 bytes; n_heads a multiple of
- * n_kv_heads; n_k at most 2^30, n_items x n_q x n_heads below 2^22.  out overlaps no input. */
+ * n_kv_heads; n_k at most 2^30, n_items x n_q x n_heads below 2^22; scale finite.  out overlaps no input,
+ * and its rows do not overlap each other: each of its strides is at least what the smaller ones span. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of q, k, v and out */
     int n_items, n_q, n_k;
@@ -382,7 +383,7 @@ int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void
 
 /* A key/value cache in 8 bits: n_slots sequences of up to `capacity` tokens (a multiple
  * of PKX_CACHE8_BLOCK).  A block of PKX_CACHE8_BLOCK tokens of one slot and head has one
- * scale; an element is k * k_scale.  d_head: a multiple of 16 up to 128; 16-byte aligned. */
+ * scale; an element is k * k_scale, and scales are finite and not negative.  d_head: a multiple of 16 up to 128; 16-byte aligned. */
 #define PKX_CACHE8_BLOCK 32
 typedef struct {
     int n_slots, n_kv_heads, d_head, capacity;
@@ -463,7 +464,7 @@ int pkx_beam_select(const pkx_beam_select_args* a, void* ws, size_t ws_bytes, vo
 /* Reordering: row b * n_beams + w of every dst = row b * n_beams + parent[b][w] of its src, `bytes` of it
  * (prediction-network states, cache tables, ...); rows whose parent is out of range are left as they were.
  * states: host array of at most PKX_BEAM_MAX_STATES; row strides in bytes, at least `bytes` (src: or 0).
- * No src, from its first row to its last, overlaps a dst. */
+ * No src, from its first row to its last, overlaps a dst, and no row of a dst another dst's. */
 #define PKX_BEAM_MAX_STATES 32
 typedef struct {
     const void* src;

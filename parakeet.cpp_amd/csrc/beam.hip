@@ -626,7 +626,6 @@ void launch_beam_reorder(const int* parent, int B, int W, const BeamState* state
         ++p.n;
     }
     if (p.n == 0) return;
-    require(p.rows < (1 << 23), "beam reorder: too many rows for one call");
     int64_t z = (most + 1023) / 1024;                        // four pieces a thread
     z = z > 64 ? 64 : z;
     launch(reorder_kernel, dim3((unsigned)p.rows, p.n, (unsigned)z), dim3(256), 0, s, p);

@@ -151,18 +151,19 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int
 
 void launch_cache8_append(const CacheAppendParams& p, hipStream_t s) {
     if (p.R == 0 || p.n_new == 0) return;
-    const int blocks = (p.n_new + kCacheBlock - 2) / kCacheBlock + 1;     // wherever the first token falls in its block
-    const int64_t x = (int64_t)p.R * blocks;
+    const int64_t blocks = ((int64_t)p.n_new + kCacheBlock - 2) / kCacheBlock + 1;     // wherever the first token falls in its block
+    const int64_t x = p.R * blocks;
     require(x < (1 << 22) && p.c.Hkv <= 65535, "cache append: at most 2^22 blocks of 32 tokens in one call");
     const dim3 grid((unsigned)x, p.c.Hkv, 2);
-    if (p.f32) launch(cache8_append_kernel<true>, grid, dim3(256), 0, s, p, blocks);
-    else launch(cache8_append_kernel<false>, grid, dim3(256), 0, s, p, blocks);
+    if (p.f32) launch(cache8_append_kernel<true>, grid, dim3(256), 0, s, p, (int)blocks);
+    else launch(cache8_append_kernel<false>, grid, dim3(256), 0, s, p, (int)blocks);
 }
 
 void launch_cache8_read(const CacheReadParams& p, hipStream_t s) {
-    const int64_t per = (int64_t)p.n * p.c.Hkv * (p.c.dk / 8);
-    if (p.R == 0 || per == 0 || (!p.k && !p.v)) return;
-    const int64_t chunks = (per + 255) / 256;
+    if (p.R == 0 || p.n == 0 || (!p.k && !p.v)) return;
+    // (in f64: no product of the sizes that a call may name wraps)
+    require((double)p.R * p.n * p.c.Hkv < (double)(1 << 30), "cache read: at most 2^30 rows of d_head values in one call");
+    const int64_t per = (int64_t)p.n * p.c.Hkv * (p.c.dk / 8), chunks = (per + 255) / 256;
     require(p.R * chunks < (1 << 22), "cache read: at most 2^33 values in one call");
     launch(cache8_read_kernel, dim3((unsigned)(p.R * chunks)), dim3(256), 0, s, p, (int)per, (int)chunks);
 }

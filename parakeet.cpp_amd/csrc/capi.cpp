@@ -1,9 +1,12 @@
 // extern "C" boundary (include/pkx.h).  Every entry point catches all C++
 // exceptions and reports them through a thread-local last-error string, the
 // same no-throw convention as the reference C API (src/parakeet_capi.cpp:207-225).
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
 
 #include "../../include/pkx.h"
 #include "decoder.hpp"
@@ -150,9 +153,22 @@ bool is_f32(int type, const char* what) {
     return type == PKX_TYPE_F32;
 }
 
-// Rows of an output that do not run into each other.
+// Rows of an output that do not run into each other: each stride at least what the
+// smaller ones span.
 void need_apart(int64_t a, int64_t na, int64_t b, int64_t nb, int64_t c, int64_t nc, int64_t row, const char* what) {
-    need((na <= 1 || a >= row) && (nb <= 1 || b >= row) && (nc <= 1 || c >= row), what);
+    std::pair<int64_t, int64_t> dim[3] = {{a, na}, {b, nb}, {c, nc}};
+    std::sort(dim, dim + 3);
+    double span = (double)row;
+    for (const auto& [stride, n] : dim) {
+        if (n <= 1) continue;
+        need((double)stride >= span, what);
+        span += (double)stride * (double)(n - 1);
+    }
+}
+
+// What the kernels' 32-bit indexes hold; in f64, where no product of sizes wraps.
+void need_rows(int items, int n_q, int heads) {
+    need((double)items * n_q * heads < (double)(1 << 22), "attention: at most 2^22 rows x heads in one call");
 }
 
 // A strided operand read or written in 16-byte pieces.
@@ -179,6 +195,9 @@ pkx::DecAttnParams cross_params(const pkx_cross_attn* a) {
     p.Hkv = a->n_kv_heads;
     p.G = a->n_heads / a->n_kv_heads;
     p.dk = a->d_head;
+    need_rows(a->n_items, a->n_q, a->n_heads);
+    need(std::isfinite(a->scale * 2.0f), "cross attention: scale is not finite");
+    need(!a->k_mask || a->k_mask_item >= 0, "cross attention: negative stride of k_mask");
     p.scale = a->scale;
     p.q = a->q; p.q_item = a->q_item; p.q_row = a->q_row; p.q_head = a->q_head;
     p.k = a->k; p.k_item = a->k_item; p.k_row = a->k_row; p.k_head = a->k_head;
@@ -227,6 +246,8 @@ pkx::DecAttnParams cache_attn_params(const pkx_cache8* c, const pkx_cache8_attn*
     p.Hkv = o.Hkv;
     p.G = a->n_heads / o.Hkv;
     p.dk = o.dk;
+    need_rows(a->n_rows, a->n_q, a->n_heads);
+    need(std::isfinite(a->scale * 2.0f), "cache attention: scale is not finite");
     p.scale = a->scale;
     p.causal = a->causal != 0;
     p.q = a->q; p.q_item = a->q_row; p.q_row = a->q_tok; p.q_head = a->q_head;
@@ -824,6 +845,7 @@ int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_
         need(n_states >= 0 && n_states <= pkx::kMaxBeamStates, "beam reorder: at most PKX_BEAM_MAX_STATES states");
         if (n_items == 0 || n_states == 0) return;
         need(parent && states, "null argument");
+        need((double)n_items * n_beams < (double)(1 << 23), "beam reorder: too many rows for one call");
         pkx::BeamState p[pkx::kMaxBeamStates];
         const int64_t rows = (int64_t)n_items * n_beams;
         for (int i = 0; i < n_states; ++i) {

@@ -144,6 +144,30 @@ def test_beam_refusals():
     assert [x.strip() for x in out[22:]] == ["0"] * 2
 
 
+def test_refusals_of_values_and_of_sizes_whose_products_wrap():
+    """A scale that is not finite, rows of an output that lie in each other, and sizes whose products pass 64 bits."""
+    out = _run("""
+        top = (1 << 31) - 1
+        for kw in (dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=3e38), dict(k_mask=A, k_mask_item=-1),
+                   dict(out_item=64, out_row=64, out_head=64), dict(out_item=256, out_row=256, out_head=64), dict(out_row=192),
+                   dict(n_items=top, n_q=top, n_heads=top, n_kv_heads=top, out_item=1 << 62, out_row=1 << 40)):
+            said(L.pkx_cross_attention(cross(**kw), None, 0, None))
+        n = C.c_size_t()
+        said(L.pkx_cross_attention_workspace(cross(n_items=top, n_q=top, n_heads=top, n_kv_heads=top), C.byref(n)))
+        for kw in (dict(scale=float("nan")), dict(out_row=64, out_tok=64, out_head=64)):
+            said(L.pkx_cache8_attention(cache(), attn(n_q=2, **kw), None, 0, None))
+        said(L.pkx_cache8_append(cache(), toks(n_rows=1, n_new=top), None))
+        said(L.pkx_cache8_read(cache(), top, top, A, A, A, A, None))
+        said(L.pkx_cache8_read(cache(n_kv_heads=top, n_slots=1), 1, top, A, A, A, A, None))
+        said(L.pkx_beam_reorder(A, top, top, (pkx.BeamState * 1)(pkx.BeamState(A, A, 1 << 60, 1 << 60, 16)), 1, None))
+    """)
+    words = ["scale", "scale", "scale", "k_mask", "overlap", "overlap", "overlap", "2^22", "2^22", "scale", "overlap", "2^22", "2^30",
+             "2^30", "too many"]
+    assert len(out) == len(words)
+    for line, w in zip(out, words):
+        assert line.startswith("1 ") and w in line, (line, w)
+
+
 def test_workspace_follows_the_sizes():
     """No workspace where the rows fill the chip; with few rows and many keys partial sums for every split."""
     out = _run("""
