@@ -467,11 +467,12 @@ __global__ __launch_bounds__(256, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn
         }
         float ks8[8], vs8[8];
         if constexpr (TABLE) {
+            const float kept_vs = t.ok ? t.vs : 0.f;       // (of a key left out: anything, NaN too)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int r = (i < 4 ? 0 : 12) + 4 * g + i;
                 ks8[i] = __shfl(t.ks, r, 64);
-                vs8[i] = __shfl(t.vs, r, 64);
+                vs8[i] = __shfl(kept_vs, r, 64);
             }
         }
         float vf = 1.0f, pf[8];
@@ -499,37 +500,43 @@ __global__ __launch_bounds__(256, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn
         const float mx = fmaxf(m, xgroup_max(max3(max3(sc[0], sc[1], sc[2]), max3(sc[3], sc[4], sc[5]), fmaxf(sc[6], sc[7]))));
         const float alpha = __builtin_amdgcn_exp2f(m - mx);
         m = mx;
+        // weights, and so l and O, are 2^14 p where they go to f16: down to 2^-28
+        // of the largest they keep its 11 bits, then 2^-39 of it
+        const float off = KV == KV_F32 ? mx : mx - 14.0f;
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            pf[e] = __builtin_amdgcn_exp2f(sc[e] - mx);
+            pf[e] = __builtin_amdgcn_exp2f(sc[e] - off);
             sum += pf[e];
         }
         l = l * alpha + sum;
         if constexpr (KV == KV_I8) {
             if constexpr (TABLE) {
-                // weights p vs of keys with different scales: divided by
-                // their largest, so that f16 keeps it whatever the scales
-                float top = 0.f;
+                // weights p vs of keys with different scales: their largest
+                // becomes 2^14, so that f16 keeps it whatever the scales (a largest
+                // below 2^-110 is as good as none, and its inverse would not be finite)
+                float top = 0x1p-110f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     pf[e] *= vs8[e];
                     top = fmaxf(top, pf[e]);
                 }
                 top = xgroup_max(top);
-                const float inv = top > 0.f ? 1.0f / top : 0.f;
+                const float inv = 0x1p14f / top;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] *= inv;
-                vf = top;
+                vf = top * 0x1p-14f;
             } else {
                 vf = t.vs;
             }
         }
         if constexpr (SPLIT) {
-            vf *= 0x1p-14f;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float a = pf[2 * e] * 0x1p14f, bq = pf[2 * e + 1] * 0x1p14f;
+                float a = pf[2 * e], bq = pf[2 * e + 1];
+                // the products as rounded here: fused into the conversions, the two
+                // uses of hi below could differ by one of its steps
+                if constexpr (TABLE) asm("" : "+v"(a), "+v"(bq));
                 const f16 ah = (f16)a, bh = (f16)bq;
                 ph[e] = pack_f16((float)ah, (float)bh);
                 pl[e] = pack_f16(a - (float)ah, bq - (float)bh);
@@ -1153,8 +1160,6 @@ size_t dec_attention_workspace(const DecAttnParams& p) {
 void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_t s) {
     if (p.B == 0 || p.n_q == 0) return;
     const Shape sh = attn_shape(p);
-    require((int64_t)p.B * p.Hkv * sh.mt * sh.splits < (1 << 22) && (int64_t)p.B * p.Hkv * p.n_q * p.G < (1 << 22),
-            "attention: at most 2^22 rows x heads in one call");
     const size_t need = dec_attention_workspace(p);
     require(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need),
             "attention: the workspace is smaller than its size query says, or not 16-byte aligned");
@@ -1163,8 +1168,8 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     p.split_keys = sh.keys;
     if (need) {
         const size_t parts = (size_t)p.B * p.Hkv * p.n_q * p.G * sh.splits;
-        p.part_ml = (float2*)ws;
-        p.part_o = (float*)((char*)ws + parts * sizeof(float2));
+        p.part_o = (float*)ws;
+        p.part_ml = (float2*)(p.part_o + parts * p.dk);
     }
     if (p.kv == KV_F16) launch_width<KV_F16, false, false>(p, sh, s);
     else if (p.kv == KV_F32) launch_width<KV_F32, true, false>(p, sh, s);

@@ -269,6 +269,83 @@ def test_cache_attention(gpu, stream, type, R, nq, H, Hkv, d, n, causal, table):
             check_attention(got[r, :m, h], want, type == "f16", d, f"cache r{r} h{h}")
 
 
+@pytest.mark.parametrize("type", ["f16", "f32"])
+def test_cache_attention_unused_slots_may_hold_anything(gpu, stream, type):
+    """Positions whose table entry is out of range, with NaN scales in every slot and block that no entry names."""
+    rng = np.random.default_rng(3)
+    S, H, cap, d, n = 4, 2, 160, 64, 150
+    c = HostCache(gpu, stream, S, H, cap, d, rng)
+    tab = np.full((2, n), 1, np.int32)
+    tab[:, 70:] = 2
+    tab[0, ::3], tab[1, 32:64], tab[1, 140:] = -1, S, 1 << 30
+    for a in (c.ks, c.vs):
+        a[[0, 3]], a[1, :, 3:], a[2, :, :2] = NAN, NAN, NAN
+    c.dev.k_scale.upload(c.ks, stream)
+    c.dev.v_scale.upload(c.vs, stream)
+    dt = np.float16 if type == "f16" else np.float32
+    q = rng.standard_normal((2, 1, H, d)).astype(dt)
+    out = gpu.DeviceArray(q.shape, dt)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n, n]), stream), max_len=n, table=dev(gpu, tab, stream))(stream)
+    got = out.numpy(stream)
+    for r in range(2):
+        ok = (tab[r] >= 0) & (tab[r] < S)
+        K, V = (np.nan_to_num(ref.values(x, y, np.where(ok, tab[r], 0), np.arange(n))) for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        for h in range(H):
+            want = ref.attention(q[r, :, h], K[:, h], V[:, h], d ** -0.5, ok[None])
+            check_attention(got[r, :, h], want, type == "f16", d, f"r{r} h{h}")
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("table", [False, True])
+def test_cache_attention_weights_near_nothing(gpu, stream, type, table):
+    """Blocks whose weights run from 1 down to below the least normal f32: what is added for them is finite."""
+    rng = np.random.default_rng(4)
+    d, n = 16, 32 * 24
+    c = HostCache(gpu, stream, 1, 1, n, d, rng)
+    c.k[:] = 0
+    c.k[0, 0, :, 0] = 100 - np.arange(n) // 32 * 8       # block b: scores of 8 (12 - b) + a little, in units of log 2
+    c.k[0, 0, :, 1] = np.arange(n) % 3
+    c.ks[:] = 1
+    c.vs[:] = 1e-3
+    c.dev.k.upload(c.k, stream)
+    c.dev.k_scale.upload(c.ks, stream)
+    c.dev.v_scale.upload(c.vs, stream)
+    dt = np.float16 if type == "f16" else np.float32
+    q = np.zeros((1, 1, 1, d), dt)
+    q[..., :2] = np.log(2), 0.125
+    out = gpu.DeviceArray(q.shape, dt)
+    extra = dict(table=dev(gpu, np.zeros((1, n), np.int32), stream)) if table else {}
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n]), stream), scale=1.0, **extra)(stream)
+    K, V = (ref.values(x, y, np.zeros(n, int), np.arange(n))[:, 0] for x, y in ((c.k, c.ks), (c.v, c.vs)))
+    check_attention(out.numpy(stream)[0, :, 0], ref.attention(q[0, :, 0], K, V, 1.0, np.ones((1, n), bool)), type == "f16", d, "near nothing")
+
+
+@pytest.mark.parametrize("kind", ["cross", "cache"])
+def test_many_small_weights_are_kept(gpu, stream, kind):
+    """One key far above 20000 others of weight 100.5 x 2^-24 each: rounded to f16 as they are they would be 0.5% off
+    together; scaled into its normal range they are off by at most half a step, 2^-11, and the output by another."""
+    n, d = 20032, 16
+    s0 = float(-np.log2(100.5 * 2.0 ** -24))
+    k, v = np.zeros((1, n, 1, d), np.float32), np.ones((1, n, 1, d), np.float32)
+    k[0, 0, 0, 0], v[0, 0] = 1, 0
+    out = gpu.DeviceArray((1, 1, 1, d), np.float16)
+    q = np.zeros((1, 1, 1, d), np.float16)
+    q[..., 0] = 16
+    scale = s0 * np.log(2) / 16
+    if kind == "cross":
+        gpu.CrossAttention(dev(gpu, q, stream), *(dev(gpu, x.astype(np.float16), stream) for x in (k, v)), out, scale=scale)(stream)
+    else:
+        c = gpu.Cache8(1, 1, d, n)
+        gpu.CacheAppend(c, dev(gpu, k, stream), dev(gpu, v, stream), start=dev(gpu, i32([0]), stream))(stream)
+        gpu.CacheAttention(c, dev(gpu, q, stream), out, dev(gpu, i32([n]), stream), scale=scale)(stream)
+    rest = (n - 1) * 2.0 ** -s0
+    want = rest / (1 + rest)
+    # (a factor of 2^-24 relative in f32 moves the score of 17.3 by 2e-6 nats: nothing beside 2^-11)
+    err = np.abs(out.numpy(stream).astype(np.float64) - want).max()
+    print(f"[{kind}] error {err:.2e} of {want:.4f}", flush=True)
+    assert err <= 2.0 ** -10 * want
+
+
 def test_cache_far_slots(gpu, stream):
     """A slot, and a position, whose byte offset passes 2^32."""
     rng = np.random.default_rng(8)
