@@ -697,7 +697,6 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     constexpr bool SPLIT = KV == KV_I8 && QF32;
     constexpr int ES = KV == KV_F16 ? 2 : 1, NQ = SPLIT ? D / 4 : D / 8, NJ = D / 16;
     constexpr int PIECES = D * ES / 16, KP = KT * PIECES / 256;     // 16-byte pieces of a key row; of a thread
-    constexpr int NKP = KP > 0 ? KP : 1;
     constexpr int DV = D / 32;                                      // value dimensions of a thread
     constexpr int KC = D / 8;                                       // 16-byte pieces of a key row in LDS
     constexpr int JB = NJ < 4 ? NJ : 4;                             // value products in flight
@@ -767,14 +766,14 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     }
 
     // the step in flight
-    uint32_t kr[NKP][4], vr[8][DV * ES / 4 > 0 ? DV * ES / 4 : 1];
+    uint32_t kr[KP][4], vr[8][DV * ES > 4 ? DV * ES / 4 : 1];
     uint32_t mr8 = 1;
     float ksr[2] = {1.f, 1.f}, vsr[2] = {1.f, 1.f};
     const int oct = t >> 5, d0 = (t & 31) * DV;            // value work: keys of octet oct, dimensions d0 .. d0 + DV
     const int v_key = 32 * (oct >> 2) + 4 * (oct & 3);
     const uint32_t v_at = (uint32_t)v_key * v_row + (d0 < p.dk ? d0 : 0) * ES;
     constexpr int KSTEP = 256 / PIECES;                    // key work: piece k_ch of keys k_key + n KSTEP
-    const int k_key = t / PIECES % KT, k_ch = t % PIECES;
+    const int k_key = t / PIECES, k_ch = t % PIECES;
     const uint32_t k_at = (uint32_t)k_key * k_row + (16 * k_ch < p.dk * ES ? 16 * k_ch : 0);
     // LDS addresses that differ in more than a constant (see stage for the permutation)
     auto key_turn = [](int key) { return KC == 16 ? key & 15 : KC == 8 ? (key >> 1) & 7 : (key >> 2) & 3; };
@@ -801,34 +800,31 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const auto kt = step_rsrc(kb + (int64_t)t0 * k_row, rows * k_row + p.dk * ES);
         const auto vt = step_rsrc(vb + (int64_t)t0 * v_row, rows * v_row + p.dk * ES);
 #pragma unroll
-        for (int n = 0; n < NKP; ++n) buffer_words(kr[n], kt, k_at + n * KSTEP * k_row);
+        for (int n = 0; n < KP; ++n) buffer_words(kr[n], kt, k_at + n * KSTEP * k_row);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t at = v_at + (i < 4 ? i : 12 + i) * v_row;
-            if constexpr (DV * ES == 1) vr[i][0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(vt, at, 0, 0);
-            else if constexpr (DV * ES == 2) vr[i][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vt, at, 0, 0);
+            if constexpr (DV * ES == 2) vr[i][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vt, at, 0, 0);
             else buffer_words(vr[i], vt, at);
         }
     };
     auto stage = [&](uint64_t keep) {
-        if (KP > 0 || t < KT * PIECES) {
 #pragma unroll
-            for (int n = 0; n < NKP; ++n) {
-                const int key = k_key + n * KSTEP, ch = k_ch, x = key_turn(k_key);    // KSTEP % 16 = 0
-                f16* row = sk + key * D;
-                if constexpr (KV == KV_F16) {
-                    *(int4v*)(row + 8 * (ch ^ x)) = (int4v){(int)kr[n][0], (int)kr[n][1], (int)kr[n][2], (int)kr[n][3]};
-                } else {
+        for (int n = 0; n < KP; ++n) {
+            const int key = k_key + n * KSTEP, ch = k_ch, x = key_turn(k_key);    // KSTEP % 16 = 0
+            f16* row = sk + key * D;
+            if constexpr (KV == KV_F16) {
+                *(int4v*)(row + 8 * (ch ^ x)) = (int4v){(int)kr[n][0], (int)kr[n][1], (int)kr[n][2], (int)kr[n][3]};
+            } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        int4v w;
+                for (int h = 0; h < 2; ++h) {
+                    int4v w;
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            w[2 * e] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c010c00));
-                            w[2 * e + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c030c02));
-                        }
-                        *(int4v*)(row + 8 * ((2 * ch + h) ^ x)) = w;
+                    for (int e = 0; e < 2; ++e) {
+                        w[2 * e] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c010c00));
+                        w[2 * e + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, kr[n][2 * h + e], 0x0c030c02));
                     }
+                    *(int4v*)(row + 8 * ((2 * ch + h) ^ x)) = w;
                 }
             }
         }
@@ -1103,18 +1099,12 @@ template <bool F32> __global__ __launch_bounds__(256) void dec_join_rows_kernel(
 
 // Rows a workgroup takes and how many ways the keys are split over workgroups.
 struct Shape { bool wide; int rows, mt, splits, keys; };
-Shape attn_shape(const DecAttnParams& p) {
+Shape split_shape(const DecAttnParams& p, bool wide) {
     Shape s;
     const int64_t M = (int64_t)p.n_q * p.G, units = (int64_t)p.B * p.Hkv;
     const int tiles = cdiv(p.n_k > 0 ? p.n_k : 1, 32);
-    // dec_tile_kernel's rows share what they read and convert, but it needs the
-    // chip full of 128-row tiles: by tiles of 16 rows x 32 keys, 512 x 12 run in
-    // 8.7 us on dec_attn_kernel and 11.9 on it, 896 x 12 in 14.2 and 12.3, 512 x 118
-    // in 80 and 40; 8-bit, where lengths differ and rows see part of the keys,
-    // 832 x 34 in 18.3 and 22.8
-    const int64_t work = units * cdiv(M, 16) * tiles;
-    s.wide = p.kv != KV_F32 && !p.table && M >= 64 && work >= (p.kv == KV_F16 ? 10000 : 32000);
-    s.rows = s.wide ? 128 : 16;
+    s.wide = wide;
+    s.rows = wide ? 128 : 16;
     s.mt = cdiv(M, s.rows);
     const int64_t wgs = units * s.mt;
     int64_t want = wgs >= 512 ? 1 : 512 / wgs;             // about two workgroups per CU
@@ -1124,16 +1114,36 @@ Shape attn_shape(const DecAttnParams& p) {
     // rounds (of about 0.5 us; f32 heads above 64 one round, of 2 us) or eight steps
     // (1 us), four where there are few rows to join
     int per = (cdiv(tiles, want) + 3) / 4 * 4;
-    const int least = p.kv == KV_F32 && p.dk > 64 ? 4 : s.wide && units * M <= 1024 ? 8 : 16;
+    const int least = p.kv == KV_F32 && p.dk > 64 ? 4 : wide && units * M <= 1024 ? 8 : 16;
     if (per < least) per = least;
     s.splits = cdiv(tiles, per);
     s.keys = per * 32;
     return s;
 }
+Shape attn_shape(const DecAttnParams& p) {
+    // dec_tile_kernel's rows share what they read and convert, but its time goes by
+    // the steps of a workgroup, however few workgroups there are and rows they have.
+    // By tiles of 16 rows x 32 keys, 16 of them a full step, f16:
+    //   tiles  steps x rounds   16-row form   128-row form, us
+    //    3328        2               8.7           7.0    (d_head 64: 8 items x 8 heads x 200 rows, 128 keys)
+    //    6656        4              11.7           9.3    (256 keys)
+    //    6144        6               9.0          12.0    (16 x 8 x 64 rows, 375 keys)
+    //    9984        6              22.1          17.7    (d_head 128: 8 x 8 x 200 rows, 375 keys)
+    //    4608        8              11.8          20.2    (4 x 8 x 130 rows, 500 keys)
+    // 8-bit keys (where rows see part of the keys and lengths differ): with d_head 64
+    // no gain in most (37.6 against 44.1 at 112896 tiles, 119 against 120 at 448000), with
+    // 128 40.3 against 41.0 at 54912, 232 against 165 at 448000.
+    const int64_t M = (int64_t)p.n_q * p.G;
+    if (p.kv == KV_F32 || p.table || M < 64) return split_shape(p, false);
+    const Shape wide = split_shape(p, true);
+    const int64_t units = (int64_t)p.B * p.Hkv, tiles = units * cdiv(M, 16) * cdiv(p.n_k, 32);
+    const int64_t steps = (int64_t)(p.n_k < wide.keys ? cdiv(p.n_k, 64) : wide.keys / 64) * cdiv(units * wide.mt * wide.splits, 256);
+    return (p.kv == KV_F16 ? steps > 0 && tiles >= 1500 * steps : p.dk > 64 && tiles >= 60000) ? wide : split_shape(p, false);
+}
 
 template <int KV, bool QF32, int D, bool TABLE> void launch_shape(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)p.B * p.Hkv * sh.mt * sh.splits));
-    if constexpr (KV != KV_F32 && !TABLE)
+    if constexpr (KV == KV_F16 || (KV == KV_I8 && D > 64 && !TABLE))
         if (sh.wide) {
             if (p.causal && KV == KV_I8) launch(dec_tile_kernel<KV, QF32, D, KV == KV_I8>, grid, dim3(256), 0, s, p);
             else launch(dec_tile_kernel<KV, QF32, D, false>, grid, dim3(256), 0, s, p);

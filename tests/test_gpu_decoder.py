@@ -43,7 +43,7 @@ CROSS = [
     ("f16", 1, 65, 300, 4, 1, 128), ("f16", 1, 64, 1, 1, 1, 24), ("f16", 2, 300, 515, 1, 1, 32), ("f16", 1, 200, 130, 2, 2, 128),
     ("f32", 1, 1, 125, 8, 8, 64), ("f32", 3, 4, 33, 4, 2, 128), ("f32", 2, 5, 7, 3, 3, 8), ("f32", 2, 37, 211, 2, 2, 64),
     # enough rows and keys for the many-row kernel, every head width, rows and keys that end inside a tile
-    ("f16", 3, 130, 300, 48, 24, 64), ("f16", 2, 200, 515, 32, 32, 32), ("f16", 1, 257, 700, 32, 8, 128), ("f16", 2, 150, 430, 40, 40, 80),
+    ("f16", 3, 130, 300, 48, 24, 64), ("f16", 2, 200, 515, 32, 32, 32), ("f16", 1, 257, 700, 36, 9, 128), ("f16", 2, 150, 430, 40, 40, 80),
     ("f16", 1, 200, 3000, 16, 2, 40),
     # no keys at all
     ("f16", 2, 3, 0, 2, 1, 64), ("f16", 1, 70, 0, 1, 1, 64), ("f32", 2, 3, 0, 2, 1, 64), ("f32", 1, 70, 0, 1, 1, 32),
@@ -215,10 +215,10 @@ CACHE = [
     ("f32", 1, 1, 8, 8, 64, 18, True, False), ("f32", 6, 1, 4, 4, 128, 100, True, True), ("f32", 2, 70, 2, 1, 64, 200, True, False),
     # many rows over few keys: a weight's two f16 terms that do not add up to it are seen
     ("f32", 4, 128, 8, 8, 64, 48, False, False),
-    # the many-row kernel: causal and not, every head width, keys split and whole
-    ("f16", 6, 200, 16, 16, 64, 900, True, False), ("f16", 6, 257, 16, 16, 32, 650, False, False), ("f16", 6, 150, 32, 16, 128, 715, True, False),
-    ("f16", 6, 130, 32, 8, 80, 1000, False, False), ("f32", 6, 200, 16, 16, 64, 900, True, False), ("f32", 6, 257, 16, 16, 32, 650, True, False),
-    ("f32", 6, 150, 32, 16, 128, 715, False, False), ("f32", 6, 600, 16, 16, 16, 333, True, False),
+    # the many-row kernel: causal and not, keys split and whole; sizes just short of it
+    ("f16", 6, 150, 32, 16, 128, 1100, True, False), ("f16", 6, 130, 32, 8, 80, 1230, False, False),
+    ("f32", 6, 150, 32, 16, 128, 1100, False, False), ("f32", 6, 130, 32, 8, 112, 1230, True, False),
+    ("f16", 6, 200, 16, 16, 64, 900, True, False), ("f32", 6, 257, 16, 16, 32, 650, True, False),
     ("f32", 1, 3, 2, 1, 32, 3000, True, False), ("f32", 3, 5, 2, 2, 16, 64, False, False), ("f32", 2, 80, 2, 2, 80, 111, True, True),
 ]
 
