@@ -377,8 +377,13 @@ __device__ __forceinline__ void work_of(int bid, const DecAttnParams& p, int mt,
     kh = u - b * p.Hkv;
 }
 
+// Workgroups to a CU: as many as the registers allow without spilling (f32,
+// d_head 128, 54 rows x 334 keys x 56 heads: 25.4 us at one, 22.1 at two; f32, 64: one
+// more than three spills, 18.1 -> 19.4).
+constexpr int attn_wgs(int kv, int d) { return d > 64 ? 2 : kv == KV_F32 && d > 32 ? 3 : 4; }
+
 template <int KV, bool QF32, int D, bool TABLE>
-__global__ __launch_bounds__(256, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn_kernel(DecAttnParams p) {
+__global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnParams p) {
     using TL = Tile<KV, D>;
     constexpr bool SPLIT = KV == KV_I8 && QF32;            // q and p as two f16 terms
     constexpr int NQ = KV == KV_F32 ? D / 4 : SPLIT ? D / 4 : D / 8;
@@ -576,7 +581,7 @@ __global__ __launch_bounds__(256, KV != KV_F32 && D <= 64 ? 4 : 1) void dec_attn
 
     if (k0 + 32 * wk < k1) {
         int t0 = k0 + 32 * wk;
-        if constexpr (KV == KV_F32) {      // (a second tile in flight gained nothing: the matrix pipe is what these wait for)
+        if constexpr (KV == KV_F32) {      // (a second tile in flight gained nothing, eight key shares lost 10 to 40%)
             for (; t0 < k1; t0 += STEP) {
                 Tile<KV, D> a;
                 load_tile<KV, D>(a, s, t0, lane);
