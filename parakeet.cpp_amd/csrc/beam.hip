@@ -12,22 +12,28 @@
 //
 // The W largest of many values: with the values in 64 groups, the W-th largest
 // of the groups' maxima bounds the W-th largest value from below, and only a few
-// values more than W reach it.  The bound is found bit by bit on an order-preserving integer (a ballot
-// and a count per bit, its top 20 bits: a lower bound is all that is wanted);
-// the values that reach it go to a list in LDS and are ranked there by counting.
-// Where more reach it than the list holds (ties), W rounds of a maximum over
-// the workgroup take over.
+// values more than W reach it.  The bound is found bit by bit on an
+// order-preserving integer (a ballot and a count per bit, its top 20 bits: a lower
+// bound is all that is wanted); the values that reach it go to a list in LDS and
+// are ranked there by counting.  Where more reach it than the list holds (ties),
+// W rounds of a maximum over the workgroup take over.  (W rounds for every call
+// instead of the bound: 25.1, 41.1 and 145 us for the calls below.)
 //
 // Few words (all of an item in one workgroup's registers): select_small, one
 // launch.  Otherwise select_rows, a workgroup per row or chunk of one, writes
 // the chunk's maximum, sum and list; select_item, a workgroup per item, forms
 // the scores and ranks them.
+//
+// Measured, with the reordering of the states, us: 1 item x 4 beams x 1025 words
+// (f32) 9.1, 16 x 8 x 8193 (f16) 13.8, 32 x 16 x 32769 (f32) 29.2.  A launch that
+// does nothing takes 2.5 to 3, so the first two are launches and dependent steps; the
+// last reads its 67 MB of logits at 3.7 TB/s in 18 (a copy reaches 5.1).
 #include "decoder.hpp"
 
 namespace pkx {
 namespace {
 
-constexpr int kPer = 32;                        // logits a lane holds
+constexpr int kPer = 32, kSmallPer = 16, kFew = 8;      // logits a lane holds: of a chunk, of an item, of a short row
 constexpr int kRowThreads = 256, kChunk = kRowThreads * kPer;
 constexpr int kSmallThreads = 1024, kItemThreads = 1024;
 constexpr int kList = 128;                      // candidates of a chunk
@@ -95,13 +101,15 @@ __device__ __forceinline__ float exp_below(float d) {
 
 // n logits of a row over `threads` threads, VEC adjacent ones a thread and step:
 // 16 bytes (rows of odd length are aligned to their elements only), or one where
-// that leaves threads without any.  Register i of thread t is
+// that leaves threads without any (f16, 4 beams x 1025 words: 8.0 us with 16 bytes, 6.4
+// with one; 16 x 8 x 700: 9.1 and 7.8).  PER registers, used or not, are what a
+// short row costs (4 x 1025, f32: 7.2 us with 32, 6.4 with 8).  Register i of thread t is
 // logit word(i), -inf where there is none.  The thread whose piece the row's
 // end cuts reads the row's last 16 bytes instead and leaves out what its
 // neighbour has, so that no load waits on a branch.
-template <bool F32, int VEC> struct RowRegs {
-    static constexpr int G = kPer / VEC;
-    float x[kPer];
+template <bool F32, int VEC, int PER> struct RowRegs {
+    static constexpr int G = PER / VEC;
+    float x[PER];
     int n, o0, step, groups, last;
     __device__ __forceinline__ int piece(int g) const { return o0 + g * step; }
     __device__ __forceinline__ int cut(int g) const { return piece(g) < last ? piece(g) : last; }
@@ -131,7 +139,7 @@ template <bool F32, int VEC> struct RowRegs {
 #pragma unroll
             for (int g = 0; g < G; ++g) raw[g] = *(const words*)((const uint8_t*)logits + (first + cut(g)) * (F32 ? 4 : 2));
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
+            for (int i = 0; i < PER; ++i) {
                 const int g = i / VEC, e = i % VEC;
                 float v;
                 if constexpr (F32) v = __int_as_float(raw[g][e]);
@@ -143,7 +151,7 @@ template <bool F32, int VEC> struct RowRegs {
     __device__ __forceinline__ float max() const {
         float m = x[0];
 #pragma unroll
-        for (int i = 1; i < kPer; ++i) m = fmaxf(m, x[i]);
+        for (int i = 1; i < PER; ++i) m = fmaxf(m, x[i]);
         return m;
     }
     // sum of e^(x - m) for a maximum m over these and other lanes, NaN where a logit is NaN or +inf
@@ -276,7 +284,7 @@ __device__ __forceinline__ double beam_score(const BeamSelectParams& p, int64_t 
 __device__ __forceinline__ bool is_dead(double score, double lse) { return score == -INFINITY || !(lse < 1e300 && lse > -1e300); }
 
 // One workgroup per item, all its logits in registers: `per` waves a beam.
-template <bool F32, int VEC> __global__ __launch_bounds__(kSmallThreads) void select_small_kernel(BeamSelectParams p, int per) {
+template <bool F32, int VEC, int PER> __global__ __launch_bounds__(kSmallThreads) void select_small_kernel(BeamSelectParams p, int per) {
     __shared__ Hits hits;
     __shared__ float smax[16];
     __shared__ double ssum[16];
@@ -288,7 +296,7 @@ template <bool F32, int VEC> __global__ __launch_bounds__(kSmallThreads) void se
     const int w = wave / per, first = w * per, t = threadIdx.x - first * 64, threads = per * 64;
     const bool on = w < p.W;
     const int64_t row = (int64_t)b * p.W + (on ? w : 0);
-    RowRegs<F32, VEC> r;
+    RowRegs<F32, VEC, PER> r;
     r.load(p.logits, row * p.row, on ? p.V : 0, t, threads);       // a finished beam's too: nothing waits on done
     const bool fin = on && p.done && p.done[row];
     const double score = beam_score(p, row);
@@ -361,8 +369,10 @@ template <bool F32, int VEC> __global__ __launch_bounds__(kSmallThreads) void se
     }
 }
 
-// One workgroup per chunk of a row: its maximum, sum and candidates.
-template <bool F32, int VEC> __global__ __launch_bounds__(kRowThreads) void select_rows_kernel(BeamSelectParams p, SelectWork ws) {
+// One workgroup per chunk of a row: its maximum, sum and candidates.  Chunks of up
+// to 8192 logits, read once, all loads in flight at once; 512 rows of 32769 f32 take
+// 17.9 us, two thirds of it VALU issue (an exponential and an f64 sum per logit).
+template <bool F32, int VEC, int PER> __global__ __launch_bounds__(kRowThreads) void select_rows_kernel(BeamSelectParams p, SelectWork ws) {
     __shared__ float smax[4];
     __shared__ double ssum[4];
     __shared__ uint32_t keys[kRowThreads];
@@ -373,7 +383,7 @@ template <bool F32, int VEC> __global__ __launch_bounds__(kRowThreads) void sele
     if (p.done && p.done[row]) return;                       // its one candidate needs no logits
     const int base = (int)(unit - row * ws.chunks) * ws.len;
     const int n = p.V - base < ws.len ? p.V - base : ws.len;
-    RowRegs<F32, VEC> r;
+    RowRegs<F32, VEC, PER> r;
     r.load(p.logits, row * p.row + base, n, t, kRowThreads);
     const float lane_max = r.max();
     const float wm = wave_max_dpp(lane_max);
@@ -414,7 +424,9 @@ template <bool F32, int VEC> __global__ __launch_bounds__(kRowThreads) void sele
     if (t == 0) ws.stat[unit] = ChunkStat{m, listed, (ssum[0] + ssum[1]) + (ssum[2] + ssum[3])};
 }
 
-// One workgroup per item over its chunks' lists.
+// One workgroup per item over its chunks' lists: a chain of dependent steps (statistics,
+// f64 exponentials and a logarithm, bound, ranking) of 6.6 us for 8 beams x 2 chunks, 8.9
+// for 16 x 5, however many items there are up to the chip's 256 CUs.
 __global__ __launch_bounds__(kItemThreads) void select_item_kernel(BeamSelectParams p, SelectWork ws) {
     constexpr int WAVES = kItemThreads / 64;
     __shared__ Hits hits;
@@ -543,6 +555,8 @@ struct ReorderParams {
     int width[kMaxBeamStates];       // bytes a thread moves at a time
 };
 
+// All states in one launch: rows x states x pieces.  4 states of 2560 bytes x 128 rows
+// 2.9 us, near an empty launch.
 __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
     const BeamState& s = p.st[blockIdx.y];
     const int width = p.width[blockIdx.y];
@@ -561,11 +575,14 @@ __global__ __launch_bounds__(256) void reorder_kernel(ReorderParams p) {
     }
 }
 
-// waves a beam where an item fits one workgroup's registers, 0 where it does not
+// waves a beam where an item fits one workgroup's registers, 0 where it does not.
+// One launch against two, us: 1 item x 4 beams x 1025 words 6.4 and 8.6, 16 x 4 x 4096
+// 9.4 and 10.8, 16 x 16 x 1024 11.2 and 11.8; with 32 logits a lane 16 x 4 x 8192 took
+// 13.8 and 11.6, so 16 is the limit.
 int small_waves(const BeamSelectParams& p) {
     if (p.W > 16) return 0;
     const int per = 16 / p.W;
-    return p.V <= per * 64 * kPer ? per : 0;
+    return p.V <= per * 64 * kSmallPer ? per : 0;
 }
 
 SelectWork select_work(const BeamSelectParams& p) {
@@ -587,9 +604,10 @@ void launch_beam_select(const BeamSelectParams& p, void* ws, size_t ws_bytes, hi
     const int wide = p.f32 ? 4 : 8;
     require(p.B < (1 << 22), "beam select: at most 2^22 items in one call");
     if (const int per = small_waves(p)) {
-        const bool one = p.V < per * 64 * wide;
-        auto* k = p.f32 ? (one ? select_small_kernel<true, 1> : select_small_kernel<true, 4>)
-                        : (one ? select_small_kernel<false, 1> : select_small_kernel<false, 8>);
+        const int threads = per * 64;
+        auto* k = p.V < threads * wide ? (p.f32 ? select_small_kernel<true, 1, kFew> : select_small_kernel<false, 1, kFew>)
+                  : !p.f32             ? select_small_kernel<false, 8, kSmallPer>
+                                       : p.V <= threads * kFew ? select_small_kernel<true, 4, kFew> : select_small_kernel<true, 4, kSmallPer>;
         launch(k, dim3(p.B), dim3(kSmallThreads), 0, s, p, per);
         return;
     }
@@ -601,9 +619,9 @@ void launch_beam_select(const BeamSelectParams& p, void* ws, size_t ws_bytes, hi
     require(lists < ((size_t)1 << 23), "beam select: too many beams and words for one call");
     w.stat = (ChunkStat*)ws;
     w.list = (Entry*)((char*)ws + lists * sizeof(ChunkStat));
-    const bool one = p.V < kRowThreads * wide;
-    auto* k = p.f32 ? (one ? select_rows_kernel<true, 1> : select_rows_kernel<true, 4>)
-                    : (one ? select_rows_kernel<false, 1> : select_rows_kernel<false, 8>);
+    auto* k = p.V < kRowThreads * wide ? (p.f32 ? select_rows_kernel<true, 1, kFew> : select_rows_kernel<false, 1, kFew>)
+              : !p.f32                 ? select_rows_kernel<false, 8, kPer>
+                                       : w.len <= kRowThreads * kFew ? select_rows_kernel<true, 4, kFew> : select_rows_kernel<true, 4, kPer>;
     launch(k, dim3((unsigned)lists), dim3(kRowThreads), 0, s, p, w);
     launch(select_item_kernel, dim3(p.B), dim3(kItemThreads), 0, s, p, w);
 }

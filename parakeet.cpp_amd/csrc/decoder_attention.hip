@@ -25,7 +25,17 @@
 // (0x6400 | (b ^ 0x80) = 1024 + b + 128, minus 1152: exact), the scale of a
 // block multiplies the scores and the tile's P V product in f32.  With f32
 // queries, q and p are split into two f16 terms of 22 bits together, so the
-// int8 products keep f32's accuracy at twice the matrix instructions.
+// int8 products keep f32's accuracy at twice the matrix instructions (the f32 ones
+// have a sixteenth of the f16 ones' rate).
+//
+// Measured, us (a copy moves 5.1 TB/s, a launch that does nothing takes 2.5 to 3):
+//   f16 1 row x 8 heads x 64, 125 keys                     4.4   launch, dependent loads
+//   f16 16 x 4 rows x 8 heads x 128, up to 375 keys        7.8   15 MB at 2.0 TB/s; latency
+//   f16 4 x 8 rows x 16 (8) heads x 64, 3750 keys         10.0 + 3.9 to join: 31 MB, 3.1 TB/s
+//   f32 3 x 37 rows x 8 heads x 64, up to 211 keys         8.0   latency, matrix pipe
+//   int8 128 beams x 8 heads x 64, up to 448 keys, table  14.3   VALU issue 68%
+//   int8 4 rows x 16 (4) heads x 128, up to 32768 keys    23.4 + 4.7 to join: 92 MB, 3.9 TB/s
+//   int8, f32 8 x 200 rows x 8 heads x 64, up to 1025     18.0   VALU issue 65%: conversions
 #include "decoder.hpp"
 
 namespace pkx {
@@ -696,6 +706,12 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
 // far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
 // different scales add up in one accumulator, which is rescaled when v grows.
 // 2^14 rides in the exponent, and r too where f16's 11 bits are what is kept.
+//
+// f16, 16 x 448 rows x 8 heads x 128, 750 keys: 42.6 us alone, 38.2 in a stream of
+// such calls (575 TFLOP/s; a large product of the library reaches 1071), 118 on
+// dec_attn_kernel.  VALU issue 49%, matrix pipe 30%, LDS 30%: a wave's softmax stands
+// between its products, and 226 registers leave two waves a SIMD to overlap them.
+// Tried: 16 rows a wave and eight waves (57 us), two LDS buffers (44.4).
 template <int KV, bool QF32, int D, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     constexpr int QT = 2, NW = 4, ROWS = 16 * QT * NW, KT = 64;
@@ -1192,7 +1208,9 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     else p.table ? launch_width<KV_I8, false, true>(p, sh, s) : launch_width<KV_I8, false, false>(p, sh, s);
     if (sh.splits > 1) {
         const int64_t rows = (int64_t)p.B * p.Hkv * p.n_q * p.G;
-        if (rows <= 1024) {                        // threads by the row leave the chip short of them
+        // threads by the row leave the chip short of them: 64 rows x 29 splits 9.1 us, by
+        // the workgroup 4.7; 2048 x 15 4.8 and 4.8; 12800 x 3 5.0 and 7.5
+        if (rows <= 1024) {
             auto* k = p.q_f32 ? dec_join_kernel<true> : dec_join_kernel<false>;
             launch(k, dim3((unsigned)rows), dim3(256), 0, s, p);
         } else {

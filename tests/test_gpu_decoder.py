@@ -167,7 +167,7 @@ class HostCache:
 
 
 @pytest.mark.parametrize("type", ["f16", "f32"])
-@pytest.mark.parametrize("d,new", [(64, 1), (16, 5), (80, 40), (128, 100), (48, 31), (32, 33)])
+@pytest.mark.parametrize("d,new", [(64, 1), (128, 1), (16, 1), (48, 1), (80, 1), (112, 1), (16, 5), (80, 40), (128, 100), (48, 31), (32, 33)])
 def test_cache_append(gpu, stream, type, d, new):
     """Bytes and scales equal to the restatement's, whatever the position in a block; rows out of range, past the
     capacity, of count 0 and naming a slot again; NaN, infinities and zeros among the values; the rest untouched."""
@@ -391,7 +391,7 @@ def check_select(got, want, scores, label):
 
 @pytest.mark.parametrize("type", ["f16", "f32"])
 @pytest.mark.parametrize("B,W,V", [(1, 1, 1), (2, 4, 1025), (1, 32, 33), (3, 8, 3), (2, 5, 2048), (1, 7, 2049), (2, 16, 9001),
-                                   (1, 3, 70000), (5, 2, 64), (1, 32, 70001), (2, 17, 700), (1, 1, 32768), (1, 1, 32769)])
+                                   (1, 3, 70000), (5, 2, 64), (1, 32, 70001), (2, 17, 700), (1, 20, 1500), (1, 1, 32768), (1, 1, 32769)])
 def test_beam_select(gpu, stream, type, B, W, V):
     """Random logits; then equal ones (ties to the lowest index), finished beams, dead beams, -inf words."""
     print(f"[beam] {type} B={B} W={W} V={V}", flush=True)
