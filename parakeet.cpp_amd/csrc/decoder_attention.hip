@@ -128,6 +128,7 @@ struct KeySource {
     int n_slots;
     int64_t k_slot, s_slot;      // bytes and scales between slots (keys and values alike)
     bool far;                    // a slot's offset may not fit 32 bits
+    uint32_t span;               // otherwise: bytes from k (and v) to the last slot's end
 };
 
 // A buffer resource of one step's rows, built from scalars.
@@ -200,37 +201,50 @@ template <int D> __device__ __forceinline__ void load_tile_by_table(Tile<KV_I8, 
     slot = in ? slot : 0;
     t.ks = s.ks[slot * s.s_slot + tb / kCacheBlock];
     t.vs = s.vs[slot * s.s_slot + tb / kCacheBlock];
-    const uint8_t* kb = s.k + (int64_t)tb * s.k_row;
-    const uint8_t* vb = s.v + (int64_t)tb * s.v_row;
-    auto fetch = [&](auto&& at_k, auto&& at_v) {
+    if (!s.far) {        // through resources of all slots, offsets of 32 bits
+        const uint32_t mine_at = (uint32_t)slot * (uint32_t)s.k_slot + (tb + row) * s.k_row;
+        const auto kr = step_rsrc(s.k, s.span), vr = step_rsrc(s.v, s.span);
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             constexpr int N = TL::NK == 2 ? 2 : 4;
+            const uint32_t at = (uint32_t)__shfl((int)mine_at, 16 * kt + c, 64);
 #pragma unroll
             for (int n = 0; n < TL::NK / N; ++n) {
                 uint32_t d[N];
-                load_words(d, at_k(16 * kt + c, s.k_at[n]));
+                buffer_words(d, kr, at + s.k_at[n]);
 #pragma unroll
                 for (int i = 0; i < N; ++i) t.k[kt][N * n + i] = d[i];
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint8_t* x = at_v((i < 4 ? 0 : 12) + 4 * g + i, s.v_at);
-            if constexpr (D == 32) t.v[i][0] = *(const uint16_t*)x;
-            else load_words(t.v[i], x);
+            const uint32_t at = (uint32_t)__shfl((int)mine_at, (i < 4 ? 0 : 12) + 4 * g + i, 64) + s.v_at;
+            if constexpr (D == 32) t.v[i][0] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(vr, at, 0, 0);
+            else buffer_words(t.v[i], vr, at);
         }
+        return;
+    }
+    const int64_t mine_at = slot * s.k_slot + (int64_t)(tb + row) * s.k_row;
+    auto from = [&](int r) {
+        return (int64_t)((uint64_t)(uint32_t)__shfl((int)(mine_at >> 32), r, 64) << 32 | (uint32_t)__shfl((int)mine_at, r, 64));
     };
-    if (!s.far) {
-        const uint32_t mine_at = (uint32_t)slot * (uint32_t)s.k_slot + row * s.k_row;
-        fetch([&](int r, uint32_t d) { return kb + ((uint32_t)__shfl((int)mine_at, r, 64) + d); },
-              [&](int r, uint32_t d) { return vb + ((uint32_t)__shfl((int)mine_at, r, 64) + d); });
-    } else {
-        const int64_t mine_at = slot * s.k_slot + row * s.k_row;
-        auto from = [&](int r) {
-            return (int64_t)((uint64_t)(uint32_t)__shfl((int)(mine_at >> 32), r, 64) << 32 | (uint32_t)__shfl((int)mine_at, r, 64));
-        };
-        fetch([&](int r, uint32_t d) { return kb + (from(r) + d); }, [&](int r, uint32_t d) { return vb + (from(r) + d); });
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        constexpr int N = TL::NK == 2 ? 2 : 4;
+        const uint8_t* x = s.k + from(16 * kt + c);
+#pragma unroll
+        for (int n = 0; n < TL::NK / N; ++n) {
+            uint32_t d[N];
+            load_words(d, x + s.k_at[n]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) t.k[kt][N * n + i] = d[i];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint8_t* x = s.v + from((i < 4 ? 0 : 12) + 4 * g + i) + s.v_at;
+        if constexpr (D == 32) t.v[i][0] = *(const uint16_t*)x;
+        else load_words(t.v[i], x);
     }
 }
 
@@ -429,6 +443,7 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
             s.n_slots = p.n_slots;
             s.k_slot = p.k_item;
             s.far = p.n_slots * p.k_item > 0x7fffffffll;
+            s.span = (uint32_t)(p.n_slots * p.k_item - kh * p.k_head);
         }
     } else {
         s.k = (const uint8_t*)p.k + (b * p.k_item + kh * p.k_head) * TL::ES;
@@ -527,17 +542,15 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
         l = l * alpha + sum;
         if constexpr (KV == KV_I8) {
             if constexpr (TABLE) {
-                // weights p vs of keys with different scales: their largest
-                // becomes 2^14, so that f16 keeps it whatever the scales (a largest
-                // below 2^-110 is as good as none, and its inverse would not be finite)
-                float top = 0x1p-110f;
+                // weights p vs of keys with different scales: their largest becomes
+                // 2^14, so that f16 keeps it exactly whatever the scales (a power of two instead
+                // doubled the error of outputs that one key decides; the reciprocal's last
+                // bit is one of 2^-23).  A largest below 2^-110 is as good as none, and its
+                // reciprocal would not be finite
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    pf[e] *= vs8[e];
-                    top = fmaxf(top, pf[e]);
-                }
-                top = xgroup_max(top);
-                const float inv = 0x1p14f / top;
+                for (int e = 0; e < 8; ++e) pf[e] *= vs8[e];
+                const float top = xgroup_max(max3(max3(pf[0], pf[1], pf[2]), max3(pf[3], pf[4], pf[5]), max3(pf[6], pf[7], 0x1p-110f)));
+                const float inv = __builtin_amdgcn_rcpf(top) * 0x1p14f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] *= inv;
                 vf = top * 0x1p-14f;

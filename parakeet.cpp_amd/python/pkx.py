@@ -605,7 +605,9 @@ def quantize_gguf(in_path, out_path, qtype: str):
 # Each object binds its buffers once (a decode loop calls the same ones every step)
 # and keeps them and its workspace alive; calling it starts the kernels on `stream`.
 # An object's calls share its workspace: they must not overlap.  Arrays are
-# DeviceArrays or anything with .ptr, .shape and .dtype.
+# DeviceArrays or anything with .ptr, .shape and .dtype; .strides, in elements, may
+# stand beside them and are taken for queries, keys, values, outputs, logits, masks
+# and tables, and refused for the rest unless packed.
 def _type(a):
     t = {"float32": TYPE_F32, "float16": TYPE_F16}.get(np.dtype(a.dtype).name)
     if t is None:
@@ -617,18 +619,28 @@ def _ptr(a):
     return None if a is None else a.ptr
 
 
-def _expect(a, shape, dtype, what):
-    if a is not None and (tuple(a.shape) != tuple(shape) or np.dtype(a.dtype) != np.dtype(dtype)):
-        raise PkxError(f"{what}: {np.dtype(dtype).name} {list(shape)} is wanted, got {np.dtype(a.dtype).name} {list(a.shape)}")
+def _packed(shape):
+    return tuple(int(np.prod(shape[i + 1:])) for i in range(len(shape)))
 
 
 def _strides(a):
-    """Elements between items, rows and heads of a packed [item][row][head][dim] array, or the array's own .strides."""
+    """Elements between an array's items, rows, ..., its last dimension's adjacent: its own .strides, or a packed array's."""
     own = getattr(a, "strides", None)
-    if own is not None:
-        return tuple(own)[:3]
-    _, t, h, d = a.shape
-    return t * h * d, h * d, d
+    n = len(a.shape) - 1
+    if own is None:
+        return _packed(a.shape)[:n]
+    if len(own) < n or (len(own) > n and own[n] != 1 and a.shape[n] > 1):
+        raise PkxError(f"strides {list(own)} of an array {list(a.shape)}: the last dimension's elements are adjacent")
+    return tuple(own)[:n]
+
+
+def _expect(a, shape, dtype, what, strided=False):
+    if a is None:
+        return
+    if tuple(a.shape) != tuple(shape) or np.dtype(a.dtype) != np.dtype(dtype):
+        raise PkxError(f"{what}: {np.dtype(dtype).name} {list(shape)} is wanted, got {np.dtype(a.dtype).name} {list(a.shape)}")
+    if not strided and any(n > 1 and x != y for n, x, y in zip(a.shape, _strides(a), _packed(a.shape))):
+        raise PkxError(f"{what}: a packed {list(shape)} is wanted")
 
 
 class _Bound:
@@ -656,10 +668,10 @@ class CrossAttention(_Bound):
         (B, nq, H, d), (_, nk, Hkv, _) = q.shape, k.shape
         for a, n, dt in ((k, (B, nk, Hkv, d), q.dtype), (v, (B, nk, Hkv, d), q.dtype), (out, q.shape, q.dtype),
                          (q_len, (B,), np.int32), (k_len, (B,), np.int32), (k_mask, (B, nk), np.uint8)):
-            _expect(a, n, dt, "cross attention")
+            _expect(a, n, dt, "cross attention", strided=len(n) > 1)
         a = CrossAttnArgs(_type(q), B, nq, nk, H, Hkv, d, d ** -0.5 if scale is None else scale, q.ptr, *_strides(q),
                           k.ptr, *_strides(k), v.ptr, *_strides(v), out.ptr, *_strides(out), _ptr(q_len), _ptr(k_len),
-                          _ptr(k_mask), nk)
+                          _ptr(k_mask), nk if k_mask is None else _strides(k_mask)[0])
         self._bind("pkx_cross_attention", (C.byref(a),), (a, q, k, v, out, q_len, k_len, k_mask),
                    "pkx_cross_attention_workspace")
 
@@ -689,12 +701,12 @@ class Cache8:
         self.args = Cache8Args(S, H, d, cap, k.ptr, v.ptr, k_scale.ptr, v_scale.ptr)
 
 
-def _table_row(table, rows):
+def _table_row(table, rows, positions):
     if table is None:
         return 0
-    if len(table.shape) != 2 or table.shape[0] != rows or np.dtype(table.dtype) != np.int32:
-        raise PkxError(f"cache table: int32 [{rows}][positions] is wanted, got {table.dtype} {list(table.shape)}")
-    return table.shape[1]
+    if len(table.shape) != 2 or table.shape[0] != rows or table.shape[1] < positions or np.dtype(table.dtype) != np.int32:
+        raise PkxError(f"cache table: int32 [{rows}][>= {positions}] is wanted, got {table.dtype} {list(table.shape)}")
+    return _strides(table)[0]
 
 
 class CacheAppend(_Bound):
@@ -704,9 +716,9 @@ class CacheAppend(_Bound):
         R, n, H, d = k.shape
         for a, m, dt in ((k, (R, n, cache.n_kv_heads, cache.d_head), k.dtype), (v, k.shape, k.dtype),
                          (start, (R,), np.int32), (slot, (R,), np.int32), (count, (R,), np.int32)):
-            _expect(a, m, dt, "cache append")
+            _expect(a, m, dt, "cache append", strided=len(m) > 1)
         a = Cache8Tokens(_type(k), R, n, k.ptr, *_strides(k), v.ptr, *_strides(v), _ptr(slot), start.ptr, _ptr(count),
-                         _ptr(table), _table_row(table, R))
+                         _ptr(table), _table_row(table, R, cache.capacity))
         self._bind("pkx_cache8_append", (C.byref(cache.args), C.byref(a)), (cache, a, k, v, start, slot, count, table))
 
 
@@ -730,10 +742,10 @@ class CacheAttention(_Bound):
         R, n, H, d = q.shape
         for a, m, dt in ((q, (R, n, H, cache.d_head), q.dtype), (out, q.shape, q.dtype), (length, (R,), np.int32),
                          (slot, (R,), np.int32), (q_len, (R,), np.int32)):
-            _expect(a, m, dt, "cache attention")
+            _expect(a, m, dt, "cache attention", strided=len(m) > 1)
         a = Cache8AttnArgs(_type(q), R, n, H, int(causal), d ** -0.5 if scale is None else scale, q.ptr, *_strides(q),
                            out.ptr, *_strides(out), _ptr(slot), length.ptr, _ptr(q_len), _ptr(table),
-                           _table_row(table, R), max_len)
+                           _table_row(table, R, min(max_len or cache.capacity, cache.capacity)), max_len)
         self._bind("pkx_cache8_attention", (C.byref(cache.args), C.byref(a)),
                    (cache, a, q, out, length, slot, q_len, table), "pkx_cache8_attention_workspace")
 
@@ -746,7 +758,10 @@ class BeamSelect(_Bound):
         for a, dt in ((scores, np.float32), (parent, np.int32), (token, np.int32), (new_scores, np.float32),
                       (done, np.uint8), (new_done, np.uint8)):
             _expect(a, (B, W), dt, "beam select")
-        a = BeamSelectArgs(_type(logits), B, W, V, end_id, logits.ptr, V, scores.ptr, _ptr(done), parent.ptr, token.ptr,
+        item, row = _strides(logits)
+        if B > 1 and item != W * row:
+            raise PkxError("beam select: the rows of logits [B][W][V] are equally far apart")
+        a = BeamSelectArgs(_type(logits), B, W, V, end_id, logits.ptr, row, scores.ptr, _ptr(done), parent.ptr, token.ptr,
                            new_scores.ptr, _ptr(new_done))
         self._bind("pkx_beam_select", (C.byref(a),), (a, logits, scores, parent, token, new_scores, done, new_done),
                    "pkx_beam_select_workspace")
@@ -762,6 +777,8 @@ class BeamReorder(_Bound):
         for i, (s, d) in enumerate(states):
             if tuple(s.shape) != tuple(d.shape) or np.dtype(s.dtype) != np.dtype(d.dtype) or s.shape[0] != B * W:
                 raise PkxError(f"beam reorder: states are pairs of the same [{B * W}][...], got {list(s.shape)} and {list(d.shape)}")
+            for x in (s, d):
+                _expect(x, s.shape, s.dtype, "beam reorder")
             n = int(np.prod(s.shape[1:])) * np.dtype(s.dtype).itemsize
             a[i] = BeamState(s.ptr, d.ptr, n, n, n)
         self._bind("pkx_beam_reorder", (parent.ptr, B, W, a, len(states)), (parent, a, states))

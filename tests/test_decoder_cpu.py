@@ -168,6 +168,36 @@ def test_refusals_of_values_and_of_sizes_whose_products_wrap():
         assert line.startswith("1 ") and w in line, (line, w)
 
 
+def test_binding_refuses_strides_it_would_not_pass_on():
+    out = _run("""
+        import numpy as np
+        class V:
+            def __init__(self, shape, dtype=np.float32, strides=None):
+                self.ptr, self.shape, self.dtype, self.strides = A, shape, np.dtype(dtype), strides
+        q, kv, n = V((2, 1, 4, 64)), V((2, 9, 2, 64)), V((2,), np.int32)
+        cache = pkx.Cache8.wrap(*(V((2, 2, 96, 64), np.int8) for _ in range(2)), *(V((2, 2, 3)) for _ in range(2)))
+        sel = lambda x, s=None: pkx.BeamSelect(x, s or V((2, 4)), *(V((2, 4), np.int32) for _ in range(2)), V((2, 4)))
+        for f in (lambda: pkx.CrossAttention(q, kv, kv, V((2, 1, 4, 64), strides=(512, 512, 128, 2))),
+                  lambda: pkx.CrossAttention(q, kv, kv, q, k_len=V((2,), np.int32, (2,))),
+                  lambda: sel(V((2, 4, 50), strides=(400, 50, 1))),
+                  lambda: sel(V((2, 4, 50)), V((2, 4), strides=(8, 1))),
+                  lambda: pkx.CacheAppend(cache, q, q, n),
+                  lambda: pkx.CacheAttention(cache, q, q, n, table=V((2, 95), np.int32, (200, 1))),
+                  lambda: pkx.BeamReorder(V((1, 2), np.int32), [(V((2, 6)), V((2, 6), strides=(8, 1)))])):
+            try:
+                f()
+                print("taken")
+            except pkx.PkxError as e:
+                print("refused", e)
+        a = pkx.CrossAttention(q, kv, kv, q, k_mask=V((2, 9), np.uint8, (16, 1)))._keep[0]
+        b = sel(V((2, 4, 50), strides=(256, 64, 1)))._keep[0]
+        c = pkx.CacheAttention(cache, q, q, n, table=V((2, 50), np.int32, (77, 1)), max_len=50)._keep[1]
+        print(a.k_mask_item, b.logits_row, c.table_row)
+    """)
+    assert len(out) == 8 and all(x.startswith("refused") for x in out[:7]), out
+    assert out[7] == "16 64 77"
+
+
 def test_workspace_follows_the_sizes():
     """No workspace where the rows fill the chip; with few rows and many keys partial sums for every split."""
     out = _run("""

@@ -89,6 +89,31 @@ def test_cross_attention(gpu, stream, type, B, nq, nk, H, Hkv, d, masked):
             check_attention(got[b, :n, h], want, type == "f16", d, f"cross b{b} h{h}")
 
 
+def test_rows_of_masks_logits_and_tables_further_apart(gpu, stream):
+    """The middle of larger buffers of masks, logits and tables gives what packed copies give."""
+    rng = np.random.default_rng(12)
+    q, k, v = (dev(gpu, rng.standard_normal((2, n, 2, 32)).astype(np.float16), stream) for n in (3, 50, 50))
+    mask = (rng.random((2, 64)) < 0.5).astype(np.uint8)
+    outs = [gpu.DeviceArray((2, 3, 2, 32), np.float16) for _ in range(2)]
+    gpu.CrossAttention(q, k, v, outs[0], k_mask=View(dev(gpu, mask, stream), 5, (2, 50), (64, 1)))(stream)
+    gpu.CrossAttention(q, k, v, outs[1], k_mask=dev(gpu, np.ascontiguousarray(mask[:, 5:55]), stream))(stream)
+    assert np.array_equal(*(o.numpy(stream) for o in outs))
+    c = HostCache(gpu, stream, 3, 2, 64, 32, rng)
+    table = rng.integers(0, 3, (2, 90)).astype(np.int32)
+    n = dev(gpu, i32([60, 33]), stream)
+    gpu.CacheAttention(c.dev, q, outs[0], n, table=View(dev(gpu, table, stream), 7, (2, 64), (90, 1)))(stream)
+    gpu.CacheAttention(c.dev, q, outs[1], n, table=dev(gpu, np.ascontiguousarray(table[:, 7:71]), stream))(stream)
+    assert np.array_equal(*(o.numpy(stream) for o in outs))
+    x = rng.standard_normal((2, 4, 128)).astype(np.float32)
+    score = dev(gpu, rng.standard_normal((2, 4)).astype(np.float32), stream)
+    got = []
+    for logits in (View(dev(gpu, x, stream), 3, (2, 4, 101), (4 * 128, 128, 1)), dev(gpu, np.ascontiguousarray(x[..., 3:104]), stream)):
+        o = [gpu.DeviceArray((2, 4), t) for t in (np.int32, np.int32, np.float32)]
+        gpu.BeamSelect(logits, score, *o)(stream)
+        got.append([a.numpy(stream) for a in o])
+    assert all(np.array_equal(a, b) for a, b in zip(*got))
+
+
 def test_cross_attention_strides_and_streams(gpu, stream):
     """Head-major buffers, the middle of larger ones, two streams at once, and what surrounds the output kept."""
     rng = np.random.default_rng(5)
