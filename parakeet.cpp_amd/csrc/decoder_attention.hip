@@ -58,11 +58,21 @@ __device__ __forceinline__ float xgroup_sum(float x) {
 }
 
 // v_max3_f32 as it is: the compiler puts a canonicalising v_max before every
-// fmaxf of a matrix product's result
+// fmaxf of a matrix product's result.  It keeps no waits around inline assembly
+// either: matrix products go through settled() first, and what comes out through an
+// ordinary instruction before a lane swap reads it.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
     return r;
+}
+__device__ __forceinline__ float max8(float4v x, float4v y) {
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], y[0], y[1]), max3(y[2], y[3], y[3]));
+}
+// 20 wait states, enough for the longest matrix instruction's result (19)
+__device__ __forceinline__ void settled(float4v (&s)[2][4]) {
+    asm("s_nop 15\n\ts_nop 3"
+        : "+v"(s[0][0]), "+v"(s[0][1]), "+v"(s[0][2]), "+v"(s[0][3]), "+v"(s[1][0]), "+v"(s[1][1]), "+v"(s[1][2]), "+v"(s[1][3]));
 }
 
 // bits 0 .. n - 1
@@ -252,6 +262,18 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
     const half2v h = {(f16)a, (f16)b};
     return __builtin_bit_cast(uint32_t, h);
 }
+// Two values as pairs of f16 terms: what the rounding leaves is exact in f32.  The first
+// terms are formed twice, and once from a product fused into the conversion they could
+// differ by one of their steps, so either they are taken from their register (fewer
+// instructions: 8 prompts of 200 rows 18.6 -> 17.6 us) or the values are (fewer
+// registers, where all are in use).
+template <bool VALUES> __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+    if constexpr (VALUES) asm("" : "+v"(a), "+v"(b));
+    hi = pack_f16(a, b);
+    if constexpr (!VALUES) asm("" : "+v"(hi));
+    const half2v h = __builtin_bit_cast(half2v, hi);
+    lo = pack_f16(fmaf((float)h[0], -1.0f, a), fmaf((float)h[1], -1.0f, b));
+}
 
 // Row m of an item and key head as lane group g's fragments (LAYOUT: the kind
 // of keys whose order of dimensions they meet); returns its query index.  Rows past the queries are zeros.
@@ -316,12 +338,7 @@ __device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, 
 #pragma unroll
         for (int n = 0; n < D / 32; ++n)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = x[n][2 * e] * f, bq = x[n][2 * e + 1] * f;
-                const f16 ah = (f16)a, bh = (f16)bq;
-                q[4 * n + e] = pack_f16((float)ah, (float)bh);
-                q[D / 8 + 4 * n + e] = pack_f16(a - (float)ah, bq - (float)bh);
-            }
+            for (int e = 0; e < 4; ++e) split_f16<false>(x[n][2 * e] * f, x[n][2 * e + 1] * f, q[4 * n + e], q[D / 8 + 4 * n + e]);
     }
     return i;
 }
@@ -509,17 +526,11 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
         uint32_t ph[4], pl[4];
         const float4v s0 = tile_scores<KV, D, QF32, NQ>(t.k[0], q);
         const float4v s1 = tile_scores<KV, D, QF32, NQ>(t.k[1], q);
-        float f = qf;
-        if constexpr (KV == KV_I8 && !TABLE) f *= t.ks;
         float sc[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            sc[e] = s0[e] * f;
-            sc[4 + e] = s1[e] * f;
-            if constexpr (TABLE) {
-                sc[e] *= ks8[e];
-                sc[4 + e] *= ks8[4 + e];
-            }
+            sc[e] = s0[e] * (TABLE ? qf * ks8[e] : KV == KV_I8 ? qf * t.ks : qf);
+            sc[4 + e] = s1[e] * (TABLE ? qf * ks8[4 + e] : KV == KV_I8 ? qf * t.ks : qf);
         }
         if (!whole || t0 + 32 > all) {
             const uint32_t see = keep >> (4 * g) & low_bits(lim - t0 - 4 * g);
@@ -527,7 +538,8 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
             for (int e = 0; e < 8; ++e)
                 if (!(see & (1u << (e < 4 ? e : 12 + e)))) sc[e] = -INFINITY;
         }
-        const float mx = fmaxf(m, xgroup_max(max3(max3(sc[0], sc[1], sc[2]), max3(sc[3], sc[4], sc[5]), fmaxf(sc[6], sc[7]))));
+        const float top = max8((float4v){sc[0], sc[1], sc[2], sc[3]}, (float4v){sc[4], sc[5], sc[6], sc[7]});
+        const float mx = xgroup_max(fmaxf(m, top));
         const float alpha = __builtin_amdgcn_exp2f(m - mx);
         m = mx;
         // weights, and so l and O, are 2^14 p where they go to f16: down to 2^-28
@@ -549,7 +561,8 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
                 // reciprocal would not be finite
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] *= vs8[e];
-                const float top = xgroup_max(max3(max3(pf[0], pf[1], pf[2]), max3(pf[3], pf[4], pf[5]), max3(pf[6], pf[7], 0x1p-110f)));
+                float top = max8((float4v){pf[0], pf[1], pf[2], pf[3]}, (float4v){pf[4], pf[5], pf[6], pf[7]});
+                top = xgroup_max(fmaxf(top, 0x1p-110f));
                 const float inv = __builtin_amdgcn_rcpf(top) * 0x1p14f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) pf[e] *= inv;
@@ -560,15 +573,7 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
         }
         if constexpr (SPLIT) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float a = pf[2 * e], bq = pf[2 * e + 1];
-                // the products as rounded here: fused into the conversions, the two
-                // uses of hi below could differ by one of its steps
-                if constexpr (TABLE) asm("" : "+v"(a), "+v"(bq));
-                const f16 ah = (f16)a, bh = (f16)bq;
-                ph[e] = pack_f16((float)ah, (float)bh);
-                pl[e] = pack_f16(a - (float)ah, bq - (float)bh);
-            }
+            for (int e = 0; e < 4; ++e) split_f16<false>(pf[2 * e], pf[2 * e + 1], ph[e], pl[e]);
         } else if constexpr (KV != KV_F32) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) ph[e] = pack_f16(pf[2 * e], pf[2 * e + 1]);
@@ -909,6 +914,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                     }
         }
         if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(0);
+        settled(s);
         const bool cut = keep != ~0ull || t0 + KT > all_wave;
         float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f;
         if constexpr (KV == KV_I8) {
@@ -944,8 +950,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
             float mx = m[qt];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float4v x = s[qt][2 * h], y = s[qt][2 * h + 1];
-                mx = fmaxf(mx, max3(max3(x[0], x[1], x[2]), max3(x[3], y[0], y[1]), max3(y[2], y[3], y[3])) * f[h]);
+                mx = fmaxf(mx, max8(s[qt][2 * h], s[qt][2 * h + 1]) * f[h]);
             }
             mx = fmaxf(m[qt], xgroup_max(mx));
             alpha[qt] = __builtin_amdgcn_exp2f(m[qt] - mx) * grow;
@@ -966,17 +971,8 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                 l[qt] = RIDES ? fmaf(sum, ri[h], l[qt]) : l[qt] + sum;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float a = SPLIT ? pf[2 * e] * rv[h] : pf[2 * e], bq = SPLIT ? pf[2 * e + 1] * rv[h] : pf[2 * e + 1];
-                    // the products as rounded here: fused into the conversions, the two
-                    // uses of hi below could differ by one of its steps
-                    if constexpr (SPLIT) asm("" : "+v"(a), "+v"(bq));
-                    if constexpr (SPLIT) {
-                        const f16 ah = (f16)a, bh = (f16)bq;
-                        ph[qt][h][e] = pack_f16((float)ah, (float)bh);
-                        pl[qt][h][e] = pack_f16(a - (float)ah, bq - (float)bh);
-                    } else {
-                        ph[qt][h][e] = pack_f16(a, bq);
-                    }
+                    if constexpr (SPLIT) split_f16<true>(pf[2 * e] * rv[h], pf[2 * e + 1] * rv[h], ph[qt][h][e], pl[qt][h][e]);
+                    else ph[qt][h][e] = pack_f16(pf[2 * e], pf[2 * e + 1]);
                 }
             }
         }
