@@ -35,7 +35,7 @@
 //   f32 3 x 37 rows x 8 heads x 64, up to 211 keys         8.0   latency, matrix pipe
 //   int8 128 beams x 8 heads x 64, up to 448 keys, table  14.3   VALU issue 68%
 //   int8 4 rows x 16 (4) heads x 128, up to 32768 keys    23.4 + 4.7 to join: 92 MB, 3.9 TB/s
-//   int8, f32 8 x 200 rows x 8 heads x 64, up to 1025     18.0   VALU issue 65%: conversions
+//   int8, f32 8 x 200 rows x 8 heads x 64, up to 1025     17.6   VALU issue 65%: conversions
 #include "decoder.hpp"
 
 namespace pkx {

@@ -239,7 +239,7 @@ CACHE = [
     ("f16", 2, 8, 2, 2, 16, 333, False, False), ("f16", 2, 40, 4, 2, 128, 90, False, True), ("f16", 1, 2, 16, 1, 48, 1, True, False),
     ("f32", 1, 1, 8, 8, 64, 18, True, False), ("f32", 6, 1, 4, 4, 128, 100, True, True), ("f32", 2, 70, 2, 1, 64, 200, True, False),
     # many rows over few keys: a weight's two f16 terms that do not add up to it are seen
-    ("f32", 4, 128, 8, 8, 64, 48, False, False),
+    ("f32", 4, 128, 8, 8, 64, 48, False, False), ("f32", 2, 1500, 64, 64, 128, 150, False, False),
     # the many-row kernel: causal and not, keys split and whole; sizes just short of it
     ("f16", 6, 150, 32, 16, 128, 1100, True, False), ("f16", 6, 130, 32, 8, 80, 1230, False, False),
     ("f32", 6, 150, 32, 16, 128, 1100, False, False), ("f32", 6, 130, 32, 8, 112, 1230, True, False),
