@@ -29,7 +29,7 @@ struct DecAttnParams {
     const uint8_t* mask = nullptr;  int64_t mask_item = 0;   // [B][n_k], 0: the key is not attended
     int B = 0, n_q = 0, n_k = 0, Hkv = 0, G = 1, dk = 0;
     int causal = 0;      // query i of n sees keys t <= len - n + i
-    float scale = 1.0f;
+    float scale = 1.0f, scale_lo = 0.0f;      // in launches: scale log2 e, what its rounding left
     int splits = 1, split_keys = 0;
     float* part_o = nullptr;      // [row][split][D]
     float2* part_ml = nullptr;    // [row][split] {running maximum (log2 units), sum}

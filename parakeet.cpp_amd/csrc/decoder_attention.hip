@@ -35,13 +35,13 @@
 //   f32 3 x 37 rows x 8 heads x 64, up to 211 keys         8.0   latency, matrix pipe
 //   int8 128 beams x 8 heads x 64, up to 448 keys, table  14.3   VALU issue 68%
 //   int8 4 rows x 16 (4) heads x 128, up to 32768 keys    23.4 + 4.7 to join: 92 MB, 3.9 TB/s
-//   int8, f32 8 x 200 rows x 8 heads x 64, up to 1025     17.6   VALU issue 65%: conversions
+//   int8, f32 8 x 200 rows x 8 heads x 64, up to 1025     19.0   VALU issue 65%: conversions
 #include "decoder.hpp"
 
 namespace pkx {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr float kNoMax = -3.0e38f;   // below every score: m - m' is finite from the start
 
 __device__ __forceinline__ float xgroup_max(float x) {
@@ -265,7 +265,7 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
 // Two values as pairs of f16 terms: what the rounding leaves is exact in f32.  The first
 // terms are formed twice, and once from a product fused into the conversion they could
 // differ by one of their steps, so either they are taken from their register (fewer
-// instructions: 8 prompts of 200 rows 18.6 -> 17.6 us) or the values are (fewer
+// instructions: 8 prompts of 200 rows 18.6 us, so 17.6) or the values are (fewer
 // registers, where all are in use).
 template <bool VALUES> __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
     if constexpr (VALUES) asm("" : "+v"(a), "+v"(b));
@@ -278,13 +278,14 @@ template <bool VALUES> __device__ __forceinline__ void split_f16(float a, float 
 // Row m of an item and key head as lane group g's fragments (LAYOUT: the kind
 // of keys whose order of dimensions they meet); returns its query index.  Rows past the queries are zeros.
 template <int KV, bool QF32, int D, int LAYOUT, int NQ>
-__device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, int kh, int cnt, int g, uint32_t (&q)[NQ], float& qf) {
+__device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, int kh, int cnt, int g, uint32_t (&q)[NQ], float& qf, float& qf_lo) {
     const int i = udiv_small(m, p.G), h = kh * p.G + (m - i * p.G);
     const bool live = i < cnt;
     // rows past the queries and pieces past the head's dimensions read another
     // row's or piece instead and become zeros: the loads wait on no branch
     const int64_t at = b * p.q_item + (live ? i * p.q_row : 0) + h * p.q_head;
     qf = p.scale;
+    qf_lo = p.scale_lo;
     if constexpr (KV == KV_F32) {
         float4v x[D / 16];
 #pragma unroll
@@ -335,6 +336,7 @@ __device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, 
         ex = ex < -100 ? -100 : ex;
         const float f = ldexpf(1.0f, 14 - ex);
         qf *= ldexpf(1.0f, ex - 14);
+        qf_lo *= ldexpf(1.0f, ex - 14);
 #pragma unroll
         for (int n = 0; n < D / 32; ++n)
 #pragma unroll
@@ -347,32 +349,40 @@ __device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, 
 template <int KV, int D, bool QF32, int NQ>
 __device__ __forceinline__ float4v tile_scores(const uint32_t (&k)[Tile<KV, D>::NK], const uint32_t (&q)[NQ]) {
     float4v acc = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (KV == KV_F32) {
+    if constexpr (KV == KV_F32) {      // two sums of half the length, for their rounding
+        float4v odd = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < D / 4; ++i)
+        for (int i = 0; i < D / 4; i += 2) {
             acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i]), __uint_as_float(q[i]), acc, 0, 0, 0);
+            odd = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[i + 1]), __uint_as_float(q[i + 1]), odd, 0, 0, 0);
+        }
+        acc += odd;
     } else {
+        // (the second terms' products first: the sum is rounded at its full size in
+        // those of the first only)
+        half8v a[D / 32];
 #pragma unroll
         for (int s = 0; s < D / 32; ++s) {
-            int4v a;
+            int4v w;
             if constexpr (KV == KV_F16) {
-                a = (int4v){(int)k[4 * s], (int)k[4 * s + 1], (int)k[4 * s + 2], (int)k[4 * s + 3]};
+                w = (int4v){(int)k[4 * s], (int)k[4 * s + 1], (int)k[4 * s + 2], (int)k[4 * s + 3]};
             } else {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    a[2 * h] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c010c00));
-                    a[2 * h + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c030c02));
+                    w[2 * h] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c010c00));
+                    w[2 * h + 1] = i8_pair_f16(__builtin_amdgcn_perm(0, k[2 * s + h], 0x0c030c02));
                 }
             }
-            const half8v af = __builtin_bit_cast(half8v, a);
-            const int4v b = {(int)q[4 * s], (int)q[4 * s + 1], (int)q[4 * s + 2], (int)q[4 * s + 3]};
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, __builtin_bit_cast(half8v, b), acc, 0, 0, 0);
-            if constexpr (KV == KV_I8 && QF32) {
-                const int o = D / 8 + 4 * s;
-                const int4v bl = {(int)q[o], (int)q[o + 1], (int)q[o + 2], (int)q[o + 3]};
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(af, __builtin_bit_cast(half8v, bl), acc, 0, 0, 0);
-            }
+            a[s] = __builtin_bit_cast(half8v, w);
         }
+#pragma unroll
+        for (int part = KV == KV_I8 && QF32 ? 1 : 0; part >= 0; --part)
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s) {
+                const int o = part * (D / 8) + 4 * s;
+                const int4v b = {(int)q[o], (int)q[o + 1], (int)q[o + 2], (int)q[o + 3]};
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a[s], __builtin_bit_cast(half8v, b), acc, 0, 0, 0);
+            }
     }
     return acc;
 }
@@ -419,7 +429,7 @@ __device__ __forceinline__ void work_of(int bid, const DecAttnParams& p, int mt,
 }
 
 // Workgroups to a CU: as many as the registers allow without spilling (f32,
-// d_head 128, 54 rows x 334 keys x 56 heads: 25.4 us at one, 22.1 at two; f32, 64: one
+// d_head 128, 54 rows x 334 keys x 56 heads: 25.4 us at one, 22.1 at two (20.3 by now); f32, 64: one
 // more than three spills, 18.1 -> 19.4).
 constexpr int attn_wgs(int kv, int d) { return d > 64 ? 2 : kv == KV_F32 && d > 32 ? 3 : 4; }
 
@@ -479,8 +489,8 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
 
     // queries: B operand, column c = row m0 + c
     uint32_t q[NQ];
-    float qf;            // factor of the scores
-    const int qi = load_query<KV, QF32, D, KV>(p, m0 + c, b, kh, cnt, g, q, qf);
+    float qf, qf_lo;     // factor of the scores, what its rounding left
+    const int qi = load_query<KV, QF32, D, KV>(p, m0 + c, b, kh, cnt, g, q, qf, qf_lo);
     const int lim = p.causal ? T - cnt + qi + 1 : T;       // keys below it are seen
 
     float4v o[NJ];
@@ -526,29 +536,47 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
         uint32_t ph[4], pl[4];
         const float4v s0 = tile_scores<KV, D, QF32, NQ>(t.k[0], q);
         const float4v s1 = tile_scores<KV, D, QF32, NQ>(t.k[1], q);
-        float sc[8];
+        // f32: the factor f of a score in two terms, and a weight's exponent s f - max
+        // rounded as a whole, since an error of 2^-24 of a score of 17 is one of 7e-7 of
+        // its weight (with the table, where every key has a factor of its own, neither: 128
+        // beams x 8 heads x 64 took 19.4 us instead of 15.0)
+        float sv[8], fe[8], fl[8], sc[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            sc[e] = s0[e] * (TABLE ? qf * ks8[e] : KV == KV_I8 ? qf * t.ks : qf);
-            sc[4 + e] = s1[e] * (TABLE ? qf * ks8[4 + e] : KV == KV_I8 ? qf * t.ks : qf);
+        for (int e = 0; e < 8; ++e) {
+            sv[e] = e < 4 ? s0[e & 3] : s1[e & 3];
+            const float ks = TABLE ? ks8[e] : KV == KV_I8 ? t.ks : 1.0f;
+            fe[e] = KV == KV_I8 ? qf * ks : qf;
+            if constexpr (QF32 && !TABLE) fl[e] = KV == KV_I8 ? fmaf(qf_lo, ks, fmaf(qf, ks, -fe[e])) : qf_lo;
+            sc[e] = sv[e] * fe[e];
         }
-        if (!whole || t0 + 32 > all) {
-            const uint32_t see = keep >> (4 * g) & low_bits(lim - t0 - 4 * g);
+        const bool cut = !whole || t0 + 32 > all;
+        const uint32_t see = keep >> (4 * g) & low_bits(lim - t0 - 4 * g);
+        auto leave_out = [&](float (&x)[8]) {
+            if (cut) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (!(see & (1u << (e < 4 ? e : 12 + e)))) sc[e] = -INFINITY;
-        }
+                for (int e = 0; e < 8; ++e)
+                    if (!(see & (1u << (e < 4 ? e : 12 + e)))) x[e] = -INFINITY;
+            }
+        };
+        leave_out(sc);
         const float top = max8((float4v){sc[0], sc[1], sc[2], sc[3]}, (float4v){sc[4], sc[5], sc[6], sc[7]});
         const float mx = xgroup_max(fmaxf(m, top));
         const float alpha = __builtin_amdgcn_exp2f(m - mx);
         m = mx;
-        // weights, and so l and O, are 2^14 p where they go to f16: down to 2^-28
-        // of the largest they keep its 11 bits, then 2^-39 of it
-        const float off = KV == KV_F32 ? mx : mx - 14.0f;
+        if constexpr (QF32 && !TABLE) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sc[e] = fmaf(sv[e], fl[e], fmaf(sv[e], fe[e], -mx));
+            leave_out(sc);
+        } else {
+            // weights, and so l and O, are 2^14 p where they go to f16 alone: down to
+            // 2^-28 of the largest they keep its 11 bits, then 2^-39 of it
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sc[e] -= QF32 ? mx : mx - 14.0f;
+        }
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            pf[e] = __builtin_amdgcn_exp2f(sc[e] - off);
+            pf[e] = __builtin_amdgcn_exp2f(sc[e]);
             sum += pf[e];
         }
         l = l * alpha + sum;
@@ -568,12 +596,15 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
                 for (int e = 0; e < 8; ++e) pf[e] *= inv;
                 vf = top * 0x1p-14f;
             } else {
-                vf = t.vs;
+                vf = SPLIT ? t.vs * 0x1p-14f : t.vs;
             }
         }
         if constexpr (SPLIT) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) split_f16<false>(pf[2 * e], pf[2 * e + 1], ph[e], pl[e]);
+            for (int e = 0; e < 4; ++e) {
+                const float up = TABLE ? 1.0f : 0x1p14f;
+                split_f16<false>(pf[2 * e] * up, pf[2 * e + 1] * up, ph[e], pl[e]);
+            }
         } else if constexpr (KV != KV_F32) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) ph[e] = pack_f16(pf[2 * e], pf[2 * e + 1]);
@@ -723,7 +754,7 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
 // Weights go to f16 as 2^14 p r, r = (value scale of the block) / (largest so
 // far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
 // different scales add up in one accumulator, which is rescaled when v grows.
-// 2^14 rides in the exponent, and r too where f16's 11 bits are what is kept.
+// 2^14 and r ride in the exponent where f16's 11 bits are what is kept.
 //
 // f16, 16 x 448 rows x 8 heads x 128, 750 keys: 42.6 us alone, 38.2 in a stream of
 // such calls (575 TFLOP/s; a large product of the library reaches 1071), 118 on
@@ -776,7 +807,8 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     int lim[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        const int i = load_query<KV, QF32, D, KV_F16>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt]);
+        float lo;
+        const int i = load_query<KV, QF32, D, KV_F16>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt], lo);
         lim[qt] = CAUSAL ? T - cnt + i + 1 : T;
         if (p.scale < 0.f) {       // the factor is not negative: maxima are taken before it
             qf[qt] = -qf[qt];
@@ -929,6 +961,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                 rv[h] = vref > 0.f ? fmaxf(vs[h] / vref, 0x1p-60f) : 1.f;
                 ri[h] = 1.0f / rv[h];
                 rl[h] = __builtin_amdgcn_logf(rv[h]);
+                if constexpr (SPLIT) rv[h] *= 0x1p14f;
             }
         }
         uint32_t ph[QT][2][4], pl[QT][2][4];
@@ -960,7 +993,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
             for (int h = 0; h < 2; ++h) {
                 // where p goes to f16 alone the factor r rides in the exponent
                 constexpr bool RIDES = KV == KV_I8 && !SPLIT;
-                const float off = 14.0f - mx + (RIDES ? rl[h] : 0.f);
+                const float off = SPLIT ? -mx : 14.0f - mx + (RIDES ? rl[h] : 0.f);
                 float pf[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -1021,7 +1054,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const float ll = l[qt];
         const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
         if (i >= cnt) continue;
-        const float unit = KV == KV_I8 ? vref : 1.0f;
+        const float unit = SPLIT ? vref * 0x1p-14f : KV == KV_I8 ? vref : 1.0f;
         if (p.splits > 1) {
             const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
             if (g == 0) p.part_ml[at] = float2{m[qt], ll};
@@ -1203,7 +1236,9 @@ void launch_dec_attention(DecAttnParams p, void* ws, size_t ws_bytes, hipStream_
     const size_t need = dec_attention_workspace(p);
     require(need == 0 || (ws && (uintptr_t)ws % 16 == 0 && ws_bytes >= need),
             "attention: the workspace is smaller than its size query says, or not 16-byte aligned");
-    p.scale *= kLog2e;
+    const double scale = (double)p.scale * kLog2e;
+    p.scale = (float)scale;
+    p.scale_lo = (float)(scale - p.scale);
     p.splits = sh.splits;
     p.split_keys = sh.keys;
     if (need) {
