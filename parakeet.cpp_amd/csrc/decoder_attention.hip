@@ -740,6 +740,13 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
     store(wk, x, mm, ll);
 }
 
+// Exponent field of the power of two at or above a finite scale x >= 0, 0 for none.
+__device__ __forceinline__ int scale_exponent(float x) {
+    const uint32_t u = (uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x));
+    const int e = (int)((u + 0x7fffffu) >> 23);
+    return u == 0 ? 0 : e < 1 ? 1 : e > 254 ? 254 : e;
+}
+
 // Many query rows against the same keys: 128 rows a workgroup, 32 a wave, the
 // keys in steps of 64 through LDS, where every wave reads them.  8-bit keys
 // become f16 on the way in, once for the workgroup.  The value rows are turned
@@ -751,9 +758,15 @@ __global__ __launch_bounds__(256, attn_wgs(KV, D)) void dec_attn_kernel(DecAttnP
 // (64 of 4 bytes here: with a permutation that repeats after 8 rows the reads of
 // 256-byte rows took twice as long).
 //
-// Weights go to f16 as 2^14 p r, r = (value scale of the block) / (largest so
-// far, v): 2^14 keeps small weights out of f16's subnormals, r lets blocks of
-// different scales add up in one accumulator, which is rescaled when v grows.
+// Weights go to f16 as 2^14 p r, r = (value scale of the block) / u: 2^14 keeps
+// small weights out of f16's subnormals, r lets the two blocks of a step add up in
+// one accumulator, whose unit u is the power of two at or above the larger of
+// their scales.  The accumulator is brought from step to step's unit along with
+// the running maximum, without a rounding; two blocks more than 2^6 apart are taken
+// one after the other.  So r is at least 2^-7 and a weight keeps f16's 11 bits
+// down to 2^-21 of the largest, whatever other blocks hold that the row does not
+// see or has no weight for.  (u stays above 2^-72 of its largest so far, for the
+// accumulator's range in f32; r falls below 2^-7 only from there on.)
 // 2^14 and r ride in the exponent where f16's 11 bits are what is kept.
 //
 // f16, 16 x 448 rows x 8 heads x 128, 750 keys: 42.6 us alone, 38.2 in a stream of
@@ -827,7 +840,8 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     const int k1 = ke < hi ? (int)ke : hi;
 
     float4v o[QT][NJ];
-    float m[QT], l[QT], vref = 0.f;
+    float m[QT], l[QT];
+    int unit_e = 0, unit_top = 0;     // exponent field of the accumulator's unit (0: no value yet), its largest
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         m[qt] = kNoMax;
@@ -950,15 +964,17 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const bool cut = keep != ~0ull || t0 + KT > all_wave;
         float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f;
         if constexpr (KV == KV_I8) {
-            const float top = fmaxf(vref, fmaxf(vs[0], vs[1]));
-            if (top > vref) {
-                grow = vref / top;
-                vref = top;
+            const int e0 = scale_exponent(vs[0]), e1 = scale_exponent(vs[1]), e = e0 > e1 ? e0 : e1;
+            if (e != 0) {
+                unit_top = e > unit_top ? e : unit_top;
+                const int to = e > unit_top - 72 ? e : unit_top - 72;
+                grow = ldexpf(1.0f, unit_e - to);
+                unit_e = to;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // (a block of zeros: any factor, so that the weights' sum survives)
-                rv[h] = vref > 0.f ? fmaxf(vs[h] / vref, 0x1p-60f) : 1.f;
+                // (a block of zeros: a factor that leaves nothing in f16 but the weights' sum in f32)
+                rv[h] = fmaxf(ldexpf(vs[h], 127 - unit_e), 0x1p-60f);
                 ri[h] = 1.0f / rv[h];
                 rl[h] = __builtin_amdgcn_logf(rv[h]);
                 if constexpr (SPLIT) rv[h] *= 0x1p14f;
@@ -1036,14 +1052,27 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     };
 
     if (k0 < k1) load(k0);
-    for (int t0 = k0; t0 < k1; t0 += KT) {
-        const uint64_t keep = __ballot(t0 + lane < T && mr8 != 0);     // the same in every wave
-        const float ks[2] = {ksr[0], ksr[1]}, vs[2] = {vsr[0], vsr[1]};
+    bool second = false;       // the second half of a step whose blocks' scales are far apart: loaded and staged again
+    for (int t0 = k0; t0 < k1;) {
+        uint64_t keep = __ballot(t0 + lane < T && mr8 != 0);           // the same in every wave
+        const float ks[2] = {ksr[0], ksr[1]};
+        float vs[2] = {vsr[0], vsr[1]};
         stage(keep);
         __syncthreads();
-        if (t0 + KT < k1) load(t0 + KT);
+        int next = t0 + KT;
+        if constexpr (KV == KV_I8) {
+            const int e0 = scale_exponent(vs[0]), e1 = scale_exponent(vs[1]);
+            if (e0 != 0 && e1 != 0 && (e0 > e1 + 6 || e1 > e0 + 6)) {
+                keep &= second ? 0xffffffff00000000ull : 0xffffffffull;
+                vs[0] = vs[1] = second ? vs[1] : vs[0];
+                second = !second;
+                next = second ? t0 : next;
+            }
+        }
+        if (next < k1) load(next);
         if (!CAUSAL || t0 < hi_wave) compute(t0, keep, ks, vs);
         __syncthreads();
+        t0 = next;
     }
 
 #pragma unroll
@@ -1054,7 +1083,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const float ll = l[qt];
         const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
         if (i >= cnt) continue;
-        const float unit = SPLIT ? vref * 0x1p-14f : KV == KV_I8 ? vref : 1.0f;
+        const float unit = KV == KV_I8 ? ldexpf(unit_e != 0 ? 1.0f : 0.f, unit_e - (SPLIT ? 141 : 127)) : 1.0f;
         if (p.splits > 1) {
             const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
             if (g == 0) p.part_ml[at] = float2{m[qt], ll};

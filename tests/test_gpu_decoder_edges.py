@@ -1,0 +1,85 @@
+"""The attention decoder operators where their arithmetic or their addresses are at an end, against decoder_ref.py."""
+import numpy as np
+import pytest
+
+import decoder_ref as ref
+from test_gpu_decoder import HostCache, dev, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def small_weights(q, k, v, scale, keep, least):
+    """sum over kept keys of min(p, least) |v|: what rounding weights to multiples of `least` may lose."""
+    s = np.where(keep, np.asarray(q, np.float64) @ np.asarray(k, np.float64).T * scale, -np.inf)
+    p = np.exp(s - s.max(1, keepdims=True))
+    return np.minimum(p, least) @ np.abs(np.asarray(v, np.float64))
+
+
+def check_scaled(got, q, k, v, scale, keep, f16, d, label):
+    """Within the roundings of every key's own block, however large the other blocks' values are: the bound of
+    decoder_ref with a weight's absolute error at most 2^-32 (a sixteen-bit term of 2^14 p r, r at least 2^-7, is
+    off by 2^-25 at most where it is subnormal) and never more than the weight."""
+    want = list(ref.attention(q, k, v, scale, keep))
+    low = small_weights(q, k, v, scale, keep, 2.0 ** -32)
+    want[2] = 0 * want[2]
+    err, bound = np.abs(got.astype(np.float64) - want[0]), ref.attention_bound(want, f16, d) + low
+    worst = float((err / bound).max())
+    print(f"[{label}] largest error {err.max():.2e} of values up to {np.abs(want[0]).max():.2e}, {worst:.2f} of its bound", flush=True)
+    assert np.isfinite(got).all() and worst <= 1.0
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("nq", [2, 256])
+@pytest.mark.parametrize("d", [80, 128])
+def test_cache_blocks_of_small_values_next_to_large_ones(gpu, stream, type, nq, d):
+    """Rows whose weights all lie in one block with values 2^40 below the other blocks' (few rows, and enough for the
+    many-row kernel): first, last, either half of a 64-key step."""
+    print(f"[scales] {type} nq={nq} d={d}", flush=True)
+    rng = np.random.default_rng(nq + d)
+    R, H, n = 4, 16, 1920
+    c = HostCache(gpu, stream, R, H, n, d, rng)
+    wanted = [0, n // 32 - 1, 20, 33]
+    c.k[:] = 0
+    c.k[..., 1] = rng.integers(-127, 128, c.k.shape[:-1])
+    c.ks[:] = 2.0 ** -7
+    c.vs[:] = 2.0 ** 34 * rng.uniform(0.6, 1, c.vs.shape)
+    for r, b in enumerate(wanted):
+        c.k[r, :, 32 * b:32 * b + 32, 0] = 127
+        c.vs[r, :, b] = 2.0 ** -6 * rng.uniform(0.6, 1, H)
+    for a, x in ((c.dev.k, c.k), (c.dev.k_scale, c.ks), (c.dev.v_scale, c.vs)):
+        a.upload(x, stream)
+    dt = np.float16 if type == "f16" else np.float32
+    q = np.zeros((R, nq, H, d), dt)
+    q[..., 0] = 101          # other blocks: weights e^-100
+    q[..., 1] = rng.standard_normal(q.shape[:-1])
+    out = gpu.DeviceArray(q.shape, dt)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream), causal=False, scale=1.0)(stream)
+    got = out.numpy(stream)
+    for r in range(R):
+        K, V = (ref.values(x, y, np.full(n, r), np.arange(n)) for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        for h in (0, H - 1):
+            check_scaled(got[r, :, h], q[r, :, h], K[:, h], V[:, h], 1.0, np.ones((nq, n), bool), type == "f16", d, f"r{r} h{h}")
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+def test_cache_blocks_that_a_row_does_not_see(gpu, stream, type):
+    """Causal rows in front of a block whose values are 2^40 times those that they see."""
+    rng = np.random.default_rng(40)
+    R, H, n, nq, d = 4, 16, 1920, 256, 128
+    c = HostCache(gpu, stream, R, H, n, d, rng)
+    first = [n - 32, n - 64, n - 128, n - 160]
+    c.vs[:] = 2.0 ** -6 * rng.uniform(0.6, 1, c.vs.shape)
+    for r, t in enumerate(first):
+        c.vs[r, :, t // 32:] = 2.0 ** 34
+    c.dev.v_scale.upload(c.vs, stream)
+    dt = np.float16 if type == "f16" else np.float32
+    q = (rng.standard_normal((R, nq, H, d)) * 0.7).astype(dt)
+    out = gpu.DeviceArray(q.shape, dt)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream))(stream)
+    got = out.numpy(stream)
+    for r in range(R):
+        K, V = (ref.values(x, y, np.full(n, r), np.arange(n)) for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        m = first[r] - (n - nq)          # rows that see nothing of it
+        keep = np.arange(n)[None] <= (n - nq + np.arange(m))[:, None]
+        for h in (0, H - 1):
+            check_scaled(got[r, :m, h], q[r, :m, h], K[:, h], V[:, h], d ** -0.5, keep, type == "f16", d, f"r{r} h{h}")
