@@ -391,6 +391,14 @@ typedef struct {
     float *k_scale, *v_scale;            /* dev [n_slots][n_kv_heads][capacity / PKX_CACHE8_BLOCK] */
 } pkx_cache8;
 
+/* Clear: the scales of row r's slot become 0, so that it reads as zeros and holds nothing of what it held.  A slot's
+ * scales are cleared, here or by the caller, before a sequence whose first append to it does not start a block: an
+ * append inside a block takes the block's scale for that of tokens it is to keep, and a larger one left from another
+ * sequence, or from fresh memory, coarsens the new tokens without an error.  That is what happens to beams that share
+ * a prompt in one slot and go on in their own.  Rows with a slot out of range are skipped. */
+int pkx_cache8_clear(const pkx_cache8* c, int n_rows, const int32_t* slot /* dev [n_rows], or NULL: row r is slot r */,
+                     void* stream);
+
 /* Append: tokens 0..count[r] of row r become positions start[r].. of its slot.  With s the
  * block's scale (0 where the block starts with a new token), s' = max(s, max|x| / 127) over the
  * block's new elements x of that head, a new element is held as round(x / s') within +-127 and an

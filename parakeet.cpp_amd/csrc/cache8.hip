@@ -1,4 +1,4 @@
-// The 8-bit key/value cache: appending tokens and reading them back.
+// The 8-bit key/value cache: clearing slots, appending tokens and reading them back.
 //
 // A block is 32 tokens of one slot and head; its scale is s = max |x| / 127
 // over the values appended to it so far, and a value is held as
@@ -171,6 +171,17 @@ template <bool F32> __global__ __launch_bounds__(256) void cache8_append_one_ker
     }
 }
 
+// The scales of a slot, 8 bytes for 64 x d_head held: a launch and little else, once a sequence.
+__global__ __launch_bounds__(256) void cache8_clear_kernel(Cache8 c, const int* slots) {
+    const int r = blockIdx.x, slot = slots ? slots[r] : r;
+    if ((unsigned)slot >= (unsigned)c.n_slots) return;
+    const int64_t n = (int64_t)c.Hkv * (c.cap / kCacheBlock), step = (int64_t)gridDim.y * 256;
+    for (int64_t i = (int64_t)blockIdx.y * 256 + threadIdx.x; i < n; i += step) {
+        c.k_scale[slot * n + i] = 0.f;
+        c.v_scale[slot * n + i] = 0.f;
+    }
+}
+
 // Eight values of K and V per thread: tokens start[r] .. + n of row r's slot as q * scale.
 // Bound by what it writes, 4 bytes a value: 128 rows x 32 tokens x 8 heads x 64, 16.8 MB,
 // 7.2 us.
@@ -208,6 +219,12 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(CacheReadParams p, int
 }
 
 }  // namespace
+
+void launch_cache8_clear(const Cache8& c, int rows, const int* slot, hipStream_t s) {
+    if (rows == 0) return;
+    const int64_t pieces = ((int64_t)c.Hkv * (c.cap / kCacheBlock) + 1023) / 1024;     // four scales a thread
+    launch(cache8_clear_kernel, dim3((unsigned)rows, (unsigned)(pieces < 64 ? pieces : 64)), dim3(256), 0, s, c, slot);
+}
 
 void launch_cache8_append(const CacheAppendParams& p, hipStream_t s) {
     if (p.R == 0 || p.n_new == 0) return;

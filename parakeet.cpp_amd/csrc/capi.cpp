@@ -757,6 +757,15 @@ int pkx_cross_attention(const pkx_cross_attn* a, void* ws, size_t ws_bytes, void
     });
 }
 
+int pkx_cache8_clear(const pkx_cache8* c, int n_rows, const int32_t* slot, void* s) {
+    return guarded([&] {
+        const pkx::Cache8 o = cache_params(c);
+        need(n_rows >= 0, "cache clear: negative size");
+        need(slot || n_rows <= o.n_slots, "cache clear: more rows than slots");
+        need_device(st(s));
+        pkx::launch_cache8_clear(o, n_rows, slot, st(s));
+    });
+}
 int pkx_cache8_append(const pkx_cache8* c, const pkx_cache8_tokens* t, void* s) {
     return guarded([&] {
         pkx::CacheAppendParams p;

@@ -43,6 +43,9 @@ struct Cache8 {
     int8_t *k = nullptr, *v = nullptr;
     float *k_scale = nullptr, *v_scale = nullptr;
 };
+// The scales of row r's slot (slot NULL: slot r) become 0.
+void launch_cache8_clear(const Cache8& c, int rows, const int* slot, hipStream_t s);
+
 struct CacheAppendParams {
     Cache8 c;
     bool f32 = false;

@@ -149,6 +149,7 @@ SIGS = {
     "pkx_streaming_step": ([_vp, _vp, C.c_int, C.c_int, _vp, _ip, _vp], C.c_int),
     "pkx_cross_attention_workspace": ([_P(CrossAttnArgs), _P(_sz)], C.c_int),
     "pkx_cross_attention": ([_P(CrossAttnArgs), _vp, _sz, _vp], C.c_int),
+    "pkx_cache8_clear": ([_P(Cache8Args), _i32, _vp, _vp], C.c_int),
     "pkx_cache8_append": ([_P(Cache8Args), _P(Cache8Tokens), _vp], C.c_int),
     "pkx_cache8_read": ([_P(Cache8Args), _i32, _i32, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "pkx_cache8_attention_workspace": ([_P(Cache8Args), _P(Cache8AttnArgs), _P(_sz)], C.c_int),
@@ -677,12 +678,15 @@ class CrossAttention(_Bound):
 
 
 class Cache8:
-    """A key/value cache in 8 bits (pkx_cache8): k, v int8 [S][Hkv][capacity][d], scales f32 [S][Hkv][capacity / 32]."""
+    """A key/value cache in 8 bits (pkx_cache8): k, v int8 [S][Hkv][capacity][d], scales f32 [S][Hkv][capacity / 32].
+
+    A new cache's scales are zeros; a slot that is used again is cleared first (CacheClear) unless its next sequence
+    starts at the start of a block there."""
 
     def __init__(self, n_slots, n_kv_heads, d_head, capacity):
         n = (n_slots, n_kv_heads, capacity)
         self._set(*(DeviceArray(n + (d_head,), np.int8) for _ in range(2)),
-                  *(DeviceArray(n[:2] + (capacity // CACHE8_BLOCK,), np.float32) for _ in range(2)))
+                  *(DeviceArray.from_numpy(np.zeros(n[:2] + (capacity // CACHE8_BLOCK,), np.float32)) for _ in range(2)))
 
     @classmethod
     def wrap(cls, k, v, k_scale, v_scale):
@@ -707,6 +711,15 @@ def _table_row(table, rows, positions):
     if len(table.shape) != 2 or table.shape[0] != rows or table.shape[1] < positions or np.dtype(table.dtype) != np.int32:
         raise PkxError(f"cache table: int32 [{rows}][>= {positions}] is wanted, got {table.dtype} {list(table.shape)}")
     return _strides(table)[0]
+
+
+class CacheClear(_Bound):
+    """pkx_cache8_clear: slot [R] int32, or None: every slot."""
+
+    def __init__(self, cache, slot=None):
+        n = cache.n_slots if slot is None else slot.shape[0]
+        _expect(slot, (n,), np.int32, "cache clear")
+        self._bind("pkx_cache8_clear", (C.byref(cache.args), n, _ptr(slot)), (cache, slot))
 
 
 class CacheAppend(_Bound):

@@ -3,9 +3,15 @@ import numpy as np
 import pytest
 
 import decoder_ref as ref
-from test_gpu_decoder import HostCache, dev, i32
+from test_gpu_decoder import HostCache as DecoderCache, check_attention, dev, i32
 
 pytestmark = pytest.mark.gpu
+
+
+class HostCache(DecoderCache):
+    def same_scales(self, stream):
+        for a, b in ((self.dev.k_scale, self.ks), (self.dev.v_scale, self.vs)):
+            assert np.array_equal(a.numpy(stream), b, equal_nan=True)
 
 
 def small_weights(q, k, v, scale, keep, least):
@@ -83,3 +89,63 @@ def test_cache_blocks_that_a_row_does_not_see(gpu, stream, type):
         keep = np.arange(n)[None] <= (n - nq + np.arange(m))[:, None]
         for h in (0, H - 1):
             check_scaled(got[r, :m, h], q[r, :m, h], K[:, h], V[:, h], d ** -0.5, keep, type == "f16", d, f"r{r} h{h}")
+
+
+def test_new_cache_is_clear(gpu, stream):
+    """The scales of a new cache are zeros, whatever the memory held."""
+    old = [gpu.DeviceArray((3, 2, 64 // 32), np.float32) for _ in range(64)]
+    for a in old:
+        a.upload(np.full(a.shape, np.nan, np.float32), stream)
+    del old, a
+    for _ in range(8):
+        c = gpu.Cache8(3, 2, 32, 64)
+        assert not c.k_scale.numpy(stream).any() and not c.v_scale.numpy(stream).any()
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("prompt,d", [(50, 64), (33, 48), (31, 128)])
+def test_beams_share_a_prompt_in_slots_that_held_another_sequence(gpu, stream, type, prompt, d):
+    """A prompt in one slot that the beams' tables name, every beam's tokens from there on in its own slot, whose scales
+    are another sequence's (large, NaN) until they are cleared; a slot of another item is left as it was."""
+    print(f"[prompt] {type} {prompt} d={d}", flush=True)
+    rng = np.random.default_rng(prompt)
+    W, H, cap, steps = 4, 2, 128, 20
+    c = HostCache(gpu, stream, W + 2, H, cap, d, rng)
+    c.ks[:], c.vs[:] = 1e6, np.nan
+    c.dev.k_scale.upload(c.ks, stream)
+    c.dev.v_scale.upload(c.vs, stream)
+    slots = i32([4, 0, 3, 1])
+    gpu.CacheClear(c.dev, dev(gpu, i32([4, 0, -1, 3, 1, W + 2, 0]), stream))(stream)
+    c.ks[slots], c.vs[slots] = 0, 0
+    c.same_scales(stream)
+    dt = np.float16 if type == "f16" else np.float32
+    table, slot = dev(gpu, np.full((W, cap), -1, np.int32), stream), dev(gpu, slots, stream)
+    where = np.full((W, cap), -1)
+    where[:, :prompt] = slots[0]
+    x = [rng.standard_normal((1, prompt, H, d)).astype(dt) for _ in range(2)]
+    gpu.CacheAppend(c.dev, *(dev(gpu, a, stream) for a in x), start=dev(gpu, i32([0]), stream), slot=dev(gpu, slots[:1], stream))(stream)
+    for ints, scale, a in ((c.k, c.ks, x[0]), (c.v, c.vs, x[1])):
+        ref.append(ints, scale, a, slots[:1], [0], [prompt])
+    table.upload(i32(where), stream)
+    for t in range(prompt, prompt + steps):
+        x = [rng.standard_normal((W, 1, H, d)).astype(dt) for _ in range(3)]
+        gpu.CacheAppend(c.dev, *(dev(gpu, a, stream) for a in x[:2]), start=dev(gpu, i32([t] * W), stream), slot=slot, table=table)(stream)
+        for ints, scale, a in ((c.k, c.ks, x[0]), (c.v, c.vs, x[1])):
+            ref.append(ints, scale, a, slots, [t] * W, [1] * W)
+        where[:, t] = slots
+        out = gpu.DeviceArray((W, 1, H, d), dt)
+        gpu.CacheAttention(c.dev, dev(gpu, x[2], stream), out, dev(gpu, i32([t + 1] * W), stream), table=table)(stream)
+        got = out.numpy(stream)
+        for r in range(W):
+            K, V = (ref.values(a, b, where[r, :t + 1], np.arange(t + 1)) for a, b in ((c.k, c.ks), (c.v, c.vs)))
+            for h in range(H):
+                want = ref.attention(x[2][r, :, h], K[:, h], V[:, h], d ** -0.5, np.ones((1, t + 1), bool))
+                check_attention(got[r, :, h], want, type == "f16", d, f"t{t} r{r} h{h}")
+    c.same_scales(stream)
+    assert np.array_equal(c.dev.k.numpy(stream), c.k) and np.array_equal(c.dev.v.numpy(stream), c.v)
+    back = gpu.DeviceArray((W, steps, H, d), np.float32)
+    gpu.CacheRead(c.dev, back, None, start=dev(gpu, i32([prompt] * W), stream), slot=slot)(stream)
+    for r in range(W):
+        assert np.array_equal(back.numpy(stream)[r], ref.values(c.k, c.ks, np.full(steps, slots[r]), prompt + np.arange(steps)))
+    gpu.CacheClear(c.dev)(stream)
+    assert not c.dev.k_scale.numpy(stream).any() and not c.dev.v_scale.numpy(stream).any()
