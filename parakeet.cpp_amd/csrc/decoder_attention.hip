@@ -816,15 +816,15 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     const uint32_t k_row = (uint32_t)p.k_row * ES, v_row = (uint32_t)p.v_row * ES;
 
     uint32_t q[QT][NQ];
-    float qf[QT];
+    float qf[QT], qf_lo[QT];     // factor of the scores, what its rounding left
     int lim[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-        float lo;
-        const int i = load_query<KV, QF32, D, KV_F16>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt], lo);
+        const int i = load_query<KV, QF32, D, KV_F16>(p, m0 + 16 * qt + c, b, kh, cnt, g, q[qt], qf[qt], qf_lo[qt]);
         lim[qt] = CAUSAL ? T - cnt + i + 1 : T;
         if (p.scale < 0.f) {       // the factor is not negative: maxima are taken before it
             qf[qt] = -qf[qt];
+            qf_lo[qt] = -qf_lo[qt];
 #pragma unroll
             for (int n = 0; n < NQ; ++n) q[qt][n] ^= 0x80008000u;
         }
@@ -985,8 +985,19 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) {
             // (not zero, as for a block of zeros: -inf stays -inf)
-            const float f[2] = {fmaxf(KV == KV_I8 ? qf[qt] * ks[0] : qf[qt], 1e-37f),
-                                fmaxf(KV == KV_I8 ? qf[qt] * ks[1] : qf[qt], 1e-37f)};
+            float f[2], fl[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                f[h] = KV == KV_I8 ? qf[qt] * ks[h] : qf[qt];
+                if constexpr (SPLIT) {
+                    // in two terms, as in dec_attn_kernel, the first rounded down: the second is
+                    // not negative then, nor zero, and -inf stays -inf
+                    const bool above = fmaf(qf_lo[qt], ks[h], fmaf(qf[qt], ks[h], -f[h])) < 0.f;
+                    f[h] = __uint_as_float(__float_as_uint(f[h]) - (above ? 1 : 0));
+                    fl[h] = fmaxf(fmaf(qf_lo[qt], ks[h], fmaf(qf[qt], ks[h], -f[h])), 0x1p-126f);
+                }
+                f[h] = fmaxf(f[h], 1e-37f);
+            }
             if (cut) {
                 const int below = lim[qt] - t0 - 4 * g;
                 const uint32_t see[2] = {(uint32_t)keep >> (4 * g) & low_bits(below), (uint32_t)(keep >> 32) >> (4 * g) & low_bits(below - 32)};
@@ -1014,7 +1025,9 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float x = s[qt][2 * h + (e >> 2)][e & 3];
-                    pf[e] = __builtin_amdgcn_exp2f(fmaf(x, f[h], off));
+                    float y = fmaf(x, f[h], off);
+                    if constexpr (SPLIT) y = fmaf(x, fl[h], y);
+                    pf[e] = __builtin_amdgcn_exp2f(y);
                 }
                 const float sum = ((pf[0] + pf[1]) + (pf[2] + pf[3])) + ((pf[4] + pf[5]) + (pf[6] + pf[7]));
                 l[qt] = RIDES ? fmaf(sum, ri[h], l[qt]) : l[qt] + sum;

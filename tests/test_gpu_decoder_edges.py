@@ -149,3 +149,34 @@ def test_beams_share_a_prompt_in_slots_that_held_another_sequence(gpu, stream, t
         assert np.array_equal(back.numpy(stream)[r], ref.values(c.k, c.ks, np.full(steps, slots[r]), prompt + np.arange(steps)))
     gpu.CacheClear(c.dev)(stream)
     assert not c.dev.k_scale.numpy(stream).any() and not c.dev.v_scale.numpy(stream).any()
+
+
+@pytest.mark.parametrize("nq", [2, 256])
+@pytest.mark.parametrize("scale", [1.0, -1.0])
+def test_f32_queries_with_large_scores_on_the_cache(gpu, stream, nq, scale):
+    """Scores of 8128 nats whose keys differ by one at most, formed without a rounding but for the factors: a weight is
+    off by the roundings of its exponent, its two terms and the sums, not by 2^-24 of the score."""
+    rng = np.random.default_rng(nq)
+    R, H, n, d = 4, 16, 1920, 128
+    c = HostCache(gpu, stream, R, H, n, d, rng)
+    c.k[:] = 0
+    at = 32 * np.arange(n // 32) + rng.integers(0, 32, n // 32)      # one key a block
+    c.k[:, :, at, 0] = 127
+    c.ks[:] = 1 + rng.integers(0, 1 << 10, c.ks.shape) * 2.0 ** -23
+    for a, x in ((c.dev.k, c.k), (c.dev.k_scale, c.ks)):
+        a.upload(x, stream)
+    q = np.zeros((R, nq, H, d), np.float32)
+    q[..., 0] = 64 * scale
+    out = gpu.DeviceArray(q.shape, np.float32)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream), causal=False, scale=scale)(stream)
+    got, worst = out.numpy(stream).astype(np.float64), 0.0
+    for r in range(R):
+        K, V = (x[r].astype(np.float64) * np.repeat(y[r].astype(np.float64), 32, 1)[..., None] for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        for h in (0, H - 1):
+            o, a = ref.attention(q[r, :, h], K[h], V[h], scale, np.ones((nq, n), bool))[:2]
+            # a weight: 2^-22 of two terms, 2^-23 each of its exponential and of exponents below 1; n / 32 sums of
+            # 2^-24 and rescalings of as much; all of it once more in the sum that divides
+            bound = a * 2 * (2.0 ** -22 + 2 * 2.0 ** -23 + 2 * (n // 32) * 2.0 ** -24)
+            worst = max(worst, float((np.abs(got[r, :, h] - o) / bound).max()))
+    print(f"[large scores] nq={nq} {worst:.2f} of the bound", flush=True)
+    assert worst <= 1
