@@ -758,16 +758,18 @@ __device__ __forceinline__ int scale_exponent(float x) {
 // (64 of 4 bytes here: with a permutation that repeats after 8 rows the reads of
 // 256-byte rows took twice as long).
 //
-// Weights go to f16 as 2^14 p r, r = (value scale of the block) / u: 2^14 keeps
-// small weights out of f16's subnormals, r lets the two blocks of a step add up in
-// one accumulator, whose unit u is the power of two at or above the larger of
-// their scales.  The accumulator is brought from step to step's unit along with
-// the running maximum, without a rounding; two blocks more than 2^6 apart are taken
-// one after the other.  So r is at least 2^-7 and a weight keeps f16's 11 bits
-// down to 2^-21 of the largest, whatever other blocks hold that the row does not
-// see or has no weight for.  (u stays above 2^-72 of its largest so far, for the
-// accumulator's range in f32; r falls below 2^-7 only from there on.)
-// 2^14 and r ride in the exponent where f16's 11 bits are what is kept.
+// Weights go to f16 as 2^14 p: 2^14 keeps small ones out of f16's subnormals, and rides
+// in the exponent.  With 8-bit keys the accumulator's unit is the block's value scale,
+// whatever scales other blocks have that a row does not see or has no weight for.
+// f16: it changes from block to block, along with the running maximum before a step's first block and
+// by a product of its own between the two (2% of the time; the ratio of the scales in the
+// weights instead cost a dominating weight, else exact, its rounding: 6 x 150 rows x 32
+// heads x 128, 1100 tokens were off by 2.7e-4 of their size, so by 2.33e-4; the rounding of the output is 2.07e-4).
+// f32: the unit is the power of two at or above the larger scale of a step's two blocks,
+// so that it changes without a rounding and a weight's two terms carry r = scale / unit;
+// blocks more than 2^6 apart are taken one after the other, so r is at least 2^-7 and the terms
+// keep 22 bits of a weight down to 2^-9 of the largest, 11 of it down to 2^-21.
+// (The unit stays above 2^-72 of its largest so far, for the accumulator's range; r goes below that only from there on.)
 //
 // f16, 16 x 448 rows x 8 heads x 128, 750 keys: 42.6 us alone, 38.2 in a stream of
 // such calls (575 TFLOP/s; a large product of the library reaches 1071), 118 on
@@ -777,7 +779,7 @@ __device__ __forceinline__ int scale_exponent(float x) {
 template <int KV, bool QF32, int D, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
     constexpr int QT = 2, NW = 4, ROWS = 16 * QT * NW, KT = 64;
-    constexpr bool SPLIT = KV == KV_I8 && QF32;
+    constexpr bool SPLIT = KV == KV_I8 && QF32, RIDES = KV == KV_I8 && !QF32;
     constexpr int ES = KV == KV_F16 ? 2 : 1, NQ = SPLIT ? D / 4 : D / 8, NJ = D / 16;
     constexpr int PIECES = D * ES / 16, KP = KT * PIECES / 256;     // 16-byte pieces of a key row; of a thread
     constexpr int DV = D / 32;                                      // value dimensions of a thread
@@ -841,7 +843,9 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
 
     float4v o[QT][NJ];
     float m[QT], l[QT];
-    int unit_e = 0, unit_top = 0;     // exponent field of the accumulator's unit (0: no value yet), its largest
+    // the accumulator's unit (0: no value yet) and its largest; f32: their exponent fields
+    float unit = 0.f, unit_top = 0.f;
+    int unit_e = 0, top_e = 0;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         m[qt] = kNoMax;
@@ -962,22 +966,30 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         if constexpr (KV == KV_F16) __builtin_amdgcn_s_setprio(0);
         settled(s);
         const bool cut = keep != ~0ull || t0 + KT > all_wave;
-        float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f;
-        if constexpr (KV == KV_I8) {
+        float rv[2] = {1.f, 1.f}, ri[2] = {1.f, 1.f}, rl[2] = {0.f, 0.f}, grow = 1.f, grow2 = 1.f;
+        if constexpr (RIDES) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                // (a block of zeros: a factor that leaves nothing in f16 but the weights' sum in f32)
+                const float to = vs[h] > 0.f ? fmaxf(fmaxf(vs[h], unit_top * 0x1p-72f), 0x1p-126f) : unit;
+                const float inv = __builtin_amdgcn_rcpf(to), r = vs[h] > 0.f ? fmaxf(vs[h] * inv, 0x1p-60f) : 0x1p-60f;
+                (h == 0 ? grow : grow2) = to > 0.f ? unit * inv : 1.f;
+                unit = to;
+                unit_top = fmaxf(unit_top, to);
+                ri[h] = __builtin_amdgcn_rcpf(r);
+                rl[h] = __builtin_amdgcn_logf(r);
+            }
+        } else if constexpr (KV == KV_I8) {
             const int e0 = scale_exponent(vs[0]), e1 = scale_exponent(vs[1]), e = e0 > e1 ? e0 : e1;
             if (e != 0) {
-                unit_top = e > unit_top ? e : unit_top;
-                const int to = e > unit_top - 72 ? e : unit_top - 72;
+                top_e = e > top_e ? e : top_e;
+                const int to = e > top_e - 72 ? e : top_e - 72;
                 grow = ldexpf(1.0f, unit_e - to);
                 unit_e = to;
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // (a block of zeros: a factor that leaves nothing in f16 but the weights' sum in f32)
-                rv[h] = fmaxf(ldexpf(vs[h], 127 - unit_e), 0x1p-60f);
-                ri[h] = 1.0f / rv[h];
-                rl[h] = __builtin_amdgcn_logf(rv[h]);
-                if constexpr (SPLIT) rv[h] *= 0x1p14f;
+                rv[h] = fmaxf(ldexpf(vs[h], 127 - unit_e), 0x1p-60f) * 0x1p14f;
             }
         }
         uint32_t ph[QT][2][4], pl[QT][2][4];
@@ -1018,8 +1030,6 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
             m[qt] = mx;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                // where p goes to f16 alone the factor r rides in the exponent
-                constexpr bool RIDES = KV == KV_I8 && !SPLIT;
                 const float off = SPLIT ? -mx : 14.0f - mx + (RIDES ? rl[h] : 0.f);
                 float pf[8];
 #pragma unroll
@@ -1050,6 +1060,14 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
                 half8v a[JB];
 #pragma unroll
                 for (int j = 0; j < JB; ++j) a[j] = *(const half8v*)(sv + va[h][(j0 + j) & 1] + 16 * (j0 + j) * KT);
+                if constexpr (RIDES) {
+                    if (h == 1) {
+#pragma unroll
+                        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+                            for (int j = 0; j < JB; ++j) o[qt][j0 + j] *= grow2;
+                    }
+                }
 #pragma unroll
                 for (int part = 0; part < (SPLIT ? 2 : 1); ++part)
 #pragma unroll
@@ -1073,7 +1091,7 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         stage(keep);
         __syncthreads();
         int next = t0 + KT;
-        if constexpr (KV == KV_I8) {
+        if constexpr (SPLIT) {
             const int e0 = scale_exponent(vs[0]), e1 = scale_exponent(vs[1]);
             if (e0 != 0 && e1 != 0 && (e0 > e1 + 6 || e1 > e0 + 6)) {
                 keep &= second ? 0xffffffff00000000ull : 0xffffffffull;
@@ -1096,17 +1114,17 @@ __global__ __launch_bounds__(256, 2) void dec_tile_kernel(DecAttnParams p) {
         const float ll = l[qt];
         const int mr = m0 + 16 * qt + c, i = udiv_small(mr, p.G), h = kh * p.G + (mr - i * p.G);
         if (i >= cnt) continue;
-        const float unit = KV == KV_I8 ? ldexpf(unit_e != 0 ? 1.0f : 0.f, unit_e - (SPLIT ? 141 : 127)) : 1.0f;
+        const float out_unit = SPLIT ? ldexpf(unit_e != 0 ? 1.0f : 0.f, unit_e - 141) : RIDES ? unit : 1.0f;
         if (p.splits > 1) {
             const int64_t at = ((int64_t)(b * p.Hkv + kh) * M + mr) * p.splits + split;
             if (g == 0) p.part_ml[at] = float2{m[qt], ll};
             if (ll == 0.f) continue;
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
-                if (16 * j + 4 * g < p.dk) *(float4v*)(p.part_o + at * p.dk + 16 * j + 4 * g) = o[qt][j] * unit;
+                if (16 * j + 4 * g < p.dk) *(float4v*)(p.part_o + at * p.dk + 16 * j + 4 * g) = o[qt][j] * out_unit;
             continue;
         }
-        const float f = ll != 0.f ? unit / ll : 0.f;
+        const float f = ll != 0.f ? out_unit / ll : 0.f;
         const int64_t at = b * p.o_item + i * p.o_row + h * p.o_head + 4 * g;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {

@@ -180,3 +180,27 @@ def test_f32_queries_with_large_scores_on_the_cache(gpu, stream, nq, scale):
             worst = max(worst, float((np.abs(got[r, :, h] - o) / bound).max()))
     print(f"[large scores] nq={nq} {worst:.2f} of the bound", flush=True)
     assert worst <= 1
+
+
+@pytest.mark.parametrize("nq", [2, 256])
+@pytest.mark.parametrize("causal", [False, True])
+def test_one_dominating_key_of_the_cache_is_exact_in_f16(gpu, stream, nq, causal):
+    """A weight of 1 (the others' sum is below 2^-100) is exact in f16, whatever the blocks' scales: the output is the
+    key's value rounded to f16, half a step of 2^-11, and a few f32 roundings."""
+    rng = np.random.default_rng(nq + causal)
+    R, H, n, d = 4, 16, 1920, 128
+    c = HostCache(gpu, stream, R, H, n, d, rng)
+    c.k[:] = 0
+    at = np.array([5, 32 * 7 + 31, 32 * 40, n - 257])
+    c.k[np.arange(R), :, at, 0] = 127
+    c.ks[:] = 1
+    for a, x in ((c.dev.k, c.k), (c.dev.k_scale, c.ks)):
+        a.upload(x, stream)
+    q = np.zeros((R, nq, H, d), np.float16)
+    q[..., 0] = 1
+    out = gpu.DeviceArray(q.shape, np.float16)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream), causal=causal, scale=1.0)(stream)
+    got = out.numpy(stream).astype(np.float64)
+    for r in range(R):
+        v = c.v[r, :, at[r]].astype(np.float64) * c.vs[r, :, at[r] // 32, None]
+        assert (np.abs(got[r] - v[None]) <= (2.0 ** -11 + 2.0 ** -17) * np.abs(v) + 2.0 ** -25).all(), r
