@@ -472,7 +472,7 @@ int pkx_beam_select(const pkx_beam_select_args* a, void* ws, size_t ws_bytes, vo
 /* Reordering: row b * n_beams + w of every dst = row b * n_beams + parent[b][w] of its src, `bytes` of it
  * (prediction-network states, cache tables, ...); rows whose parent is out of range are left as they were.
  * states: host array of at most PKX_BEAM_MAX_STATES; row strides in bytes, at least `bytes` (src: or 0).
- * No src, from its first row to its last, overlaps a dst, and no row of a dst another dst's. */
+ * Neither parent nor a src, from its first row to its last, overlaps a dst, and no row of a dst another dst's. */
 #define PKX_BEAM_MAX_STATES 32
 typedef struct {
     const void* src;

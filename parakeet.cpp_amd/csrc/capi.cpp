@@ -861,9 +861,16 @@ int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_
             const pkx_beam_state& x = states[i];
             need(x.bytes >= 0 && (x.src_row >= x.bytes || x.src_row == 0) && x.dst_row >= x.bytes,
                  "beam reorder: row strides must be at least the row's bytes");
+            // (no span below wraps then, whichever state comes first)
+            need((double)rows * (double)std::max({x.src_row, x.dst_row, x.bytes}) < 0x1p62, "beam reorder: rows past the address space");
+        }
+        for (int i = 0; i < n_states; ++i) {
+            const pkx_beam_state& x = states[i];
             if (x.bytes > 0) {
                 need(x.src && x.dst, "beam reorder: null state");
                 const uintptr_t b = (uintptr_t)x.dst, be = b + (rows - 1) * x.dst_row + x.bytes;
+                const uintptr_t pa = (uintptr_t)parent, pe = pa + rows * sizeof(int32_t);
+                need(pe <= b || be <= pa, "beam reorder: parent overlaps a destination");
                 for (int j = 0; j < n_states; ++j) {
                     const uintptr_t a = (uintptr_t)states[j].src, ae = a + (rows - 1) * states[j].src_row + states[j].bytes;
                     need(states[j].bytes <= 0 || ae <= b || be <= a, "beam reorder: a source overlaps a destination");
