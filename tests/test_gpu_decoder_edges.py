@@ -204,3 +204,72 @@ def test_one_dominating_key_of_the_cache_is_exact_in_f16(gpu, stream, nq, causal
     for r in range(R):
         v = c.v[r, :, at[r]].astype(np.float64) * c.vs[r, :, at[r] // 32, None]
         assert (np.abs(got[r] - v[None]) <= (2.0 ** -11 + 2.0 ** -17) * np.abs(v) + 2.0 ** -25).all(), r
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("d", [32, 48, 128])
+def test_cache_far_slots_by_table(gpu, stream, type, d):
+    """Slots that together pass 2 GiB (3 of 2^30 bytes), rows that mix them by table up to the last position, entries out
+    of range between; every width of the kernel's loads."""
+    print(f"[far table] {type} d={d}", flush=True)
+    rng = np.random.default_rng(d)
+    S, H, G = 3, 2, 2
+    cap = (1 << 29) // d // 32 * 32
+    k, v = gpu.DeviceArray((S, H, cap, d), np.int8), gpu.DeviceArray((S, H, cap, d), np.int8)
+    assert S * H * cap * d > 1 << 31
+    sc = [rng.uniform(0.005, 0.02, (S, H, cap // 32)).astype(np.float32) for _ in range(2)]
+    c = gpu.Cache8.wrap(k, v, *(dev(gpu, a, stream) for a in sc))
+    pos = np.concatenate([a + np.arange(40) for a in (0, cap // 2 + 5, cap - 40)])
+    ints = [rng.integers(-127, 128, (S, H, len(pos), d)).astype(np.int8) for _ in range(2)]
+    for a, x in ((k, ints[0]), (v, ints[1])):
+        for s in range(S):
+            for h in range(H):
+                for i in range(0, len(pos), 40):
+                    run = np.ascontiguousarray(x[s, h, i:i + 40])
+                    gpu.check(gpu.lib().pkx_memcpy_h2d(a.ptr + ((s * H + h) * cap + int(pos[i])) * d, run.ctypes.data, run.nbytes, stream.handle))
+    table = np.full((2, cap), -1, np.int32)
+    table[1] = S
+    who = rng.integers(-1, S + 1, (2, len(pos)))
+    who[:, ::5] = 2
+    table[:, pos] = who
+    dt = np.float16 if type == "f16" else np.float32
+    q = rng.standard_normal((2, 1, H * G, d)).astype(dt)
+    out = gpu.DeviceArray(q.shape, dt)
+    lens = [cap, cap - 3]
+    gpu.CacheAttention(c, dev(gpu, q, stream), out, dev(gpu, i32(lens), stream), table=dev(gpu, table, stream))(stream)
+    got = out.numpy(stream)
+    for r in range(2):
+        keep = (who[r] >= 0) & (who[r] < S) & (pos < lens[r])
+        sl = np.where(keep, who[r], 0)
+        K, V = (x[sl, :, np.arange(len(pos))] * y[sl, :, pos // 32][..., None] for x, y in zip(ints, sc))
+        for h in range(H * G):
+            want = ref.attention(q[r, :, h], K[:, h // G], V[:, h // G], d ** -0.5, keep[None])
+            check_attention(got[r, :, h], want, type == "f16", d, f"far table r{r} h{h}")
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("R,nq,H,n,d,table", [(2, 3, 4, 130, 64, False), (2, 3, 4, 130, 48, True), (4, 256, 16, 1920, 128, False)])
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+@pytest.mark.parametrize("causal", [False, True])
+def test_cache_attention_scales(gpu, stream, type, R, nq, H, n, d, table, scale, causal):
+    """Any factor on 8-bit keys: negative, zero (the mean of the seen values), large; few rows, by table, many rows."""
+    rng = np.random.default_rng(n + nq)
+    c = HostCache(gpu, stream, R, H, (n + 31) // 32 * 32, d, rng)
+    dt = np.float16 if type == "f16" else np.float32
+    q = rng.standard_normal((R, nq, H, d)).astype(dt)
+    out, tab = gpu.DeviceArray(q.shape, dt), rng.integers(-1, R, (R, n)).astype(np.int32)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream), causal=causal, scale=scale, max_len=n,
+                       table=dev(gpu, tab, stream) if table else None)(stream)
+    got, pos = out.numpy(stream), np.arange(n)
+    for r in (0, R - 1):
+        where = tab[r] if table else np.full(n, r)
+        K, V = (ref.values(x, y, np.maximum(where, 0), pos) for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        keep = np.broadcast_to(where >= 0, (nq, n))
+        if causal:
+            keep = keep & (pos[None] <= (n - nq + np.arange(nq))[:, None])
+        for h in (0, H - 1):
+            # at scale 3 most weights are tiny, and some outputs are made of them alone.  A weight goes to f16 (f32: a
+            # second term) as 2^14 p, or by table as 2^14 p v / (largest p v of the tile), v the block's value scale: where
+            # that is subnormal the step is 2^-24 and half of it 2^-39 of the largest, times at most 50 by the
+            # table for the scales of 0.001 to 0.05 here: below 2^-33, and check_scaled allows 2^-32
+            check_scaled(got[r, :, h], q[r, :, h], K[:, h], V[:, h], scale, keep, type == "f16", d, f"scale {scale} r{r} h{h}")
