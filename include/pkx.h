@@ -432,7 +432,8 @@ int pkx_cache8_read(const pkx_cache8* c, int n_rows, int n, const int32_t* slot,
  * position is left out).  Beams share their histories that way: every beam appends to a slot of its own
  * with the table, and after a selection the table's rows, not the cache, are reordered by parent.
  * A slot out of range (without table) has no positions.  f16: int8 keys and values exact in f16,
- * queries as given, weights rounded to f16; f32: queries and weights as two f16 terms, 22 bits. */
+ * queries as given, weights rounded to f16; f32: queries and weights as two f16 terms, 22 bits.  Weights too
+ * small for that many bits are off by at most 2^-32 of the row's largest (by table: products with value scales). */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of q and out */
     int n_rows, n_q, n_heads, causal;

@@ -310,8 +310,9 @@ __device__ __forceinline__ int load_query(const DecAttnParams& p, int m, int b, 
             for (int e = 0; e < 4; ++e) q[4 * n + e] = live && key_dim<LAYOUT, D>(n, g) < p.dk ? x[n][e] : 0;
     } else {
         // q = (hi + lo) / f with f the power of two that takes the row's
-        // largest value to [2^13, 2^14): hi has 11 bits, lo the next 11,
-        // and what both drop is below 2^-37 of the largest
+        // largest value to [2^13, 2^14): hi has 11 bits, lo the next 11, so
+        // that at most 2^-23 of a value is dropped, or 2^-38 of the
+        // largest where lo is subnormal
         float4v y[D / 32][2];
 #pragma unroll
         for (int n = 0; n < D / 32; ++n) {
@@ -1254,8 +1255,16 @@ Shape attn_shape(const DecAttnParams& p) {
     //    9984        6              22.1          17.7    (d_head 128: 8 x 8 x 200 rows, 375 keys)
     //    4608        8              11.8          20.2    (4 x 8 x 130 rows, 500 keys)
     // 8-bit keys (where rows see part of the keys and lengths differ): with d_head 64
-    // no gain in most (37.6 against 44.1 at 112896 tiles, 119 against 120 at 448000), with
-    // 128 40.3 against 41.0 at 54912, 232 against 165 at 448000.
+    // no gain in most (37.6 against 44.1 at 112896 tiles, 119 against 120 at 448000).  With
+    // 128 dimensions, f16, by tiles alone:
+    //   27456  24.5  30.1  (8 x 8 x 200 rows, 1025 keys)      61440  39.0  40.4  (4 x 16 x 256, 1920)
+    //   32256  24.9  28.9  (4 x 16 x 128, 2000)               64512  44.8  41.3  (2 x 16 x 512, 2000)
+    //   36864  32.8  30.7  (32 x 8 x 130, 512)                67200  48.4  48.3  (6 x 32 x 150, 1100)
+    //   54912  39.5  39.8  (8 x 16 x 200, 1025)              141056   100  65.5  (2 x 64 x 600, 900)
+    // Even at the bound; away from its middle it misses full rounds of full tiles (50176:
+    // 53.3 30.3, 8 x 16 x 448 rows, 448 keys) and takes tiles that are half empty (65536: 44.5
+    // 50.0, 16 x 32 x 64, 1000).  f32 the same within 10% (67200: 61.8 66.0; 141056: 135 92.2).
+    // (Rounds are of the chip's 256 CUs, written in: the workspace can be asked for without a device.)
     const int64_t M = (int64_t)p.n_q * p.G;
     if (p.kv == KV_F32 || p.table || M < 64) return split_shape(p, false);
     const Shape wide = split_shape(p, true);
@@ -1274,6 +1283,13 @@ template <int KV, bool QF32, int D, bool TABLE> void launch_shape(const DecAttnP
         }
     launch(dec_attn_kernel<KV, QF32, D, TABLE>, grid, dim3(256), 0, s, p);
 }
+// Head widths above 64 take 128's registers and matrix instructions.  us at 64, 80, 96, 128:
+//   f16 16 x 4 rows x 8 heads, 375 keys            6.0   8.0   8.2   8.1
+//   f16 16 x 448 rows x 8 heads, 750 keys         27.6  38.9  39.6  40.2
+//   f32 8 x 54 rows x 8 heads, 334 keys            9.5  18.4  18.3  18.6
+//   int8 4 rows x 16 (4) heads, 32768 keys        16.4  21.9  22.5  27.3
+//   int8 128 beams x 8 heads, 448 keys, table     13.5  22.0  22.2  22.7
+//   int8, f32 8 x 200 rows x 8 heads, 1025 keys   18.1  30.0  30.3  31.6
 template <int KV, bool QF32, bool TABLE> void launch_width(const DecAttnParams& p, const Shape& sh, hipStream_t s) {
     if (p.dk <= 32) launch_shape<KV, QF32, 32, TABLE>(p, sh, s);
     else if (p.dk <= 64) launch_shape<KV, QF32, 64, TABLE>(p, sh, s);

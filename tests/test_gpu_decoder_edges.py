@@ -273,3 +273,36 @@ def test_cache_attention_scales(gpu, stream, type, R, nq, H, n, d, table, scale,
             # that is subnormal the step is 2^-24 and half of it 2^-39 of the largest, times at most 50 by the
             # table for the scales of 0.001 to 0.05 here: below 2^-33, and check_scaled allows 2^-32
             check_scaled(got[r, :, h], q[r, :, h], K[:, h], V[:, h], scale, keep, type == "f16", d, f"scale {scale} r{r} h{h}")
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("nq", [2, 256])
+@pytest.mark.parametrize("causal", [False, True])
+def test_cache_blocks_of_scale_zero(gpu, stream, type, nq, causal):
+    """Blocks whose value or key scale is 0, whatever integers stand there: first ones, both or one half of a step, all;
+    tiny and large scales between them."""
+    rng = np.random.default_rng(nq)
+    R, H, n, d = 4, 16, 1920, 128
+    c = HostCache(gpu, stream, R, H, n, d, rng)
+    c.vs[0] = 0
+    c.vs[1, :, :5] = 0
+    c.vs[2, :, ::2] = 0
+    c.vs[2, :, 1::4] *= 2.0 ** -9
+    c.vs[3, :, 2:] = 0
+    c.ks[1, :, 7:20] = 0
+    c.ks[2] = 0
+    for a, x in ((c.dev.k_scale, c.ks), (c.dev.v_scale, c.vs)):
+        a.upload(x, stream)
+    dt = np.float16 if type == "f16" else np.float32
+    q = (rng.standard_normal((R, nq, H, d)) * 0.7).astype(dt)
+    out = gpu.DeviceArray(q.shape, dt)
+    gpu.CacheAttention(c.dev, dev(gpu, q, stream), out, dev(gpu, i32([n] * R), stream), causal=causal)(stream)
+    got, pos = out.numpy(stream), np.arange(n)
+    assert not got[0].any()
+    for r in range(R):
+        K, V = (ref.values(x, y, np.full(n, r), pos) for x, y in ((c.k, c.ks), (c.v, c.vs)))
+        keep = np.ones((nq, n), bool)
+        if causal:
+            keep = keep & (pos[None] <= (n - nq + np.arange(nq))[:, None])
+        for h in (0, H - 1):
+            check_scaled(got[r, :, h], q[r, :, h], K[:, h], V[:, h], d ** -0.5, keep, type == "f16", d, f"zero scales r{r} h{h}")
