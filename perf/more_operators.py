@@ -6,7 +6,7 @@
   rules   penalties for repeated tokens, biases and grammar masks on logits, the histories read through beams' tables
 
 run() with own = False states the operators in elementary torch operations; with own = True it calls the framework
-(pkx.BlockNorm, pkx.QuantizeRows, pkx.LinearI8, pkx.Rotary, pkx.LogitRules).
+(pkx.BlockNorm, pkx.LinearI8, pkx.Rotary, pkx.LogitRules).
 """
 import math
 import os
@@ -137,11 +137,9 @@ def prepare(case, seed):
             st["gate"] = randn(-(-M // st["per"]), d).to(dt)
     elif case["kind"] == "linear":
         M, N, K = case["M"], case["N"], case["K"]
-        wide = (K + 15) // 16 * 16
         st.update(x=(randn(M, K) * (0.5 + rand(M, 1))).to(dt), w=(40 * randn(N, K)).round().clamp(-127, 127).to(torch.int8),
                   w_scale=0.0005 + 0.0005 * rand(N), bias=0.1 * randn(N) if case["bias"] else None,
-                  add=randn(M, N).to(dt) if case["add"] else None, y=torch.zeros((M, N), device="cuda", dtype=dt),
-                  q=torch.zeros((M, wide), device="cuda", dtype=torch.int8), x_scale=torch.zeros((M,), device="cuda"))
+                  add=randn(M, N).to(dt) if case["add"] else None, y=torch.zeros((M, N), device="cuda", dtype=dt))
     elif case["kind"] == "rotary":
         R, n, H, Hkv, dk, rot = (case[x] for x in ("R", "n", "H", "Hkv", "dk", "rot"))
         f = torch.pow(torch.full((rot // 2,), 10000.0, device="cuda", dtype=torch.float64),
@@ -209,10 +207,8 @@ def _plan(st):
                               gate=d.get("gate"), rows_per_gate=st["per"], gate_fn=case["fn"], alpha=case["alpha"], pre=case["pre"],
                               pre_w=d.get("pre_w"), pre_b=d.get("pre_b"), eps=st["eps"])]
     if case["kind"] == "linear":
-        q = _Dev(st["q"][:, :case["K"]])
-        w = pkx.WeightI8(d["w"], d["w_scale"])
-        return [pkx.QuantizeRows(d["x"], q, d["x_scale"]),
-                pkx.LinearI8(q, d["x_scale"], w, d["y"], bias=d.get("bias"), act=case["act"], add=d.get("add"))]
+        w = pkx.WeightI8(d["w"], d["w_scale"])      # laid out once; the call quantises the tokens
+        return [pkx.LinearI8(d["x"], w, d["y"], bias=d.get("bias"), act=case["act"], add=d.get("add"))]
     if case["kind"] == "rotary":
         H, Hkv = case["H"], case["Hkv"]
         return [pkx.Rotary(d["freq"], [(_Dev(st["qkv"][:, :, :H]), d["q_out"]), (_Dev(st["qkv"][:, :, H:H + Hkv]), d["k_out"])],
