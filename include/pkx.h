@@ -483,6 +483,133 @@ typedef struct {
 int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_beam_state* states, int n_states,
                      void* stream);
 
+/* ---- the rest of a decoder's block ------------------------------------------------
+ * No counterpart in the reference: what stands between the calls above in an attention
+ * decoder, as products and norms in their training framework do.  The same manner: the
+ * caller's buffers, kernels on the stream and nothing else, capturable; calls of size zero do nothing. */
+
+/* Block norm: for every row, with u = post(y) and h = pre(x_out) before its rounding to x's type,
+ *   x_out = x + alpha * g * u      g = gate, sigmoid(gate) or 1 without one
+ * post and pre are PKX_NORM_NONE (the value itself), PKX_NORM_LAYER (less its mean, over sqrt(variance + eps))
+ * or PKX_NORM_RMS (over sqrt(mean square + eps)), then times their weight and plus their bias, f32 [d], each NULL or not
+ * (NONE takes neither).  Without y, x_out = x; without x, x_out = alpha * g * u.  x_out may be x and h may be y
+ * (same rows); other overlaps of an output are refused.  Row m has the gate's row m / rows_per_gate.
+ * h in 8 bits (h_i8): as pkx_quantize_rows holds it, with its scale.  Moments are summed in f64, the rest is f32.
+ * d up to PKX_NORM_MAX_WIDTH, n_rows below 2^22; row strides in elements, at least d where a row is written. */
+enum { PKX_NORM_NONE = 0, PKX_NORM_LAYER = 1, PKX_NORM_RMS = 2 };
+enum { PKX_GATE_LINEAR = 0, PKX_GATE_SIGMOID = 1 };
+#define PKX_NORM_MAX_WIDTH 16384
+typedef struct {
+    int type, x_type;                    /* PKX_TYPE_F32 or PKX_TYPE_F16: of y, gate and h; of x and x_out (F32 where type is) */
+    int h_i8;                            /* h is int8_t [n_rows][d] with h_scale */
+    int d;
+    int64_t n_rows;
+    const void* x;     int64_t x_row;    /* dev, or NULL */
+    const void* y;     int64_t y_row;    /* dev, or NULL (one of x and y is there) */
+    const void* gate;  int64_t gate_row; /* dev [ceil(n_rows / rows_per_gate)][d], or NULL */
+    int64_t rows_per_gate;               /* at least 1 */
+    int gate_fn, post, pre;              /* PKX_GATE_*, PKX_NORM_*, PKX_NORM_* */
+    float post_eps, pre_eps, alpha;      /* eps finite and not negative, alpha finite */
+    const float *post_w, *post_b, *pre_w, *pre_b;
+    void* x_out;       int64_t x_out_row;   /* dev, or NULL */
+    void* h;           int64_t h_row;    /* dev, or NULL (one of x_out and h is there) */
+    float* h_scale;                      /* dev [n_rows], with h_i8 */
+} pkx_block_norm_args;
+int pkx_block_norm(const pkx_block_norm_args* a, void* stream);
+
+/* Rows in 8 bits: scale[m] = max |x[m]| / 127 over the finite values of row m of x [n_rows][n], and
+ * q[m][k] = round(x / scale) within +-127, each step one f32 operation, ties to even; NaN is held as 0, an
+ * infinity as +-127, a row without a finite value other than 0 has scale 0 (and infinities are 0 then).  Weights and tokens of pkx_linear_i8.  type: PKX_TYPE_F32 or
+ * PKX_TYPE_F16 of x; strides in elements, q's at least n; n_rows below 2^22. */
+int pkx_quantize_rows(int type, const void* x, int64_t x_row, int64_t n_rows, int n, int8_t* q, int64_t q_row,
+                      float* scale, void* stream);
+
+/* Weights of pkx_linear_i8: int8 w [n_out][n_in] (w_row bytes between rows) laid out once into `packed`
+ * (dev, pkx_i8_weight_bytes of it, 16-byte aligned).  n_in up to PKX_I8_MAX_DEPTH, where sums in 32 bits are exact. */
+#define PKX_I8_MAX_DEPTH 131072
+int pkx_i8_weight_bytes(int n_out, int n_in, size_t* bytes);
+int pkx_i8_weight_pack(const int8_t* w, int64_t w_row, int n_out, int n_in, void* packed, void* stream);
+
+/* y[m][n] = add[m][n] + alpha * act(x_scale[m] * w_scale[n] * sum over k of x[m][k] w[n][k] + bias[n]), the sums exact.
+ * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22, and what
+ * they hold past n_in does not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows
+ * does (x_scale NULL).  y and add are f32 or f16, and add may be y; y overlaps nothing else.  Strides in elements.
+ * n_rows and n_out below 2^22. */
+enum { PKX_TYPE_I8 = 24 };               /* ggml's number of its 8-bit integers */
+enum { PKX_ACT_NONE = 0, PKX_ACT_SILU = 1 };
+typedef struct {
+    int x_type, type;                    /* of x; of y and add */
+    int n_rows, n_out, n_in;
+    const void* x;     int64_t x_row;
+    const float* x_scale;                /* dev [n_rows], with PKX_TYPE_I8 */
+    const void* w;                       /* pkx_i8_weight_pack's */
+    const float* w_scale;                /* dev [n_out] */
+    const float* bias;                   /* dev [n_out], or NULL */
+    int act;                             /* PKX_ACT_* */
+    float alpha;                         /* finite */
+    const void* add;   int64_t add_row;  /* dev [n_rows][n_out], or NULL */
+    void* y;           int64_t y_row;
+} pkx_linear_i8_args;
+int pkx_linear_i8_workspace(const pkx_linear_i8_args* a, size_t* bytes);
+int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* stream);
+
+/* Rotary positions: token i < count[r] of row r is at position t = pos[r][i], or start[r] + i, and in every head of every part
+ * the pair (a, b) of frequency j < rot / 2 becomes
+ *   (a cos(t freq[j]) - b sin(t freq[j]), b cos(t freq[j]) + a sin(t freq[j])) * mult
+ * Pairs are elements (2 j, 2 j + 1) (interleaved) or (j, j + rot / 2); elements from rot on are copied.  Tokens
+ * from count[r] on are left as they were.  Angles are formed and reduced in f64, products are f32.  A part is an operand of its own head
+ * count (queries, keys); dst may be src with the same strides, else it overlaps no src; parts' dsts lie apart.
+ * Strides in elements (row, token, head), not negative; positions may be negative (the turn undone).
+ * d_head up to 512, rot even and at most d_head. */
+#define PKX_ROTARY_MAX_PARTS 4
+typedef struct {
+    const void* src;  int64_t src_row, src_tok, src_head;
+    void* dst;        int64_t dst_row, dst_tok, dst_head;
+    int n_heads;
+} pkx_rotary_part;
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16 */
+    int n_rows, n_tok, d_head, rot, interleaved;
+    float mult;                          /* finite; 1: a rotation */
+    const double* freq;                  /* dev [rot / 2], radians a position */
+    const int32_t* start;                /* dev [n_rows], or NULL: 0 */
+    const int32_t* pos;  int64_t pos_row;   /* dev [n_rows][n_tok], or NULL: start[r] + i */
+    const int32_t* count;                /* dev [n_rows], or NULL: n_tok (clamped to 0..n_tok) */
+    int n_parts;
+    pkx_rotary_part part[PKX_ROTARY_MAX_PARTS];
+} pkx_rotary_args;
+int pkx_rotary(const pkx_rotary_args* a, void* stream);
+/* The frequencies (host) freq[j] = base^(-2 j / rot), for contexts `factor` times as long as the trained one: those that
+ * turn less than `low` times in `context` positions are divided by factor, those that turn more than `high` times kept, and
+ * in between the two are mixed linearly in the turns.  context 0: all are divided.  factor 1: none.  base > 0, factor > 0, high > low. */
+int pkx_rotary_frequencies(double base, int rot, double factor, double context, double low, double high, double* freq);
+
+/* Rules on logits, before pkx_beam_select or an argmax: with c the times that word v is among the last `window` (0: all)
+ * of row r's first len[r] tokens,
+ *   x = c == 0 ? x : (x > 0 ? x / repetition[r] : x * repetition[r]) - presence[r] - frequency[r] * c
+ *   x = x + bias[v], then -inf where the mask has no bit for v
+ * in f32.  Token t of row r is tokens[s][t] with s = slot[r], or table[r][t] (a position whose slot is out of range is left
+ * out): the histories lie as a cache's tokens do, and beams share them through the same tables.  Tokens outside the vocabulary do not count.  bias and
+ * mask are sets of rows that rows of logits name: row bias_index[r] of n_bias (NULL: r), none where that is out of range,
+ * and likewise the mask, whose word v / 32 has the bit v % 32.  out may be logits with the same rows; other overlaps are refused.
+ * vocab up to 2^22; strides in elements. */
+typedef struct {
+    int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of logits and out */
+    int n_rows, vocab;
+    const void* logits;  int64_t logits_row;
+    void* out;           int64_t out_row;
+    const int32_t* tokens;               /* dev [n_slots][capacity], or NULL: no penalties */
+    int n_slots, capacity;
+    const int32_t* len;                  /* dev [n_rows] (clamped to 0..capacity) */
+    const int32_t* slot;                 /* dev [n_rows], or NULL: row r is slot r */
+    const int32_t* table;  int64_t table_row;   /* dev [n_rows][>= capacity], or NULL */
+    int window;
+    const float *repetition, *presence, *frequency;   /* dev [n_rows], or NULL: 1, 0, 0 */
+    const float* bias;     int64_t bias_row;  int n_bias;  const int32_t* bias_index;
+    const uint32_t* mask;  int64_t mask_row;  int n_mask;  const int32_t* mask_index;   /* mask_row in words */
+} pkx_logit_rules_args;
+int pkx_logit_rules(const pkx_logit_rules_args* a, void* stream);
+
 /* ---- profiling ----------------------------------------------------------------
  * No counterpart in the reference (its benchmarks time whole calls).
  * family_mask selects kernel families by bit (bit i = family i in the order

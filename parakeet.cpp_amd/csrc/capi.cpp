@@ -7,8 +7,10 @@
 #include <mutex>
 #include <string>
 #include <utility>
+#include <vector>
 
 #include "../../include/pkx.h"
+#include "block.hpp"
 #include "decoder.hpp"
 #include "mel.hpp"
 #include "model.hpp"
@@ -289,6 +291,101 @@ pkx::BeamSelectParams beam_params(const pkx_beam_select_args* a) {
     p.token = a->token;
     p.new_scores = a->new_scores;
     p.new_done = a->new_done;
+    return p;
+}
+// A strided operand as the bytes it touches: `row` adjacent ones at every multiple of each dimension's stride.
+struct Span {
+    uintptr_t at;
+    int64_t row;
+    std::pair<int64_t, int64_t> dim[3];   // stride in bytes, count; largest stride first
+    int dims = 0;
+
+    Span(const void* p, int64_t bytes, std::initializer_list<std::pair<int64_t, int64_t>> all) : at((uintptr_t)p), row(bytes) {
+        for (const auto& d : all)
+            if (d.second > 1) dim[dims++] = d;
+        std::sort(dim, dim + dims, [](const auto& a, const auto& b) { return a.first > b.first; });
+    }
+    double bytes(int from = 0) const {    // from the first byte to the last, of the dimensions from `from` on
+        double n = (double)row;
+        for (int i = from; i < dims; ++i) n += (double)dim[i].first * (double)(dim[i].second - 1);
+        return n;
+    }
+};
+
+// Whether two operands have no byte in common, as far as their strides say it: one ends before the other begins, or their
+// largest strides are the same and within one period (two column ranges of the same rows) they lie apart.
+bool apart(const Span& a, const Span& b) {
+    if (a.at > b.at) return apart(b, a);
+    if ((double)(b.at - a.at) >= a.bytes()) return true;
+    uint64_t from = b.at - a.at;
+    for (int i = 0; i < a.dims && i < b.dims; ++i) {
+        if (a.dim[i].first != b.dim[i].first || a.dim[i].first <= 0) return false;
+        const double period = (double)a.dim[i].first, na = a.bytes(i + 1), nb = b.bytes(i + 1);
+        // b's place in a's period; neither may run into the next one
+        from %= (uint64_t)a.dim[i].first;
+        if (na > period || (double)from + nb > period) return false;
+        if ((double)from >= na) return true;
+    }
+    return false;
+}
+bool same(const Span& a, const Span& b) {
+    if (a.at != b.at || a.row != b.row || a.dims != b.dims) return false;
+    return std::equal(a.dim, a.dim + a.dims, b.dim);
+}
+
+// Rows of n elements of e bytes, `count` of them `stride` elements apart.
+Span rows_of(const void* p, int64_t n, int64_t e, int64_t stride, int64_t count) { return Span(p, n * e, {{stride * e, count}}); }
+
+// Addresses and extents that 64-bit byte arithmetic holds.
+void need_rows_of(const void* p, int e, int64_t stride, int64_t count, int64_t least, const char* what) {
+    need(p && (uintptr_t)p % e == 0 && (stride >= least || (count <= 1 && stride >= 0)), what);
+    need((double)stride * (double)count * e < 0x1p62, what);
+}
+
+void need_i8_weight(int n_out, int n_in) {
+    need(n_out >= 0 && n_out < (1 << 22) && n_in >= 1 && n_in <= PKX_I8_MAX_DEPTH, "8-bit weights: n_out below 2^22 and n_in 1 to PKX_I8_MAX_DEPTH");
+    need(pkx::i8_weight_bytes(n_out, n_in) < (int64_t(1) << 35), "8-bit weights: 32 GiB or more");
+}
+pkx::LinearI8Params linear_i8_params(const pkx_linear_i8_args* a) {
+    need(a, "null argument");
+    pkx::LinearI8Params p;
+    p.y_f32 = is_f32(a->type, "8-bit linear: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(a->x_type == PKX_TYPE_I8 || a->x_type == PKX_TYPE_F32 || a->x_type == PKX_TYPE_F16,
+         "8-bit linear: x_type must be PKX_TYPE_I8, PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(a->n_rows >= 0 && a->n_out >= 0 && a->n_in >= 1 && a->n_in <= PKX_I8_MAX_DEPTH,
+         "8-bit linear: negative size, or n_in outside 1 to PKX_I8_MAX_DEPTH");
+    need(a->n_rows < (1 << 22) && a->n_out < (1 << 22) && (double)a->n_rows * a->n_out < 0x1p36,
+         "8-bit linear: n_rows and n_out below 2^22, and 2^36 outputs in one call");
+    need(a->act == PKX_ACT_NONE || a->act == PKX_ACT_SILU, "8-bit linear: act must be PKX_ACT_NONE or PKX_ACT_SILU");
+    need(std::isfinite(a->alpha), "8-bit linear: alpha is not finite");
+    p.M = a->n_rows;
+    p.N = a->n_out;
+    p.K = a->n_in;
+    p.w = a->w;
+    p.w_scale = a->w_scale;
+    p.bias = a->bias;
+    p.silu = a->act == PKX_ACT_SILU;
+    p.alpha = a->alpha;
+    p.add = a->add;
+    p.add_row = a->add_row;
+    p.y = a->y;
+    p.y_row = a->y_row;
+    return p;
+}
+// Quantised tokens in the workspace: rows of whole 16 bytes, then their scales.
+int64_t i8_row(const pkx_linear_i8_args* a) { return ((int64_t)a->n_in + 15) / 16 * 16; }
+size_t i8_workspace(const pkx_linear_i8_args* a) {
+    return a->x_type == PKX_TYPE_I8 || a->n_rows == 0 || a->n_out == 0 ? 0 : (size_t)a->n_rows * (i8_row(a) + 4);
+}
+pkx::QuantizeRowsParams quantize_rows_params(int type, const void* x, int64_t x_row, int64_t n_rows, int n) {
+    pkx::QuantizeRowsParams p;
+    p.f32 = is_f32(type, "quantise rows: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+    need(n_rows >= 0 && n_rows < (1 << 22) && n >= 0, "quantise rows: negative size, or 2^22 rows");
+    if (n_rows > 0) need_rows_of(x, p.f32 ? 4 : 2, x_row, n_rows, 0, "quantise rows: x is null, misaligned or of a negative stride");
+    p.rows = n_rows;
+    p.d = n;
+    p.x = x;
+    p.x_row = x_row;
     return p;
 }
 }  // namespace
@@ -880,6 +977,293 @@ int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_
         }
         need_device(st(s));
         pkx::launch_beam_reorder(parent, n_items, n_beams, p, n_states, st(s));
+    });
+}
+
+int pkx_block_norm(const pkx_block_norm_args* a, void* s) {
+    return guarded([&] {
+        need(a, "null argument");
+        pkx::BlockNormParams p;
+        p.f32 = is_f32(a->type, "block norm: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+        p.x_f32 = is_f32(a->x_type, "block norm: x_type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+        need(p.x_f32 || !p.f32, "block norm: an f16 x goes with f16 y, gate and h");
+        need(a->n_rows >= 0 && a->n_rows < (1 << 22), "block norm: negative size, or 2^22 rows");
+        need(a->d >= 1 && a->d <= PKX_NORM_MAX_WIDTH, "block norm: d must be 1 to PKX_NORM_MAX_WIDTH");
+        for (int kind : {a->post, a->pre})
+            need(kind == PKX_NORM_NONE || kind == PKX_NORM_LAYER || kind == PKX_NORM_RMS, "block norm: post and pre must be PKX_NORM_*");
+        need(a->gate_fn == PKX_GATE_LINEAR || a->gate_fn == PKX_GATE_SIGMOID, "block norm: gate_fn must be PKX_GATE_*");
+        need(a->post_eps >= 0 && a->pre_eps >= 0 && std::isfinite(a->post_eps) && std::isfinite(a->pre_eps),
+             "block norm: eps must be finite and not negative");
+        need(std::isfinite(a->alpha), "block norm: alpha is not finite");
+        need(a->x || a->y, "block norm: neither x nor y");
+        need(a->x_out || a->h, "block norm: neither x_out nor h");
+        need(!a->gate || (a->y && a->rows_per_gate >= 1), "block norm: a gate needs y, and rows_per_gate of at least 1");
+        need(a->post == PKX_NORM_NONE ? !a->post_w && !a->post_b : a->y != nullptr, "block norm: post without y, or weights without post");
+        need(a->pre == PKX_NORM_NONE ? !a->pre_w && !a->pre_b : a->h != nullptr, "block norm: pre without h, or weights without pre");
+        need(!a->h_i8 || (a->h && a->h_scale), "block norm: 8 bits without h or h_scale");
+        if (a->n_rows == 0) return;
+        const int e = p.f32 ? 4 : 2, ex = p.x_f32 ? 4 : 2, eh = a->h_i8 ? 1 : e;
+        const int64_t rows = a->n_rows, d = a->d, gates = a->gate ? (rows - 1) / a->rows_per_gate + 1 : 0;
+        if (a->x) need_rows_of(a->x, ex, a->x_row, rows, 0, "block norm: x is misaligned or of a negative stride");
+        if (a->y) need_rows_of(a->y, e, a->y_row, rows, 0, "block norm: y is misaligned or of a negative stride");
+        if (a->gate) need_rows_of(a->gate, e, a->gate_row, gates, 0, "block norm: gate is misaligned or of a negative stride");
+        if (a->x_out) need_rows_of(a->x_out, ex, a->x_out_row, rows, d, "block norm: x_out is misaligned, or its rows overlap");
+        if (a->h) need_rows_of(a->h, eh, a->h_row, rows, d, "block norm: h is misaligned, or its rows overlap");
+        const Span none(nullptr, 0, {});
+        const Span x = a->x ? rows_of(a->x, d, ex, a->x_row, rows) : none, y = a->y ? rows_of(a->y, d, e, a->y_row, rows) : none;
+        const Span g = a->gate ? rows_of(a->gate, d, e, a->gate_row, gates) : none;
+        const Span o = a->x_out ? rows_of(a->x_out, d, ex, a->x_out_row, rows) : none;
+        const Span h = a->h ? rows_of(a->h, d, eh, a->h_row, rows) : none;
+        const Span hs = a->h_i8 ? rows_of(a->h_scale, 1, 4, 1, rows) : none;
+        for (const Span* w : {&o, &h, &hs}) {
+            if (!w->at) continue;
+            for (const Span* in : {&x, &y, &g})
+                need(!in->at || apart(*w, *in) || (w == &o && in == &x && same(o, x)) || (w == &h && in == &y && same(h, y) && !a->h_i8),
+                     "block norm: an output overlaps an input");
+            for (const float* v : {a->post_w, a->post_b, a->pre_w, a->pre_b})
+                need(!v || apart(*w, Span(v, 4 * d, {})), "block norm: an output overlaps a weight");
+            for (const Span* w2 : {&o, &h, &hs}) need(w == w2 || !w2->at || apart(*w, *w2), "block norm: the outputs overlap");
+        }
+        p.h_i8 = a->h_i8 != 0;
+        p.rows = rows;
+        p.d = a->d;
+        p.x = a->x; p.x_row = a->x_row;
+        p.y = a->y; p.y_row = a->y_row;
+        p.gate = a->gate; p.gate_row = a->gate_row;
+        p.rows_per_gate = a->gate && a->rows_per_gate < rows ? (int)a->rows_per_gate : (int)rows;
+        p.sigmoid = a->gate_fn == PKX_GATE_SIGMOID;
+        p.post = a->post;
+        p.pre = a->pre;
+        p.post_w = a->post_w; p.post_b = a->post_b; p.post_eps = a->post_eps;
+        p.pre_w = a->pre_w; p.pre_b = a->pre_b; p.pre_eps = a->pre_eps;
+        p.alpha = a->alpha;
+        p.x_out = a->x_out; p.x_out_row = a->x_out_row;
+        p.h = a->h; p.h_row = a->h_row;
+        p.h_scale = a->h_scale;
+        need_device(st(s));
+        pkx::launch_block_norm(p, st(s));
+    });
+}
+
+int pkx_quantize_rows(int type, const void* x, int64_t x_row, int64_t n_rows, int n, int8_t* q, int64_t q_row, float* scale, void* s) {
+    return guarded([&] {
+        pkx::QuantizeRowsParams p = quantize_rows_params(type, x, x_row, n_rows, n);
+        if (n_rows == 0) return;
+        need_rows_of(q, 1, q_row, n_rows, n, "quantise rows: q is null, or its rows overlap");
+        need(scale && (uintptr_t)scale % 4 == 0, "quantise rows: scale is null or misaligned");
+        const Span in = rows_of(x, n, p.f32 ? 4 : 2, x_row, n_rows), out = rows_of(q, n, 1, q_row, n_rows), sc = rows_of(scale, 1, 4, 1, n_rows);
+        need(apart(in, out) && apart(in, sc) && apart(out, sc), "quantise rows: an output overlaps x or the other one");
+        p.q = q;
+        p.q_row = q_row;
+        p.scale = scale;
+        need_device(st(s));
+        pkx::launch_quantize_rows(p, st(s));
+    });
+}
+
+int pkx_i8_weight_bytes(int n_out, int n_in, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        need_i8_weight(n_out, n_in);
+        *bytes = (size_t)pkx::i8_weight_bytes(n_out, n_in);
+    });
+}
+int pkx_i8_weight_pack(const int8_t* w, int64_t w_row, int n_out, int n_in, void* packed, void* s) {
+    return guarded([&] {
+        need_i8_weight(n_out, n_in);
+        if (n_out == 0) return;
+        need_rows_of(w, 1, w_row, n_out, 0, "8-bit weights: w is null or of a negative stride");
+        need(packed && (uintptr_t)packed % 16 == 0, "8-bit weights: packed is null or not 16-byte aligned");
+        need(apart(rows_of(w, n_in, 1, w_row, n_out), Span(packed, pkx::i8_weight_bytes(n_out, n_in), {})), "8-bit weights: packed overlaps w");
+        need_device(st(s));
+        pkx::launch_i8_weight_pack(w, w_row, n_out, n_in, packed, st(s));
+    });
+}
+
+int pkx_linear_i8_workspace(const pkx_linear_i8_args* a, size_t* bytes) {
+    return guarded([&] {
+        need(bytes, "null argument");
+        linear_i8_params(a);
+        *bytes = i8_workspace(a);
+    });
+}
+int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* s) {
+    return guarded([&] {
+        pkx::LinearI8Params p = linear_i8_params(a);
+        if (p.M == 0 || p.N == 0) return;
+        const int e = p.y_f32 ? 4 : 2;
+        const int64_t M = p.M, N = p.N, K = p.K;
+        need(p.w && (uintptr_t)p.w % 16 == 0, "8-bit linear: w is null or not 16-byte aligned");
+        need(p.w_scale && (uintptr_t)p.w_scale % 4 == 0 && (uintptr_t)p.bias % 4 == 0, "8-bit linear: w_scale is null, or it or bias misaligned");
+        need_rows_of(p.y, e, p.y_row, M, N, "8-bit linear: y is null or misaligned, or its rows overlap");
+        if (p.add) need_rows_of(p.add, e, p.add_row, M, 0, "8-bit linear: add is misaligned or of a negative stride");
+        const Span y = rows_of(p.y, N, e, p.y_row, M);
+        if (p.add) {
+            const Span add = rows_of(p.add, N, e, p.add_row, M);
+            need(apart(y, add) || same(y, add), "8-bit linear: y overlaps add without being it");
+        }
+        need(apart(y, Span(p.w, pkx::i8_weight_bytes(N, K), {})) && apart(y, Span(p.w_scale, 4 * N, {})) &&
+                 (!p.bias || apart(y, Span(p.bias, 4 * N, {}))), "8-bit linear: y overlaps the weights, their scales or the bias");
+        if (a->x_type == PKX_TYPE_I8) {
+            need_rows_of(a->x, 16, a->x_row, M, K, "8-bit linear: x is null, not 16-byte aligned or of rows shorter than n_in");
+            need(a->x_row % 16 == 0 && a->x_row >= K && a->x_row < (1 << 22), "8-bit linear: x_row must be a multiple of 16, at least n_in and below 2^22");
+            need(a->x_scale && (uintptr_t)a->x_scale % 4 == 0, "8-bit linear: x_scale is null or misaligned");
+            need(apart(y, rows_of(a->x, i8_row(a), 1, a->x_row, M)) && apart(y, Span(a->x_scale, 4 * M, {})), "8-bit linear: y overlaps x or its scales");
+            p.x = (const int8_t*)a->x;
+            p.x_row = a->x_row;
+            p.x_scale = a->x_scale;
+            need_device(st(s));
+            pkx::launch_linear_i8(p, st(s));
+            return;
+        }
+        need(!a->x_scale, "8-bit linear: x_scale goes with PKX_TYPE_I8");
+        pkx::QuantizeRowsParams q = quantize_rows_params(a->x_type, a->x, a->x_row, M, a->n_in);
+        need(ws && (uintptr_t)ws % 16 == 0, "8-bit linear: the workspace is null or not 16-byte aligned");
+        need(ws_bytes >= i8_workspace(a), "8-bit linear: the workspace is too small");
+        need(apart(y, rows_of(a->x, K, q.f32 ? 4 : 2, a->x_row, M)), "8-bit linear: y overlaps x");
+        q.q = (int8_t*)ws;
+        q.q_row = i8_row(a);
+        q.scale = (float*)((char*)ws + M * q.q_row);
+        p.x = q.q;
+        p.x_row = q.q_row;
+        p.x_scale = q.scale;
+        need_device(st(s));
+        pkx::launch_quantize_rows(q, st(s));
+        pkx::launch_linear_i8(p, st(s));
+    });
+}
+
+int pkx_rotary(const pkx_rotary_args* a, void* s) {
+    return guarded([&] {
+        need(a, "null argument");
+        pkx::RotaryParams p;
+        p.f32 = is_f32(a->type, "rotary: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+        need(a->n_rows >= 0 && a->n_tok >= 0, "rotary: negative size");
+        need(a->d_head >= 1 && a->d_head <= pkx::kMaxRotaryWidth, "rotary: d_head must be 1 to 512");
+        need(a->rot >= 0 && a->rot % 2 == 0 && a->rot <= a->d_head, "rotary: rot must be even and at most d_head");
+        need(a->n_parts >= 0 && a->n_parts <= PKX_ROTARY_MAX_PARTS, "rotary: at most PKX_ROTARY_MAX_PARTS parts");
+        need(std::isfinite(a->mult), "rotary: mult is not finite");
+        need(!a->pos || a->pos_row >= 0, "rotary: negative stride of pos");
+        for (int i = 0; i < a->n_parts; ++i) need(a->part[i].n_heads >= 0 && a->part[i].n_heads <= 4096, "rotary: a part has 0 to 4096 heads");
+        if (a->n_rows == 0 || a->n_tok == 0) return;
+        need(a->freq && (uintptr_t)a->freq % 8 == 0, "rotary: freq is null or misaligned");
+        const int e = p.f32 ? 4 : 2;
+        const int64_t R = a->n_rows, n = a->n_tok;
+        std::vector<Span> src, dst;
+        for (int i = 0; i < a->n_parts; ++i) {
+            const pkx_rotary_part& x = a->part[i];
+            if (x.n_heads == 0) continue;
+            need(x.src && x.dst && ((uintptr_t)x.src | (uintptr_t)x.dst) % e == 0, "rotary: a part's src or dst is null or misaligned");
+            need(x.src_row >= 0 && x.src_tok >= 0 && x.src_head >= 0 && x.dst_row >= 0 && x.dst_tok >= 0 && x.dst_head >= 0, "rotary: negative stride");
+            need_apart(x.dst_row, R, x.dst_tok, n, x.dst_head, x.n_heads, a->d_head, "rotary: rows of a dst overlap");
+            src.emplace_back(x.src, (int64_t)a->d_head * e, std::initializer_list<std::pair<int64_t, int64_t>>{{x.src_row * e, R}, {x.src_tok * e, n}, {x.src_head * e, x.n_heads}});
+            dst.emplace_back(x.dst, (int64_t)a->d_head * e, std::initializer_list<std::pair<int64_t, int64_t>>{{x.dst_row * e, R}, {x.dst_tok * e, n}, {x.dst_head * e, x.n_heads}});
+            need(src.back().bytes() < 0x1p62 && dst.back().bytes() < 0x1p62, "rotary: strides past the address space");
+            pkx::RotaryPart& o = p.part[p.parts++];
+            o = pkx::RotaryPart{x.src, x.src_row, x.src_tok, x.src_head, x.dst, x.dst_row, x.dst_tok, x.dst_head, x.n_heads};
+        }
+        for (size_t i = 0; i < dst.size(); ++i) {
+            for (size_t j = 0; j < dst.size(); ++j) {
+                need(apart(dst[i], src[j]) || (i == j && same(dst[i], src[i])), "rotary: a dst overlaps a src without being its own");
+                need(i == j || apart(dst[i], dst[j]), "rotary: two dsts overlap");
+            }
+            need(a->rot == 0 || apart(dst[i], Span(a->freq, 4 * (int64_t)a->rot, {})), "rotary: a dst overlaps freq");
+            need((!a->start || apart(dst[i], Span(a->start, 4 * R, {}))) && (!a->count || apart(dst[i], Span(a->count, 4 * R, {}))) &&
+                     (!a->pos || apart(dst[i], rows_of(a->pos, n, 4, a->pos_row, R))), "rotary: a dst overlaps start, pos or count");
+        }
+        p.R = a->n_rows;
+        p.n = a->n_tok;
+        p.dk = a->d_head;
+        p.rot = a->rot;
+        p.interleaved = a->interleaved != 0;
+        p.mult = a->mult;
+        p.freq = a->freq;
+        p.start = a->start;
+        p.pos = a->pos;
+        p.pos_row = a->pos_row;
+        p.count = a->count;
+        need_device(st(s));
+        pkx::launch_rotary(p, st(s));
+    });
+}
+int pkx_rotary_frequencies(double base, int rot, double factor, double context, double low, double high, double* freq) {
+    return guarded([&] {
+        need(freq, "null argument");
+        need(rot >= 0 && rot % 2 == 0 && rot <= pkx::kMaxRotaryWidth, "rotary: rot must be even and at most 512");
+        need(base > 0 && std::isfinite(base) && factor > 0 && std::isfinite(factor), "rotary: base and factor must be positive and finite");
+        need(context >= 0 && std::isfinite(context) && (context == 0 || (high > low && std::isfinite(high - low))), "rotary: context must not be negative, and high above low");
+        for (int j = 0; j < rot / 2; ++j) {
+            const double f = std::pow(base, -2.0 * j / rot);
+            double keep = 0;
+            if (context > 0) keep = std::min(1.0, std::max(0.0, (context * f / (2 * M_PI) - low) / (high - low)));
+            freq[j] = f * (keep + (1 - keep) / factor);
+        }
+    });
+}
+
+int pkx_logit_rules(const pkx_logit_rules_args* a, void* s) {
+    return guarded([&] {
+        need(a, "null argument");
+        pkx::LogitRulesParams p;
+        p.f32 = is_f32(a->type, "logit rules: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
+        need(a->n_rows >= 0 && a->vocab >= 0 && a->window >= 0, "logit rules: negative size");
+        need(a->vocab <= (1 << 22), "logit rules: a vocabulary of at most 2^22 words");
+        if (a->n_rows == 0 || a->vocab == 0) return;
+        const int e = p.f32 ? 4 : 2;
+        const int64_t R = a->n_rows, V = a->vocab;
+        need_rows_of(a->logits, e, a->logits_row, R, 0, "logit rules: logits are null, misaligned or of a negative stride");
+        need_rows_of(a->out, e, a->out_row, R, V, "logit rules: out is null or misaligned, or its rows overlap");
+        const Span in = rows_of(a->logits, V, e, a->logits_row, R), out = rows_of(a->out, V, e, a->out_row, R);
+        need(same(in, out) || apart(in, out), "logit rules: out overlaps logits without being them");
+        if (a->tokens) {
+            need(a->n_slots >= 1 && a->capacity >= 0, "logit rules: no slots, or a negative capacity");
+            need((double)a->n_slots * a->capacity < 0x1p60 && a->table_row >= 0 && (double)a->table_row * R < 0x1p60, "logit rules: tokens or table past the address space");
+            need(a->len, "logit rules: null len");
+            need(a->slot || a->table || R <= a->n_slots, "logit rules: more rows than slots");
+            need(!a->table || a->table_row >= a->capacity, "logit rules: table rows are shorter than the capacity");
+            need(apart(out, Span(a->tokens, 4 * (int64_t)a->n_slots * a->capacity, {})) && apart(out, Span(a->len, 4 * R, {})) &&
+                     (!a->slot || apart(out, Span(a->slot, 4 * R, {}))) && (!a->table || apart(out, rows_of(a->table, a->capacity, 4, a->table_row, R))),
+                 "logit rules: out overlaps the tokens, their lengths, slots or table");
+            p.tokens = a->tokens;
+            p.n_slots = a->n_slots;
+            p.cap = a->capacity;
+            p.len = a->len;
+            p.slot = a->slot;
+            p.table = a->table;
+            p.table_row = a->table_row;
+            p.window = a->window;
+            p.repetition = a->repetition;
+            p.presence = a->presence;
+            p.frequency = a->frequency;
+            for (const float* v : {a->repetition, a->presence, a->frequency})
+                need(!v || apart(out, Span(v, 4 * R, {})), "logit rules: out overlaps a penalty");
+        }
+        if (a->bias) {
+            need(a->n_bias >= 0 && (uintptr_t)a->bias % 4 == 0 && a->bias_row >= 0 && (double)a->bias_row * a->n_bias < 0x1p60, "logit rules: bias is misaligned, or of a negative count or stride");
+            need(a->n_bias == 0 || apart(out, rows_of(a->bias, V, 4, a->bias_row, a->n_bias)), "logit rules: out overlaps bias");
+            need(!a->bias_index || apart(out, Span(a->bias_index, 4 * R, {})), "logit rules: out overlaps bias_index");
+            p.bias = a->bias;
+            p.bias_row = a->bias_row;
+            p.n_bias = a->n_bias;
+            p.bias_index = a->bias_index;
+        }
+        if (a->mask) {
+            need(a->n_mask >= 0 && (uintptr_t)a->mask % 4 == 0 && a->mask_row >= 0 && (double)a->mask_row * a->n_mask < 0x1p60, "logit rules: mask is misaligned, or of a negative count or stride");
+            need(a->n_mask == 0 || apart(out, rows_of(a->mask, (V + 31) / 32, 4, a->mask_row, a->n_mask)), "logit rules: out overlaps mask");
+            need(!a->mask_index || apart(out, Span(a->mask_index, 4 * R, {})), "logit rules: out overlaps mask_index");
+            p.mask = a->mask;
+            p.mask_row = a->mask_row;
+            p.n_mask = a->n_mask;
+            p.mask_index = a->mask_index;
+        }
+        p.R = a->n_rows;
+        p.V = a->vocab;
+        p.x = a->logits;
+        p.x_row = a->logits_row;
+        p.out = a->out;
+        p.out_row = a->out_row;
+        need_device(st(s));
+        pkx::launch_logit_rules(p, st(s));
     });
 }
 

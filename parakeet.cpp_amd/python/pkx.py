@@ -45,7 +45,9 @@ class Config(C.Structure):
 
 
 _i32, _i64, _sz = C.c_int, C.c_int64, C.c_size_t
-TYPE_F32, TYPE_F16 = 0, 1
+TYPE_F32, TYPE_F16, TYPE_I8 = 0, 1, 24
+NORMS, GATES, ACTS = {"none": 0, "layer": 1, "rms": 2}, {"linear": 0, "sigmoid": 1}, {"none": 0, "silu": 1}
+ROTARY_MAX_PARTS = 4
 CACHE8_BLOCK, BEAM_MAX_STATES = 32, 32
 
 
@@ -82,6 +84,37 @@ class BeamSelectArgs(C.Structure):
 
 class BeamState(C.Structure):
     _fields_ = [("src", _vp), ("dst", _vp), ("src_row", _i64), ("dst_row", _i64), ("bytes", _i64)]
+
+
+class BlockNormArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "x_type", "h_i8", "d")] + [("n_rows", _i64)] +
+                [f for n in ("x", "y", "gate") for f in [(n, _vp), (n + "_row", _i64)]] + [("rows_per_gate", _i64)] +
+                [(n, _i32) for n in ("gate_fn", "post", "pre")] + [(n, C.c_float) for n in ("post_eps", "pre_eps", "alpha")] +
+                [(n, _vp) for n in ("post_w", "post_b", "pre_w", "pre_b")] +
+                [f for n in ("x_out", "h") for f in [(n, _vp), (n + "_row", _i64)]] + [("h_scale", _vp)])
+
+
+class LinearI8Args(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("x_type", "type", "n_rows", "n_out", "n_in")] + [("x", _vp), ("x_row", _i64)] +
+                [(n, _vp) for n in ("x_scale", "w", "w_scale", "bias")] + [("act", _i32), ("alpha", C.c_float)] +
+                [("add", _vp), ("add_row", _i64), ("y", _vp), ("y_row", _i64)])
+
+
+class RotaryPart(C.Structure):
+    _fields_ = [f for n in ("src", "dst") for f in [(n, _vp)] + [(n + "_" + x, _i64) for x in ("row", "tok", "head")]] + [("n_heads", _i32)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_rows", "n_tok", "d_head", "rot", "interleaved")] + [("mult", C.c_float)] +
+                [("freq", _vp), ("start", _vp), ("pos", _vp), ("pos_row", _i64), ("count", _vp), ("n_parts", _i32),
+                 ("part", RotaryPart * ROTARY_MAX_PARTS)])
+
+
+class LogitRulesArgs(C.Structure):
+    _fields_ = ([(n, _i32) for n in ("type", "n_rows", "vocab")] + [f for n in ("logits", "out") for f in [(n, _vp), (n + "_row", _i64)]] +
+                [("tokens", _vp), ("n_slots", _i32), ("capacity", _i32), ("len", _vp), ("slot", _vp), ("table", _vp),
+                 ("table_row", _i64), ("window", _i32)] + [(n, _vp) for n in ("repetition", "presence", "frequency")] +
+                [f for n in ("bias", "mask") for f in [(n, _vp), (n + "_row", _i64), ("n_" + n, _i32), (n + "_index", _vp)]])
 
 
 _P = C.POINTER
@@ -157,6 +190,15 @@ SIGS = {
     "pkx_beam_select_workspace": ([_P(BeamSelectArgs), _P(_sz)], C.c_int),
     "pkx_beam_select": ([_P(BeamSelectArgs), _vp, _sz, _vp], C.c_int),
     "pkx_beam_reorder": ([_vp, _i32, _i32, _P(BeamState), _i32, _vp], C.c_int),
+    "pkx_block_norm": ([_P(BlockNormArgs), _vp], C.c_int),
+    "pkx_quantize_rows": ([_i32, _vp, _i64, _i64, _i32, _vp, _i64, _vp, _vp], C.c_int),
+    "pkx_i8_weight_bytes": ([_i32, _i32, _P(_sz)], C.c_int),
+    "pkx_i8_weight_pack": ([_vp, _i64, _i32, _i32, _vp, _vp], C.c_int),
+    "pkx_linear_i8_workspace": ([_P(LinearI8Args), _P(_sz)], C.c_int),
+    "pkx_linear_i8": ([_P(LinearI8Args), _vp, _sz, _vp], C.c_int),
+    "pkx_rotary": ([_P(RotaryArgs), _vp], C.c_int),
+    "pkx_rotary_frequencies": ([C.c_double, _i32] + [C.c_double] * 4 + [_P(C.c_double)], C.c_int),
+    "pkx_logit_rules": ([_P(LogitRulesArgs), _vp], C.c_int),
     "pkx_model_set_profiling": ([_vp, C.c_uint, C.c_int], C.c_int),
     "pkx_model_profile_read": ([_vp, C.POINTER(C.c_double), C.POINTER(C.c_int64)], C.c_int),
 }
@@ -795,3 +837,146 @@ class BeamReorder(_Bound):
             n = int(np.prod(s.shape[1:])) * np.dtype(s.dtype).itemsize
             a[i] = BeamState(s.ptr, d.ptr, n, n, n)
         self._bind("pkx_beam_reorder", (parent.ptr, B, W, a, len(states)), (parent, a, states))
+
+
+# ---- the rest of a decoder's block ------------------------------------------------
+def _row(a):
+    """Elements between the rows of a matrix [M][n]."""
+    return 0 if a is None else _strides(a)[0]
+
+
+def _kind(kinds, name, what):
+    if name not in kinds:
+        raise PkxError(f"{what}: one of {', '.join(kinds)} is wanted, got {name!r}")
+    return kinds[name]
+
+
+class BlockNorm(_Bound):
+    """pkx_block_norm: x_out = x + alpha * g * post(y), h = pre(x_out).
+
+    x, x_out [M][d] f32 or f16; y, gate, h f32 or f16, gate [ceil(M / rows_per_gate)][d]; h int8 with h_scale [M] f32;
+    weights and biases [d] f32.  x, y, gate and x_out may be missing."""
+
+    def __init__(self, x=None, h=None, y=None, x_out=None, post="none", post_w=None, post_b=None, gate=None, rows_per_gate=1,
+                 gate_fn="linear", alpha=1.0, pre="none", pre_w=None, pre_b=None, eps=1e-5, post_eps=None, pre_eps=None, h_scale=None):
+        like = x if x is not None else y
+        if like is None or len(like.shape) != 2:
+            raise PkxError("block norm: x or y [rows][d] is wanted")
+        M, d = like.shape
+        i8 = h is not None and np.dtype(h.dtype) == np.int8
+        narrow = [a for a in (y, gate, None if i8 else h) if a is not None]
+        stream_ = [a for a in (x, x_out) if a is not None]
+        dt = np.dtype((narrow or stream_)[0].dtype)
+        dx = np.dtype((stream_ or narrow)[0].dtype)
+        if i8 and h_scale is None:
+            raise PkxError("block norm: h in 8 bits needs h_scale")
+        if not i8 and h_scale is not None:
+            raise PkxError("block norm: h_scale goes with h in 8 bits")
+        for a, n, t in ((x, (M, d), dx), (x_out, (M, d), dx), (y, (M, d), dt), (h, (M, d), np.int8 if i8 else dt),
+                        (gate, (-(-M // max(int(rows_per_gate), 1)), d), dt)):
+            _expect(a, n, t, "block norm", strided=True)
+        for a, n in ((post_w, d), (post_b, d), (pre_w, d), (pre_b, d), (h_scale, M)):
+            _expect(a, (n,), np.float32, "block norm")
+        a = BlockNormArgs(_type((narrow or stream_)[0]), _type((stream_ or narrow)[0]), int(i8), d, M, _ptr(x), _row(x), _ptr(y), _row(y),
+                          _ptr(gate), _row(gate), int(rows_per_gate), _kind(GATES, gate_fn, "block norm gate"), _kind(NORMS, post, "block norm"),
+                          _kind(NORMS, pre, "block norm"), eps if post_eps is None else post_eps, eps if pre_eps is None else pre_eps, alpha,
+                          _ptr(post_w), _ptr(post_b), _ptr(pre_w), _ptr(pre_b), _ptr(x_out), _row(x_out), _ptr(h), _row(h), _ptr(h_scale))
+        self._bind("pkx_block_norm", (C.byref(a),), (a, x, h, y, x_out, post_w, post_b, gate, pre_w, pre_b, h_scale))
+
+
+class QuantizeRows(_Bound):
+    """pkx_quantize_rows: x [M][n] f32 or f16 -> q [M][n] int8, scale [M] f32."""
+
+    def __init__(self, x, q, scale):
+        M, n = x.shape
+        _expect(q, (M, n), np.int8, "quantise rows", strided=True)
+        _expect(scale, (M,), np.float32, "quantise rows")
+        self._bind("pkx_quantize_rows", (_type(x), x.ptr, _row(x), M, n, q.ptr, _row(q), scale.ptr), (x, q, scale))
+
+
+class WeightI8:
+    """Weights of LinearI8: w [N][K] int8 laid out once (pkx_i8_weight_pack), scale [N] f32, kept as it is."""
+
+    def __init__(self, w, scale, stream=None):
+        (N, K), n = w.shape, C.c_size_t()
+        _expect(w, (N, K), np.int8, "8-bit weights", strided=True)
+        _expect(scale, (N,), np.float32, "8-bit weights")
+        check(lib().pkx_i8_weight_bytes(N, K, C.byref(n)))
+        self.shape, self.scale, self.packed = (N, K), scale, DeviceArray((n.value,), np.uint8)
+        check(lib().pkx_i8_weight_pack(w.ptr, _row(w), N, K, self.packed.ptr, _sh(stream)))
+        # the layout may be read on another stream next, and w be freed
+        check(lib().pkx_stream_synchronize(_sh(stream)))
+
+    @classmethod
+    def quantize(cls, w, stream=None):
+        """From w [N][K] f32 or f16: a scale for each of the N output channels."""
+        q, scale = DeviceArray(w.shape, np.int8), DeviceArray((w.shape[0],), np.float32)
+        QuantizeRows(w, q, scale)(stream)
+        return cls(q, scale, stream)
+
+
+class LinearI8(_Bound):
+    """pkx_linear_i8: y [M][N] = add + alpha * act(x w^T + bias), w a WeightI8; x [M][K] f32 or f16, or int8 with x_scale [M]."""
+
+    def __init__(self, x, w, y, x_scale=None, bias=None, act="none", add=None, alpha=1.0):
+        (M, K), (N, Kw) = x.shape, w.shape
+        i8 = np.dtype(x.dtype) == np.int8
+        if K != Kw or i8 != (x_scale is not None):
+            raise PkxError(f"8-bit linear: x [M][{Kw}] is wanted, with x_scale if it is int8, got {np.dtype(x.dtype).name} {list(x.shape)}")
+        _expect(y, (M, N), y.dtype, "8-bit linear", strided=True)
+        _expect(add, (M, N), y.dtype, "8-bit linear", strided=True)
+        _expect(x_scale, (M,), np.float32, "8-bit linear")
+        _expect(bias, (N,), np.float32, "8-bit linear")
+        a = LinearI8Args(TYPE_I8 if i8 else _type(x), _type(y), M, N, K, x.ptr, _row(x), _ptr(x_scale), w.packed.ptr, w.scale.ptr,
+                         _ptr(bias), _kind(ACTS, act, "8-bit linear"), alpha, _ptr(add), _row(add), y.ptr, _row(y))
+        self._bind("pkx_linear_i8", (C.byref(a),), (a, x, w, y, x_scale, bias, add), "pkx_linear_i8_workspace")
+
+
+def rotary_frequencies(rot, base=10000.0, factor=1.0, context=0, low=1.0, high=32.0):
+    """pkx_rotary_frequencies as a float64 array [rot / 2]."""
+    f = np.zeros(rot // 2, np.float64)
+    check(lib().pkx_rotary_frequencies(base, rot, factor, context, low, high, f.ctypes.data_as(_P(C.c_double))))
+    return f
+
+
+class Rotary(_Bound):
+    """pkx_rotary: parts are (src, dst) pairs [R][n][heads][d] (dst may be src); freq [rot / 2] f64; start, count [R], pos [R][n] int32."""
+
+    def __init__(self, freq, parts, start=None, pos=None, count=None, interleaved=False, mult=1.0):
+        if not 1 <= len(parts) <= ROTARY_MAX_PARTS:
+            raise PkxError(f"rotary: 1 to {ROTARY_MAX_PARTS} parts are wanted, got {len(parts)}")
+        (R, n, _, d), rot = parts[0][0].shape, 2 * freq.shape[0]
+        _expect(freq, (rot // 2,), np.float64, "rotary")
+        a = RotaryArgs(_type(parts[0][0]), R, n, d, rot, int(interleaved), mult, freq.ptr, _ptr(start), _ptr(pos), _row(pos), _ptr(count), len(parts))
+        for i, (src, dst) in enumerate(parts):
+            for x in (src, dst):
+                _expect(x, (R, n, src.shape[2], d), parts[0][0].dtype, "rotary", strided=True)
+            a.part[i] = RotaryPart(src.ptr, *_strides(src), dst.ptr, *_strides(dst), src.shape[2])
+        _expect(start, (R,), np.int32, "rotary")
+        _expect(count, (R,), np.int32, "rotary")
+        _expect(pos, (R, n), np.int32, "rotary", strided=True)
+        self._bind("pkx_rotary", (C.byref(a),), (a, freq, parts, start, pos, count))
+
+
+class LogitRules(_Bound):
+    """pkx_logit_rules: logits, out [R][V]; tokens [slots][capacity] int32 with length [R] and slot [R] or table [R][capacity];
+    repetition, presence, frequency [R] f32; bias [rows][V] f32, mask [rows][ceil(V / 32)] int32 or uint32, their indexes [R] int32."""
+
+    def __init__(self, logits, out, tokens=None, length=None, slot=None, table=None, window=0, repetition=None, presence=None,
+                 frequency=None, bias=None, bias_index=None, mask=None, mask_index=None):
+        R, V = logits.shape
+        _expect(out, (R, V), logits.dtype, "logit rules", strided=True)
+        slots, cap = (0, 0) if tokens is None else tokens.shape
+        _expect(tokens, (slots, cap), np.int32, "logit rules")
+        for x, t in ((length, np.int32), (slot, np.int32), (repetition, np.float32), (presence, np.float32), (frequency, np.float32),
+                     (bias_index, np.int32), (mask_index, np.int32)):
+            _expect(x, (R,), t, "logit rules")
+        n_bias, n_mask = (0 if x is None else x.shape[0] for x in (bias, mask))
+        _expect(bias, (n_bias, V), np.float32, "logit rules", strided=True)
+        if mask is not None:
+            _expect(mask, (n_mask, (V + 31) // 32), np.int32 if np.dtype(mask.dtype) == np.int32 else np.uint32, "logit rules", strided=True)
+        a = LogitRulesArgs(_type(logits), R, V, logits.ptr, _row(logits), out.ptr, _row(out), _ptr(tokens), slots, cap, _ptr(length),
+                           _ptr(slot), _ptr(table), _table_row(table, R, cap), int(window), _ptr(repetition), _ptr(presence), _ptr(frequency),
+                           _ptr(bias), _row(bias), n_bias, _ptr(bias_index), _ptr(mask), _row(mask), n_mask, _ptr(mask_index))
+        self._bind("pkx_logit_rules", (C.byref(a),),
+                   (a, logits, out, tokens, length, slot, table, repetition, presence, frequency, bias, bias_index, mask, mask_index))
