@@ -60,6 +60,9 @@ struct LinearI8Params {
     void* y = nullptr;  int64_t y_row = 0;
 };
 void launch_linear_i8(const LinearI8Params& p, hipStream_t s);
+// The same from rows as they come, in one launch, for the few and short ones that linear_i8_fused() names.
+bool linear_i8_fused(int M, int K);
+void launch_linear_i8_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s);
 
 constexpr int kRotaryParts = 4, kMaxRotaryWidth = 512;
 struct RotaryPart {

@@ -144,28 +144,18 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(BlockNorm
     if (!p.h) return;
     if (p.pre != NORM_NONE) normalise<T, NV>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, first, t, d, p.inv_d, ps);
     if constexpr (I8) {
-        float top = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
-            if (8 * (t + k * T) < d) {
-                if (8 * (t + k * T) + 8 > d)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (8 * (t + k * T) + e >= d) x[k][e] = 0.f;
-                top = finite_max8(x[k], top);
-            }
-        top = wave_max_full(top);
-        if constexpr (T > 64) {
-            if ((threadIdx.x & 63) == 0) top_part[threadIdx.x >> 6] = top;
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < T / 64; ++i) top = fmaxf(top, top_part[i]);
-        }
-        const float s = top / 127.0f;
+            for (int e = 0; e < 8; ++e)
+                if (8 * (t + k * T) + e >= d) x[k][e] = 0.f;    // weights and biases are not read there
+        const RowTop top = row_top<T, NV>(x, top_part);
+        const float s = top.top / 127.0f;
         if (t == 0) p.h_scale[r] = s;
+        const RowQuantiser held(s, top.plain);
         int8_t* o = (int8_t*)p.h + r * p.h_row;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) store_bytes8(o, quantised8(x[k], s), 8 * (t + k * T), d);
+        for (int k = 0; k < NV; ++k) store_bytes8(o, held(x[k]), 8 * (t + k * T), d);
     } else {
         ET* o = (ET*)p.h + r * p.h_row;
 #pragma unroll

@@ -21,39 +21,45 @@ typedef int int16v __attribute__((ext_vector_type(16)));
 // A row is read once and kept in registers up to 8 T NV values; longer rows are read twice.
 template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_rows_kernel(QuantizeRowsParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1;
-    __shared__ float part[T / 64];
+    __shared__ float part[T / 64], more[T / 64];
     const int t = threadIdx.x % T, d = p.d;
     const int64_t r = (int64_t)blockIdx.x * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0);
     if (r >= p.rows) return;
     const ET* x = (const ET*)p.x + r * p.x_row;
-    float v[NV][8], top = 0.f;
+    float v[NV][8];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        load_row8(v[k], x, 8 * (t + k * T), d);
-        top = finite_max8(v[k], top);
-    }
-    for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
-        float w[8];
-        load_row8(w, x, i, d);
-        top = finite_max8(w, top);
-    }
-    top = wave_max_full(top);
-    if constexpr (T > 64) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
-        __syncthreads();
+    for (int k = 0; k < NV; ++k) load_row8(v[k], x, 8 * (t + k * T), d);
+    RowTop top = row_top<T, NV>(v, part);
+    const bool longer = d > 8 * T * NV;
+    if (longer) {                            // only the longest rows' kernel: T > 64
+        float w[1][8] = {}, m = 0.f;
+        bool plain = true;
+        for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
+            RowMax seen;
+            load_row8(w[0], x, i, d);
+            seen.add(w[0]);
+            plain &= seen.odd == 0.f;
+            m = finite_max8(w[0], m);
+        }
+        w[0][0] = m;
 #pragma unroll
-        for (int i = 0; i < T / 64; ++i) top = fmaxf(top, part[i]);
+        for (int e = 1; e < 8; ++e) w[0][e] = 0.f;
+        const RowTop rest = row_top<T, 1>(w, more);
+        top.top = fmaxf(top.top, rest.top);
+        top.plain &= __syncthreads_and(plain);
     }
-    const float s = top / 127.0f;
+    const float s = top.top / 127.0f;
     if (t == 0) p.scale[r] = s;
+    const RowQuantiser held(s, top.plain);
     int8_t* q = p.q + r * p.q_row;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) store_bytes8(q, quantised8(v[k], s), 8 * (t + k * T), d);
-    for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
-        float w[8];
-        load_row8(w, x, i, d);
-        store_bytes8(q, quantised8(w, s), i, d);
-    }
+    for (int k = 0; k < NV; ++k) store_bytes8(q, held(v[k]), 8 * (t + k * T), d);
+    if (longer)
+        for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
+            float w[8];
+            load_row8(w, x, i, d);
+            store_bytes8(q, held(w), i, d);
+        }
 }
 
 template <typename ET> void launch_quantize_typed(const QuantizeRowsParams& p, hipStream_t s) {
@@ -80,98 +86,236 @@ __global__ __launch_bounds__(256) void i8_pack_kernel(const int8_t* w, int64_t w
 }
 
 // ---- epilogue --------------------------------------------------------------
-// CNT channels from n0 on of token m.
-template <typename YT, int CNT>
-__device__ __forceinline__ void finish(const LinearI8Params& p, const int* acc, int m, int n0, float xs) {
-    const int64_t row = (int64_t)m;
-    YT* y = (YT*)p.y + row * p.y_row + n0;
-    const YT* add = p.add ? (const YT*)p.add + row * p.add_row + n0 : nullptr;
+// v / (1 + e^-v).  e^-v as 2^t (1 + r ln 2) with t = -v log2 e in f32 and r what its rounding left; the
+// reciprocal of 1 + e^-v to half a step by a Newton step.  About 10 instructions where expf
+// and a division take 35.
+// An f16 result takes the bare exponential and reciprocal (|v| 2^-23 relative, far below its 2^-11):
+// 2000 x 4096 outputs 1.2 us less.
+template <typename YT> __device__ __forceinline__ float silu_of(float v) {
+    if constexpr (sizeof(YT) == 2) return silu_dev(v);
+    const float t = v * -1.4426950408889634f;
+    const float r = fmaf(v, -1.4426950408889634f, -t) + v * -1.925963033500e-8f;   // log2 e less its f32
+    float e = __builtin_amdgcn_exp2f(t);
+    e = t < 127.f ? fmaf(e, r * 0.69314718056f, e) : e;
+    const float d = 1.0f + e;
+    float q = __builtin_amdgcn_rcpf(d);
+    q = d < 1e38f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
+    return v * q;
+}
+
+// What a lane needs of CNT channels from n0 < N on, for any number of tokens.
+template <typename YT, int CNT> struct Channels {
     typedef YT vec __attribute__((ext_vector_type(CNT)));
     typedef vec vecu __attribute__((aligned(sizeof(YT))));
     typedef float fvec __attribute__((ext_vector_type(CNT)));
     typedef fvec fvecu __attribute__((aligned(4)));
-    if (n0 + CNT <= p.N) {
-        const fvec ws = *(const fvecu*)(p.w_scale + n0);
-        fvec b = {};
-        if (p.bias) b = *(const fvecu*)(p.bias + n0);
+    typedef int ivec __attribute__((ext_vector_type(CNT)));
+    fvec ws, b = {};
+    int n0;
+    bool whole;
+
+    __device__ __forceinline__ Channels(const LinearI8Params& p, int n) : n0(n), whole(n + CNT <= p.N) {
+        if (whole) {
+            ws = *(const fvecu*)(p.w_scale + n0);
+            if (p.bias) b = *(const fvecu*)(p.bias + n0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < CNT; ++e) {
+                const int at = n0 + e < p.N ? n0 + e : n0;
+                ws[e] = p.w_scale[at];
+                if (p.bias) b[e] = p.bias[at];
+            }
+        }
+    }
+    __device__ __forceinline__ void store(const LinearI8Params& p, ivec acc, int m, float xs) const {
+        YT* y = (YT*)p.y + (int64_t)m * p.y_row + n0;
+        const YT* add = p.add ? (const YT*)p.add + (int64_t)m * p.add_row + n0 : nullptr;
         vec a = {};
-        if (add) a = *(const vecu*)add;
+        if (add) {
+            if (whole) a = *(const vecu*)add;
+            else
+#pragma unroll
+                for (int e = 0; e < CNT; ++e)
+                    if (n0 + e < p.N) a[e] = add[e];
+        }
+        float v[CNT];
+#pragma unroll
+        for (int e = 0; e < CNT; ++e) v[e] = (float)acc[e] * (xs * ws[e]) + b[e];
+        if (p.silu)
+#pragma unroll
+            for (int e = 0; e < CNT; ++e) v[e] = silu_of<YT>(v[e]);
         vec o;
 #pragma unroll
         for (int e = 0; e < CNT; ++e) {
-            float v = (float)acc[e] * (xs * ws[e]);
-            if (p.bias) v += b[e];
-            if (p.silu) v = v / (1.0f + expf(-v));
-            v *= p.alpha;
-            if (add) v += (float)a[e];
-            o[e] = (YT)v;
+            v[e] *= p.alpha;
+            if (add) v[e] += (float)a[e];
+            o[e] = (YT)v[e];
         }
-        *(vecu*)y = o;
-        return;
-    }
+        if (whole) *(vecu*)y = o;
+        else
 #pragma unroll
-    for (int e = 0; e < CNT; ++e) {
-        if (n0 + e >= p.N) break;
-        float v = (float)acc[e] * (xs * p.w_scale[n0 + e]);
-        if (p.bias) v += p.bias[n0 + e];
-        if (p.silu) v = v / (1.0f + expf(-v));
-        v *= p.alpha;
-        if (add) v += (float)add[e];
-        y[e] = (YT)v;
+            for (int e = 0; e < CNT; ++e)
+                if (n0 + e < p.N) y[e] = o[e];
     }
-}
+};
 
 // ---- few tokens ------------------------------------------------------------
-// 16 channels x 16 MT tokens to a workgroup, K shared out over its waves block by
-// block (a wave reads 1 KB of weights and MT KB of tokens per step, straight into
-// the fragments) and the partial sums joined through LDS.
-template <typename YT, int MT, int W> __global__ __launch_bounds__(W * 64) void i8_rows_kernel(LinearI8Params p, int mtiles) {
-    __shared__ int4v part[W][MT][64];
+// 16 channels x 16 tokens to a workgroup, K shared out over its eight waves block by
+// block (a wave reads 1 KB of weights and 1 KB of tokens per block, straight into
+// the fragments, four blocks at a time) and the partial sums joined through LDS.
+// 64 tokens to a workgroup read the weights once instead of four times, but are fewer workgroups: 64 x 1024 x 4096
+// 9.7 us instead of 4.8.  1 x 8192 x 8192: 11.2 us, 67 MB at 6 TB/s.
+constexpr int kRowWaves = 8;
+template <typename YT>
+__device__ __forceinline__ void rows_finish(const LinearI8Params& p, int4v acc, int4v (&part)[kRowWaves][64], int nh, int m0, const float* xs) {
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int unit = blockIdx.x, nh = udiv_small(unit, mtiles), m0 = (unit - nh * mtiles) * 16 * MT;
+    part[w][lane] = acc;
+    __syncthreads();
+    // slots 16 h + 4 g + r of the block are these four channels
+    const int g = lane >> 4, h = nh & 1, n0 = (nh >> 1) * kI8ColBlock + 16 * (g & 1) + 4 * (2 * h + (g >> 1));
+    const int m = m0 + (lane & 15);
+    if (w != 0 || m >= p.M || n0 >= p.N) return;
+    const Channels<YT, 4> ch(p, n0);
+    int4v s = part[0][lane];
+#pragma unroll
+    for (int j = 1; j < kRowWaves; ++j) s += part[j][lane];
+    ch.store(p, s, m, xs[m]);
+}
+
+template <typename YT> __global__ __launch_bounds__(kRowWaves * 64) void i8_rows_kernel(LinearI8Params p, int mtiles) {
+    constexpr int W = kRowWaves, U = 4;
+    __shared__ int4v part[W][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int nh = udiv_small(blockIdx.x, mtiles), m0 = (blockIdx.x - nh * mtiles) * 16;
     const int kblocks = (p.K + kI8DepthPad - 1) / kI8DepthPad * (kI8DepthPad / kI8DepthBlock);
-    const int8_t* wp = (const int8_t*)p.w + (int64_t)(nh >> 1) * kblocks * 2048;
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wp, (int64_t)kblocks * 2048);
-    const int k16 = (p.K + 15) & ~15, rows = p.M - m0 < 16 * MT ? p.M - m0 : 16 * MT;
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc((const int8_t*)p.w + (int64_t)(nh >> 1) * kblocks * 2048, (int64_t)kblocks * 2048);
+    const int k16 = (p.K + 15) & ~15, rows = p.M - m0 < 16 ? p.M - m0 : 16;
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (int64_t)m0 * p.x_row, (int64_t)(rows - 1) * p.x_row + k16);
     const uint32_t wo = ((lane >> 4) * 32 + 16 * (nh & 1) + (lane & 15)) * 16;
     const uint32_t xo = (uint32_t)((lane & 15) * p.x_row + 16 * (lane >> 4));
-    int4v acc[MT] = {};
-    for (int kb = w; kb < kblocks; kb += W) {
-        const int4v a = __builtin_amdgcn_raw_buffer_load_b128(rw, wo, kb * 2048, 0);
-        int4v b[MT];
+    int4v acc = {};
+    for (int k0 = w; k0 < kblocks; k0 += U * W) {
+        int4v a[U], b[U];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) b[i] = __builtin_amdgcn_raw_buffer_load_b128(rx, xo + (uint32_t)(16 * i * p.x_row) + kb * 64, 0, 0);
+        for (int u = 0; u < U; ++u) {        // blocks past the last: zeros, and no token read
+            const int kb = k0 + u * W;
+            a[u] = __builtin_amdgcn_raw_buffer_load_b128(rw, kb < kblocks ? wo + kb * 2048 : OOB, 0, 0);
+            b[u] = __builtin_amdgcn_raw_buffer_load_b128(rx, kb < kblocks ? xo + kb * 64 : OOB, 0, 0);
+        }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b[i], acc[i], 0, 0, 0);
+        for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u], acc, 0, 0, 0);
     }
+    rows_finish<YT>(p, acc, part, nh, m0, p.x_scale);
+}
+
+// Few tokens as they come, quantised by every workgroup for itself: one launch instead of two where that costs less than
+// a launch.  Each wave asks for its first blocks of weights, then the rows are shared out: `wpr` waves to a row, up
+// to 8 x 64 x NV values a wave, held in LDS in rows 16 bytes apart in banks.  1 x 4096 x 1024: 3.7 us, in two launches
+// 5.2; 16 x 4096 x 1024 5.0 and 5.6; 16 x 4096 x 2048 7.1 and 5.9, so up to 2^14 values.
+template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) void i8_rows_fused_kernel(LinearI8Params p, const XT* x, int64_t x_row, int wpr) {
+    constexpr int W = kRowWaves, U = 8;
+    extern __shared__ __align__(16) uint8_t held[];          // [M][kpad + 16]
+    __shared__ int4v part[W][64];
+    __shared__ float tops[W], scale[16];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nh = blockIdx.x;
+    const int kpad = (p.K + kI8DepthPad - 1) / kI8DepthPad * kI8DepthPad, kblocks = kpad / kI8DepthBlock, ld = kpad + 16;
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc((const int8_t*)p.w + (int64_t)(nh >> 1) * kblocks * 2048, (int64_t)kblocks * 2048);
+    const uint32_t wo = ((lane >> 4) * 32 + 16 * (nh & 1) + (lane & 15)) * 16;
+    int4v a[U];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) part[w][i][lane] = acc[i];
+    for (int u = 0; u < U; ++u) a[u] = __builtin_amdgcn_raw_buffer_load_b128(rw, w + u * W < kblocks ? wo + (w + u * W) * 2048 : OOB, 0, 0);
+
+    const int slots = W / wpr, sub = w % wpr;
+    auto load = [&](int r, float (&v)[NV][8]) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) load_row8(v[k], x + r * x_row, 8 * (lane + 64 * (sub + wpr * k)), p.K);
+    };
+    auto hold = [&](int r, const float (&v)[NV][8], RowTop top) {
+        const float s = top.top / 127.0f;
+        if (lane == 0 && sub == 0) scale[r] = s;
+        const RowQuantiser q(s, top.plain);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int at = 8 * (lane + 64 * (sub + wpr * k));
+            if (at < kpad) *(int2v*)(held + r * ld + at) = q(v[k]);      // zeros past K
+        }
+    };
+    if (wpr == 1) {
+        for (int r = w; r < p.M; r += slots) {
+            float v[NV][8];
+            load(r, v);
+            hold(r, v, row_top<64, NV>(v, nullptr));
+        }
+    } else {                                 // one row at most to a wave
+        const int r = w / wpr;
+        float v[NV][8] = {};
+        if (r < p.M) load(r, v);
+        RowTop top = row_top<64, NV>(v, nullptr);
+        if (lane == 0) tops[w] = top.plain ? top.top : -top.top;
+        __syncthreads();
+        for (int i = 0; i < wpr; ++i) {
+            const float o = tops[w - sub + i];
+            top.plain &= __builtin_bit_cast(int, o) >= 0;
+            top.top = fmaxf(top.top, fabsf(o));
+        }
+        if (r < p.M) hold(r, v, top);
+    }
     __syncthreads();
-    for (int i = w; i < MT; i += W) {
-        int4v s = part[0][i][lane];
+    const int row = (lane & 15) < p.M ? lane & 15 : p.M - 1;         // tokens past the last give sums that nobody reads
+    const uint8_t* xr = held + row * ld + 16 * (lane >> 4);
+    int4v acc = {};
+    for (int k0 = w; k0 < kblocks; k0 += U * W) {
+        if (k0 > w)
 #pragma unroll
-        for (int j = 1; j < W; ++j) s += part[j][i][lane];
-        const int m = m0 + 16 * i + (lane & 15), g = lane >> 4, h = nh & 1;
-        // slots 16 h + 4 g + r of the block are these four channels
-        const int n0 = (nh >> 1) * kI8ColBlock + 16 * (g & 1) + 4 * (2 * h + (g >> 1));
-        if (m < p.M && n0 < p.N) finish<YT, 4>(p, (const int*)&s, m, n0, p.x_scale[m]);
+            for (int u = 0; u < U; ++u) a[u] = __builtin_amdgcn_raw_buffer_load_b128(rw, k0 + u * W < kblocks ? wo + (k0 + u * W) * 2048 : OOB, 0, 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * W >= kblocks) break;
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], *(const int4v*)(xr + (k0 + u * W) * 64), acc, 0, 0, 0);
+        }
     }
+    rows_finish<YT>(p, acc, part, nh, 0, scale);
 }
 
 // ---- many tokens -----------------------------------------------------------
 // WM x WN waves of TM x TN tiles of 32 tokens x 32 channels.  Tokens go through
 // LDS (rows of 128 bytes, their 16-byte pieces permuted by the row so that the
 // reads of a tile fall into different banks), weights straight into the fragments.
+//
+// Slab k (128 inputs) is computed in step k.  Its weights were asked for in step k - WD + 1, its tokens, by loads
+// straight into LDS, in step k - WD - 1, and waited for by every wave before the barrier that opens step
+// k - 1; so the first fragments of step k are read during step k - 1 and no wave
+// waits for LDS after a barrier.  Small tiles, whose products of a quarter slab are over before LDS
+// answers, have read the whole of slab k by then (AHEAD).  Step k fills the stage that is free: slab k's, read
+// ahead, or else slab k - 1's.
+// A barrier of the workgroup's waves behind their own LDS reads and all but the last N of their vector-memory
+// operations; no memory operation passes it.
+template <int N> __device__ __forceinline__ void join() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | ((N >> 4) << 14) | (0x7 << 4));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 template <typename YT, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM * WN * 64) void i8_tile_kernel(LinearI8Params p, int mtiles, int ntiles) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params p, int mtiles, int ntiles) {
     constexpr int W = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, ROWS = BM / 8 / W;   // DMA instructions of a wave per slab
+    constexpr bool AHEAD = TM * TN <= 4;
+    // weights of two slabs in turn; of four: no faster (512 x 4096 x 4096 on 64 x 128 tiles 15.9 and 15.8 us), more registers
+    constexpr int WD = 2, ST = AHEAD ? WD + 1 : WD + 2, STAGE = BM * 128;    // ST stages of tokens
     static_assert(BM / 8 % W == 0, "rows of a slab go evenly over the waves");
-    __shared__ __align__(16) uint8_t slab[2][BM * 128];
+    constexpr int SUMS = W * 32 * TN * 128;      // 32 tokens' sums of every wave, at the end
+    __shared__ __align__(16) uint8_t slab[ST * STAGE > SUMS ? ST * STAGE : SUMS];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wid % WM, wn = wid / WM;
+    // an XCD's tiles are neighbours: eight rows of tiles at a time, column by column (8192^3: 482 us; one row at a
+    // time 563, 16 rows 565, 32 rows 603)
+    constexpr int group = 8;
     const int tile = xcd_tile(blockIdx.x, mtiles * ntiles);
-    const int tn = tile / mtiles, m0 = (tile - tn * mtiles) * BM, n0 = tn * BN;
+    const int g = tile / (group * ntiles), in = tile - g * group * ntiles;
+    const int gm = mtiles - g * group < group ? mtiles - g * group : group;
+    const int tn = in / gm, m0 = (g * group + in - tn * gm) * BM, n0 = tn * BN;
     const int slabs = (p.K + kI8DepthPad - 1) / kI8DepthPad, kblocks = 2 * slabs;
     const int k16 = (p.K + 15) & ~15, rows = p.M - m0 < BM ? p.M - m0 : BM;
     const __amdgpu_buffer_rsrc_t rx = make_rsrc(p.x + (int64_t)m0 * p.x_row, (int64_t)(rows - 1) * p.x_row + k16);
@@ -182,85 +326,164 @@ __global__ __launch_bounds__(WM * WN * 64) void i8_tile_kernel(LinearI8Params p,
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
         const int r = (wid * ROWS + i) * 8 + (lane >> 3);
-        xo[i] = (uint32_t)(r * p.x_row + 16 * ((lane & 7) ^ (r & 7)));
+        xo[i] = (uint32_t)(r * p.x_row + 16 * ((lane & 7) ^ (r >> 1 & 7)));
     }
     uint32_t wo[TN];
 #pragma unroll
     for (int j = 0; j < TN; ++j) wo[j] = (uint32_t)((wn * TN + j) * kblocks * 2048 + lane * 16);
-    const uint8_t* arow[2];
+    uint32_t ao[4];                          // a lane's pieces of a stage, tile 0
 #pragma unroll
-    for (int b = 0; b < 2; ++b) arow[b] = slab[b] + (wm * TM * 32 + (lane & 31)) * 128;
-    const int half = lane >> 5, sw = lane & 7;
+    for (int q = 0; q < 4; ++q) ao[q] = (uint32_t)((wm * TM * 32 + (lane & 31)) * 128 + 16 * ((2 * q + (lane >> 5)) ^ (lane >> 1 & 7)));
 
     int16v acc[TM][TN] = {};
-    int4v wf[2][4][TN];
-    auto fetch = [&](int k, int b) {
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) lds_dma16(rx, slab[b] + (wid * ROWS + i) * 1024, xo[i], k * 128);
+    int4v wf[WD][4][TN], xf[2][AHEAD ? 4 : 1][TM];
+    // past the last slab nothing is read: a resource of no bytes, so that every step issues the same loads
+    const __amdgpu_buffer_rsrc_t none = make_rsrc(p.w, 0);
+    auto fetch = [&](int k, int stage, int i) {      // a wave's i-th 1 KB of slab k
+        lds_dma16(k < slabs ? rx : none, slab + stage * STAGE + (wid * ROWS + i) * 1024, xo[i], k * 128);
     };
-    auto fetch_w = [&](int k, int4v (&f)[4][TN]) {
+    auto fetch_w = [&](int k, int q, int4v (&f)[4][TN]) {
+        const __amdgpu_buffer_rsrc_t r = k < slabs ? rw : none;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) f[q][j] = __builtin_amdgcn_raw_buffer_load_b128(rw, wo[j] + q * 1024, k * 4096, 0);
+        for (int j = 0; j < TN; ++j) f[q][j] = __builtin_amdgcn_raw_buffer_load_b128(r, wo[j] + q * 1024, k * 4096, 0);
     };
-    auto step = [&](int k, int b) {
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (k + 1 < slabs) {
-            fetch(k + 1, b ^ 1);
-            fetch_w(k + 1, wf[b ^ 1]);
-        }
+    auto read = [&](int stage, int q, int4v (&f)[TM]) {
+        const uint8_t* st = slab + stage * STAGE;
+#pragma unroll
+        for (int i = 0; i < TM; ++i) f[i] = *(const int4v*)(st + ao[q] + i * 32 * 128);
+    };
+    int stage = 0;                           // slab k's
+    auto step = [&](int k, int u, int4v (&w)[4][TN], int4v (&next)[4][TN]) {     // u: k modulo WD
+        // slab k + 1 is there; what the last WD - 1 steps asked for may still be on its way
+        join<(WD - 1) * (ROWS + 4 * TN)>();
+        const int after = stage == ST - 1 ? 0 : stage + 1, before = stage == 0 ? ST - 1 : stage - 1;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            int4v xf[TM];
+            if (AHEAD) read(after, q, xf[(u + 1) & 1][q]);
+            else if (q < 3) read(stage, q + 1, xf[(q + 1) & 1][0]);
+            else read(after, 0, xf[0][0]);
 #pragma unroll
-            for (int i = 0; i < TM; ++i) xf[i] = *(const int4v*)(arow[b] + i * 32 * 128 + 16 * ((2 * q + half) ^ sw));
+            for (int i = 0; i < TM; ++i) {
+                // loads in the middle of the products, a few at a time: in one burst they fill the queue and hold up what is behind them
+                if (i == TM / 2) {
+                    __builtin_amdgcn_sched_barrier(0);
+                    fetch_w(k + WD - 1, q, next);
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                    for (int d = q * ROWS / 4; d < (q + 1) * ROWS / 4; ++d) fetch(k + WD + 1, AHEAD ? stage : before, d);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[b][q][j], xf[i], acc[i][j], 0, 0, 0);
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(w[q][j], AHEAD ? xf[u & 1][q][i] : xf[q & 1][0][i], acc[i][j], 0, 0, 0);
+            }
         }
+        stage = after;
     };
-    fetch(0, 0);
-    fetch_w(0, wf[0]);
-    int k = 0;
-    for (; k + 1 < slabs; k += 2) {
-        step(k, 0);
-        step(k + 1, 1);
+    // in the order in which the steps before the first would have issued them, so that step 0's count holds
+#pragma unroll
+    for (int k = 0; k < WD + 1; ++k) {
+        if (k >= 2)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) fetch_w(k - 2, q, wf[k - 2]);
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i) fetch(k, k, i);
     }
-    if (k < slabs) step(k, 0);
+    join<(WD - 1) * (ROWS + 4 * TN) + ROWS>();
+#pragma unroll
+    for (int q = 0; q < (AHEAD ? 4 : 1); ++q) read(0, q, xf[0][q]);
+    for (int k = 0; k < slabs; k += WD) {
+#pragma unroll
+        for (int u = 0; u < WD; ++u)
+            if (k + u < slabs) step(k + u, u, wf[u], wf[(u + WD - 1) % WD]);
+    }
 
+    // A wave's sums pass through LDS (32 tokens at a time, their 16-byte pieces permuted by the row), so that
+    // neighbouring lanes write neighbouring pieces of a row: as the matrix instructions leave them a store would touch 64
+    // half lines (16 MB of f16 took 6 us that way).
+    constexpr int E = 16 / sizeof(YT), PER = 32 * TN / E, STEP = 64 / PER, PIECES = 8 * TN;
+    join<0>();
+    auto swizzle = [](int r) { return TN == 1 ? r >> 1 & 7 : r & (PIECES - 1); };   // 16 rows' pieces in 64 banks
+    uint8_t* own = slab + wid * 32 * TN * 128;
+    const int n = n0 + wn * TN * 32 + E * (lane % PER);
+    if (n0 + wn * TN * 32 >= p.N) return;
+    const Channels<YT, E> ch(p, n < p.N ? n : p.N - 1);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int m = m0 + (wm * TM + i) * 32 + (lane & 31);
-        if (m >= p.M) continue;
-        const float xs = p.x_scale[m];
+        const int r0 = lane & 31;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int n = n0 + (wn * TN + j) * 32 + 16 * half;
-            if (n < p.N) finish<YT, 16>(p, (const int*)&acc[i][j], m, n, xs);
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const int piece = 8 * j + 4 * (lane >> 5) + g;
+                *(int4v*)(own + r0 * TN * 128 + 16 * (piece ^ swizzle(r0))) = int4v{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+            }
+#pragma unroll
+        for (int r1 = 0; r1 < 32; r1 += STEP) {
+            const int r = r1 + lane / PER, m = m0 + (wm * TM + i) * 32 + r;
+            typename Channels<YT, E>::ivec v;
+#pragma unroll
+            for (int h = 0; h < E / 4; ++h) {
+                const int4v c = *(const int4v*)(own + r * TN * 128 + 16 * (((E / 4) * (lane % PER) + h) ^ swizzle(r)));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * h + e] = c[e];
+            }
+            if (m < p.M && n < p.N) ch.store(p, v, m, p.x_scale[m]);
         }
     }
 }
 
+template <typename YT, int WM, int WN, int TM, int TN> void launch_tiles(const LinearI8Params& p, hipStream_t s) {
+    const int mt = cdiv(p.M, 32 * WM * TM), nt = cdiv(p.N, 32 * WN * TN);
+    launch(i8_tile_kernel<YT, WM, WN, TM, TN>, dim3(mt * nt), dim3(WM * WN * 64), 0, s, p, mt, nt);
+}
+
+// The form whose estimated time is least, in us a 1024 of K, from what a round of 256 workgroups takes of it:
+//   rows 16 x 16          0.6   64 x 1024 x 4096 4.8 us (32 x 128 tiles: 9.1); 64 x 4096 x 4096 12.7 (8.3); launch and ends 3, tiles 4
+//   tiles of 32 x 128     1.3   128 x 4096 x 4096 8.7 us (64 x 128: 10.1); several to a CU
+//   tiles of 64 x 128     2.4   512 x 4096 x 4096 15.8 us (32 x 128: 17.8, 128 x 256: 27.7); several to a CU
+//   tiles of 128 x 256    9.6   2000 x 4096 x 1024 16.1 us (64 x 128: 17.3, 256 x 256: 22); one to a CU
+//   tiles of 256 x 256   16     16384 x 4096 x 4096 264 us (128 x 256: 318); one to a CU
 template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s) {
-    if (p.M <= 64) {
-        const int mt = p.M <= 16 ? 1 : 2, mtiles = cdiv(p.M, 16 * mt), units = 2 * cdiv(p.N, 32) * mtiles;
-        if (mt == 1) launch(i8_rows_kernel<YT, 1, 8>, dim3(units), dim3(512), 0, s, p, mtiles);
-        else launch(i8_rows_kernel<YT, 2, 8>, dim3(units), dim3(512), 0, s, p, mtiles);
-        return;
-    }
-    if ((int64_t)cdiv(p.M, 256) * cdiv(p.N, 256) >= 200) {
-        const int mt = cdiv(p.M, 256), nt = cdiv(p.N, 256);
-        launch(i8_tile_kernel<YT, 2, 4, 4, 2>, dim3(mt * nt), dim3(512), 0, s, p, mt, nt);
-        return;
-    }
-    const int mt = cdiv(p.M, 128), nt = cdiv(p.N, 128);
-    launch(i8_tile_kernel<YT, 2, 2, 2, 2>, dim3(mt * nt), dim3(256), 0, s, p, mt, nt);
+    const float depth = p.K / 1024.0f, cus = 256.0f;
+    const auto tiles = [&](int bm, int bn) { return (float)cdiv(p.M, bm) * cdiv(p.N, bn); };
+    const auto shared = [&](float n) { return fmaxf(1.0f, n / cus); };   // rounds where a CU holds several workgroups
+    const auto alone = [&](float n) { return ceilf(n / cus); };
+    const float t32 = 1.3f * shared(tiles(32, 128)), t64 = 2.4f * shared(tiles(64, 128));
+    const float t128 = 9.6f * alone(tiles(128, 256)), t256 = 16.0f * alone(tiles(256, 256));
+    const float best = fminf(fminf(t32, t64), fminf(t128, t256));
+    const float units = 2.0f * tiles(16, 32);
+    if (units < (float)(1 << 22) && 3.0f + 0.6f * fmaxf(0.8f, units / cus) * depth < 4.0f + best * depth) {
+        const int mtiles = cdiv(p.M, 16);
+        launch(i8_rows_kernel<YT>, dim3(2 * cdiv(p.N, 32) * mtiles), dim3(512), 0, s, p, mtiles);
+    } else if (t256 == best) launch_tiles<YT, 2, 4, 4, 2>(p, s);
+    else if (t128 == best) launch_tiles<YT, 2, 4, 2, 2>(p, s);
+    else if (t64 == best) launch_tiles<YT, 1, 4, 2, 1>(p, s);
+    else launch_tiles<YT, 1, 4, 1, 1>(p, s);
+}
+
+// Waves to a row of the fused form: all eight for one token, one from five tokens on.
+int fused_waves(int M) { return M == 1 ? 8 : M == 2 ? 4 : M <= 4 ? 2 : 1; }
+
+template <typename YT, typename XT> void launch_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s) {
+    const int wpr = fused_waves(p.M), kpad = cdiv(p.K, kI8DepthPad) * kI8DepthPad;
+    const uint32_t lds = p.M * (kpad + 16);
+    const int per = cdiv(kpad, 512 * wpr);
+    const dim3 grid(2 * cdiv(p.N, 32));
+    if (per <= 1) launch(i8_rows_fused_kernel<YT, XT, 1>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
+    else if (per <= 2) launch(i8_rows_fused_kernel<YT, XT, 2>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
+    else launch(i8_rows_fused_kernel<YT, XT, 4>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
 }
 
 }  // namespace
+
+bool linear_i8_fused(int M, int K) {
+    const int kpad = cdiv(K, kI8DepthPad) * kI8DepthPad;
+    return M <= 16 && kpad <= 4 * 512 * fused_waves(M) && M * kpad <= 16384;
+}
+void launch_linear_i8_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s) {
+    if (p.M == 0 || p.N == 0) return;
+    if (p.y_f32) q.f32 ? launch_fused<float, float>(p, q, s) : launch_fused<float, f16>(p, q, s);
+    else q.f32 ? launch_fused<f16, float>(p, q, s) : launch_fused<f16, f16>(p, q, s);
+}
 
 void launch_quantize_rows(const QuantizeRowsParams& p, hipStream_t s) {
     if (p.rows == 0) return;

@@ -86,6 +86,17 @@ __device__ __forceinline__ float wave_max_full(float v) {
     return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
 }
 
+// The largest magnitude of a row, and whether it holds an infinity or a NaN: `odd` is 0 times every value, NaN then.
+struct RowMax {
+    float top = 0.f, odd = 0.f;
+    __device__ __forceinline__ void add(const float (&v)[8]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            top = fmaxf(top, fabsf(v[e]));
+            odd = fmaf(v[e], 0.f, odd);
+        }
+    }
+};
 // The largest finite magnitude among v and top.
 __device__ __forceinline__ float finite_max8(const float (&v)[8], float top) {
 #pragma unroll
@@ -95,17 +106,77 @@ __device__ __forceinline__ float finite_max8(const float (&v)[8], float top) {
     }
     return top;
 }
-// clamp(round(x / s), -127, 127), ties to even; NaN is held as 0, 0 where the scale is 0.
-__device__ __forceinline__ int2v quantised8(const float (&v)[8], float s) {
-    int2v w = {};
+
+struct RowTop { float top; bool plain; };    // the largest finite magnitude of a row; whether all of it is finite
+// Of the NV x 8 values a lane, T lanes to the row: part [T / 64] joins the waves of a row, whose sign bits mark the odd ones.
+template <int T, int NV> __device__ __forceinline__ RowTop row_top(const float (&v)[NV][8], float* part) {
+    RowMax seen;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float r = s != 0.f ? rintf(v[e] / s) : 0.f;
-        r = r != r ? 0.f : fminf(fmaxf(r, -127.f), 127.f);
-        w[e >> 2] |= (int)((unsigned)((int)r & 0xFF) << (8 * (e & 3)));
+    for (int k = 0; k < NV; ++k) seen.add(v[k]);
+    RowTop o{seen.top, __ballot(seen.odd != 0.f) == 0};
+    if (!o.plain) {
+        o.top = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) o.top = finite_max8(v[k], o.top);
     }
-    return w;
+    o.top = wave_max_full(o.top);
+    if constexpr (T > 64) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = o.plain ? o.top : -o.top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) {
+            o.plain &= __builtin_bit_cast(int, part[i]) >= 0;
+            o.top = fmaxf(o.top, fabsf(part[i]));
+        }
+    }
+    return o;
 }
+
+// Rows held in 8 bits: q = clamp(round(x / s), -127, 127) with the division one correctly rounded f32
+// operation, ties to even; NaN is held as 0, everything as 0 where the scale is 0.
+//
+// The division by r = RN(1 / s): q0 = x r is within 2 units in the last place, each step q + (x - q s) r (the
+// remainder exact) squares that, and after two the quotient is the correctly rounded
+// one (Markstein's theorem; s of an all-ones significand excepted).  5 operations instead of about
+// 20: 16384 x 4096 f16 took 52-62 us of VALU time with divisions.  Rows with an infinity or a NaN, and scales
+// whose remainders might be subnormal, are divided outright.  A finite |x / s| is at most 127 (1 + 2^-23), so that adding
+// 1.5 2^23 rounds it to an integer whose byte is the lowest of the sum.
+struct RowQuantiser {
+    float s, r;
+    bool fast;
+    __device__ __forceinline__ RowQuantiser(float scale, bool plain) : s(scale) {
+        const uint32_t b = __builtin_bit_cast(uint32_t, s);
+        fast = plain && s > 1e-25f && s < 1e25f && (b & 0x7FFFFF) != 0x7FFFFF;
+        r = fast ? 1.0f / s : 0.f;
+    }
+    __device__ __forceinline__ int2v operator()(const float (&v)[8]) const {
+        int2v w = {};
+        if (fast) {
+            uint32_t u[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                float q = v[e] * r;
+                q = fmaf(fmaf(-q, s, v[e]), r, q);
+                q = fmaf(fmaf(-q, s, v[e]), r, q);
+                u[e] = __builtin_bit_cast(uint32_t, q + 12582912.f);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t a = __builtin_amdgcn_perm(u[4 * h + 1], u[4 * h], 0x0c0c0400u);
+                const uint32_t b = __builtin_amdgcn_perm(u[4 * h + 3], u[4 * h + 2], 0x04000c0cu);
+                w[h] = (int)(a | b);
+            }
+            return w;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float q = s != 0.f ? rintf(v[e] / s) : 0.f;
+            q = q != q ? 0.f : fminf(fmaxf(q, -127.f), 127.f);
+            w[e >> 2] |= (int)((unsigned)((int)q & 0xFF) << (8 * (e & 3)));
+        }
+        return w;
+    }
+};
 __device__ __forceinline__ void store_bytes8(int8_t* row, int2v w, int i, int d) {
     if (i + 8 <= d) {
         *(int2u*)(row + i) = w;
