@@ -25,7 +25,7 @@ template <int T> __device__ __forceinline__ Moments row_sum(Moments m, double (&
     m.s = wave_sum_f64(m.s);
     m.t = wave_sum_f64(m.t);
     if constexpr (T > 64) {
-        const int w = threadIdx.x >> 6;
+        const int w = threadIdx.x % T >> 6;
         __syncthreads();                     // the last sums have been read
         if ((threadIdx.x & 63) == 0) {
             part[2 * w] = m.s;
@@ -42,22 +42,50 @@ template <int T> __device__ __forceinline__ Moments row_sum(Moments m, double (&
     return m;
 }
 
+// A lane's part of a vector of d, asked for before it is needed.
+template <int T, int NV> struct Part {
+    float v[NV][8];
+    bool there = false;
+    template <typename S> __device__ __forceinline__ void ask(const S* p, int t, int d) {
+        there = p != nullptr;
+        if (there)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) load_row8(v[k], p, 8 * (t + k * T), d);
+    }
+};
+
 // v becomes its norm: LayerNorm or RMS, times w, plus b (either may be missing).
 template <int T, int NV>
-__device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const float* w, const float* b, float eps, float first, int t,
+__device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const Part<T, NV>& w, const Part<T, NV>& b, float eps, float first, int t,
                                           int d, double inv_d, double (&part)[2 * (T / 64)]) {
     const bool layer = kind == NORM_LAYER;
-    const double c = layer ? (double)first : 0.0;
     Moments m = {0, 0};
+    if (layer) {
+        const double c = (double)first;
 #pragma unroll
-    for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            if (8 * (t + k * T) + 8 > d)     // what lies past the row's end adds nothing
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = 8 * (t + k * T) + e;
-            const double x = i < d ? (double)v[k][e] - c : 0.0;
-            m.s += x;
-            m.t = fma(x, x, m.t);
+                for (int e = 0; e < 8; ++e)
+                    if (8 * (t + k * T) + e >= d) v[k][e] = first;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const double x = (double)v[k][e] - c;
+                m.s += x;
+                m.t = fma(x, x, m.t);
+            }
         }
+    } else {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            if (8 * (t + k * T) + 8 > d)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (8 * (t + k * T) + e >= d) v[k][e] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) m.t = fma((double)v[k][e], (double)v[k][e], m.t);
+        }
+    }
     m = row_sum<T>(m, part);
     const double mu = layer ? m.s * inv_d : 0.0;
     const double var = m.t * inv_d - mu * mu + (double)eps;
@@ -65,112 +93,139 @@ __device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const flo
     double r = __builtin_amdgcn_rsq(var);
     r = r * (1.5 - 0.5 * var * r * r);
     const float inv = (float)r;
-    const double mean = c + mu;
-    const float hi = (float)mean, lo = (float)(mean - hi);     // v - mean exactly where v is near it
+    if (layer) {
+        const double mean = (double)first + mu;
+        const float hi = (float)mean, lo = (float)(mean - hi);     // v - mean exactly where v is near it
 #pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int i = 8 * (t + k * T);
-        if (i >= d) continue;
-        float ww[8], bb[8];
-        if (w) load_row8(ww, w, i, d);
-        if (b) load_row8(bb, b, i, d);
+        for (int k = 0; k < NV; ++k)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float x = layer ? (v[k][e] - hi) - lo : v[k][e];
-            x *= inv;
-            if (w) x *= ww[e];
-            if (b) x += bb[e];
-            v[k][e] = x;
-        }
+            for (int e = 0; e < 8; ++e) v[k][e] = (v[k][e] - hi) - lo;
     }
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[k][e] *= inv;
+    if (w.there)
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] *= w.v[k][e];
+    if (b.there)
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[k][e] += b.v[k][e];
 }
 
-// One row to T lanes: a wave up to 2048 channels, a workgroup beyond.
-template <typename ET, typename XT, bool I8, int T, int NV>
+// One row to T lanes: a wave up to 1024 channels, a workgroup beyond.
+template <typename ET, typename XT, bool I8, int T, int NV, bool EARLY>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(BlockNormParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1;
     __shared__ double part[kRows][2 * (T / 64)];
-    __shared__ float top_part[T / 64];
+    __shared__ float top_part[kRows][T / 64], x0[kRows];
     const int t = threadIdx.x % T, d = p.d;
     const int mine = kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0;
-    const int64_t r = (int64_t)blockIdx.x * kRows + mine;
+    const int r = blockIdx.x * kRows + mine;
     if (r >= p.rows) return;                 // whole waves; T > 64 has one row to a workgroup
     double (&ps)[2 * (T / 64)] = part[mine];
 
-    const XT* xr = (const XT*)p.x + r * p.x_row;
-    const ET* yr = (const ET*)p.y + r * p.y_row;
-    float x[NV][8], y[NV][8];
-#pragma unroll
-    for (int k = 0; k < NV; ++k) {
-        const int i = 8 * (t + k * T);
-        if (p.x) load_row8(x[k], xr, i, d);
-        if (p.y) load_row8(y[k], yr, i, d);
+    // EARLY: everything that the row needs is asked for at once, which is what a few rows wait for (2000 x 1024: 9.0 us,
+    // 9.8 with each vector read where it is used); many rows need the registers for more rows at a time (8192 x 4090 f32
+    // 136 us, early 166)
+    const XT* xr = p.x ? (const XT*)p.x + r * p.x_row : nullptr;
+    const ET* yr = p.y ? (const ET*)p.y + r * p.y_row : nullptr;
+    const ET* gr = p.gate ? (const ET*)p.gate + udiv_small(r, p.rows_per_gate) * p.gate_row : nullptr;
+    Part<T, NV> x, y, gate, post_w, post_b, pre_w, pre_b;
+    y.ask(yr, t, d);
+    const float first_y = p.post == NORM_LAYER ? (float)yr[0] : 0.f;
+    x.ask(xr, t, d);
+    if (EARLY) {
+        gate.ask(gr, t, d);
+        post_w.ask(p.post_w, t, d);
+        post_b.ask(p.post_b, t, d);
+        pre_w.ask(p.pre_w, t, d);
+        pre_b.ask(p.pre_b, t, d);
     }
-    if (p.y) {
-        if (p.post != NORM_NONE) normalise<T, NV>(y, p.post, p.post_w, p.post_b, p.post_eps, (float)yr[0], t, d, p.inv_d, ps);
-        const ET* gr = (const ET*)p.gate + (p.gate ? (r / p.rows_per_gate) * p.gate_row : 0);
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            const int i = 8 * (t + k * T);
-            if (p.gate) {
-                float g[8];
-                load_row8(g, gr, i, d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (p.sigmoid) g[e] = 1.0f / (1.0f + expf(-g[e]));
-                    y[k][e] *= g[e];
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[k][e] = p.x ? x[k][e] + p.alpha * y[k][e] : p.alpha * y[k][e];
+    if (y.there) {
+        if (!EARLY) {
+            post_w.ask(p.post_w, t, d);
+            post_b.ask(p.post_b, t, d);
         }
+        if (p.post != NORM_NONE) normalise<T, NV>(y.v, p.post, post_w, post_b, p.post_eps, first_y, t, d, p.inv_d, ps);
+        if (!EARLY) gate.ask(gr, t, d);
+        if (gate.there) {
+            if (p.sigmoid)
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) gate.v[k][e] = 1.0f / (1.0f + expf(-gate.v[k][e]));
+#pragma unroll
+            for (int k = 0; k < NV; ++k)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y.v[k][e] *= gate.v[k][e];
+        }
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x.v[k][e] = x.there ? x.v[k][e] + p.alpha * y.v[k][e] : p.alpha * y.v[k][e];
     }
     // the first element of x', for every lane
     float first = 0.f;
     if (p.pre == NORM_LAYER) {
-        if constexpr (T == 64) first = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x[0][0]), 0));
+        if constexpr (T == 64) first = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x.v[0][0]), 0));
         else {
-            __shared__ float x0;
-            if (t == 0) x0 = x[0][0];
+            if (t == 0) x0[mine] = x.v[0][0];
             __syncthreads();
-            first = x0;
+            first = x0[mine];
         }
     }
     if (p.x_out) {
         XT* o = (XT*)p.x_out + r * p.x_out_row;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) store_row8(o, x[k], 8 * (t + k * T), d);
+        for (int k = 0; k < NV; ++k) store_row8(o, x.v[k], 8 * (t + k * T), d);
     }
     if (!p.h) return;
-    if (p.pre != NORM_NONE) normalise<T, NV>(x, p.pre, p.pre_w, p.pre_b, p.pre_eps, first, t, d, p.inv_d, ps);
+    if (!EARLY) {
+        pre_w.ask(p.pre_w, t, d);
+        pre_b.ask(p.pre_b, t, d);
+    }
+    if (p.pre != NORM_NONE) normalise<T, NV>(x.v, p.pre, pre_w, pre_b, p.pre_eps, first, t, d, p.inv_d, ps);
     if constexpr (I8) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                if (8 * (t + k * T) + e >= d) x[k][e] = 0.f;    // weights and biases are not read there
-        const RowTop top = row_top<T, NV>(x, top_part);
+                if (8 * (t + k * T) + e >= d) x.v[k][e] = 0.f;    // weights and biases are not read there
+        const RowTop top = row_top<T, NV>(x.v, top_part[mine]);
         const float s = top.top / 127.0f;
         if (t == 0) p.h_scale[r] = s;
         const RowQuantiser held(s, top.plain);
         int8_t* o = (int8_t*)p.h + r * p.h_row;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) store_bytes8(o, held(x[k]), 8 * (t + k * T), d);
+        for (int k = 0; k < NV; ++k) store_bytes8(o, held(x.v[k]), 8 * (t + k * T), d);
     } else {
         ET* o = (ET*)p.h + r * p.h_row;
 #pragma unroll
-        for (int k = 0; k < NV; ++k) store_row8(o, x[k], 8 * (t + k * T), d);
+        for (int k = 0; k < NV; ++k) store_row8(o, x.v[k], 8 * (t + k * T), d);
     }
 }
 
+template <typename ET, typename XT, bool I8, int T, int NV, bool EARLY> void launch_rows(const BlockNormParams& p, hipStream_t s) {
+    constexpr int kRows = T < 256 ? 256 / T : 1;
+    launch(block_norm_kernel<ET, XT, I8, T, NV, EARLY>, dim3((unsigned)((p.rows + kRows - 1) / kRows)), dim3(T * kRows), 0, s, p);
+}
+// Early up to 16 waves a CU, as many as the registers then hold.
+template <typename ET, typename XT, bool I8, int T, int NV> void launch_width(const BlockNormParams& p, hipStream_t s) {
+    if (p.rows * (T / 64) <= 4096 && !(T == 1024 && NV == 2)) launch_rows<ET, XT, I8, T, NV, T != 1024 || NV != 2>(p, s);
+    else launch_rows<ET, XT, I8, T, NV, false>(p, s);
+}
 template <typename ET, typename XT, bool I8> void launch_typed(const BlockNormParams& p, hipStream_t s) {
-    const unsigned rows = (unsigned)p.rows;
-    if (p.d <= 512) launch(block_norm_kernel<ET, XT, I8, 64, 1>, dim3((rows + 3) / 4), dim3(256), 0, s, p);
-    else if (p.d <= 1024) launch(block_norm_kernel<ET, XT, I8, 64, 2>, dim3((rows + 3) / 4), dim3(256), 0, s, p);
-    else if (p.d <= 2048) launch(block_norm_kernel<ET, XT, I8, 256, 1>, dim3(rows), dim3(256), 0, s, p);
-    else if (p.d <= 4096) launch(block_norm_kernel<ET, XT, I8, 256, 2>, dim3(rows), dim3(256), 0, s, p);
-    else if (p.d <= 8192) launch(block_norm_kernel<ET, XT, I8, 1024, 1>, dim3(rows), dim3(1024), 0, s, p);
-    else launch(block_norm_kernel<ET, XT, I8, 1024, 2>, dim3(rows), dim3(1024), 0, s, p);
+    if (p.d <= 512) launch_width<ET, XT, I8, 64, 1>(p, s);
+    else if (p.d <= 1024) launch_width<ET, XT, I8, 128, 1>(p, s);
+    else if (p.d <= 2048) launch_width<ET, XT, I8, 256, 1>(p, s);
+    else if (p.d <= 4096) launch_width<ET, XT, I8, 256, 2>(p, s);
+    else if (p.d <= 8192) launch_width<ET, XT, I8, 1024, 1>(p, s);
+    else launch_width<ET, XT, I8, 1024, 2>(p, s);
 }
 
 }  // namespace

@@ -54,6 +54,14 @@ template <typename T> __device__ __forceinline__ void store_row8(T* row, const f
         if (i + e < d) row[i + e] = (T)v[e];
 }
 
+// A barrier for what a workgroup shares in LDS: it waits for no load that is on its way to a register, as __syncthreads does.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 __device__ __forceinline__ double readlane_f64(double v, int lane) {
     const long long b = __builtin_bit_cast(long long, v);
     const unsigned lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
@@ -121,7 +129,7 @@ template <int T, int NV> __device__ __forceinline__ RowTop row_top(const float (
     }
     o.top = wave_max_full(o.top);
     if constexpr (T > 64) {
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = o.plain ? o.top : -o.top;
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x % T >> 6] = o.plain ? o.top : -o.top;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < T / 64; ++i) {
