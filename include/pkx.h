@@ -526,13 +526,13 @@ int pkx_quantize_rows(int type, const void* x, int64_t x_row, int64_t n_rows, in
 
 /* Weights of pkx_linear_i8: int8 w [n_out][n_in] (w_row bytes between rows) laid out once into `packed`
  * (dev, pkx_i8_weight_bytes of it, 16-byte aligned).  n_in up to PKX_I8_MAX_DEPTH, where sums in 32 bits are exact. */
-#define PKX_I8_MAX_DEPTH 131072
+#define PKX_I8_MAX_DEPTH 131071
 int pkx_i8_weight_bytes(int n_out, int n_in, size_t* bytes);
 int pkx_i8_weight_pack(const int8_t* w, int64_t w_row, int n_out, int n_in, void* packed, void* stream);
 
 /* y[m][n] = add[m][n] + alpha * act(x_scale[m] * w_scale[n] * sum over k of x[m][k] w[n][k] + bias[n]), the sums exact.
- * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22, and what
- * they hold past n_in does not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows
+ * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22; every
+ * row can be read to its next multiple of 16, and what it holds past n_in does not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows
  * does (x_scale NULL).  y and add are f32 or f16, and add may be y; y overlaps nothing else.  Strides in elements.
  * n_rows and n_out below 2^22. */
 enum { PKX_TYPE_I8 = 24 };               /* ggml's number of its 8-bit integers */
@@ -592,7 +592,7 @@ int pkx_rotary_frequencies(double base, int rot, double factor, double context, 
  * out): the histories lie as a cache's tokens do, and beams share them through the same tables.  Tokens outside the vocabulary do not count.  bias and
  * mask are sets of rows that rows of logits name: row bias_index[r] of n_bias (NULL: r), none where that is out of range,
  * and likewise the mask, whose word v / 32 has the bit v % 32.  out may be logits with the same rows; other overlaps are refused.
- * vocab up to 2^22; strides in elements. */
+ * vocab up to 2^22, capacity up to 2^30; strides in elements. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of logits and out */
     int n_rows, vocab;

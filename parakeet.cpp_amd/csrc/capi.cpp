@@ -377,6 +377,10 @@ int64_t i8_row(const pkx_linear_i8_args* a) { return ((int64_t)a->n_in + 15) / 1
 size_t i8_workspace(const pkx_linear_i8_args* a) {
     return a->x_type == PKX_TYPE_I8 || a->n_rows == 0 || a->n_out == 0 || pkx::linear_i8_fused(a->n_rows, a->n_in) ? 0 : (size_t)a->n_rows * (i8_row(a) + 4);
 }
+// Every element where it was: a stride counts where its dimension has more than one.
+bool in_place(const pkx::RotaryPart& p, int64_t rows, int64_t toks) {
+    return p.src == p.dst && (rows <= 1 || p.s_row == p.d_row) && (toks <= 1 || p.s_tok == p.d_tok) && (p.heads <= 1 || p.s_head == p.d_head);
+}
 pkx::QuantizeRowsParams quantize_rows_params(int type, const void* x, int64_t x_row, int64_t n_rows, int n) {
     pkx::QuantizeRowsParams p;
     p.f32 = is_f32(type, "quantise rows: type must be PKX_TYPE_F32 or PKX_TYPE_F16");
@@ -1165,11 +1169,11 @@ int pkx_rotary(const pkx_rotary_args* a, void* s) {
             dst.emplace_back(x.dst, (int64_t)a->d_head * e, std::initializer_list<std::pair<int64_t, int64_t>>{{x.dst_row * e, R}, {x.dst_tok * e, n}, {x.dst_head * e, x.n_heads}});
             need(src.back().bytes() < 0x1p62 && dst.back().bytes() < 0x1p62, "rotary: strides past the address space");
             pkx::RotaryPart& o = p.part[p.parts++];
-            o = pkx::RotaryPart{x.src, x.src_row, x.src_tok, x.src_head, x.dst, x.dst_row, x.dst_tok, x.dst_head, x.n_heads};
+            o = pkx::RotaryPart{x.src, x.src_row, x.src_tok, x.src_head, x.dst, x.dst_row, x.dst_tok, x.dst_head, x.n_heads, 1};
         }
         for (size_t i = 0; i < dst.size(); ++i) {
             for (size_t j = 0; j < dst.size(); ++j) {
-                need(apart(dst[i], src[j]) || (i == j && same(dst[i], src[i])), "rotary: a dst overlaps a src without being its own");
+                need(apart(dst[i], src[j]) || (i == j && in_place(p.part[i], R, n)), "rotary: a dst overlaps a src without being its own");
                 need(i == j || apart(dst[i], dst[j]), "rotary: two dsts overlap");
             }
             need(a->rot == 0 || apart(dst[i], Span(a->freq, 4 * (int64_t)a->rot, {})), "rotary: a dst overlaps freq");
@@ -1221,7 +1225,7 @@ int pkx_logit_rules(const pkx_logit_rules_args* a, void* s) {
         const Span in = rows_of(a->logits, V, e, a->logits_row, R), out = rows_of(a->out, V, e, a->out_row, R);
         need(same(in, out) || apart(in, out), "logit rules: out overlaps logits without being them");
         if (a->tokens) {
-            need(a->n_slots >= 1 && a->capacity >= 0, "logit rules: no slots, or a negative capacity");
+            need(a->n_slots >= 1 && a->capacity >= 0 && a->capacity <= (1 << 30), "logit rules: no slots, or a capacity that is negative or above 2^30");
             need((double)a->n_slots * a->capacity < 0x1p60 && a->table_row >= 0 && (double)a->table_row * R < 0x1p60, "logit rules: tokens or table past the address space");
             need(a->len, "logit rules: null len");
             need(a->slot || a->table || R <= a->n_slots, "logit rules: more rows than slots");

@@ -1,7 +1,7 @@
 // Products of 8-bit tokens and 8-bit weights, a scale for each token and each
 // output channel:
 //   y[m][n] = add[m][n] + alpha act(xs[m] ws[n] sum_k x[m][k] w[n][k] + bias[n]).
-// Sums are exact in i32 (K up to 2^17: 127 * 127 * 2^17 < 2^31); everything after them is f32.
+// Sums are exact in i32 (128 * 128 * K < 2^31 for K below 2^17); everything after them is f32.
 //
 // The weights are the A operand of the matrix instructions and the tokens the B
 // operand, so that a lane ends with one token and consecutive channels.  Their
@@ -80,8 +80,11 @@ __global__ __launch_bounds__(256) void i8_pack_kernel(const int8_t* w, int64_t w
     const int nb = (int)(block / kblocks), kb = (int)(block - (int64_t)nb * kblocks);
     const int n = nb * kI8ColBlock + tail_col(slot), k0 = kb * kI8DepthBlock + 16 * group;
     int4v v = {};
-    for (int e = 0; e < 16; ++e)
-        if (n < N && k0 + e < K) v[e >> 2] |= (int)((unsigned)(w[n * w_row + k0 + e] & 0xFF) << (8 * (e & 3)));
+    typedef int4v int4u __attribute__((aligned(1)));
+    if (n < N && k0 + 16 <= K) v = *(const int4u*)(w + n * w_row + k0);
+    else
+        for (int e = 0; e < 16; ++e)
+            if (n < N && k0 + e < K) v[e >> 2] |= (int)((unsigned)(w[n * w_row + k0 + e] & 0xFF) << (8 * (e & 3)));
     *(int4v*)(out + at * 16) = v;
 }
 
@@ -96,11 +99,12 @@ template <typename YT> __device__ __forceinline__ float silu_of(float v) {
     const float t = v * -1.4426950408889634f;
     const float r = fmaf(v, -1.4426950408889634f, -t) + v * -1.925963033500e-8f;   // log2 e less its f32
     float e = __builtin_amdgcn_exp2f(t);
-    e = t < 127.f ? fmaf(e, r * 0.69314718056f, e) : e;
-    const float d = 1.0f + e;
+    e = fabsf(t) < 127.f ? fmaf(e, r * 0.69314718056f, e) : e;     // else 0, or nothing beside 1, or past all that f32 holds
+    // (the hardware's reciprocal is 0 where it would be subnormal: large sums by 2^-64, and v with them)
+    const float by = e > 0x1p60f ? 0x1p-64f : 1.0f, d = (1.0f + e) * by;
     float q = __builtin_amdgcn_rcpf(d);
-    q = d < 1e38f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
-    return v * q;
+    q = d <= 3.402823466e38f ? fmaf(fmaf(-d, q, 1.0f), q, q) : q;
+    return v * by * q;
 }
 
 // What a lane needs of CNT channels from n0 < N on, for any number of tokens.
@@ -340,7 +344,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
     // past the last slab nothing is read: a resource of no bytes, so that every step issues the same loads
     const __amdgpu_buffer_rsrc_t none = make_rsrc(p.w, 0);
     auto fetch = [&](int k, int stage, int i) {      // a wave's i-th 1 KB of slab k
-        lds_dma16(k < slabs ? rx : none, slab + stage * STAGE + (wid * ROWS + i) * 1024, xo[i], k * 128);
+        // the whole offset in the lane's part: only that is held against the end of the tokens
+        lds_dma16(k < slabs ? rx : none, slab + stage * STAGE + (wid * ROWS + i) * 1024, xo[i] + k * 128, 0);
     };
     auto fetch_w = [&](int k, int q, int4v (&f)[4][TN]) {
         const __amdgpu_buffer_rsrc_t r = k < slabs ? rw : none;

@@ -35,85 +35,119 @@ __device__ __forceinline__ float2v cos_sin_turns(double x) {
     return float2v{(k == 1 || k == 2) ? -a : a, k >= 2 ? -b : b};
 }
 
-// One workgroup per TOK tokens of a row: their angles once into LDS, then all heads.
-// An item is up to eight pairs of a head, or eight of its other dimensions.
-template <typename ET, int TOK> __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int groups) {
-    extern __shared__ float2v turn[];        // [TOK][rot / 2]
-    const int r = udiv_small(blockIdx.x, groups), i0 = (blockIdx.x - r * groups) * TOK;
+// One workgroup per `tok` tokens of a row and part (blockIdx.y): their angles once into LDS, then the part's heads, IT items a
+// thread at a time.  An item is 8 elements of a head (4 pairs of neighbours, or elements past rot), or 8 pairs of halves; the
+// first ones are asked for before the angles are formed.  WHOLE: every item is, so nothing looks for an end.
+template <typename ET, bool INTER, bool WHOLE, int IT>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
+    extern __shared__ float2v turn[];        // [tok][rot / 2]
+    const RotaryPart q = p.part[blockIdx.y];
+    const int r = udiv_small(blockIdx.x, most), i0 = (blockIdx.x - r * most) * q.tok;
     int n = p.count ? p.count[r] : p.n;
     n = n > p.n ? p.n : n;
     if (i0 >= n) return;
-    const int toks = n - i0 < TOK ? n - i0 : TOK, pairs = p.rot / 2;
+    const int toks = n - i0 < q.tok ? n - i0 : q.tok, pairs = p.rot / 2, rest = p.dk - p.rot;
+    const int turned = INTER ? (p.rot + 7) / 8 : (pairs + 7) / 8, items = turned + (rest + 7) / 8, per = q.heads * items;
+    const int all = toks * per;
+    const ET* from = (const ET*)q.src + r * q.s_row + i0 * q.s_tok;
+    ET* to = (ET*)q.dst + r * q.d_row + i0 * q.d_tok;
+
+    auto get = [](float (&v)[8], const ET* row, int i, int d) {
+        if constexpr (WHOLE) load8u(v, row + i);
+        else load_row8(v, row, i, d);
+    };
+    auto put = [](ET* row, const float (&v)[8], int i, int d) {
+        if constexpr (WHOLE) store8u(row + i, v);
+        else store_row8(row, v, i, d);
+    };
+    // at: an item's first pair, or -1 - its first element past rot; whole elements and pairs beyond an item's end are zeros
+    float a[IT][8], b[IT][8] = {};
+    const ET* src[IT];
+    ET* dst[IT];
+    int at[IT], tok[IT];
+    auto load = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < IT; ++u) {
+            const int j = j0 + 256 * u < all ? j0 + 256 * u : 0;
+            tok[u] = udiv_small(j, per);
+            const int hi = j - tok[u] * per, h = udiv_small(hi, items), it = hi - h * items;
+            src[u] = from + tok[u] * q.s_tok + h * q.s_head;
+            dst[u] = to + tok[u] * q.d_tok + h * q.d_head;
+            at[u] = it >= turned ? -1 - 8 * (it - turned) : INTER ? 4 * it : 8 * it;
+            if (j0 + 256 * u >= all) dst[u] = nullptr;
+            const bool other = at[u] < 0;
+            if (other && src[u] == dst[u]) dst[u] = nullptr;
+            get(a[u], src[u] + (other ? p.rot : 0), other ? -1 - at[u] : INTER ? 2 * at[u] : at[u], other ? rest : INTER ? p.rot : pairs);
+            if (!INTER && !other) get(b[u], src[u] + pairs, at[u], pairs);
+        }
+    };
+    auto turn_and_store = [&]() {
+#pragma unroll
+        for (int u = 0; u < IT; ++u) {
+            if (!dst[u]) continue;
+            const bool other = at[u] < 0;
+            const float2v* cs = turn + tok[u] * pairs + (other ? 0 : at[u]);
+            float o[8], o2[8];
+#pragma unroll
+            for (int e = 0; e < (INTER ? 4 : 8); ++e) {
+                const float2v c = (WHOLE ? !other : !other && at[u] + e < pairs) ? cs[e] : float2v{0.f, 0.f};
+                const float v = INTER ? a[u][2 * (e & 3)] : a[u][e], w = INTER ? a[u][2 * (e & 3) + 1] : b[u][e];
+                const float x = v * c[0] - w * c[1], y = w * c[0] + v * c[1];
+                if (INTER) {
+                    o[2 * (e & 3)] = other ? v : x;
+                    o[2 * (e & 3) + 1] = other ? w : y;
+                } else {
+                    o[e] = other ? v : x;
+                    o2[e] = y;
+                }
+            }
+            put(dst[u] + (other ? p.rot : 0), o, other ? -1 - at[u] : INTER ? 2 * at[u] : at[u], other ? rest : INTER ? p.rot : pairs);
+            if (!INTER && !other) put(dst[u] + pairs, o2, at[u], pairs);
+        }
+    };
+
+    load(threadIdx.x);
     const int64_t first = p.start ? p.start[r] : 0;
     for (int j = threadIdx.x; j < toks * pairs; j += 256) {
         const int i = udiv_small(j, pairs), f = j - i * pairs;
-        const int64_t at = p.pos ? p.pos[r * p.pos_row + i0 + i] : first + i0 + i;
-        const float2v cs = cos_sin_turns((double)at * p.freq[f] * 0.159154943091895335769);
+        const int64_t where = p.pos ? p.pos[r * p.pos_row + i0 + i] : first + i0 + i;
+        const float2v cs = cos_sin_turns((double)where * p.freq[f] * 0.159154943091895335769);
         turn[j] = float2v{cs[0] * p.mult, cs[1] * p.mult};
     }
     __syncthreads();
-    const int turned = (pairs + 7) / 8, rest = p.dk - p.rot, items = turned + (rest + 7) / 8;
-    for (int z = 0; z < p.parts; ++z) {
-        const RotaryPart& a = p.part[z];
-        const bool copy = a.src != a.dst;
-        const int per = a.heads * items, all = toks * per;
-        for (int j = threadIdx.x; j < all; j += 256) {
-            const int i = udiv_small(j, per), hi = j - i * per, h = udiv_small(hi, items), it = hi - h * items;
-            const ET* src = (const ET*)a.src + r * a.s_row + (int64_t)(i0 + i) * a.s_tok + h * a.s_head;
-            ET* dst = (ET*)a.dst + r * a.d_row + (int64_t)(i0 + i) * a.d_tok + h * a.d_head;
-            if (it >= turned) {
-                if (!copy) continue;
-                float v[8];
-                load_row8(v, src + p.rot, 8 * (it - turned), rest);
-                store_row8(dst + p.rot, v, 8 * (it - turned), rest);
-                continue;
-            }
-            const int f = 8 * it;
-            float u[8], v[8], x[8], y[8];
-            if (p.interleaved) {             // pairs f .. f + 8: elements 2 f .. 2 f + 16
-                load_row8(u, src, 2 * f, p.rot);
-                load_row8(v, src, 2 * f + 8, p.rot);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = u[2 * e]; y[e] = u[2 * e + 1];
-                    x[4 + e] = v[2 * e]; y[4 + e] = v[2 * e + 1];
-                }
-            } else {
-                load_row8(x, src, f, pairs);
-                load_row8(y, src + pairs, f, pairs);
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float2v cs = f + e < pairs ? turn[i * pairs + f + e] : float2v{0.f, 0.f};
-                const float s = x[e] * cs[0] - y[e] * cs[1], t = y[e] * cs[0] + x[e] * cs[1];
-                x[e] = s;
-                y[e] = t;
-            }
-            if (p.interleaved) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    u[2 * e] = x[e]; u[2 * e + 1] = y[e];
-                    v[2 * e] = x[4 + e]; v[2 * e + 1] = y[4 + e];
-                }
-                store_row8(dst, u, 2 * f, p.rot);
-                store_row8(dst, v, 2 * f + 8, p.rot);
-            } else {
-                store_row8(dst, x, f, pairs);
-                store_row8(dst + pairs, y, f, pairs);
-            }
-        }
+    for (int j = threadIdx.x;;) {
+        turn_and_store();
+        j += 256 * IT;
+        if (j >= all) break;
+        load(j);
     }
+}
+
+template <typename ET, bool INTER, bool WHOLE, int IT> void launch_typed(RotaryParams p, hipStream_t s) {
+    const int pairs = p.rot / 2, items = cdiv(INTER ? p.rot : pairs, 8) + cdiv(p.dk - p.rot, 8);
+    int most = 1, lds = 0;
+    for (int z = 0; z < p.parts; ++z) {      // as many tokens as give every thread its IT items, within 32 KB of angles
+        int tok = 256 * IT / (p.part[z].heads * items);
+        if (tok * pairs > 4096) tok = 4096 / pairs;
+        tok = tok < 1 ? 1 : tok > p.n ? p.n : tok;
+        p.part[z].tok = tok;
+        most = cdiv(p.n, tok) > most ? cdiv(p.n, tok) : most;
+        lds = tok * pairs * 8 > lds ? tok * pairs * 8 : lds;
+    }
+    require((double)p.R * most < (double)(1 << 22), "rotary: too many tokens for one call");
+    launch(rotary_kernel<ET, INTER, WHOLE, IT>, dim3(p.R * most, p.parts), dim3(256), lds, s, p, most);
+}
+template <typename ET> void launch_pairs(const RotaryParams& p, hipStream_t s) {
+    const bool rest = (p.dk - p.rot) % 8 == 0;
+    if (p.interleaved) rest && p.rot % 8 == 0 ? launch_typed<ET, true, true, 4>(p, s) : launch_typed<ET, true, false, 1>(p, s);
+    else rest && p.rot % 16 == 0 ? launch_typed<ET, false, true, 2>(p, s) : launch_typed<ET, false, false, 1>(p, s);
 }
 
 }  // namespace
 
 void launch_rotary(const RotaryParams& p, hipStream_t s) {
     if (p.R == 0 || p.n == 0 || p.parts == 0) return;
-    constexpr int kTok = 4;
-    const int groups = p.n == 1 ? 1 : cdiv(p.n, kTok);
-    require((double)p.R * groups < (double)(1 << 22), "rotary: too many tokens for one call");
-    if (p.n == 1) launch(p.f32 ? rotary_kernel<float, 1> : rotary_kernel<f16, 1>, dim3(p.R), dim3(256), p.rot / 2 * 8, s, p, 1);
-    else launch(p.f32 ? rotary_kernel<float, kTok> : rotary_kernel<f16, kTok>, dim3(p.R * groups), dim3(256), kTok * p.rot / 2 * 8, s, p, groups);
+    p.f32 ? launch_pairs<float>(p, s) : launch_pairs<f16>(p, s);
 }
 
 }  // namespace pkx

@@ -68,7 +68,7 @@ def quantised(x):
     return np.where(s[:, None] == 0, 0, q).astype(np.int8), s
 
 
-def linear_i8(q, s, w, ws, bias, act, alpha, add):
+def linear_i8(q, s, w, ws, bias, act, alpha, add, f16=False):
     """-> (y, its f32 error) of ints q [M][K], w [N][K]; the sums are whole numbers."""
     acc = (q.astype(np.float64) @ w.astype(np.float64).T)
     v = acc * s.astype(np.float64)[:, None] * ws.astype(np.float64)[None]
@@ -78,8 +78,10 @@ def linear_i8(q, s, w, ws, bias, act, alpha, add):
         err = err + U * np.abs(v)
     if act == "silu":
         y = v / (1 + np.exp(-v))
-        # |d silu / dv| <= 1.1; exp to 2^-23 relative, weighted by its share of the sum, a sum and a division
-        err, v = 1.1 * err + 5 * U * np.abs(y), y
+        # |d silu / dv| <= 1.1; then e^-v to 3 U (the hardware's exponential to a unit in the last place, 2 U, and a product), whose
+        # share of 1 + e^-v is at most 1, that sum (U), its reciprocal (U after a Newton step) and the product (U).  An f16 result takes
+        # the exponential of v log2 e rounded once (|v| U) and a reciprocal to a unit in the last place (2 U).
+        err, v = 1.1 * err + (6 + (1 + np.abs(v) if f16 else 0)) * U * np.abs(y), y
     v, err = alpha * v, abs(alpha) * err + U * np.abs(alpha * v)
     if add is not None:
         v = v + add.astype(np.float64)

@@ -94,8 +94,8 @@ def test_quantise_and_weight_refusals():
         q(type=8); q(M=-1); q(M=1 << 22); q(n=-1); q(x=None); q(x=MB + 1); q(xr=-64); q(qr=63); q(o=None); q(s=None); q(s=3 * MB + 2); q(o=MB + 100); q(s=MB)
         q(s=2 * MB + 64)
         n = C.c_size_t()
-        said(L.pkx_i8_weight_bytes(8, 0, C.byref(n))); said(L.pkx_i8_weight_bytes(8, 131073, C.byref(n))); said(L.pkx_i8_weight_bytes(-1, 8, C.byref(n)))
-        said(L.pkx_i8_weight_bytes(1 << 22, 8, C.byref(n))); said(L.pkx_i8_weight_bytes(4000000, 131072, C.byref(n))); said(L.pkx_i8_weight_bytes(8, 8, None))
+        said(L.pkx_i8_weight_bytes(8, 0, C.byref(n))); said(L.pkx_i8_weight_bytes(8, 131072, C.byref(n))); said(L.pkx_i8_weight_bytes(-1, 8, C.byref(n)))
+        said(L.pkx_i8_weight_bytes(1 << 22, 8, C.byref(n))); said(L.pkx_i8_weight_bytes(4000000, 131071, C.byref(n))); said(L.pkx_i8_weight_bytes(8, 8, None))
         w = lambda w=MB, r=64, N=8, K=64, p=2 * MB: said(L.pkx_i8_weight_pack(w, r, N, K, p, None))
         w(w=None); w(r=-1); w(p=None); w(p=2 * MB + 8); w(p=MB + 64)
         q(M=0, x=None, o=None, s=None); w(N=0, w=None)
@@ -111,7 +111,7 @@ def test_quantise_and_weight_refusals():
 def test_linear_refusals():
     out = _run("""
         nan = float("nan")
-        cases = [dict(x_type=8), dict(type=24), dict(n_rows=-1), dict(n_in=0), dict(n_in=131073), dict(n_out=1 << 22), dict(n_rows=1 << 20, n_out=1 << 20),
+        cases = [dict(x_type=8), dict(type=24), dict(n_rows=-1), dict(n_in=0), dict(n_in=131072), dict(n_out=1 << 22), dict(n_rows=1 << 20, n_out=1 << 20),
                  dict(act=2), dict(alpha=nan), dict(w=None), dict(w=MB + 8), dict(w_scale=None), dict(bias=MB + 2), dict(y=None), dict(y=5 * MB + 1),
                  dict(y_row=63), dict(add=6 * MB + 1, add_row=64), dict(add=5 * MB + 64, add_row=64), dict(add=5 * MB, add_row=0), dict(y=3 * MB), dict(y=4 * MB),
                  dict(bias=5 * MB), dict(x=None), dict(x=MB + 8), dict(x_row=40), dict(x_row=32), dict(x_row=1 << 22), dict(x_scale=None), dict(y=MB), dict(y=2 * MB)]
@@ -154,7 +154,9 @@ def test_rotary_refusals():
                       ([part(dst=MB + 128)], {}), ([part(), part(src=3 * MB)], {}), ([part(dst=9 * MB)], {}), ([part()], dict(start=2 * MB)),
                       # queries turned onto the keys beside them
                       ([part(**qkv(0), **dst(1)), part(**qkv(1), **dst(2))], {}),
-                      ([part(dst_row=768, dst=MB, src_row=1536)], {})):
+                      ([part(dst_row=768, dst=MB, src_row=1536)], {}),
+                      # in place, but transposed
+                      ([part(dst=MB, src_row=192, src_tok=64, src_head=576, dst_row=64, dst_tok=192, dst_head=576)], dict(n_rows=3, n_tok=3))):
             said(L.pkx_rotary(rot(p, **kw), None))
         said(L.pkx_rotary(None, None))
         f = (C.c_double * 8)()
@@ -165,30 +167,30 @@ def test_rotary_refusals():
         for kw in (dict(n_rows=0), dict(n_tok=0), dict(n_rows=0, freq=None)):
             said(L.pkx_rotary(rot([part()], **kw), None))
     """)
-    _refused(out[:32], ["type", "negative", "d_head", "d_head", "rot must", "rot must", "at most", "mult", "pos", "heads", "heads", "freq", "freq", "null or", "null or",
-                        "negative stride", "overlap", "overlaps a src", "two dsts", "overlaps freq", "overlaps start", "overlaps a src", "overlaps a src", "null",
+    _refused(out[:33], ["type", "negative", "d_head", "d_head", "rot must", "rot must", "at most", "mult", "pos", "heads", "heads", "freq", "freq", "null or", "null or",
+                        "negative stride", "overlap", "overlaps a src", "two dsts", "overlaps freq", "overlaps start", "overlaps a src", "overlaps a src", "overlaps a src", "null",
                         "base", "rot must", "rot must", "factor", "context", "high", "base", "null"])
-    assert [x.strip() for x in out[32:]] == ["0"] * 3
+    assert [x.strip() for x in out[33:]] == ["0"] * 3
 
 
 def test_logit_rules_refusals():
     out = _run("""
         cases = [dict(type=24), dict(n_rows=-1), dict(vocab=-1), dict(window=-1), dict(vocab=(1 << 22) + 1), dict(logits=None), dict(logits=MB + 2), dict(logits_row=-1),
-                 dict(out=None), dict(out_row=99), dict(out=MB + 4), dict(out=MB, out_row=200), dict(n_slots=0), dict(capacity=-1), dict(len=None), dict(n_slots=3),
+                 dict(out=None), dict(out_row=99), dict(out=MB + 4), dict(out=MB, out_row=200), dict(n_slots=0), dict(capacity=-1), dict(capacity=(1 << 30) + 1), dict(len=None), dict(n_slots=3),
                  dict(table=5 * MB, table_row=49), dict(out=3 * MB), dict(out=4 * MB), dict(slot=2 * MB), dict(repetition=2 * MB + 400),
                  dict(bias=5 * MB + 2, bias_row=100, n_bias=1), dict(bias=5 * MB, bias_row=-1, n_bias=1), dict(bias=2 * MB, bias_row=100, n_bias=1),
                  dict(bias=5 * MB, bias_row=100, n_bias=1, bias_index=2 * MB), dict(mask=5 * MB, mask_row=4, n_mask=-1), dict(mask=2 * MB, mask_row=4, n_mask=1),
-                 dict(mask=5 * MB, mask_row=4, n_mask=1, mask_index=2 * MB), dict(n_slots=(1 << 31) - 1, capacity=(1 << 31) - 1)]
+                 dict(mask=5 * MB, mask_row=4, n_mask=1, mask_index=2 * MB), dict(n_slots=(1 << 31) - 1, capacity=1 << 30)]
         for kw in cases:
             said(L.pkx_logit_rules(rules(**kw), None))
         said(L.pkx_logit_rules(None, None))
         for kw in (dict(n_rows=0), dict(vocab=0, logits=None)):
             said(L.pkx_logit_rules(rules(**kw), None))
     """)
-    _refused(out[:30], ["type", "negative", "negative", "negative", "2^22", "logits are", "logits are", "logits are", "out is", "out is", "overlaps logits", "overlaps logits",
-                        "no slots", "no slots", "null len", "more rows", "shorter", "overlaps the tokens", "overlaps the tokens", "overlaps the tokens", "overlaps a penalty",
+    _refused(out[:31], ["type", "negative", "negative", "negative", "2^22", "logits are", "logits are", "logits are", "out is", "out is", "overlaps logits", "overlaps logits",
+                        "no slots", "no slots", "2^30", "null len", "more rows", "shorter", "overlaps the tokens", "overlaps the tokens", "overlaps the tokens", "overlaps a penalty",
                         "bias is", "bias is", "overlaps bias", "overlaps bias_index", "mask is", "overlaps mask", "overlaps mask_index", "address space", "null"])
-    assert [x.strip() for x in out[30:]] == ["0"] * 2
+    assert [x.strip() for x in out[31:]] == ["0"] * 2
 
 
 def test_operands_side_by_side_are_taken():

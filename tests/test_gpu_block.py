@@ -168,8 +168,9 @@ LINEAR = [
     ("f16", 64, 1024, 4096, "none", True, True), ("f16", 65, 100, 300, "silu", True, False), ("f32", 100, 33, 1000, "none", False, False),
     ("f16", 128, 256, 64, "none", False, True), ("f32", 129, 129, 129, "silu", True, True), ("f16", 300, 1000, 257, "none", True, False),
     ("f16", 700, 4096, 512, "silu", True, False), ("f32", 2000, 777, 96, "none", True, True), ("f16", 3500, 4100, 272, "none", False, False),
-    ("f32", 4097, 4095, 16, "none", True, False), ("f16", 40, 8193, 320, "none", False, False), ("f16", 257, 2, 131072, "none", False, False),
-    ("f32", 5, 3, 131072, "none", False, False),
+    ("f32", 4097, 4095, 16, "none", True, False), ("f16", 40, 8193, 320, "none", False, False), ("f16", 257, 2, 131071, "none", False, False),
+    ("f32", 5, 3, 131071, "none", False, False), ("f16", 2000, 4096, 130, "silu", True, False), ("f32", 1990, 4000, 100, "none", False, True),
+    ("f32", 6, 500, 1500, "silu", True, False), ("f16", 3, 40, 2048, "none", True, True), ("f16", 130, 1000, 640, "none", False, False),
 ]
 
 
@@ -196,7 +197,7 @@ def test_linear_i8(gpu, stream, type, M, N, K, act, bias, add, tokens):
         big = rng.integers(-128, 128, (M, row)).astype(np.int8)
         q, s = big[:, :K], rng.uniform(0.001, 0.05, M).astype(np.float32)
         gpu.LinearI8(View(dev(gpu, big, stream), 0, (M, K), (row, 1)), wd, vy, x_scale=dev(gpu, s, stream), **kw)(stream)
-    want, err = ref.linear_i8(q, s, w, ws, b, act, kw["alpha"], a[:, 1:] if add else None)
+    want, err = ref.linear_i8(q, s, w, ws, b, act, kw["alpha"], a[:, 1:] if add else None, type == "f16")
     got = y.numpy(stream)
     check(got[:, :N], want, err, type == "f16", "y")
     assert (got[:, N:] == 5).all()
@@ -204,16 +205,19 @@ def test_linear_i8(gpu, stream, type, M, N, K, act, bias, add, tokens):
 
 def test_linear_i8_extremes(gpu, stream):
     """The largest sums, in place over what is added, weights quantised by the binding, scales of zero."""
-    K = 131072
-    x, w = np.full((2, K), 127, np.int8), np.full((33, K), 127, np.int8)
-    w[1::2] = -127
-    x[1] = -127
+    K = 131071
+    x, w = np.full((2, K), -128, np.int8), np.full((33, K), -128, np.int8)
+    w[1::2] = 127
+    x[1] = 127
     one = np.ones(33, np.float32)
     wd = gpu.WeightI8(dev(gpu, w, stream), dev(gpu, one, stream), stream)
     y = dev(gpu, np.ones((2, 33), np.float32), stream)
-    gpu.LinearI8(dev(gpu, x, stream), wd, y, x_scale=dev(gpu, np.float32([1, 0]), stream), add=y)(stream)
+    xb = np.zeros((2, K + 1), np.int8)
+    xb[:, :K] = x
+    gpu.LinearI8(View(dev(gpu, xb, stream), 0, (2, K), (K + 1, 1)), wd, y, x_scale=dev(gpu, np.float32([1, 0]), stream), add=y)(stream)
     got = y.numpy(stream)
-    assert np.array_equal(got[0], np.float32(1) + (127.0 * 127 * K * (1 - 2 * (np.arange(33) % 2))).astype(np.float32)) and (got[1] == 1).all()
+    sums = -128.0 * np.where(np.arange(33) % 2, 127, -128) * K
+    assert np.array_equal(got[0], np.float32(1) + sums.astype(np.float32)) and (got[1] == 1).all()
     rng = np.random.default_rng(8)
     wf, xf = rng.standard_normal((70, 200)).astype(np.float32), rng.standard_normal((5, 200)).astype(np.float32)
     wq, ws = ref.quantised(wf)
@@ -221,6 +225,21 @@ def test_linear_i8_extremes(gpu, stream):
     y = gpu.DeviceArray((5, 70), np.float32)
     gpu.LinearI8(dev(gpu, xf, stream), gpu.WeightI8.quantize(dev(gpu, wf, stream), stream), y)(stream)
     check(y.numpy(stream), *ref.linear_i8(q, s, wq, ws, None, "none", 1.0, None), False, "quantised weights")
+    # SiLU of what f32 and f16 hold at their ends
+    v = np.float32([np.inf, -np.inf, np.nan, 1e38, -1e38, 200, -200, 88.5, -88.5, 0, -0.0, 1e-30, -103, -87.4, -88.1, 60])
+    wd = gpu.WeightI8(dev(gpu, np.zeros((16, 16), np.int8), stream), dev(gpu, np.ones(16, np.float32), stream), stream)
+    for dt in (np.float32, np.float16):
+        for rows in (1, 40):
+            y = gpu.DeviceArray((rows, 16), dt)
+            gpu.LinearI8(dev(gpu, np.ones((rows, 16), np.float32), stream), wd, y, bias=dev(gpu, v, stream), act="silu")(stream)
+            got = y.numpy(stream)
+            with np.errstate(all="ignore"):
+                want = v.astype(np.float64) / (1 + np.exp(-v.astype(np.float64)))
+                lost = np.abs(want) * 6 * ref.U + 1.2e-38        # subnormal results may be zeros
+                if dt == np.float16:
+                    want, lost = np.where(np.abs(want) > 65519, np.copysign(np.inf, want), want), lost + 2.0 ** -23 * np.abs(v * want)
+            for r in range(rows):
+                check(got[r], want, np.where(np.isfinite(want), lost, 0), dt == np.float16, "silu")
 
 
 # ---- rotary ---------------------------------------------------------------------
