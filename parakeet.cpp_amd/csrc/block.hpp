@@ -61,7 +61,7 @@ struct LinearI8Params {
 };
 void launch_linear_i8(const LinearI8Params& p, hipStream_t s);
 // The same from rows as they come, in one launch, for the few and short ones that linear_i8_fused() names.
-bool linear_i8_fused(int M, int K);
+bool linear_i8_fused(int M, int N, int K);
 void launch_linear_i8_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s);
 
 constexpr int kRotaryParts = 4, kMaxRotaryWidth = 512;

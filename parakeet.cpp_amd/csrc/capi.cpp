@@ -375,7 +375,7 @@ pkx::LinearI8Params linear_i8_params(const pkx_linear_i8_args* a) {
 // Quantised tokens in the workspace: rows of whole 16 bytes, then their scales.
 int64_t i8_row(const pkx_linear_i8_args* a) { return ((int64_t)a->n_in + 15) / 16 * 16; }
 size_t i8_workspace(const pkx_linear_i8_args* a) {
-    return a->x_type == PKX_TYPE_I8 || a->n_rows == 0 || a->n_out == 0 || pkx::linear_i8_fused(a->n_rows, a->n_in) ? 0 : (size_t)a->n_rows * (i8_row(a) + 4);
+    return a->x_type == PKX_TYPE_I8 || a->n_rows == 0 || a->n_out == 0 || pkx::linear_i8_fused(a->n_rows, a->n_out, a->n_in) ? 0 : (size_t)a->n_rows * (i8_row(a) + 4);
 }
 // Every element where it was: a stride counts where its dimension has more than one.
 bool in_place(const pkx::RotaryPart& p, int64_t rows, int64_t toks) {
@@ -1123,7 +1123,7 @@ int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* 
         need(!a->x_scale, "8-bit linear: x_scale goes with PKX_TYPE_I8");
         pkx::QuantizeRowsParams q = quantize_rows_params(a->x_type, a->x, a->x_row, M, a->n_in);
         need(apart(y, rows_of(a->x, K, q.f32 ? 4 : 2, a->x_row, M)), "8-bit linear: y overlaps x");
-        if (pkx::linear_i8_fused(p.M, p.K)) {
+        if (pkx::linear_i8_fused(p.M, p.N, p.K)) {
             need_device(st(s));
             pkx::launch_linear_i8_fused(p, q, st(s));
             return;

@@ -21,15 +21,16 @@ typedef int int16v __attribute__((ext_vector_type(16)));
 // A row is read once and kept in registers up to 8 T NV values; longer rows are read twice.
 template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_rows_kernel(QuantizeRowsParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1;
-    __shared__ float part[T / 64], more[T / 64];
+    __shared__ float part[kRows][T / 64], more[T / 64];
     const int t = threadIdx.x % T, d = p.d;
-    const int64_t r = (int64_t)blockIdx.x * kRows + (kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0);
+    const int mine = kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0;
+    const int64_t r = (int64_t)blockIdx.x * kRows + mine;
     if (r >= p.rows) return;
     const ET* x = (const ET*)p.x + r * p.x_row;
     float v[NV][8];
 #pragma unroll
     for (int k = 0; k < NV; ++k) load_row8(v[k], x, 8 * (t + k * T), d);
-    RowTop top = row_top<T, NV>(v, part);
+    RowTop top = row_top<T, NV>(v, part[mine]);
     const bool longer = d > 8 * T * NV;
     if (longer) {                            // only the longest rows' kernel: T > 64
         float w[1][8] = {}, m = 0.f;
@@ -65,6 +66,7 @@ template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256
 template <typename ET> void launch_quantize_typed(const QuantizeRowsParams& p, hipStream_t s) {
     const unsigned rows = (unsigned)p.rows;
     if (p.d <= 512) launch(quantize_rows_kernel<ET, 64, 1>, dim3((rows + 3) / 4), dim3(256), 0, s, p);
+    else if (p.d <= 1024) launch(quantize_rows_kernel<ET, 128, 1>, dim3((rows + 1) / 2), dim3(256), 0, s, p);
     else if (p.d <= 2048) launch(quantize_rows_kernel<ET, 256, 1>, dim3(rows), dim3(256), 0, s, p);
     else if (p.d <= 4096) launch(quantize_rows_kernel<ET, 256, 2>, dim3(rows), dim3(256), 0, s, p);
     else launch(quantize_rows_kernel<ET, 1024, 2>, dim3(rows), dim3(1024), 0, s, p);
@@ -148,13 +150,15 @@ template <typename YT, int CNT> struct Channels {
         if (p.silu)
 #pragma unroll
             for (int e = 0; e < CNT; ++e) v[e] = silu_of<YT>(v[e]);
+        if (p.alpha != 1.0f)
+#pragma unroll
+            for (int e = 0; e < CNT; ++e) v[e] *= p.alpha;
+        if (add)
+#pragma unroll
+            for (int e = 0; e < CNT; ++e) v[e] += (float)a[e];
         vec o;
 #pragma unroll
-        for (int e = 0; e < CNT; ++e) {
-            v[e] *= p.alpha;
-            if (add) v[e] += (float)a[e];
-            o[e] = (YT)v[e];
-        }
+        for (int e = 0; e < CNT; ++e) o[e] = (YT)v[e];
         if (whole) *(vecu*)y = o;
         else
 #pragma unroll
@@ -183,14 +187,14 @@ __device__ __forceinline__ void rows_finish(const LinearI8Params& p, int4v acc, 
     int4v s = part[0][lane];
 #pragma unroll
     for (int j = 1; j < kRowWaves; ++j) s += part[j][lane];
-    ch.store(p, s, m, xs[m]);
+    ch.store(p, s, m, xs[m - m0]);
 }
 
 template <typename YT> __global__ __launch_bounds__(kRowWaves * 64) void i8_rows_kernel(LinearI8Params p, int mtiles) {
     constexpr int W = kRowWaves, U = 4;
     __shared__ int4v part[W][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int nh = udiv_small(blockIdx.x, mtiles), m0 = (blockIdx.x - nh * mtiles) * 16;
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), nh = udiv_small(unit, mtiles), m0 = (unit - nh * mtiles) * 16;     // an XCD reads few weights
     const int kblocks = (p.K + kI8DepthPad - 1) / kI8DepthPad * (kI8DepthPad / kI8DepthBlock);
     const __amdgpu_buffer_rsrc_t rw = make_rsrc((const int8_t*)p.w + (int64_t)(nh >> 1) * kblocks * 2048, (int64_t)kblocks * 2048);
     const int k16 = (p.K + 15) & ~15, rows = p.M - m0 < 16 ? p.M - m0 : 16;
@@ -209,19 +213,23 @@ template <typename YT> __global__ __launch_bounds__(kRowWaves * 64) void i8_rows
 #pragma unroll
         for (int u = 0; u < U; ++u) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], b[u], acc, 0, 0, 0);
     }
-    rows_finish<YT>(p, acc, part, nh, m0, p.x_scale);
+    rows_finish<YT>(p, acc, part, nh, m0, p.x_scale + m0);
 }
 
 // Few tokens as they come, quantised by every workgroup for itself: one launch instead of two where that costs less than
 // a launch.  Each wave asks for its first blocks of weights, then the rows are shared out: `wpr` waves to a row, up
 // to 8 x 64 x NV values a wave, held in LDS in rows 16 bytes apart in banks.  1 x 4096 x 1024: 3.7 us, in two launches
-// 5.2; 16 x 4096 x 1024 5.0 and 5.6; 16 x 4096 x 2048 7.1 and 5.9, so up to 2^14 values.
-template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) void i8_rows_fused_kernel(LinearI8Params p, const XT* x, int64_t x_row, int wpr) {
+// 5.2; 16 x 4096 x 1024 5.0 and 5.6; 16 x 4096 x 2048 7.1 and 5.9, so up to 2^14 values.  More tokens than 16 while the
+// workgroups are one round of the chip: 64 x 1024 x 1024 5.4 and 5.7, 64 x 4096 x 256 8.1 and 6.2.
+template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) void i8_rows_fused_kernel(LinearI8Params p, const XT* x, int64_t x_row, int wpr, int mtiles) {
     constexpr int W = kRowWaves, U = 8;
-    extern __shared__ __align__(16) uint8_t held[];          // [M][kpad + 16]
+    extern __shared__ __align__(16) uint8_t held[];          // [rows][kpad + 16]
     __shared__ int4v part[W][64];
     __shared__ float tops[W], scale[16];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nh = blockIdx.x;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), nh = udiv_small(unit, mtiles), m0 = (unit - nh * mtiles) * 16;
+    const int rows = p.M - m0 < 16 ? p.M - m0 : 16;
+    x += m0 * x_row;
     const int kpad = (p.K + kI8DepthPad - 1) / kI8DepthPad * kI8DepthPad, kblocks = kpad / kI8DepthBlock, ld = kpad + 16;
     const __amdgpu_buffer_rsrc_t rw = make_rsrc((const int8_t*)p.w + (int64_t)(nh >> 1) * kblocks * 2048, (int64_t)kblocks * 2048);
     const uint32_t wo = ((lane >> 4) * 32 + 16 * (nh & 1) + (lane & 15)) * 16;
@@ -245,7 +253,7 @@ template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) vo
         }
     };
     if (wpr == 1) {
-        for (int r = w; r < p.M; r += slots) {
+        for (int r = w; r < rows; r += slots) {
             float v[NV][8];
             load(r, v);
             hold(r, v, row_top<64, NV>(v, nullptr));
@@ -253,7 +261,7 @@ template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) vo
     } else {                                 // one row at most to a wave
         const int r = w / wpr;
         float v[NV][8] = {};
-        if (r < p.M) load(r, v);
+        if (r < rows) load(r, v);
         RowTop top = row_top<64, NV>(v, nullptr);
         if (lane == 0) tops[w] = top.plain ? top.top : -top.top;
         __syncthreads();
@@ -262,10 +270,10 @@ template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) vo
             top.plain &= __builtin_bit_cast(int, o) >= 0;
             top.top = fmaxf(top.top, fabsf(o));
         }
-        if (r < p.M) hold(r, v, top);
+        if (r < rows) hold(r, v, top);
     }
     __syncthreads();
-    const int row = (lane & 15) < p.M ? lane & 15 : p.M - 1;         // tokens past the last give sums that nobody reads
+    const int row = (lane & 15) < rows ? lane & 15 : rows - 1;         // tokens past the last give sums that nobody reads
     const uint8_t* xr = held + row * ld + 16 * (lane >> 4);
     int4v acc = {};
     for (int k0 = w; k0 < kblocks; k0 += U * W) {
@@ -278,7 +286,7 @@ template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) vo
             acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[u], *(const int4v*)(xr + (k0 + u * W) * 64), acc, 0, 0, 0);
         }
     }
-    rows_finish<YT>(p, acc, part, nh, 0, scale);
+    rows_finish<YT>(p, acc, part, nh, m0, scale);
 }
 
 // ---- many tokens -----------------------------------------------------------
@@ -469,20 +477,21 @@ template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s)
 int fused_waves(int M) { return M == 1 ? 8 : M == 2 ? 4 : M <= 4 ? 2 : 1; }
 
 template <typename YT, typename XT> void launch_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s) {
-    const int wpr = fused_waves(p.M), kpad = cdiv(p.K, kI8DepthPad) * kI8DepthPad;
-    const uint32_t lds = p.M * (kpad + 16);
+    const int wpr = fused_waves(p.M), kpad = cdiv(p.K, kI8DepthPad) * kI8DepthPad, mtiles = cdiv(p.M, 16);
+    const uint32_t lds = (p.M < 16 ? p.M : 16) * (kpad + 16);
     const int per = cdiv(kpad, 512 * wpr);
-    const dim3 grid(2 * cdiv(p.N, 32));
-    if (per <= 1) launch(i8_rows_fused_kernel<YT, XT, 1>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
-    else if (per <= 2) launch(i8_rows_fused_kernel<YT, XT, 2>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
-    else launch(i8_rows_fused_kernel<YT, XT, 4>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr);
+    const dim3 grid(2 * cdiv(p.N, 32) * mtiles);
+    if (per <= 1) launch(i8_rows_fused_kernel<YT, XT, 1>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr, mtiles);
+    else if (per <= 2) launch(i8_rows_fused_kernel<YT, XT, 2>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr, mtiles);
+    else launch(i8_rows_fused_kernel<YT, XT, 4>, grid, dim3(512), lds, s, p, (const XT*)q.x, q.x_row, wpr, mtiles);
 }
 
 }  // namespace
 
-bool linear_i8_fused(int M, int K) {
-    const int kpad = cdiv(K, kI8DepthPad) * kI8DepthPad;
-    return M <= 16 && kpad <= 4 * 512 * fused_waves(M) && M * kpad <= 16384;
+bool linear_i8_fused(int M, int N, int K) {
+    const int kpad = cdiv(K, kI8DepthPad) * kI8DepthPad, rows = M < 16 ? M : 16;
+    if (kpad > 4 * 512 * fused_waves(M) || rows * kpad > 16384) return false;
+    return M <= 16 || (double)cdiv(N, 32) * 2 * cdiv(M, 16) <= 256;
 }
 void launch_linear_i8_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s) {
     if (p.M == 0 || p.N == 0) return;

@@ -119,7 +119,7 @@ def test_linear_refusals():
             said(L.pkx_linear_i8(lin(**kw), None, 0, None))
         said(L.pkx_linear_i8(None, None, 0, None))
         n = C.c_size_t()
-        f = dict(x_type=1, x_scale=None, n_rows=100)
+        f = dict(x_type=1, x_scale=None, n_rows=100, n_in=4000, x_row=4000)
         said(L.pkx_linear_i8_workspace(lin(**f), C.byref(n)))
         said(L.pkx_linear_i8(lin(x_type=1), 7 * MB, 1 << 20, None))
         said(L.pkx_linear_i8(lin(**f), None, 0, None))
@@ -139,7 +139,7 @@ def test_linear_refusals():
     assert out[31].strip() == "0"
     _refused(out[32:39], ["x_scale", "workspace", "workspace", "workspace", "x is", "overlaps x", "null"])
     assert [x.strip() for x in out[39:41]] == ["0"] * 2
-    assert int(out[41]) >= 100 * 48 + 400 and int(out[42]) == 0
+    assert int(out[41]) >= 100 * 4000 + 400 and int(out[42]) == 0
 
 
 def test_rotary_refusals():

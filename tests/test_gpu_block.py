@@ -170,7 +170,7 @@ LINEAR = [
     ("f16", 700, 4096, 512, "silu", True, False), ("f32", 2000, 777, 96, "none", True, True), ("f16", 3500, 4100, 272, "none", False, False),
     ("f32", 4097, 4095, 16, "none", True, False), ("f16", 40, 8193, 320, "none", False, False), ("f16", 257, 2, 131071, "none", False, False),
     ("f32", 5, 3, 131071, "none", False, False), ("f16", 2000, 4096, 130, "silu", True, False), ("f32", 1990, 4000, 100, "none", False, True),
-    ("f32", 6, 500, 1500, "silu", True, False), ("f16", 3, 40, 2048, "none", True, True), ("f16", 130, 1000, 640, "none", False, False),
+    ("f32", 6, 500, 1500, "silu", True, False), ("f16", 3, 40, 2048, "none", True, True), ("f32", 41, 100, 1000, "none", True, False), ("f16", 64, 500, 33, "silu", False, True), ("f16", 130, 1000, 640, "none", False, False),
 ]
 
 
