@@ -109,8 +109,9 @@ template <typename YT> __device__ __forceinline__ float silu_of(float v) {
     return v * by * q;
 }
 
-// What a lane needs of CNT channels from n0 < N on, for any number of tokens.
-template <typename YT, int CNT> struct Channels {
+// What a lane needs of CNT channels from n0 < N on, for any number of tokens.  STREAM: y is written past the caches next to the
+// units, which keep tokens and weights for the tiles that follow (2000 x 4096 x 1024 15.9 -> 14.1 us on 128 x 256 of eight waves).
+template <typename YT, int CNT, bool STREAM> struct Channels {
     typedef YT vec __attribute__((ext_vector_type(CNT)));
     typedef vec vecu __attribute__((aligned(sizeof(YT))));
     typedef float fvec __attribute__((ext_vector_type(CNT)));
@@ -159,7 +160,8 @@ template <typename YT, int CNT> struct Channels {
         vec o;
 #pragma unroll
         for (int e = 0; e < CNT; ++e) o[e] = (YT)v[e];
-        if (whole) *(vecu*)y = o;
+        if (whole && STREAM) __builtin_nontemporal_store(o, (vecu*)y);
+        else if (whole) *(vecu*)y = o;
         else
 #pragma unroll
             for (int e = 0; e < CNT; ++e)
@@ -183,7 +185,7 @@ __device__ __forceinline__ void rows_finish(const LinearI8Params& p, int4v acc, 
     const int g = lane >> 4, h = nh & 1, n0 = (nh >> 1) * kI8ColBlock + 16 * (g & 1) + 4 * (2 * h + (g >> 1));
     const int m = m0 + (lane & 15);
     if (w != 0 || m >= p.M || n0 >= p.N) return;
-    const Channels<YT, 4> ch(p, n0);
+    const Channels<YT, 4, false> ch(p, n0);
     int4v s = part[0][lane];
 #pragma unroll
     for (int j = 1; j < kRowWaves; ++j) s += part[j][lane];
@@ -290,7 +292,7 @@ template <typename YT, typename XT, int NV> __global__ __launch_bounds__(512) vo
 }
 
 // ---- many tokens -----------------------------------------------------------
-// WM x WN waves of TM x TN tiles of 32 tokens x 32 channels.  Tokens go through
+// Four waves side by side, each TM x TN tiles of 32 tokens x 32 channels.  Tokens go through
 // LDS (rows of 128 bytes, their 16-byte pieces permuted by the row so that the
 // reads of a tile fall into different banks), weights straight into the fragments.
 //
@@ -310,9 +312,9 @@ template <int N> __device__ __forceinline__ void join() {
     asm volatile("" ::: "memory");
 }
 
-template <typename YT, int WM, int WN, int TM, int TN>
-__global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params p, int mtiles, int ntiles) {
-    constexpr int W = WM * WN, BM = 32 * WM * TM, BN = 32 * WN * TN, ROWS = BM / 8 / W;   // DMA instructions of a wave per slab
+template <typename YT, int TM, int TN>
+__global__ __launch_bounds__(256, 2) void i8_tile_kernel(LinearI8Params p, int mtiles, int ntiles) {
+    constexpr int W = 4, BM = 32 * TM, BN = 32 * W * TN, ROWS = BM / 8 / W;   // DMA instructions of a wave per slab
     constexpr bool AHEAD = TM * TN <= 4;
     // weights of two slabs in turn; of four: no faster (512 x 4096 x 4096 on 64 x 128 tiles 15.9 and 15.8 us), more registers
     constexpr int WD = 2, ST = AHEAD ? WD + 1 : WD + 2, STAGE = BM * 128;    // ST stages of tokens
@@ -320,9 +322,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
     constexpr int SUMS = W * 32 * TN * 128;      // 32 tokens' sums of every wave, at the end
     __shared__ __align__(16) uint8_t slab[ST * STAGE > SUMS ? ST * STAGE : SUMS];
     const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wid % WM, wn = wid / WM;
-    // an XCD's tiles are neighbours: eight rows of tiles at a time, column by column (8192^3: 482 us; one row at a
-    // time 563, 16 rows 565, 32 rows 603)
+    // an XCD's tiles are neighbours: eight rows of tiles at a time, column by column (8192^3 on
+    // tiles of 256 x 256: 482 us; one row at a time 563, 16 rows 565, 32 rows 603)
     constexpr int group = 8;
     const int tile = xcd_tile(blockIdx.x, mtiles * ntiles);
     const int g = tile / (group * ntiles), in = tile - g * group * ntiles;
@@ -342,10 +343,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
     }
     uint32_t wo[TN];
 #pragma unroll
-    for (int j = 0; j < TN; ++j) wo[j] = (uint32_t)((wn * TN + j) * kblocks * 2048 + lane * 16);
+    for (int j = 0; j < TN; ++j) wo[j] = (uint32_t)((wid * TN + j) * kblocks * 2048 + lane * 16);
     uint32_t ao[4];                          // a lane's pieces of a stage, tile 0
 #pragma unroll
-    for (int q = 0; q < 4; ++q) ao[q] = (uint32_t)((wm * TM * 32 + (lane & 31)) * 128 + 16 * ((2 * q + (lane >> 5)) ^ (lane >> 1 & 7)));
+    for (int q = 0; q < 4; ++q) ao[q] = (uint32_t)((lane & 31) * 128 + 16 * ((2 * q + (lane >> 5)) ^ (lane >> 1 & 7)));
 
     int16v acc[TM][TN] = {};
     int4v wf[WD][4][TN], xf[2][AHEAD ? 4 : 1][TM];
@@ -416,9 +417,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
     join<0>();
     auto swizzle = [](int r) { return TN == 1 ? r >> 1 & 7 : r & (PIECES - 1); };   // 16 rows' pieces in 64 banks
     uint8_t* own = slab + wid * 32 * TN * 128;
-    const int n = n0 + wn * TN * 32 + E * (lane % PER);
-    if (n0 + wn * TN * 32 >= p.N) return;
-    const Channels<YT, E> ch(p, n < p.N ? n : p.N - 1);
+    const int n = n0 + wid * TN * 32 + E * (lane % PER);
+    if (n0 + wid * TN * 32 >= p.N) return;
+    const Channels<YT, E, true> ch(p, n < p.N ? n : p.N - 1);
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int r0 = lane & 31;
@@ -431,8 +432,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
             }
 #pragma unroll
         for (int r1 = 0; r1 < 32; r1 += STEP) {
-            const int r = r1 + lane / PER, m = m0 + (wm * TM + i) * 32 + r;
-            typename Channels<YT, E>::ivec v;
+            const int r = r1 + lane / PER, m = m0 + i * 32 + r;
+            typename Channels<YT, E, true>::ivec v;
 #pragma unroll
             for (int h = 0; h < E / 4; ++h) {
                 const int4v c = *(const int4v*)(own + r * TN * 128 + 16 * (((E / 4) * (lane % PER) + h) ^ swizzle(r)));
@@ -444,33 +445,39 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void i8_tile_kernel(LinearI8Params
     }
 }
 
-template <typename YT, int WM, int WN, int TM, int TN> void launch_tiles(const LinearI8Params& p, hipStream_t s) {
-    const int mt = cdiv(p.M, 32 * WM * TM), nt = cdiv(p.N, 32 * WN * TN);
-    launch(i8_tile_kernel<YT, WM, WN, TM, TN>, dim3(mt * nt), dim3(WM * WN * 64), 0, s, p, mt, nt);
+template <typename YT, int TM, int TN> void launch_tiles(const LinearI8Params& p, hipStream_t s) {
+    const int mt = cdiv(p.M, 32 * TM), nt = cdiv(p.N, 128 * TN);
+    launch(i8_tile_kernel<YT, TM, TN>, dim3(mt * nt), dim3(256), 0, s, p, mt, nt);
 }
 
-// The form whose estimated time is least, in us a 1024 of K, from what a round of 256 workgroups takes of it:
-//   rows 16 x 16          0.6   64 x 1024 x 4096 4.8 us (32 x 128 tiles: 9.1); 64 x 4096 x 4096 12.7 (8.3); launch and ends 3, tiles 4
-//   tiles of 32 x 128     1.3   128 x 4096 x 4096 8.7 us (64 x 128: 10.1); several to a CU
-//   tiles of 64 x 128     2.4   512 x 4096 x 4096 15.8 us (32 x 128: 17.8, 128 x 256: 27.7); several to a CU
-//   tiles of 128 x 256    9.6   2000 x 4096 x 1024 16.1 us (64 x 128: 17.3, 256 x 256: 22); one to a CU
-//   tiles of 256 x 256   16     16384 x 4096 x 4096 264 us (128 x 256: 318); one to a CU
+// The form of the least estimated time: a start and, for each round of workgroups that the chip holds, an end and the
+// 1024s of K.  Fitted to products run back to back for 0.15 s (the card's clock is then 1.6 GHz for the large ones), us:
+//                              16 x 16   32 x 128   64 x 128   64 x 256   128 x 256
+//      64 x  1024 x 4096          5.0       9.1       10.1
+//     128 x  4096 x 4096         12.7       8.1        9.5       15.0        27.5
+//     512 x  4096 x 4096                   17.0       15.2       18.2        29.6
+//    1000 x  4096 x 1024                               8.6        9.4        13.5
+//    2000 x  4096 x 1024                   19.4       15.5       14.9        15.7    (256 x 256, eight waves: 17.9)
+//    2000 x  4096 x 4096                              44.1       38.7        37.8                            42.1
+//   16384 x  4096 x 4096                  450        327        286         242                             245
+//    8192 x  8192 x 8192                             638        547         457                             450
 template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s) {
-    const float depth = p.K / 1024.0f, cus = 256.0f;
-    const auto tiles = [&](int bm, int bn) { return (float)cdiv(p.M, bm) * cdiv(p.N, bn); };
-    const auto shared = [&](float n) { return fmaxf(1.0f, n / cus); };   // rounds where a CU holds several workgroups
-    const auto alone = [&](float n) { return ceilf(n / cus); };
-    const float t32 = 1.3f * shared(tiles(32, 128)), t64 = 2.4f * shared(tiles(64, 128));
-    const float t128 = 9.6f * alone(tiles(128, 256)), t256 = 16.0f * alone(tiles(256, 256));
-    const float best = fminf(fminf(t32, t64), fminf(t128, t256));
-    const float units = 2.0f * tiles(16, 32);
-    if (units < (float)(1 << 22) && 3.0f + 0.6f * fmaxf(0.8f, units / cus) * depth < 4.0f + best * depth) {
+    const float depth = p.K / 1024.0f;
+    const auto rounds = [&](int bm, int bn, float held) { return (float)cdiv(p.M, bm) * cdiv(p.N, bn) / held; };
+    const auto least = [](float r, float most) { return r > most ? r : most; };    // fewer workgroups take no less
+    const float units = rounds(16, 16, 256), rows = 3.0f + least(units, 0.8f) * 0.6f * depth;
+    const float t32 = 4.0f + least(rounds(32, 128, 256), 0.63f) * (0.45f + 1.5f * depth);
+    const float t64 = 4.0f + least(rounds(64, 128, 256), 1.0f) * (0.7f + 2.25f * depth);
+    const float wide64 = 4.0f + least(rounds(64, 256, 512), 0.41f) * (3.2f + 7.8f * depth);
+    const float wide128 = 5.0f + least(rounds(128, 256, 512), 0.4f) * (6.5f + 14.5f * depth);
+    const float best = fminf(fminf(t32, t64), fminf(wide64, wide128));
+    if (rows < best && units * 256 < (float)(1 << 21)) {
         const int mtiles = cdiv(p.M, 16);
         launch(i8_rows_kernel<YT>, dim3(2 * cdiv(p.N, 32) * mtiles), dim3(512), 0, s, p, mtiles);
-    } else if (t256 == best) launch_tiles<YT, 2, 4, 4, 2>(p, s);
-    else if (t128 == best) launch_tiles<YT, 2, 4, 2, 2>(p, s);
-    else if (t64 == best) launch_tiles<YT, 1, 4, 2, 1>(p, s);
-    else launch_tiles<YT, 1, 4, 1, 1>(p, s);
+    } else if (wide128 == best) launch_tiles<YT, 4, 2>(p, s);
+    else if (wide64 == best) launch_tiles<YT, 2, 2>(p, s);
+    else if (t64 == best) launch_tiles<YT, 2, 1>(p, s);
+    else launch_tiles<YT, 1, 1>(p, s);
 }
 
 // Waves to a row of the fused form: all eight for one token, one from five tokens on.

@@ -19,7 +19,8 @@ template <typename T, int E> struct Piece {
 
 // One workgroup per row and tile of at most WORDS words (`width`, a multiple of 32).  The chain is length, table, tokens,
 // counts; logits, biases and mask are asked for behind the table's entries and used when the counts are there, and no
-// barrier waits for them.  What V leaves past whole pieces of 16 bytes goes to one thread a word.
+// barrier waits for them.  What V leaves past whole pieces of 16 bytes goes to one thread a word.  512 rows x 32769: 34.5 us, of
+// which 26 are a copy's, 5 biases and masks, 3 the histories; 39.5 with stores that stay in the caches next to the units.
 constexpr int kRuleThreads = 512;
 template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p, int tiles, int width) {
     constexpr int T = kRuleThreads, E = 16 / sizeof(ET), NV = WORDS / (T * E);     // neighbouring lanes', neighbouring pieces
@@ -119,7 +120,7 @@ template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) voi
         vec y;
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = (ET)ruled((float)v[k][e], c[e], bias[k][e], bits[k] >> (i % 32 + e) & 1);
-        *(vecu*)(o + i) = y;
+        __builtin_nontemporal_store(y, (vecu*)(o + i));
     }
     if (t < rest) o[whole + t] = (ET)ruled((float)last, count ? times[whole + t] : 0u, last_bias, last_bits >> ((whole + t) % 32) & 1);
 }

@@ -21,18 +21,20 @@ __device__ __forceinline__ void load8u(float (&v)[8], const float* p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) { v[e] = a[e]; v[4 + e] = b[e]; }
 }
+// Stores past the caches next to the units: what these kernels write they do not read again, and lines kept for it push out
+// what they do (4 x 8192 tokens turned 49.3 -> 44.3 us, 2000 x 1024 normed 8.6 -> 7.6; loads past them cost a quarter more).
 __device__ __forceinline__ void store8u(f16* p, const float (&v)[8]) {
     half8v a;
 #pragma unroll
     for (int e = 0; e < 8; ++e) a[e] = (f16)v[e];
-    *(half8u*)p = a;
+    __builtin_nontemporal_store(a, (half8u*)p);
 }
 __device__ __forceinline__ void store8u(float* p, const float (&v)[8]) {
     float4v a, b;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { a[e] = v[e]; b[e] = v[4 + e]; }
-    *(float4u*)p = a;
-    *(float4u*)(p + 4) = b;
+    __builtin_nontemporal_store(a, (float4u*)p);
+    __builtin_nontemporal_store(b, (float4u*)(p + 4));
 }
 
 // Elements [i, i + 8) of a row of d; those past its end are 0 and are not read.
