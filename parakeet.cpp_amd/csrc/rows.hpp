@@ -56,6 +56,34 @@ template <typename T> __device__ __forceinline__ void store_row8(T* row, const f
         if (i + e < d) row[i + e] = (T)v[e];
 }
 
+// The same in pieces of four.
+template <typename T> __device__ __forceinline__ void load_row4(float* v, const T* row, int i, int d) {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    typedef vec vecu __attribute__((aligned(sizeof(T))));
+    if (i + 4 <= d) {
+        const vec a = *(const vecu*)(row + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (float)a[e];
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = i + e < d ? (float)row[i + e] : 0.f;
+}
+template <typename T> __device__ __forceinline__ void store_row4(T* row, const float* v, int i, int d) {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    typedef vec vecu __attribute__((aligned(sizeof(T))));
+    if (i + 4 <= d) {
+        vec a;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] = (T)v[e];
+        __builtin_nontemporal_store(a, (vecu*)(row + i));
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < d) row[i + e] = (T)v[e];
+}
+
 // A barrier for what a workgroup shares in LDS: it waits for no load that is on its way to a register, as __syncthreads does.
 __device__ __forceinline__ void lds_barrier() {
     asm volatile("" ::: "memory");
@@ -195,6 +223,17 @@ __device__ __forceinline__ void store_bytes8(int8_t* row, int2v w, int i, int d)
 #pragma unroll
     for (int e = 0; e < 8; ++e)
         if (i + e < d) row[i + e] = (int8_t)(w[e >> 2] >> (8 * (e & 3)));
+}
+
+__device__ __forceinline__ void store_bytes4(int8_t* row, int w, int i, int d) {
+    typedef int int1u __attribute__((aligned(1)));
+    if (i + 4 <= d) {
+        *(int1u*)(row + i) = w;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (i + e < d) row[i + e] = (int8_t)(w >> (8 * e));
 }
 
 }  // namespace pkx
