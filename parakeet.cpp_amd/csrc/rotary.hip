@@ -36,9 +36,9 @@ __device__ __forceinline__ float2v cos_sin_turns(double x) {
 }
 
 // One workgroup per `tok` tokens of a row and part (blockIdx.y): their angles once into LDS, then the part's heads, IT items a
-// thread at a time.  An item is 8 elements of a head (4 pairs of neighbours, or elements past rot), or 8 pairs of halves; the
-// first ones are asked for before the angles are formed.  WHOLE: every item is, so nothing looks for an end.
-template <typename ET, bool INTER, bool WHOLE, int IT>
+// thread at a time.  An item is E elements of a head, 16 bytes (pairs of neighbours, or elements past rot), or E pairs of
+// halves; the first ones are asked for before the angles are formed.  WHOLE: every item is, so nothing looks for an end.
+template <typename ET, bool INTER, bool WHOLE, int E, int IT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
     extern __shared__ float2v turn[];        // [tok][rot / 2]
     const RotaryPart q = p.part[blockIdx.y];
@@ -47,21 +47,21 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
     n = n > p.n ? p.n : n;
     if (i0 >= n) return;
     const int toks = n - i0 < q.tok ? n - i0 : q.tok, pairs = p.rot / 2, rest = p.dk - p.rot;
-    const int turned = INTER ? (p.rot + 7) / 8 : (pairs + 7) / 8, items = turned + (rest + 7) / 8, per = q.heads * items;
+    const int turned = INTER ? (p.rot + E - 1) / E : (pairs + E - 1) / E, items = turned + (rest + E - 1) / E, per = q.heads * items;
     const int all = toks * per;
     const ET* from = (const ET*)q.src + r * q.s_row + i0 * q.s_tok;
     ET* to = (ET*)q.dst + r * q.d_row + i0 * q.d_tok;
 
-    auto get = [](float (&v)[8], const ET* row, int i, int d) {
-        if constexpr (WHOLE) load8u(v, row + i);
-        else load_row8(v, row, i, d);
+    auto get = [](float (&v)[E], const ET* row, int i, int d) {
+        if constexpr (E == 8) load_row8(v, row, i, WHOLE ? i + 8 : d);
+        else load_row4(v, row, i, WHOLE ? i + 4 : d);
     };
-    auto put = [](ET* row, const float (&v)[8], int i, int d) {
-        if constexpr (WHOLE) store8u(row + i, v);
-        else store_row8(row, v, i, d);
+    auto put = [](ET* row, const float (&v)[E], int i, int d) {
+        if constexpr (E == 8) store_row8(row, v, i, WHOLE ? i + 8 : d);
+        else store_row4(row, v, i, WHOLE ? i + 4 : d);
     };
     // at: an item's first pair, or -1 - its first element past rot; whole elements and pairs beyond an item's end are zeros
-    float a[IT][8], b[IT][8] = {};
+    float a[IT][E], b[IT][E] = {};
     const ET* src[IT];
     ET* dst[IT];
     int at[IT], tok[IT];
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
             const int hi = j - tok[u] * per, h = udiv_small(hi, items), it = hi - h * items;
             src[u] = from + tok[u] * q.s_tok + h * q.s_head;
             dst[u] = to + tok[u] * q.d_tok + h * q.d_head;
-            at[u] = it >= turned ? -1 - 8 * (it - turned) : INTER ? 4 * it : 8 * it;
+            at[u] = it >= turned ? -1 - E * (it - turned) : INTER ? E / 2 * it : E * it;
             if (j0 + 256 * u >= all) dst[u] = nullptr;
             const bool other = at[u] < 0;
             if (other && src[u] == dst[u]) dst[u] = nullptr;
@@ -87,15 +87,15 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
             if (!dst[u]) continue;
             const bool other = at[u] < 0;
             const float2v* cs = turn + tok[u] * pairs + (other ? 0 : at[u]);
-            float o[8], o2[8];
+            float o[E], o2[E];
 #pragma unroll
-            for (int e = 0; e < (INTER ? 4 : 8); ++e) {
+            for (int e = 0; e < (INTER ? E / 2 : E); ++e) {
                 const float2v c = (WHOLE ? !other : !other && at[u] + e < pairs) ? cs[e] : float2v{0.f, 0.f};
-                const float v = INTER ? a[u][2 * (e & 3)] : a[u][e], w = INTER ? a[u][2 * (e & 3) + 1] : b[u][e];
+                const float v = INTER ? a[u][2 * (e % (E / 2))] : a[u][e], w = INTER ? a[u][2 * (e % (E / 2)) + 1] : b[u][e];
                 const float x = v * c[0] - w * c[1], y = w * c[0] + v * c[1];
                 if (INTER) {
-                    o[2 * (e & 3)] = other ? v : x;
-                    o[2 * (e & 3) + 1] = other ? w : y;
+                    o[2 * (e % (E / 2))] = other ? v : x;
+                    o[2 * (e % (E / 2)) + 1] = other ? w : y;
                 } else {
                     o[e] = other ? v : x;
                     o2[e] = y;
@@ -123,8 +123,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
     }
 }
 
-template <typename ET, bool INTER, bool WHOLE, int IT> void launch_typed(RotaryParams p, hipStream_t s) {
-    const int pairs = p.rot / 2, items = cdiv(INTER ? p.rot : pairs, 8) + cdiv(p.dk - p.rot, 8);
+template <typename ET, bool INTER, bool WHOLE, int E, int IT> void launch_typed(RotaryParams p, hipStream_t s) {
+    const int pairs = p.rot / 2, items = cdiv(INTER ? p.rot : pairs, E) + cdiv(p.dk - p.rot, E);
     int most = 1, lds = 0;
     for (int z = 0; z < p.parts; ++z) {      // as many tokens as give every thread its IT items, within 32 KB of angles
         int tok = 256 * IT / (p.part[z].heads * items);
@@ -135,19 +135,24 @@ template <typename ET, bool INTER, bool WHOLE, int IT> void launch_typed(RotaryP
         lds = tok * pairs * 8 > lds ? tok * pairs * 8 : lds;
     }
     require((double)p.R * most < (double)(1 << 22), "rotary: too many tokens for one call");
-    launch(rotary_kernel<ET, INTER, WHOLE, IT>, dim3(p.R * most, p.parts), dim3(256), lds, s, p, most);
+    launch(rotary_kernel<ET, INTER, WHOLE, E, IT>, dim3(p.R * most, p.parts), dim3(256), lds, s, p, most);
 }
-template <typename ET> void launch_pairs(const RotaryParams& p, hipStream_t s) {
-    const bool rest = (p.dk - p.rot) % 8 == 0;
-    if (p.interleaved) rest && p.rot % 8 == 0 ? launch_typed<ET, true, true, 4>(p, s) : launch_typed<ET, true, false, 1>(p, s);
-    else rest && p.rot % 16 == 0 ? launch_typed<ET, false, true, 2>(p, s) : launch_typed<ET, false, false, 1>(p, s);
+// Items of 16 bytes where head and pairs divide into them, of 8 for f16 where not, and of four elements with ends looked for in
+// any other case (4 x 4096 tokens x 20 heads x 80, 20 pairs of halves: 8 bytes 26.3 us, 16 with ends 37.8).
+template <typename ET, bool INTER> void launch_items(const RotaryParams& p, hipStream_t s) {
+    constexpr int E = 16 / sizeof(ET), IT = INTER ? 4 : 2;
+    const int unit = INTER ? p.rot : p.rot / 2, rest = p.dk - p.rot;
+    if (unit % E == 0 && rest % E == 0) launch_typed<ET, INTER, true, E, IT>(p, s);
+    else if (unit % 4 == 0 && rest % 4 == 0) launch_typed<ET, INTER, true, 4, IT>(p, s);
+    else launch_typed<ET, INTER, false, 4, 2>(p, s);
 }
 
 }  // namespace
 
 void launch_rotary(const RotaryParams& p, hipStream_t s) {
     if (p.R == 0 || p.n == 0 || p.parts == 0) return;
-    p.f32 ? launch_pairs<float>(p, s) : launch_pairs<f16>(p, s);
+    if (p.f32) p.interleaved ? launch_items<float, true>(p, s) : launch_items<float, false>(p, s);
+    else p.interleaved ? launch_items<f16, true>(p, s) : launch_items<f16, false>(p, s);
 }
 
 }  // namespace pkx
