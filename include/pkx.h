@@ -484,9 +484,9 @@ int pkx_beam_reorder(const int32_t* parent, int n_items, int n_beams, const pkx_
                      void* stream);
 
 /* ---- the rest of a decoder's block ------------------------------------------------
- * No counterpart in the reference: what stands between the calls above in an attention
- * decoder, as products and norms in their training framework do.  The same manner: the
- * caller's buffers, kernels on the stream and nothing else, capturable; calls of size zero do nothing. */
+ * No counterpart in the reference: what an attention decoder runs between the calls above.  The
+ * same manner: the caller's buffers, kernels on the stream and nothing else, capturable; calls of
+ * size zero do nothing. */
 
 /* Block norm: for every row, with u = post(y) and h = pre(x_out) before its rounding to x's type,
  *   x_out = x + alpha * g * u      g = gate, sigmoid(gate) or 1 without one
@@ -560,7 +560,7 @@ int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* 
  * from count[r] on are left as they were.  Angles are formed and reduced in f64, products are f32.  A part is an operand of its own head
  * count (queries, keys); dst may be src with the same strides, else it overlaps no src; parts' dsts lie apart.
  * Strides in elements (row, token, head), not negative; positions may be negative (the turn undone).
- * d_head up to 512, rot even and at most d_head. */
+ * d_head up to 512, rot even and at most d_head; n_rows * n_tok below 2^22 (more where a workgroup takes several tokens). */
 #define PKX_ROTARY_MAX_PARTS 4
 typedef struct {
     const void* src;  int64_t src_row, src_tok, src_head;
@@ -592,7 +592,7 @@ int pkx_rotary_frequencies(double base, int rot, double factor, double context, 
  * out): the histories lie as a cache's tokens do, and beams share them through the same tables.  Tokens outside the vocabulary do not count.  bias and
  * mask are sets of rows that rows of logits name: row bias_index[r] of n_bias (NULL: r), none where that is out of range,
  * and likewise the mask, whose word v / 32 has the bit v % 32.  out may be logits with the same rows; other overlaps are refused.
- * vocab up to 2^22, capacity up to 2^30; strides in elements. */
+ * vocab up to 2^22, capacity up to 2^30; n_rows times the tiles of 8192 words below 2^22; strides in elements. */
 typedef struct {
     int type;                            /* PKX_TYPE_F32 or PKX_TYPE_F16, of logits and out */
     int n_rows, vocab;

@@ -18,7 +18,8 @@ typedef int int16v __attribute__((ext_vector_type(16)));
 
 // ---- quantising rows -------------------------------------------------------
 // s = max |x| / 127 over the finite values, x held as clamp(round(x / s), -127, 127), each step one f32 operation.
-// A row is read once and kept in registers up to 8 T NV values; longer rows are read twice.
+// A row is read once and kept in registers up to 8 T NV values; longer rows are read twice.  16384 x 4096 f16 (201 MB): 37 us,
+// 5.4 TB/s.
 template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_rows_kernel(QuantizeRowsParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1;
     __shared__ float part[kRows][T / 64], more[T / 64];
@@ -412,7 +413,7 @@ __global__ __launch_bounds__(256, 2) void i8_tile_kernel(LinearI8Params p, int m
 
     // A wave's sums pass through LDS (32 tokens at a time, their 16-byte pieces permuted by the row), so that
     // neighbouring lanes write neighbouring pieces of a row: as the matrix instructions leave them a store would touch 64
-    // half lines (16 MB of f16 took 6 us that way).
+    // half lines (2000 x 4096 outputs took 6 us that way, a fill of their 16 MB 4.9).
     constexpr int E = 16 / sizeof(YT), PER = 32 * TN / E, STEP = 64 / PER, PIECES = 8 * TN;
     join<0>();
     auto swizzle = [](int r) { return TN == 1 ? r >> 1 & 7 : r & (PIECES - 1); };   // 16 rows' pieces in 64 banks

