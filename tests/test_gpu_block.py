@@ -242,6 +242,125 @@ def test_linear_i8_extremes(gpu, stream):
                 check(got[r], want, np.where(np.isfinite(want), lost, 0), dt == np.float16, "silu")
 
 
+# ---- far apart ------------------------------------------------------------------
+def _put(gpu, stream, base, at, a):
+    a = np.ascontiguousarray(a)
+    gpu.check(gpu.lib().pkx_memcpy_h2d(base.ptr + at * base.dtype.itemsize, a.ctypes.data, a.nbytes, stream.handle))
+
+
+def _get(gpu, stream, base, at, shape):
+    a = np.empty(shape, base.dtype)
+    gpu.check(gpu.lib().pkx_memcpy_d2h(a.ctypes.data, base.ptr + at * base.dtype.itemsize, a.nbytes, stream.handle))
+    return a
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+def test_far_rows(gpu, stream, type):
+    """Rows 2^31 elements apart: norm in place, quantised, products with what is added, logits."""
+    rng = np.random.default_rng(40)
+    dt, far, d, N = DT[type], 1 << 31, 300, 70
+    big = gpu.DeviceArray((2 * far + d,), dt)
+    x = rng.standard_normal((3, d)).astype(dt)
+    view = lambda n: View(big, 0, (3, n), (far, 1))  # noqa: E731
+
+    def fill(a):
+        for r in range(3):
+            _put(gpu, stream, big, r * far, a[r])
+
+    def rows(n):
+        return np.stack([_get(gpu, stream, big, r * far, (n,)) for r in range(3)])
+
+    fill(x)
+    h, y = gpu.DeviceArray((3, d), dt), rng.standard_normal((3, d)).astype(dt)
+    gpu.BlockNorm(view(d), h, y=dev(gpu, y, stream), x_out=view(d), post="layer", pre="rms")(stream)
+    r, er, hh, eh = ref.block_norm(x, y, None, 1, "linear", 1.0, "layer", None, None, "rms", None, None, 1e-5, 1e-5)
+    check(rows(d), r, er, type == "f16", "far x_out")
+    check(h.numpy(stream), hh, eh, type == "f16", "far h")
+    fill(x)
+    q, s = gpu.DeviceArray((3, d), np.int8), gpu.DeviceArray((3,), np.float32)
+    gpu.QuantizeRows(view(d), q, s)(stream)
+    want = ref.quantised(x)
+    assert np.array_equal(q.numpy(stream), want[0]) and np.array_equal(s.numpy(stream), want[1])
+    w, ws = rng.integers(-127, 128, (N, d)).astype(np.int8), rng.uniform(0.0005, 0.002, N).astype(np.float32)
+    wd = gpu.WeightI8(dev(gpu, w, stream), dev(gpu, ws, stream), stream)
+    out = gpu.DeviceArray((3, N), dt)
+    gpu.LinearI8(view(d), wd, out)(stream)
+    check(out.numpy(stream), *ref.linear_i8(*want, w, ws, None, "none", 1.0, None, type == "f16"), type == "f16", "far x")
+    gpu.LinearI8(dev(gpu, x, stream), wd, view(N), add=view(N))(stream)
+    check(rows(N), *ref.linear_i8(*want, w, ws, None, "none", 1.0, x[:, :N], type == "f16"), type == "f16", "far y")
+    fill(x)
+    bias = rng.standard_normal((3, d)).astype(np.float32)
+    gpu.LogitRules(view(d), view(d), bias=dev(gpu, bias, stream))(stream)
+    for i, got in enumerate(rows(d)):
+        check(got, *ref.rules(x[i], np.zeros(d), 1, 0, 0, bias[i], None), type == "f16", "far logits")
+
+
+@pytest.mark.parametrize("M,N", [(1100, 40), (2000, 4096)])
+def test_far_tokens_8bit(gpu, stream, M, N):
+    """8-bit tokens of the largest stride, together past 4 GiB; few channels and tiles of them."""
+    rng = np.random.default_rng(41)
+    K, row = 100, (1 << 22) - 16
+    big = gpu.DeviceArray(((M - 1) * row + 112,), np.int8)
+    x, s = rng.integers(-127, 128, (M, K)).astype(np.int8), rng.uniform(0.001, 0.05, M).astype(np.float32)
+    for m in range(M):
+        _put(gpu, stream, big, m * row, x[m])
+    w, ws = rng.integers(-127, 128, (N, K)).astype(np.int8), rng.uniform(0.0005, 0.002, N).astype(np.float32)
+    y = gpu.DeviceArray((M, N), np.float32)
+    gpu.LinearI8(View(big, 0, (M, K), (row, 1)), gpu.WeightI8(dev(gpu, w, stream), dev(gpu, ws, stream), stream), y, x_scale=dev(gpu, s, stream))(stream)
+    check(y.numpy(stream), *ref.linear_i8(x, s, w, ws, None, "none", 1.0, None), False, "far tokens")
+
+
+@pytest.mark.parametrize("M", [2, 200])
+def test_far_weights_8bit(gpu, stream, M):
+    """Weights of more than 4 GiB (rows that overlap in what they are packed from), few tokens and tiles of them; the last channels of each."""
+    rng = np.random.default_rng(42)
+    N, K = 33000, 131071
+    flat = rng.integers(-127, 128, (N - 1) * 16 + K).astype(np.int8)
+    base = dev(gpu, flat, stream)
+    ws = rng.uniform(0.0005, 0.002, N).astype(np.float32)
+    wd = gpu.WeightI8(View(base, 0, (N, K), (16, 1)), dev(gpu, ws, stream), stream)
+    x = rng.standard_normal((M, K)).astype(np.float32)
+    y = gpu.DeviceArray((M, N), np.float32)
+    gpu.LinearI8(dev(gpu, x, stream), wd, y)(stream)
+    got, (q, s) = y.numpy(stream), ref.quantised(x[-2:])
+    for n0 in (0, 16350, N - 40):
+        w = np.stack([flat[16 * n:16 * n + K] for n in range(n0, n0 + 40)])
+        check(got[-2:, n0:n0 + 40], *ref.linear_i8(q, s, w, ws[n0:n0 + 40], None, "none", 1.0, None), False, f"channels from {n0}")
+
+
+def test_far_histories(gpu, stream):
+    """Histories 2^30 tokens long, the last of them counted, by slot and by table; masks and biases whose rows lie 2^31 bytes apart."""
+    rng = np.random.default_rng(43)
+    cap, V, n = 1 << 30, 90, 40
+    words = gpu.DeviceArray((3, cap), np.int32)
+    ids = i32(rng.integers(0, V, (3, n)))
+    for s in range(3):
+        _put(gpu, stream, words, (s + 1) * cap - n, ids[s])
+    table = gpu.DeviceArray((2, cap), np.int32)
+    who = i32(rng.integers(-1, 4, (2, n)))
+    for r in range(2):
+        _put(gpu, stream, table, (r + 1) * cap - n, who[r])
+    rows = gpu.DeviceArray((1 << 29,), np.float32)           # bias at 0 and 2^29 - 128, mask words behind each
+    bias, bits = rng.standard_normal((2, V)).astype(np.float32), rng.random((2, 96)) < 0.7
+    step = (1 << 29) - 128
+    for i in range(2):
+        _put(gpu, stream, rows, i * step, np.concatenate([bias[i], np.packbits(bits[i], bitorder="little").view(np.float32)]))
+    x = rng.standard_normal((2, V)).astype(np.float32)
+    out, f = gpu.DeviceArray((2, V), np.float32), dev(gpu, np.float32([0.3, 0.4]), stream)
+    sets = View(rows, 0, (2, V), (step, 1))
+    keep = View(rows, V, (2, 3), (step, 1))
+    keep.dtype = np.dtype(np.uint32)
+    for by in ("slot", "table"):
+        where = dict(slot=dev(gpu, i32([2, 1]), stream)) if by == "slot" else dict(table=table)
+        gpu.LogitRules(dev(gpu, x, stream), out, tokens=words, length=dev(gpu, i32([cap, cap]), stream), window=n, frequency=f, bias=sets, mask=keep, **where)(stream)
+        got = out.numpy(stream)
+        for r in range(2):
+            s = np.full(n, [2, 1][r]) if by == "slot" else who[r]
+            fine = (s >= 0) & (s < 3)
+            counts = np.bincount(ids[s[fine], np.arange(n)[fine]], minlength=V)
+            check(got[r], *ref.rules(x[r], counts, 1, 0, [0.3, 0.4][r], bias[r], bits[r, :V]), False, f"far {by} {r}")
+
+
 # ---- rotary ---------------------------------------------------------------------
 ROTARY = [
     # type, R, n, heads, d, rot, interleaved, layout
@@ -308,6 +427,30 @@ def test_rotary_undone(gpu, stream):
         gpu.Rotary(f, [(d, d)], pos=dev(gpu, sign * p, stream))(stream)
     err = 2 * (9 * ref.U + 2.0 ** -51 * 1e5) * (np.abs(x[..., :32]) + np.abs(x[..., 32:])) * np.sqrt(2.0)
     assert (np.abs(d.numpy(stream) - x) <= np.concatenate([err, err], -1) * 1.01 + 2 * ref.U * np.abs(x)).all()
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("far", ["row", "token", "head"])
+def test_rotary_far(gpu, stream, type, far):
+    """Rows, tokens or heads 2^31 elements apart, in place and into packed ones."""
+    rng = np.random.default_rng(9)
+    dt, d, n, R, H = DT[type], 64, *{"row": (3, 2, 2), "token": (2, 2, 3), "head": (3, 2, 2)}[far]
+    step = {"row": (1 << 31, H * d, d), "token": (H * d, 1 << 31, d), "head": (n * d, d, 1 << 31)}[far]
+    big = gpu.DeviceArray(((1 << 31) + 4 * R * n * H * d,), dt)
+    x = rng.standard_normal((R, n, H, d)).astype(dt)
+    at = lambda r, i, h: r * step[0] + i * step[1] + h * step[2]  # noqa: E731
+    every = [(r, i, h) for r in range(R) for i in range(n) for h in range(H)]
+    for r, i, h in every:
+        _put(gpu, stream, big, at(r, i, h), x[r, i, h])
+    freq = 10000.0 ** (-np.arange(16) / 16)
+    v, packed, f, start = View(big, 0, x.shape, step), gpu.DeviceArray(x.shape, dt), dev(gpu, freq, stream), i32(np.arange(R) * 1000)
+    for dst in (packed, v):
+        gpu.Rotary(f, [(v, dst)], start=dev(gpu, start, stream))(stream)
+    got = packed.numpy(stream)
+    for r in range(R):
+        want, err = ref.rotary(x[r], start[r] + np.arange(n), freq, 32, False, 1.0)
+        check(got[r], want, err, type == "f16", f"far {far} {r}")
+    assert np.array_equal(np.stack([_get(gpu, stream, big, at(*e), (d,)) for e in every]).reshape(x.shape), got)
 
 
 # ---- rules on logits ------------------------------------------------------------
