@@ -452,25 +452,28 @@ template <typename YT, int TM, int TN> void launch_tiles(const LinearI8Params& p
 }
 
 // The form of the least estimated time: a start and, for each round of workgroups that the chip holds, an end and the
-// 1024s of K.  Fitted to products run back to back for 0.15 s (the card's clock is then 1.6 GHz for the large ones), us:
+// 1024s of K.  Fitted to products run back to back (0.15 s: the card's clock is then 1.6 GHz for the large ones), us:
 //                              16 x 16   32 x 128   64 x 128   64 x 256   128 x 256
-//      64 x  1024 x 4096          5.0       9.1       10.1
-//     128 x  4096 x 4096         12.7       8.1        9.5       15.0        27.5
-//     512 x  4096 x 4096                   17.0       15.2       18.2        29.6
-//    1000 x  4096 x 1024                               8.6        9.4        13.5
-//    2000 x  4096 x 1024                   19.4       15.5       14.9        15.7    (256 x 256, eight waves: 17.9)
-//    2000 x  4096 x 4096                              44.1       38.7        37.8                            42.1
-//   16384 x  4096 x 4096                  450        327        286         242                             245
-//    8192 x  8192 x 8192                             638        547         457                             450
+//      64 x  1024 x 4096          4.3       7.9        9.4       14.8        24.9
+//     128 x  4096 x 4096         19.6       8.1        9.5       15.0        27.4
+//     200 x  1024 x 1024          5.2       4.5        5.4        8.0        13.3
+//     512 x  4096 x 4096         72        16.7       14.9       18.2        29.6
+//    1000 x  4096 x 1024                    9.4        8.1        8.9        13.5
+//    2000 x  4096 x 1024                   18.9       14.8       13.9        15.1    (256 x 256, eight waves: 17.9)
+//    2000 x  4096 x 4096                   57.7       44.9       37.3        35.7                            42.1
+//   16384 x  4096 x 4096                  443        319        278         237                             245
+//    8192 x  8192 x 8192                  888        619        532         445                             450
+// Over 105 shapes of 32 to 16384 tokens, 40 of them not fitted to, the form taken is 1.2% slower than the best one on the mean, 26%
+// at most (1901 x 8099 x 426).
 template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s) {
     const float depth = p.K / 1024.0f;
     const auto rounds = [&](int bm, int bn, float held) { return (float)cdiv(p.M, bm) * cdiv(p.N, bn) / held; };
     const auto least = [](float r, float most) { return r > most ? r : most; };    // fewer workgroups take no less
-    const float units = rounds(16, 16, 256), rows = 3.0f + least(units, 0.8f) * 0.6f * depth;
-    const float t32 = 4.0f + least(rounds(32, 128, 256), 0.63f) * (0.45f + 1.5f * depth);
-    const float t64 = 4.0f + least(rounds(64, 128, 256), 1.0f) * (0.7f + 2.25f * depth);
-    const float wide64 = 4.0f + least(rounds(64, 256, 512), 0.41f) * (3.2f + 7.8f * depth);
-    const float wide128 = 5.0f + least(rounds(128, 256, 512), 0.4f) * (6.5f + 14.5f * depth);
+    const float units = rounds(16, 16, 256), rows = 2.65f + least(units, 0.85f) * (0.34f + 0.43f * depth);
+    const float t32 = 3.15f + least(rounds(32, 128, 256), 0.76f) * (0.22f + 1.72f * depth);
+    const float t64 = 3.74f + least(rounds(64, 128, 256), 0.77f) * (0.74f + 2.07f * depth);
+    const float wide64 = 4.26f + least(rounds(64, 256, 512), 0.4f) * (3.33f + 7.24f * depth);
+    const float wide128 = 5.98f + least(rounds(128, 256, 512), 0.45f) * (4.66f + 13.87f * depth);
     const float best = fminf(fminf(t32, t64), fminf(wide64, wide128));
     if (rows < best && units * 256 < (float)(1 << 21)) {
         const int mtiles = cdiv(p.M, 16);
