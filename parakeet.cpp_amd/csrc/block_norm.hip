@@ -20,11 +20,12 @@ namespace pkx {
 namespace {
 
 struct Moments { double s, t; };
+template <int T> constexpr int kWaves = T > 64 ? T / 64 : 1;     // of a row
 
 // Sums over the T lanes that share a row.
-template <int T> __device__ __forceinline__ Moments row_sum(Moments m, double (&part)[2 * (T / 64)]) {
-    m.s = wave_sum_f64(m.s);
-    m.t = wave_sum_f64(m.t);
+template <int T> __device__ __forceinline__ Moments row_sum(Moments m, double (&part)[2 * kWaves<T>]) {
+    m.s = lanes_sum_f64<T < 64 ? T : 64>(m.s);
+    m.t = lanes_sum_f64<T < 64 ? T : 64>(m.t);
     if constexpr (T > 64) {
         const int w = threadIdx.x % T >> 6;
         __syncthreads();                     // the last sums have been read
@@ -79,7 +80,7 @@ template <int T, int NV, int RUN> struct Part {
 // v becomes its norm: LayerNorm or RMS, times w, plus b (either may be missing).
 template <int T, int NV, int RUN>
 __device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const Part<T, NV, RUN>& w, const Part<T, NV, RUN>& b, float eps, float first, int t,
-                                          int d, double inv_d, double (&part)[2 * (T / 64)]) {
+                                          int d, double inv_d, double (&part)[2 * kWaves<T>]) {
     const bool layer = kind == NORM_LAYER;
     Moments m = {0, 0};
     if (layer) {
@@ -139,17 +140,18 @@ __device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const Par
             for (int e = 0; e < 8; ++e) v[k][e] += b.v[k][e];
 }
 
-// One row to T lanes: a wave up to 512 channels, two up to 1024, a workgroup beyond.
+// One row to T lanes: a quarter of a wave up to 128 channels, half of one up to 256, a wave up to 512, two up to 1024, a
+// workgroup beyond.
 template <typename ET, typename XT, bool I8, int T, int NV, bool EARLY>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(BlockNormParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1, RUN = sizeof(ET) == 2 ? 8 : 4;
-    __shared__ double part[kRows][2 * (T / 64)];
-    __shared__ float top_part[kRows][T / 64], x0[kRows];
+    __shared__ double part[kRows][2 * kWaves<T>];
+    __shared__ float top_part[kRows][kWaves<T>], x0[kRows];
     const int t = threadIdx.x % T, d = p.d;
-    const int mine = kRows > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / T) : 0;
+    const int mine = kRows == 1 ? 0 : T < 64 ? threadIdx.x / T : __builtin_amdgcn_readfirstlane(threadIdx.x / T);
     const int r = blockIdx.x * kRows + mine;
-    if (r >= p.rows) return;                 // whole waves: no barrier waits for them any more
-    double (&ps)[2 * (T / 64)] = part[mine];
+    if (r >= p.rows) return;                 // all lanes of a row; whole waves where there are barriers, which wait for them no more
+    double (&ps)[2 * kWaves<T>] = part[mine];
 
     // EARLY: everything that the row needs is asked for at once, which is what a few rows wait for (the kernel
     // alone, 1 x 4096 4.5 us, 4.8 with each vector read where it is used); many rows need the registers for more rows at a time
@@ -194,7 +196,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void block_norm_kernel(BlockNorm
     // the first element of x', for every lane
     float first = 0.f;
     if (p.pre == NORM_LAYER) {
-        if constexpr (T == 64) first = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x.v[0][0]), 0));
+        if constexpr (T < 64) first = __shfl(x.v[0][0], 0, T);
+        else if constexpr (T == 64) first = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x.v[0][0]), 0));
         else {
             if (t == 0) x0[mine] = x.v[0][0];
             __syncthreads();
@@ -246,11 +249,14 @@ template <typename ET, typename XT, bool I8, int T, int NV, bool EARLY> void lau
 // Early up to four waves a CU (512 x 1024, one block's two norms: 5.1 and 5.3 us; 2000 x 1024: 9.1 and 8.5).
 template <typename ET, typename XT, bool I8, int T, int NV> void launch_width(const BlockNormParams& p, hipStream_t s) {
     constexpr bool fits = T < 1024 || NV < 2;                    // the widest rows' weights would not fit the registers
-    if (fits && p.rows * (T / 64) <= 1024) launch_rows<ET, XT, I8, T, NV, fits>(p, s);
+    if (fits && p.rows * T <= 64 * 1024) launch_rows<ET, XT, I8, T, NV, fits>(p, s);
     else launch_rows<ET, XT, I8, T, NV, false>(p, s);
 }
+// Narrow rows, a head's for instance, share a wave: 32000 x 128 f16 6.4 us, a wave to each 18.9; 32000 x 256 20.8 and 25.1.
 template <typename ET, typename XT, bool I8> void launch_typed(const BlockNormParams& p, hipStream_t s) {
-    if (p.d <= 512) launch_width<ET, XT, I8, 64, 1>(p, s);
+    if (p.d <= 128) launch_width<ET, XT, I8, 16, 1>(p, s);
+    else if (p.d <= 256) launch_width<ET, XT, I8, 32, 1>(p, s);
+    else if (p.d <= 512) launch_width<ET, XT, I8, 64, 1>(p, s);
     else if (p.d <= 1024) launch_width<ET, XT, I8, 128, 1>(p, s);
     else if (p.d <= 2048) launch_width<ET, XT, I8, 256, 1>(p, s);
     else if (p.d <= 4096) launch_width<ET, XT, I8, 256, 2>(p, s);

@@ -103,24 +103,28 @@ template <int CTRL> __device__ __forceinline__ double dpp_get_f64(double v) {
     const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, 0xF, 0xF, false);
     return __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
 }
-// Sum over a whole wave, every lane active and receiving it.
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// Sum over the T = 16, 32 or 64 lanes that share a row, all of them active and receiving it (other rows' lanes need not be).
+template <int T> __device__ __forceinline__ double lanes_sum_f64(double v) {
     v += dpp_get_f64<0xB1>(v);
     v += dpp_get_f64<0x4E>(v);
     v += dpp_get_f64<0x141>(v);
     v += dpp_get_f64<0x140>(v);
-    return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
+    if constexpr (T == 16) return v;
+    const double a = readlane_f64(v, 0) + readlane_f64(v, 16), b = readlane_f64(v, 32) + readlane_f64(v, 48);
+    return T == 64 ? a + b : (threadIdx.x & 32) ? b : a;
 }
-__device__ __forceinline__ float wave_max_full(float v) {
+template <int T> __device__ __forceinline__ float lanes_max(float v) {
     v = fmaxf(v, dpp_get<0xB1>(v));
     v = fmaxf(v, dpp_get<0x4E>(v));
     v = fmaxf(v, dpp_get<0x141>(v));
     v = fmaxf(v, dpp_get<0x140>(v));
+    if constexpr (T == 16) return v;
     const int b = __builtin_bit_cast(int, v);
     const float r0 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0));
     const float r1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16));
     const float r2 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32));
     const float r3 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48));
+    if constexpr (T == 32) return (threadIdx.x & 32) ? fmaxf(r2, r3) : fmaxf(r0, r1);
     return fmaxf(fmaxf(r0, r1), fmaxf(r2, r3));
 }
 
@@ -151,13 +155,15 @@ template <int T, int NV> __device__ __forceinline__ RowTop row_top(const float (
     RowMax seen;
 #pragma unroll
     for (int k = 0; k < NV; ++k) seen.add(v[k]);
-    RowTop o{seen.top, __ballot(seen.odd != 0.f) == 0};
+    uint64_t odd = __ballot(seen.odd != 0.f);
+    if constexpr (T < 64) odd = odd >> (threadIdx.x & 63 & ~(T - 1)) & ((1ull << T) - 1);
+    RowTop o{seen.top, odd == 0};
     if (!o.plain) {
         o.top = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k) o.top = finite_max8(v[k], o.top);
     }
-    o.top = wave_max_full(o.top);
+    o.top = lanes_max<T < 64 ? T : 64>(o.top);
     if constexpr (T > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x % T >> 6] = o.plain ? o.top : -o.top;
         __syncthreads();

@@ -56,6 +56,8 @@ NORM = [
     ("f32", "f32", 2, 4097, "layer", "rms", 2, "linear"), ("f16", "f16", 3, 8192, "none", "layer", 1, "linear"),
     ("f32", "f32", 2, 8201, "layer", "layer", 1, "sigmoid"), ("f16", "f32", 2, 16383, "rms", "rms", 0, "linear"),
     ("f32", "f32", 2, 16384, "layer", "rms", 1, "linear"), ("f16", "f16", 1000, 257, "rms", "layer", 125, "sigmoid"),
+    ("f16", "f32", 37, 128, "layer", "layer", 5, "sigmoid"), ("f32", "f32", 18, 129, "layer", "rms", 1, "linear"), ("f16", "f16", 5003, 64, "none", "rms", 0, "linear"),
+    ("f16", "f16", 11, 256, "rms", "layer", 0, "linear"), ("f32", "f32", 2049, 150, "layer", "layer", 2049, "sigmoid"), ("f16", "f32", 6, 240, "layer", "layer", 1, "linear"),
 ]
 
 
@@ -116,11 +118,11 @@ def test_block_norm_parts(gpu, stream):
             check(h.numpy(stream), hh, eh, False, "h")
 
 
-def test_block_norm_hard_rows(gpu, stream):
+@pytest.mark.parametrize("d", [1500, 100, 200, 500])
+def test_block_norm_hard_rows(gpu, stream, d):
     """Rows of one value, of zeros, with a first element far out, of a mean 10^5 deviations away, of values whose squares pass f32,
     with a NaN or an infinity: each row by itself."""
     rng = np.random.default_rng(5)
-    d = 1500
     x = rng.standard_normal((8, d)).astype(np.float32)
     x[0], x[1] = 3.25, 0
     x[2, 0] = 1e6
