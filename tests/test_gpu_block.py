@@ -297,6 +297,80 @@ def test_far_rows(gpu, stream, type):
         check(got, *ref.rules(x[i], np.zeros(d), 1, 0, 0, bias[i], None), type == "f16", "far logits")
 
 
+def test_repeated_rows(gpu, stream):
+    """Inputs of stride 0 (one row for all, one head for all) and rows that overlap in what they are read from; names repeated."""
+    rng = np.random.default_rng(44)
+    M, d, N = 70, 200, 90
+    flat = rng.standard_normal(M + d).astype(np.float32)
+    base = dev(gpu, flat, stream)
+    one, slide = View(base, 0, (M, d), (0, 1)), View(base, 0, (M, d), (1, 1))
+    x1, xs = np.broadcast_to(flat[:d], (M, d)), np.stack([flat[i:i + d] for i in range(M)])
+    o, h = gpu.DeviceArray((M, d), np.float32), gpu.DeviceArray((M, d), np.float32)
+    gpu.BlockNorm(one, h, y=slide, x_out=o, gate=one, pre="layer")(stream)
+    r, er, hh, eh = ref.block_norm(x1, xs, x1, 1, "linear", 1.0, "none", None, None, "layer", None, None, 1e-5, 1e-5)
+    check(o.numpy(stream), r, er, False, "x_out")
+    check(h.numpy(stream), hh, eh, False, "h")
+    w, ws = rng.integers(-127, 128, (N, d)).astype(np.int8), rng.uniform(0.0005, 0.002, N).astype(np.float32)
+    wd = gpu.WeightI8(dev(gpu, w, stream), dev(gpu, ws, stream), stream)
+    for x, rows in ((one, x1), (slide, xs)):
+        for many in (M, 9):
+            y, v = gpu.DeviceArray((many, N), np.float32), View(base, 0, (many, d), x.strides)
+            gpu.LinearI8(v, wd, y, add=View(base, 3, (many, N), (0, 1)))(stream)
+            q, s = ref.quantised(rows[:many])
+            check(y.numpy(stream), *ref.linear_i8(q, s, w, ws, None, "none", 1.0, np.broadcast_to(flat[3:3 + N], (many, N))), False, "y")
+    f, out = dev(gpu, 10000.0 ** (-np.arange(16) / 16), stream), gpu.DeviceArray((2, 5, 3, 32), np.float32)
+    gpu.Rotary(f, [(View(base, 0, (2, 5, 3, 32), (7, 32, 0)), out)])(stream)
+    got = out.numpy(stream)
+    for i in range(2):
+        src = np.stack([np.broadcast_to(flat[7 * i + 32 * t:7 * i + 32 * t + 32], (3, 32)) for t in range(5)])
+        check(got[i], *ref.rotary(src, np.arange(5), 10000.0 ** (-np.arange(16) / 16), 32, False, 1.0), False, "turned")
+    words, out = i32(rng.integers(0, d, (2, 20))), gpu.DeviceArray((M, d), np.float32)
+    slot, freq = i32(np.arange(M) % 2), dev(gpu, np.full(M, 0.3, np.float32), stream)
+    gpu.LogitRules(one, out, tokens=dev(gpu, words, stream), length=dev(gpu, i32([20] * M), stream), slot=dev(gpu, slot, stream), frequency=freq,
+                   bias=View(base, 1, (M, d), (0, 1)), mask=View(dev(gpu, np.full(7, 0x5555FFFF, np.uint32), stream), 0, (M, 7), (0, 1)))(stream)
+    got = out.numpy(stream)
+    for r in range(M):
+        counts = np.bincount(words[slot[r]], minlength=d)
+        check(got[r], *ref.rules(x1[r], counts, 1, 0, np.float32(0.3), flat[1:1 + d], (0x5555FFFF >> (np.arange(d) % 32) & 1) != 0), False, f"rules {r}")
+
+
+def test_many_rows_graph(gpu, stream):
+    """The forms for many rows captured and replayed on changed inputs, against the same calls made directly on another stream between the replays."""
+    rng = np.random.default_rng(45)
+    M, D, N, other = 700, 1000, 900, gpu.Stream()
+    wd = gpu.WeightI8.quantize(dev(gpu, rng.standard_normal((N, D)).astype(np.float32), stream), stream)
+    freq = dev(gpu, gpu.rotary_frequencies(90), stream)
+    x = gpu.DeviceArray((M, D), np.float16)
+    sides = []
+    for _ in range(2):
+        q8, sc = gpu.DeviceArray((M, D), np.int8), gpu.DeviceArray((M,), np.float32)
+        h, y, z = (gpu.DeviceArray(s, np.float16) for s in ((M, D), (M, N), (M, N)))
+        heads = View(y, 0, (1, M, 10, 90), (M * N, N, 90))
+        calls = [gpu.BlockNorm(x, h, pre="layer"), gpu.LinearI8(h, wd, y), gpu.Rotary(freq, [(heads, heads)]), gpu.LogitRules(y, z), gpu.QuantizeRows(x, q8, sc)]
+        sides.append((calls, (h, y, z, q8, sc)))
+    x.upload(rng.standard_normal((M, D)).astype(np.float16), stream)
+    for c in sides[0][0] + sides[1][0]:
+        c(stream)
+    stream.sync()
+    hip, graph, ex = _hip(), C.c_void_p(), C.c_void_p()
+    assert hip.hipStreamBeginCapture(stream.handle, 1) == 0
+    for c in sides[0][0]:
+        c(stream)
+    assert hip.hipStreamEndCapture(stream.handle, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(ex), graph, None, None, 0) == 0
+    for step in range(3):
+        x.upload(rng.standard_normal((M, D)).astype(np.float16), stream)
+        stream.sync()
+        assert hip.hipGraphLaunch(ex, stream.handle) == 0
+        for c in sides[1][0]:
+            c(other)
+        stream.sync()
+        other.sync()
+        for a, b in zip(sides[0][1], sides[1][1]):
+            assert np.array_equal(a.numpy(stream), b.numpy(stream)), step
+    assert hip.hipGraphExecDestroy(ex) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
 @pytest.mark.parametrize("M,N", [(1100, 40), (2000, 4096)])
 def test_far_tokens_8bit(gpu, stream, M, N):
     """8-bit tokens of the largest stride, together past 4 GiB; few channels and tiles of them."""
