@@ -248,20 +248,22 @@ template <typename ET, typename XT, bool I8, int T, int NV, bool EARLY> void lau
 }
 // Early up to four waves a CU (512 x 1024, one block's two norms: 5.1 and 5.3 us; 2000 x 1024: 9.1 and 8.5).
 template <typename ET, typename XT, bool I8, int T, int NV> void launch_width(const BlockNormParams& p, hipStream_t s) {
-    constexpr bool fits = T < 1024 || NV < 2;                    // the widest rows' weights would not fit the registers
+    constexpr bool fits = NV <= 2;           // the widest rows' weights would not fit the registers
     if (fits && p.rows * T <= 64 * 1024) launch_rows<ET, XT, I8, T, NV, fits>(p, s);
     else launch_rows<ET, XT, I8, T, NV, false>(p, s);
 }
 // Narrow rows, a head's for instance, share a wave: 32000 x 128 f16 6.4 us, a wave to each 18.9; 32000 x 256 20.8 and 25.1.
+// Wide ones have eight waves (4000 x 8192 f16 113 us, 1000 x 16384 42; 16 waves 143 and 44); up to 4096 channels only while there are
+// few rows (1 x 3752 5.7 us, four waves 6.4; 8192 x 4090 f32 133 and 121).
 template <typename ET, typename XT, bool I8> void launch_typed(const BlockNormParams& p, hipStream_t s) {
     if (p.d <= 128) launch_width<ET, XT, I8, 16, 1>(p, s);
     else if (p.d <= 256) launch_width<ET, XT, I8, 32, 1>(p, s);
     else if (p.d <= 512) launch_width<ET, XT, I8, 64, 1>(p, s);
     else if (p.d <= 1024) launch_width<ET, XT, I8, 128, 1>(p, s);
     else if (p.d <= 2048) launch_width<ET, XT, I8, 256, 1>(p, s);
-    else if (p.d <= 4096) launch_width<ET, XT, I8, 256, 2>(p, s);
-    else if (p.d <= 8192) launch_width<ET, XT, I8, 1024, 1>(p, s);
-    else launch_width<ET, XT, I8, 1024, 2>(p, s);
+    else if (p.d <= 4096) p.rows <= 256 ? launch_width<ET, XT, I8, 512, 1>(p, s) : launch_width<ET, XT, I8, 256, 2>(p, s);
+    else if (p.d <= 8192) launch_width<ET, XT, I8, 512, 2>(p, s);
+    else launch_width<ET, XT, I8, 512, 4>(p, s);
 }
 
 }  // namespace

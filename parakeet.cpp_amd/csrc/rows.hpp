@@ -44,7 +44,13 @@ template <typename T> __device__ __forceinline__ void load_row8(float (&v)[8], c
         return;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = i + e < d ? (float)row[i + e] : 0.f;
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    if (i >= d) return;
+    T a[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) a[e] = row[i + e < d ? i + e : d - 1];       // the last one again: no branch for each
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = i + e < d ? (float)a[e] : 0.f;
 }
 template <typename T> __device__ __forceinline__ void store_row8(T* row, const float (&v)[8], int i, int d) {
     if (i + 8 <= d) {
