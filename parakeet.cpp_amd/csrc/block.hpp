@@ -58,6 +58,7 @@ struct LinearI8Params {
     bool y_f32 = false;
     const void* add = nullptr;  int64_t add_row = 0;
     void* y = nullptr;  int64_t y_row = 0;
+    bool lines = false;                  // y's rows begin at multiples of 64 bytes, set by the launch
 };
 void launch_linear_i8(const LinearI8Params& p, hipStream_t s);
 // The same from rows as they come, in one launch, for the few and short ones that linear_i8_fused() names.

@@ -111,7 +111,8 @@ template <typename YT> __device__ __forceinline__ float silu_of(float v) {
 }
 
 // What a lane needs of CNT channels from n0 < N on, for any number of tokens.  STREAM: y is written past the caches next to the
-// units, which keep tokens and weights for the tiles that follow (2000 x 4096 x 1024 15.9 -> 14.1 us on 128 x 256 of eight waves).
+// units, which keep tokens and weights for the tiles that follow (2000 x 4096 x 1024 16.4 -> 14.0 us), where its rows are whole lines:
+// else those caches join what two lanes write of a line (7662 x 4426 x 64 25 us, past them 38).
 template <typename YT, int CNT, bool STREAM> struct Channels {
     typedef YT vec __attribute__((ext_vector_type(CNT)));
     typedef vec vecu __attribute__((aligned(sizeof(YT))));
@@ -161,7 +162,7 @@ template <typename YT, int CNT, bool STREAM> struct Channels {
         vec o;
 #pragma unroll
         for (int e = 0; e < CNT; ++e) o[e] = (YT)v[e];
-        if (whole && STREAM) __builtin_nontemporal_store(o, (vecu*)y);
+        if (whole && STREAM && p.lines) __builtin_nontemporal_store(o, (vecu*)y);
         else if (whole) *(vecu*)y = o;
         else
 #pragma unroll
@@ -446,7 +447,8 @@ __global__ __launch_bounds__(256, 2) void i8_tile_kernel(LinearI8Params p, int m
     }
 }
 
-template <typename YT, int TM, int TN> void launch_tiles(const LinearI8Params& p, hipStream_t s) {
+template <typename YT, int TM, int TN> void launch_tiles(LinearI8Params p, hipStream_t s) {
+    p.lines = ((uintptr_t)p.y | (uintptr_t)(p.y_row * (int64_t)sizeof(YT))) % 64 == 0;
     const int mt = cdiv(p.M, 32 * TM), nt = cdiv(p.N, 128 * TN);
     launch(i8_tile_kernel<YT, TM, TN>, dim3(mt * nt), dim3(256), 0, s, p, mt, nt);
 }
