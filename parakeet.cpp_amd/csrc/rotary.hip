@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
         if constexpr (E == 8) store_row8(row, v, i, WHOLE ? i + 8 : d);
         else store_row4(row, v, i, WHOLE ? i + 4 : d);
     };
-    // at: an item's first pair, or -1 - its first element past rot; whole elements and pairs beyond an item's end are zeros
+    // at: an item's first pair, or -1 - its first element past rot; whole elements and pairs beyond a head's end are zeros
     float a[IT][E], b[IT][E] = {};
     const ET* src[IT];
     ET* dst[IT];
@@ -78,8 +78,9 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
             if (j0 + 256 * u >= all) dst[u] = nullptr;
             const bool other = at[u] < 0;
             if (other && src[u] == dst[u]) dst[u] = nullptr;
-            get(a[u], src[u] + (other ? p.rot : 0), other ? -1 - at[u] : INTER ? 2 * at[u] : at[u], other ? rest : INTER ? p.rot : pairs);
-            if (!INTER && !other) get(b[u], src[u] + pairs, at[u], pairs);
+            // what an item reads past its end is the same head's and goes nowhere; only the head's end is looked for
+            get(a[u], src[u] + (other ? p.rot : 0), other ? -1 - at[u] : INTER ? 2 * at[u] : at[u], other ? rest : p.dk);
+            if (!INTER && !other) get(b[u], src[u] + pairs, at[u], p.dk - pairs);
         }
     };
     auto turn_and_store = [&]() {
@@ -139,7 +140,7 @@ template <typename ET, bool INTER, bool WHOLE, int E, int IT> void launch_typed(
     launch(rotary_kernel<ET, INTER, WHOLE, E, IT>, dim3(p.R * most, p.parts), dim3(256), lds, s, p, most);
 }
 // Items of 16 bytes where head and pairs divide into them, of 8 for f16 where not, and of four elements with ends looked for in
-// any other case (4 x 4096 tokens x 20 heads x 80, 20 pairs of halves: 8 bytes 26.3 us, 16 with ends 37.8).
+// any other case (4 x 4096 tokens x 20 heads x 80, 20 pairs of halves: 8 bytes 26.1 us, 16 with ends 37.8; 10 pairs, with ends, 48).
 template <typename ET, bool INTER> void launch_items(const RotaryParams& p, hipStream_t s) {
     constexpr int E = 16 / sizeof(ET), IT = INTER ? 4 : 2;
     const int unit = INTER ? p.rot : p.rot / 2, rest = p.dk - p.rot;
