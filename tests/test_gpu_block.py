@@ -58,6 +58,8 @@ NORM = [
     ("f32", "f32", 2, 16384, "layer", "rms", 1, "linear"), ("f16", "f16", 1000, 257, "rms", "layer", 125, "sigmoid"),
     ("f16", "f32", 37, 128, "layer", "layer", 5, "sigmoid"), ("f32", "f32", 18, 129, "layer", "rms", 1, "linear"), ("f16", "f16", 5003, 64, "none", "rms", 0, "linear"),
     ("f16", "f16", 11, 256, "rms", "layer", 0, "linear"), ("f32", "f32", 2049, 150, "layer", "layer", 2049, "sigmoid"), ("f16", "f32", 6, 240, "layer", "layer", 1, "linear"),
+    ("f32", "f32", 1100, 500, "rms", "layer", 1, "linear"), ("f16", "f32", 600, 1000, "layer", "rms", 600, "sigmoid"), ("f32", "f32", 300, 1030, "layer", "layer", 0, "linear"),
+    ("f32", "f32", 300, 2100, "layer", "rms", 1, "linear"), ("f16", "f16", 257, 4096, "rms", "layer", 2, "linear"), ("f16", "f32", 140, 5001, "layer", "layer", 7, "sigmoid"),
 ]
 
 
