@@ -64,12 +64,14 @@ template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256
         }
 }
 
+// 4000 x 8192 f16 on 8 waves a row 16.7 us, on 16 25.6; 100 x 50000 11.8 and 9.4.
 template <typename ET> void launch_quantize_typed(const QuantizeRowsParams& p, hipStream_t s) {
     const unsigned rows = (unsigned)p.rows;
     if (p.d <= 512) launch(quantize_rows_kernel<ET, 64, 1>, dim3((rows + 3) / 4), dim3(256), 0, s, p);
     else if (p.d <= 1024) launch(quantize_rows_kernel<ET, 128, 1>, dim3((rows + 1) / 2), dim3(256), 0, s, p);
     else if (p.d <= 2048) launch(quantize_rows_kernel<ET, 256, 1>, dim3(rows), dim3(256), 0, s, p);
     else if (p.d <= 4096) launch(quantize_rows_kernel<ET, 256, 2>, dim3(rows), dim3(256), 0, s, p);
+    else if (p.d <= 8192) launch(quantize_rows_kernel<ET, 512, 2>, dim3(rows), dim3(512), 0, s, p);
     else launch(quantize_rows_kernel<ET, 1024, 2>, dim3(rows), dim3(1024), 0, s, p);
 }
 

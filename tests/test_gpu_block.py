@@ -147,7 +147,7 @@ def test_block_norm_hard_rows(gpu, stream, d):
 
 # ---- 8-bit rows and products ----------------------------------------------------
 @pytest.mark.parametrize("type", ["f16", "f32"])
-@pytest.mark.parametrize("M,n", [(1, 1), (5, 7), (3, 512), (9, 513), (2, 2048), (3, 2049), (2, 4100), (1, 16384), (2, 16385), (1, 50001), (2000, 24)])
+@pytest.mark.parametrize("M,n", [(1, 1), (5, 7), (3, 512), (9, 513), (2, 2048), (3, 2049), (2, 4100), (1, 16384), (2, 16385), (1, 50001), (2000, 24), (3, 8192), (2, 8193), (300, 5003)])
 def test_quantize_rows(gpu, stream, type, M, n):
     """Bit for bit, with NaN, infinities, rows of zeros and of subnormal values; what lies between the rows stays."""
     rng = np.random.default_rng(M + n)
