@@ -43,10 +43,11 @@ template <typename ET, bool INTER, bool WHOLE, int E, int IT>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
     extern __shared__ float2v turn[];        // [tok][rot / 2]
     const RotaryPart q = p.part[blockIdx.y];
-    const int r = udiv_small(blockIdx.x, most), i0 = (blockIdx.x - r * most) * q.tok;
+    const int r = udiv_small(blockIdx.x, most), block = blockIdx.x - r * most;
     int n = p.count ? p.count[r] : p.n;
     n = n > p.n ? p.n : n;
-    if (i0 >= n) return;
+    if ((int64_t)block * q.tok >= n) return;     // there are as many blocks as the part of the fewest tokens a block needs: past 2^31 of this one's
+    const int i0 = block * q.tok;
     const int toks = n - i0 < q.tok ? n - i0 : q.tok, pairs = p.rot / 2, rest = p.dk - p.rot;
     const int turned = INTER ? (p.rot + E - 1) / E : (pairs + E - 1) / E, items = turned + (rest + E - 1) / E, per = q.heads * items;
     const int all = toks * per;
