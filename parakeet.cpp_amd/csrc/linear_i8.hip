@@ -18,7 +18,8 @@ typedef int int16v __attribute__((ext_vector_type(16)));
 
 // ---- quantising rows -------------------------------------------------------
 // s = max |x| / 127 over the finite values, x held as clamp(round(x / s), -127, 127), each step one f32 operation.
-// A row is read once and kept in registers up to 8 T NV values; longer rows are read twice.  16384 x 4096 f16 (201 MB): 37 us,
+// A row is read once and kept in registers up to 8 T NV values; longer rows are read twice, counted in 64 bits (a lane's last step may end past
+// 2^31).  16384 x 4096 f16 (201 MB): 37 us,
 // 5.4 TB/s.
 template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256 : T) void quantize_rows_kernel(QuantizeRowsParams p) {
     constexpr int kRows = T < 256 ? 256 / T : 1;
@@ -36,9 +37,9 @@ template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256
     if (longer) {                            // only the longest rows' kernel: T > 64
         float w[1][8] = {}, m = 0.f;
         bool plain = true;
-        for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
+        for (int64_t i = 8 * (t + NV * T); i < d; i += 8 * T) {
             RowMax seen;
-            load_row8(w[0], x, i, d);
+            load_row8(w[0], x, (int)i, d);
             seen.add(w[0]);
             plain &= seen.odd == 0.f;
             m = finite_max8(w[0], m);
@@ -57,10 +58,10 @@ template <typename ET, int T, int NV> __global__ __launch_bounds__(T < 256 ? 256
 #pragma unroll
     for (int k = 0; k < NV; ++k) store_bytes8(q, held(v[k]), 8 * (t + k * T), d);
     if (longer)
-        for (int i = 8 * (t + NV * T); i < d; i += 8 * T) {
+        for (int64_t i = 8 * (t + NV * T); i < d; i += 8 * T) {
             float w[8];
-            load_row8(w, x, i, d);
-            store_bytes8(q, held(w), i, d);
+            load_row8(w, x, (int)i, d);
+            store_bytes8(q, held(w), (int)i, d);
         }
 }
 

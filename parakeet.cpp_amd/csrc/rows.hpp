@@ -37,9 +37,9 @@ __device__ __forceinline__ void store8u(float* p, const float (&v)[8]) {
     __builtin_nontemporal_store(b, (float4u*)(p + 4));
 }
 
-// Elements [i, i + 8) of a row of d; those past its end are 0 and are not read.
+// Elements [i, i + 8) of a row of d; those past its end are 0 and are not read.  d may be all that an int holds.
 template <typename T> __device__ __forceinline__ void load_row8(float (&v)[8], const T* row, int i, int d) {
-    if (i + 8 <= d) {
+    if (i <= d - 8) {
         load8u(v, row + i);
         return;
     }
@@ -228,7 +228,7 @@ struct RowQuantiser {
     }
 };
 __device__ __forceinline__ void store_bytes8(int8_t* row, int2v w, int i, int d) {
-    if (i + 8 <= d) {
+    if (i <= d - 8) {
         *(int2u*)(row + i) = w;
         return;
     }

@@ -25,3 +25,24 @@ def test_rotary_blocks_past_32_bits(gpu, stream):
     check(alone.numpy(stream)[0], want, err, True, "one head")
     want, err = ref.rotary(x, ends, freq, d, True, 1.0)
     check(np.stack([_get(gpu, stream, many, i * heads * d, (heads, d)) for i in ends]), want, err, True, "513 heads")
+
+
+def test_quantize_longest_row(gpu, stream):
+    """A row of 2^31 - 1 values, the last of them the largest: what a lane adds to its place past it is past 31 bits."""
+    n, step = (1 << 31) - 1, 1 << 26
+    rng = np.random.default_rng(51)
+    part = rng.uniform(-2, 2, step).astype(np.float16)
+    x, q, s = gpu.DeviceArray((1, n), np.float16), gpu.DeviceArray((1, n), np.int8), gpu.DeviceArray((1,), np.float32)
+    for at in range(0, n, step):
+        _put(gpu, stream, x, at, part[:min(step, n - at)])
+    _put(gpu, stream, x, n - 1, np.float16([-3]))
+    gpu.QuantizeRows(x, q, s)(stream)
+    scale = np.float32(3) / np.float32(127)
+    assert s.numpy(stream)[0] == scale
+    want = np.rint(part.astype(np.float32) / scale).astype(np.int8)
+    for at in range(0, n, step):
+        got = _get(gpu, stream, q, at, (min(step, n - at),))
+        if at + step >= n:
+            assert got[-1] == -127
+            got = got[:-1]
+        assert np.array_equal(got, want[:len(got)]), at
