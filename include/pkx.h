@@ -534,7 +534,7 @@ int pkx_i8_weight_pack(const int8_t* w, int64_t w_row, int n_out, int n_in, void
  * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22; every
  * row can be read to its next multiple of 16, and what it holds past n_in does not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows
  * does (x_scale NULL).  y and add are f32 or f16, and add may be y; y overlaps nothing else.  Strides in elements.
- * n_rows and n_out below 2^22. */
+ * n_rows and n_out below 2^22, n_rows * n_out below 2^36. */
 enum { PKX_TYPE_I8 = 24 };               /* ggml's number of its 8-bit integers */
 enum { PKX_ACT_NONE = 0, PKX_ACT_SILU = 1 };
 typedef struct {
@@ -552,6 +552,9 @@ typedef struct {
 } pkx_linear_i8_args;
 int pkx_linear_i8_workspace(const pkx_linear_i8_args* a, size_t* bytes);
 int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* stream);
+/* What a workgroup of the call's product takes, tokens x output channels (16 x 16, 32 x 128, 64 x 128, 64 x 256 or 128 x 256, by the sizes and
+ * whether x is in 8 bits), and how many workgroups there are; zeros for a call of size zero. */
+int pkx_linear_i8_tile(const pkx_linear_i8_args* a, int* tokens, int* channels, int64_t* workgroups);
 
 /* Rotary positions: token i < count[r] of row r is at position t = pos[r][i], or start[r] + i, and in every head of every part
  * the pair (a, b) of frequency j < rot / 2 becomes

@@ -64,6 +64,12 @@ void launch_linear_i8(const LinearI8Params& p, hipStream_t s);
 // The same from rows as they come, in one launch, for the few and short ones that linear_i8_fused() names.
 bool linear_i8_fused(int M, int N, int K);
 void launch_linear_i8_fused(const LinearI8Params& p, const QuantizeRowsParams& q, hipStream_t s);
+// What a workgroup of a call takes, and how many there are (16 x 16 on 512 threads, the others on 256).
+struct LinearI8Tile {
+    int tokens, channels;
+    int64_t workgroups;
+};
+LinearI8Tile linear_i8_tile(int M, int N, int K, bool i8);
 
 constexpr int kRotaryParts = 4, kMaxRotaryWidth = 512;
 struct RotaryPart {

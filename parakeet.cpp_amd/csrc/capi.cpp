@@ -1091,6 +1091,16 @@ int pkx_linear_i8_workspace(const pkx_linear_i8_args* a, size_t* bytes) {
         *bytes = i8_workspace(a);
     });
 }
+int pkx_linear_i8_tile(const pkx_linear_i8_args* a, int* tokens, int* channels, int64_t* workgroups) {
+    return guarded([&] {
+        need(tokens && channels && workgroups, "null argument");
+        const pkx::LinearI8Params p = linear_i8_params(a);
+        const pkx::LinearI8Tile t = pkx::linear_i8_tile(p.M, p.N, p.K, a->x_type == PKX_TYPE_I8);
+        *tokens = t.tokens;
+        *channels = t.channels;
+        *workgroups = t.workgroups;
+    });
+}
 int pkx_linear_i8(const pkx_linear_i8_args* a, void* ws, size_t ws_bytes, void* s) {
     return guarded([&] {
         pkx::LinearI8Params p = linear_i8_params(a);

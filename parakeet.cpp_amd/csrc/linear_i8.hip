@@ -470,22 +470,28 @@ template <typename YT, int TM, int TN> void launch_tiles(LinearI8Params p, hipSt
 //    8192 x  8192 x 8192                  888        619        532         445                             450
 // Over 105 shapes of 32 to 16384 tokens, 40 of them not fitted to, the form taken is 1.2% slower than the best one on the mean, 26%
 // at most (1901 x 8099 x 426).
-template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s) {
-    const float depth = p.K / 1024.0f;
-    const auto rounds = [&](int bm, int bn, float held) { return (float)cdiv(p.M, bm) * cdiv(p.N, bn) / held; };
+LinearI8Tile least_tile(int M, int N, int K) {
+    const float depth = K / 1024.0f;
+    const auto rounds = [&](int bm, int bn, float held) { return (float)cdiv(M, bm) * cdiv(N, bn) / held; };
     const auto least = [](float r, float most) { return r > most ? r : most; };    // fewer workgroups take no less
     const float units = rounds(16, 16, 256), rows = 2.65f + least(units, 0.85f) * (0.34f + 0.43f * depth);
-    const float t32 = 3.15f + least(rounds(32, 128, 256), 0.76f) * (0.22f + 1.72f * depth);
+    // a launch holds fewer than 2^32 threads; 2^36 results are fewer than that on the larger tiles
+    const bool small = (int64_t)cdiv(M, 32) * cdiv(N, 128) < 1 << 24;
+    const float t32 = small ? 3.15f + least(rounds(32, 128, 256), 0.76f) * (0.22f + 1.72f * depth) : __builtin_inff();
     const float t64 = 3.74f + least(rounds(64, 128, 256), 0.77f) * (0.74f + 2.07f * depth);
     const float wide64 = 4.26f + least(rounds(64, 256, 512), 0.4f) * (3.33f + 7.24f * depth);
     const float wide128 = 5.98f + least(rounds(128, 256, 512), 0.45f) * (4.66f + 13.87f * depth);
     const float best = fminf(fminf(t32, t64), fminf(wide64, wide128));
-    if (rows < best && units * 256 < (float)(1 << 21)) {
-        const int mtiles = cdiv(p.M, 16);
-        launch(i8_rows_kernel<YT>, dim3(2 * cdiv(p.N, 32) * mtiles), dim3(512), 0, s, p, mtiles);
-    } else if (wide128 == best) launch_tiles<YT, 4, 2>(p, s);
-    else if (wide64 == best) launch_tiles<YT, 2, 2>(p, s);
-    else if (t64 == best) launch_tiles<YT, 2, 1>(p, s);
+    if (rows < best && units * 256 < (float)(1 << 21)) return {16, 16, 2 * (int64_t)cdiv(N, 32) * cdiv(M, 16)};
+    const auto tile = [&](int bm, int bn) { return LinearI8Tile{bm, bn, (int64_t)cdiv(M, bm) * cdiv(N, bn)}; };
+    return wide128 == best ? tile(128, 256) : wide64 == best ? tile(64, 256) : t64 == best ? tile(64, 128) : tile(32, 128);
+}
+template <typename YT> void launch_typed(const LinearI8Params& p, hipStream_t s) {
+    const LinearI8Tile t = least_tile(p.M, p.N, p.K);
+    if (t.tokens == 16) launch(i8_rows_kernel<YT>, dim3((unsigned)t.workgroups), dim3(512), 0, s, p, cdiv(p.M, 16));
+    else if (t.tokens == 128) launch_tiles<YT, 4, 2>(p, s);
+    else if (t.channels == 256) launch_tiles<YT, 2, 2>(p, s);
+    else if (t.tokens == 64) launch_tiles<YT, 2, 1>(p, s);
     else launch_tiles<YT, 1, 1>(p, s);
 }
 
@@ -504,6 +510,11 @@ template <typename YT, typename XT> void launch_fused(const LinearI8Params& p, c
 
 }  // namespace
 
+LinearI8Tile linear_i8_tile(int M, int N, int K, bool i8) {
+    if (M == 0 || N == 0) return {0, 0, 0};
+    if (!i8 && linear_i8_fused(M, N, K)) return {16, 16, 2 * (int64_t)cdiv(N, 32) * cdiv(M, 16)};
+    return least_tile(M, N, K);
+}
 bool linear_i8_fused(int M, int N, int K) {
     const int kpad = cdiv(K, kI8DepthPad) * kI8DepthPad, rows = M < 16 ? M : 16;
     if (kpad > 4 * 512 * fused_waves(M) || rows * kpad > 16384) return false;

@@ -196,6 +196,7 @@ SIGS = {
     "pkx_i8_weight_pack": ([_vp, _i64, _i32, _i32, _vp, _vp], C.c_int),
     "pkx_linear_i8_workspace": ([_P(LinearI8Args), _P(_sz)], C.c_int),
     "pkx_linear_i8": ([_P(LinearI8Args), _vp, _sz, _vp], C.c_int),
+    "pkx_linear_i8_tile": ([_P(LinearI8Args), _P(_i32), _P(_i32), _P(_i64)], C.c_int),
     "pkx_rotary": ([_P(RotaryArgs), _vp], C.c_int),
     "pkx_rotary_frequencies": ([C.c_double, _i32] + [C.c_double] * 4 + [_P(C.c_double)], C.c_int),
     "pkx_logit_rules": ([_P(LogitRulesArgs), _vp], C.c_int),
@@ -930,6 +931,12 @@ class LinearI8(_Bound):
         a = LinearI8Args(TYPE_I8 if i8 else _type(x), _type(y), M, N, K, x.ptr, _row(x), _ptr(x_scale), w.packed.ptr, w.scale.ptr,
                          _ptr(bias), _kind(ACTS, act, "8-bit linear"), alpha, _ptr(add), _row(add), y.ptr, _row(y))
         self._bind("pkx_linear_i8", (C.byref(a),), (a, x, w, y, x_scale, bias, add), "pkx_linear_i8_workspace")
+
+    def tile(self):
+        """pkx_linear_i8_tile: (tokens, output channels) of a workgroup, and how many workgroups there are."""
+        m, n, count = _i32(), _i32(), _i64()
+        check(lib().pkx_linear_i8_tile(self._args[0], C.byref(m), C.byref(n), C.byref(count)))
+        return (m.value, n.value), count.value
 
 
 def rotary_frequencies(rot, base=10000.0, factor=1.0, context=0, low=1.0, high=32.0):
