@@ -23,3 +23,12 @@ print(tile(0, 5, 5), tile(5, 0, 5), L.pkx_linear_i8_tile(lin(), None, None, None
     assert len(out) == 8 * 6 * 3 + 1
     assert all(x.endswith("True") for x in out[:-1]), [x for x in out[:-1] if not x.endswith("True")]
     assert out[-1] == "(0, 0, 0) (0, 0, 0) 1 1"
+
+
+def test_linear_tiles_are_all_tested():
+    """The choice by sizes still sends each case of the GPU test to the tile that the case is there for, and no tile is without one."""
+    from test_gpu_block_edges import TILES as cases
+    sizes = [(c[2], c[3], c[4], {"i8": 24, "f": {"f16": 1, "f32": 0}[c[1]]}[c[9]]) for c in cases]
+    out = _run(TILES + "for a in " + repr(sizes) + ": print(tile(*a)[:2])")
+    assert out == [str(c[0]) for c in cases]
+    assert {(c[0], c[1]) for c in cases} == {(t, d) for t in ((32, 128), (64, 128), (64, 256), (128, 256)) for d in ("f16", "f32")}

@@ -46,3 +46,46 @@ def test_quantize_longest_row(gpu, stream):
             assert got[-1] == -127
             got = got[:-1]
         assert np.array_equal(got, want[:len(got)]), at
+
+
+# ---- the 8-bit product's tiles ---------------------------------------------------
+TILES = [
+    # tile, type, M, N, K (slabs of 128), act, bias, add, rows at whole lines, tokens
+    ((32, 128), "f16", 300, 1030, 1000, "silu", True, True, True, "i8"), ((32, 128), "f32", 1001, 1000, 260, "none", True, False, True, "f"),
+    ((64, 128), "f16", 2001, 1000, 700, "silu", True, True, True, "f"), ((64, 128), "f32", 2001, 1000, 700, "silu", True, True, False, "i8"),
+    ((64, 128), "f16", 700, 2050, 1100, "none", True, False, False, "i8"), ((64, 128), "f32", 1000, 6000, 384, "none", False, True, True, "f"),
+    ((64, 256), "f16", 2001, 3000, 1100, "silu", True, True, True, "f"), ((64, 256), "f16", 2001, 3000, 1100, "none", False, True, False, "i8"),
+    ((64, 256), "f32", 1000, 4099, 2040, "silu", True, True, True, "i8"), ((64, 256), "f32", 520, 6000, 2050, "none", True, False, False, "f"),
+    ((128, 256), "f16", 3000, 8200, 260, "silu", True, True, True, "f"), ((128, 256), "f16", 4100, 4099, 700, "none", True, True, False, "i8"),
+    ((128, 256), "f32", 2001, 6000, 1100, "silu", True, True, True, "i8"), ((128, 256), "f32", 4100, 3000, 1100, "none", False, True, False, "f"),
+    ((128, 256), "f32", 3000, 12300, 200, "silu", True, False, True, "f"), ((128, 256), "f16", 16400, 8200, 128, "none", True, False, True, "i8"),
+]
+
+
+@pytest.mark.parametrize("tile,type,M,N,K,act,bias,add,lines,tokens", TILES)
+def test_linear_i8_tiles(gpu, stream, tile, type, M, N, K, act, bias, add, lines, tokens):
+    """Every tile of the product, with rests in tokens, channels and inputs, even and odd numbers of slabs, results at whole lines and not: whole
+    rows of the first tiles, of the last ones and of some in between."""
+    print(f"[tiles] {tile} {type} M={M} N={N} K={K} {act} bias={bias} add={add} lines={lines} {tokens}", flush=True)
+    rng = np.random.default_rng(M + 3 * N + K + lines)
+    dt = np.dtype({"f16": np.float16, "f32": np.float32}[type])
+    w, ws = rng.integers(-127, 128, (N, K)).astype(np.int8), rng.uniform(0.0005, 0.002, N).astype(np.float32)
+    b = rng.standard_normal(N).astype(np.float32) if bias else None
+    row = -(-N * dt.itemsize // 64) * 64 // dt.itemsize + (64 // dt.itemsize if lines else 3)
+    a = rng.standard_normal((M, N)).astype(dt) if add else None
+    y = dev(gpu, np.full((M, row), 5, dt), stream)
+    kw = dict(bias=dev(gpu, b, stream), act=act, add=dev(gpu, a, stream), alpha=-0.75 if add else 1.0)
+    wd, vy = gpu.WeightI8(dev(gpu, w, stream), dev(gpu, ws, stream), stream), View(y, 0, (M, N), (row, 1))
+    if tokens == "f":
+        x = rng.standard_normal((M, K)).astype(dt)
+        call = gpu.LinearI8(dev(gpu, x, stream), wd, vy, **kw)
+    else:
+        x, s = rng.integers(-128, 128, (M, (K + 15) // 16 * 16 + 16)).astype(np.int8), rng.uniform(0.001, 0.05, M).astype(np.float32)
+        call = gpu.LinearI8(View(dev(gpu, x, stream), 0, (M, K), (x.shape[1], 1)), wd, vy, x_scale=dev(gpu, s, stream), **kw)
+    assert call.tile()[0] == tile
+    call(stream)
+    got, r = y.numpy(stream), np.unique(np.r_[0:40, 60:70, 126:130, rng.integers(0, M, 40), M - 140:M])
+    q, s = ref.quantised(x[r]) if tokens == "f" else (x[r, :K], s[r])
+    want, err = ref.linear_i8(q, s, w, ws, b, act, kw["alpha"], a[r] if add else None, type == "f16")
+    check(got[r, :N], want, err, type == "f16", "y")
+    assert (got[:, N:] == 5).all()
