@@ -89,3 +89,55 @@ def test_linear_i8_tiles(gpu, stream, tile, type, M, N, K, act, bias, add, lines
     want, err = ref.linear_i8(q, s, w, ws, b, act, kw["alpha"], a[r] if add else None, type == "f16")
     check(got[r, :N], want, err, type == "f16", "y")
     assert (got[:, N:] == 5).all()
+
+
+# ---- forms that larger or odder sizes take ---------------------------------------
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("R,V,table", [(1100, 70, True), (350, 8193, False), (130, 40001, True)])
+def test_logit_rules_many_rows(gpu, stream, type, R, V, table):
+    """More than 1024 tiles of 4096 words: tiles of up to 8192, one and several of them to a row; in place."""
+    rng = np.random.default_rng(R + V)
+    dt, cap, slots = {"f16": np.float16, "f32": np.float32}[type], 90, 40
+    x = (4 * rng.standard_normal((R, V))).astype(dt)
+    words = rng.integers(-1, V + 1, (slots, cap)).astype(np.int32)
+    words[:, :6] = 0, V - 1, min(V - 1, 4095), min(V - 1, 4096), min(V - 1, 8191), min(V - 1, 8192)
+    lens, slot, tab = (rng.integers(a, b, s).astype(np.int32) for a, b, s in ((0, cap + 2, R), (0, slots, R), (-1, slots + 1, (R, cap))))
+    rep, pres, freq = (rng.uniform(a, b, R).astype(np.float32) for a, b in ((0.5, 2), (-0.5, 1), (0, 0.3)))
+    bias, keep = rng.standard_normal((3, V)).astype(np.float32), rng.random((2, (V + 31) // 32 * 32)) < 0.5
+    bi, mi = rng.integers(-1, 4, R).astype(np.int32), rng.integers(-1, 3, R).astype(np.int32)
+    d = {k: dev(gpu, v, stream) for k, v in dict(tokens=words, length=lens, repetition=rep, presence=pres, frequency=freq, bias=bias, bias_index=bi, mask_index=mi,
+                                                 mask=np.packbits(keep, axis=1, bitorder="little").view(np.uint32), **(dict(table=tab) if table else dict(slot=slot))).items()}
+    y = dev(gpu, x, stream)
+    gpu.LogitRules(y, y, **d)(stream)
+    got = y.numpy(stream).astype(np.float64)
+    for r in range(R):
+        n = min(int(lens[r]), cap)
+        s, t = tab[r, :n] if table else np.full(n, slot[r]), np.arange(n)
+        fine = (s >= 0) & (s < slots)
+        ids = words[s[fine], t[fine]]
+        counts = np.bincount(ids[(ids >= 0) & (ids < V)], minlength=V)
+        want, err = ref.rules(x[r], counts, rep[r], pres[r], freq[r], bias[bi[r]] if 0 <= bi[r] < 3 else None, keep[mi[r], :V] if 0 <= mi[r] < 2 else None)
+        kept = np.isfinite(want)
+        assert np.array_equal(got[r][~kept], want[~kept]), r
+        assert (np.abs(got[r][kept] - want[kept]) <= ref.rounded(err[kept], want[kept], type == "f16")).all(), r
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("type,d,rot", [("f16", 80, 40), ("f16", 20, 12), ("f16", 24, 8), ("f16", 88, 88), ("f16", 100, 20), ("f32", 80, 20), ("f32", 12, 8), ("f16", 128, 0), ("f16", 26, 26)])
+@pytest.mark.parametrize("place", ["apart", "in place"])
+def test_rotary_pieces(gpu, stream, type, d, rot, inter, place):
+    """Pairs and rests that divide by eight, by four and by neither, several tokens to a workgroup, two parts."""
+    rng = np.random.default_rng(d + rot)
+    dt, n, R, heads = {"f16": np.float16, "f32": np.float32}[type], 43, 2, (5, 1)
+    x = rng.standard_normal((R, n, 6, d)).astype(dt)
+    freq = 10000.0 ** (-np.arange(rot // 2) * 2 / max(rot, 1))
+    src, f = dev(gpu, x, stream), dev(gpu, freq if rot else np.zeros(1), stream)
+    out = src if place == "in place" else dev(gpu, np.full(x.shape, 3, dt), stream)
+    part = lambda a, h0, H: View(a, h0 * d, (R, n, H, d), (n * 6 * d, 6 * d, d))  # noqa: E731
+    gpu.Rotary(View(f, 0, (rot // 2,), (1,)), [(part(src, 0, 5), part(out, 0, 5)), (part(src, 5, 1), part(out, 5, 1))], start=dev(gpu, np.int32([3, 70000]), stream),
+               interleaved=inter, mult=0.5)(stream)
+    got = out.numpy(stream)
+    for r, p in enumerate((3, 70000)):
+        want, err = ref.rotary(x[r], p + np.arange(n), freq, rot, inter, 0.5)
+        check(got[r], want, err, type == "f16", f"row {r}")
+    assert np.array_equal(got[..., rot:], x[..., rot:])
