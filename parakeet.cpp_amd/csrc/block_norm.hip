@@ -261,7 +261,7 @@ template <typename ET, typename XT, bool I8> void launch_typed(const BlockNormPa
     else if (p.d <= 512) launch_width<ET, XT, I8, 64, 1>(p, s);
     else if (p.d <= 1024) launch_width<ET, XT, I8, 128, 1>(p, s);
     else if (p.d <= 2048) launch_width<ET, XT, I8, 256, 1>(p, s);
-    else if (p.d <= 4096) p.rows <= 256 ? launch_width<ET, XT, I8, 512, 1>(p, s) : launch_width<ET, XT, I8, 256, 2>(p, s);
+    else if (p.d <= 4096) p.rows <= 256 ? launch_width<ET, XT, I8, 512, 1>(p, s) : launch_rows<ET, XT, I8, 256, 2, false>(p, s);     // past four waves a CU
     else if (p.d <= 8192) launch_width<ET, XT, I8, 512, 2>(p, s);
     else launch_width<ET, XT, I8, 512, 4>(p, s);
 }

@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import block_ref as ref
+import test_gpu_block as norm_rows
 from test_gpu_block import View, _get, _put, check, dev
 
 pytestmark = pytest.mark.gpu
@@ -141,3 +142,13 @@ def test_rotary_pieces(gpu, stream, type, d, rot, inter, place):
         want, err = ref.rotary(x[r], p + np.arange(n), freq, rot, inter, 0.5)
         check(got[r], want, err, type == "f16", f"row {r}")
     assert np.array_equal(got[..., rot:], x[..., rot:])
+
+
+# ---- block norm -----------------------------------------------------------------
+@pytest.mark.parametrize("M,d", [(128, 2049), (129, 2049), (200, 4096), (256, 3001), (257, 2500)])
+@pytest.mark.parametrize("type,xtype,post,pre,per,fn", [("f16", "f32", "layer", "rms", 7, "sigmoid"), ("f32", "f32", "rms", "layer", 0, "linear"),
+                                                       ("f16", "f16", "none", "layer", 1, "linear")])
+@pytest.mark.parametrize("i8", [False, True])
+def test_block_norm_hundreds_of_rows(gpu, stream, type, xtype, post, pre, per, fn, M, d, i8):
+    """Rows of 2049 to 4096 channels around the numbers of them at which the form changes."""
+    norm_rows.test_block_norm(gpu, stream, type, xtype, M, d, post, pre, per, fn, i8)
