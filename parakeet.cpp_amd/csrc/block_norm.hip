@@ -114,7 +114,7 @@ __device__ __forceinline__ void normalise(float (&v)[NV][8], int kind, const Par
     const double var = m.t * inv_d - mu * mu + (double)eps;
     // 1 / sqrt(var): v_rsq_f64 is good to 2^-24 or so, a Newton step squares that
     double r = __builtin_amdgcn_rsq(var);
-    r = r * (1.5 - 0.5 * var * r * r);
+    r = var < __builtin_inf() ? r * (1.5 - 0.5 * var * r * r) : r;     // of an infinite one 0, which the step would make NaN
     const float inv = (float)r;
     if (layer) {
         const double mean = (double)first + mu;

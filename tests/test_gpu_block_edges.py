@@ -152,3 +152,22 @@ def test_rotary_pieces(gpu, stream, type, d, rot, inter, place):
 def test_block_norm_hundreds_of_rows(gpu, stream, type, xtype, post, pre, per, fn, M, d, i8):
     """Rows of 2049 to 4096 channels around the numbers of them at which the form changes."""
     norm_rows.test_block_norm(gpu, stream, type, xtype, M, d, post, pre, per, fn, i8)
+
+
+@pytest.mark.parametrize("d", [100, 200, 500, 1000, 1500, 3000, 16000])
+def test_block_norm_infinite_rows(gpu, stream, d):
+    """RMS of a row with an infinity: over an infinite root, 0 where the row is finite (its bias then) and NaN at the infinity; a block's output with
+    one leaves the other channels of the residual as they were."""
+    rng = np.random.default_rng(d)
+    x, b = rng.standard_normal((3, d)).astype(np.float32), rng.standard_normal(d).astype(np.float32)
+    x[0, 7], x[2, [1, d - 1]] = np.inf, -np.inf
+    lost = np.isinf(x)
+    h = gpu.DeviceArray(x.shape, np.float32)
+    gpu.BlockNorm(dev(gpu, x, stream), h, pre="rms", pre_b=dev(gpu, b, stream))(stream)
+    got = h.numpy(stream)
+    check(got[1:2], *ref.normalised(x[1:2].astype(np.float64), np.zeros((1, d)), "rms", None, b, 1e-5), False, "finite row")
+    assert np.isnan(got[lost]).all() and all(np.array_equal(got[r][~lost[r]], b[~lost[r]]) for r in (0, 2))
+    s, o = rng.standard_normal((3, d)).astype(np.float32), gpu.DeviceArray(x.shape, np.float32)
+    gpu.BlockNorm(dev(gpu, s, stream), y=dev(gpu, x.astype(np.float16), stream), x_out=o, post="rms")(stream)
+    got = o.numpy(stream)
+    assert np.isnan(got[lost]).all() and all(np.array_equal(got[r][~lost[r]], s[r][~lost[r]]) for r in (0, 2))
