@@ -171,3 +171,21 @@ def test_block_norm_infinite_rows(gpu, stream, d):
     gpu.BlockNorm(dev(gpu, s, stream), y=dev(gpu, x.astype(np.float16), stream), x_out=o, post="rms")(stream)
     got = o.numpy(stream)
     assert np.isnan(got[lost]).all() and all(np.array_equal(got[r][~lost[r]], s[r][~lost[r]]) for r in (0, 2))
+
+
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("d", [100, 200, 500, 1000, 1500, 3000, 16000])
+def test_block_norm_ends_of_f32(gpu, stream, kind, d):
+    """Rows whose values lie further apart than f32 reaches, rows at its end and rows of subnormal values without an eps."""
+    rng = np.random.default_rng(d)
+    x = rng.standard_normal((8, d)).astype(np.float32)
+    x[0], x[0, d // 2] = -2e38, 2e38
+    x[1] = np.where(np.arange(d) % 2, 1, -1) * np.float32(3.4e38)
+    x[2] = np.where(np.arange(d) % 3, 1, -0.9) * np.float32(3.4e38)
+    x[3] *= np.float32(1e37)
+    x[4] *= np.float32(1e-40)
+    x[5] = np.arange(d) % 2 * np.float32(1.5e-45)
+    x[6] *= np.float32(1e-36)
+    h = gpu.DeviceArray(x.shape, np.float32)
+    gpu.BlockNorm(dev(gpu, x, stream), h, pre=kind, eps=0)(stream)
+    check(h.numpy(stream), *ref.normalised(x.astype(np.float64), np.zeros(x.shape), kind, None, None, 0.0), False, kind)
