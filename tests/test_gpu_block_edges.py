@@ -189,3 +189,16 @@ def test_block_norm_ends_of_f32(gpu, stream, kind, d):
     h = gpu.DeviceArray(x.shape, np.float32)
     gpu.BlockNorm(dev(gpu, x, stream), h, pre=kind, eps=0)(stream)
     check(h.numpy(stream), *ref.normalised(x.astype(np.float64), np.zeros(x.shape), kind, None, None, 0.0), False, kind)
+
+
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_silu_to_the_end_of_f32(gpu, stream, M):
+    """SiLU of values whose e^-v passes f32 while v e^v is still a normal number, and of those on both sides."""
+    v = np.r_[np.linspace(-95, -80, 301), np.linspace(-45, -38, 141), np.linspace(-4, 4, 61)].astype(np.float32)
+    wd = gpu.WeightI8(dev(gpu, np.zeros((len(v), 16), np.int8), stream), dev(gpu, np.ones(len(v), np.float32), stream), stream)
+    y = gpu.DeviceArray((M, len(v)), np.float32)
+    gpu.LinearI8(dev(gpu, np.ones((M, 16), np.float32), stream), wd, y, bias=dev(gpu, v, stream), act="silu")(stream)
+    got, x = y.numpy(stream), v.astype(np.float64)
+    want = x / (1 + np.exp(-x))
+    for r in (0, M // 2, M - 1):
+        check(got[r], want, np.abs(want) * 6 * ref.U + 2.0 ** -126, False, f"row {r}")       # what is below the normal numbers may be 0
