@@ -19,9 +19,10 @@ template <typename T, int E> struct Piece {
 
 // One workgroup per row and tile of at most WORDS words (`width`, a multiple of 32).  The chain is length, table, tokens,
 // counts; logits, biases and mask are asked for behind the table's entries and used when the counts are there, and no
-// barrier waits for them.  What V leaves past whole pieces of 16 bytes goes to one thread a word.  A row's tiles, and the beams
-// that share its history, run on one XCD, whose L2 then reads a history and a bias row once: 512 rows x 32769 f32, the last 1024 of
-// 4096 tokens, 27.2 us (34.8 with the tiles dealt over the XCDs; 4.9 TB/s of logits read and written, a copy's rate).
+// barrier waits for them (__syncthreads() waits for LDS alone).  What V leaves past whole pieces of 16 bytes goes to one thread
+// a word.  A row's tiles, and the beams that share its history, run on one XCD, whose L2 then reads a history and a bias row once:
+// 512 rows x 32769 f32, the last 1024 of 4096 tokens, 27.2 us (34.8 with the tiles dealt over the XCDs; 4.9 TB/s of logits read and
+// written, a copy's rate).
 constexpr int kRuleThreads = 512;
 template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) void logit_rules_kernel(LogitRulesParams p, int tiles, int width) {
     constexpr int T = kRuleThreads, E = 16 / sizeof(ET), NV = WORDS / (T * E);     // neighbouring lanes', neighbouring pieces
@@ -89,7 +90,7 @@ template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) voi
     if (count) {
 #pragma unroll
         for (int k = 0; k < WORDS / (4 * T); ++k) *(int4v*)(times + 4 * (t + k * T)) = int4v{0, 0, 0, 0};
-        lds_barrier();
+        __syncthreads();
         for (int i0 = from + t; i0 < n;) {
             int word[U];
 #pragma unroll
@@ -103,7 +104,7 @@ template <typename ET, int WORDS> __global__ __launch_bounds__(kRuleThreads) voi
                 if (word[u] >= 0 && w < (unsigned)words) atomicAdd(&times[w], 1u);
             }
         }
-        lds_barrier();
+        __syncthreads();
     }
     auto ruled = [&](float y, uint32_t c, float add, bool keep) {
         if (c) y = (y > 0.f ? y / rep : y * rep) - pres - freq * (float)c;

@@ -90,14 +90,6 @@ template <typename T> __device__ __forceinline__ void store_row4(T* row, const f
         if (i + e < d) row[i + e] = (T)v[e];
 }
 
-// A barrier for what a workgroup shares in LDS: it waits for no load that is on its way to a register, as __syncthreads does.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xF | (0x3 << 14) | (0x7 << 4));
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
 __device__ __forceinline__ double readlane_f64(double v, int lane) {
     const long long b = __builtin_bit_cast(long long, v);
     const unsigned lo = __builtin_amdgcn_readlane((int)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
