@@ -530,10 +530,12 @@ int pkx_quantize_rows(int type, const void* x, int64_t x_row, int64_t n_rows, in
 int pkx_i8_weight_bytes(int n_out, int n_in, size_t* bytes);
 int pkx_i8_weight_pack(const int8_t* w, int64_t w_row, int n_out, int n_in, void* packed, void* stream);
 
-/* y[m][n] = add[m][n] + alpha * act(x_scale[m] * w_scale[n] * sum over k of x[m][k] w[n][k] + bias[n]), the sums exact.
- * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22; every
- * row can be read to its next multiple of 16, and what it holds past n_in does not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows
- * does (x_scale NULL).  y and add are f32 or f16, and add may be y; y overlaps nothing else.  Strides in elements.
+/* y[m][n] = add[m][n] + alpha * act(x_scale[m] * w_scale[n] * sum over k of x[m][k] w[n][k] + bias[n]), the sums exact, the product of the
+ * scales and everything after the sums f32.
+ * x in 8 bits with its scales (PKX_TYPE_I8: rows 16-byte aligned, x_row a multiple of 16 and at least n_in, below 2^22; everything from
+ * the first row's beginning to the last row's next multiple of 16 can be read, also between rows, and what it holds past n_in does
+ * not matter), or as f32 / f16, quantised within the call as pkx_quantize_rows does (x_scale NULL).
+ * y and add are f32 or f16, and add may be y; y overlaps nothing else.  Strides in elements.
  * n_rows and n_out below 2^22, n_rows * n_out below 2^36. */
 enum { PKX_TYPE_I8 = 24 };               /* ggml's number of its 8-bit integers */
 enum { PKX_ACT_NONE = 0, PKX_ACT_SILU = 1 };
