@@ -3,7 +3,9 @@
 //   u = post(y), x' = x + alpha g u, h = pre(x').
 // Bytes bound: x, y and the gate are read once, x' and h written once, the row
 // stays in registers in between.  8192 x 4090 f32 with a gate row for each (670 MB): 121 us,
-// 5.5 TB/s.  2000 x 1024 f16 with an f32 stream (25 MB): 7.4 us.
+// 5.5 TB/s.  2000 x 1024 f16 with an f32 stream (25 MB): 7.6 us, 3.2 TB/s, where a copy of them takes
+// 4.1: a row's vectors are asked for one behind the other (each is converted to f32 where it is loaded), and its second norm's weights wait
+// for x's stores.
 //
 // Moments are summed in f64 about the row's first element c: with s = sum (v - c)
 // and t = sum (v - c)^2, mean = c + s / d and var = t / d - (s / d)^2.  c belongs
@@ -266,7 +268,8 @@ template <typename ET, typename XT, bool I8, int T, int NV> void launch_width(co
     if (fits && p.rows * T <= 64 * 1024) launch_rows<ET, XT, I8, T, NV, fits>(p, s);
     else launch_rows<ET, XT, I8, T, NV, false>(p, s);
 }
-// Narrow rows, a head's for instance, share a wave: 32000 x 128 f16 6.4 us, a wave to each 18.9; 32000 x 256 20.8 and 25.1.
+// Narrow rows, a head's for instance, share a wave.  Residual and RMS norm of f16 operands, a stream in f16 / in f32: 32000 x 128
+// 7.4 / 10.3 us, a wave to each 18.4 / 18.4; 32000 x 256 12.2 / 17.1 and 18.8 / 21.7.
 // Wide ones have eight waves (4000 x 8192 f16 113 us, 1000 x 16384 42; 16 waves 143 and 44); up to 4096 channels only while there are
 // few rows (1 x 3752 5.7 us, four waves 6.4; 8192 x 4090 f32 133 and 121).
 template <typename ET, typename XT, bool I8> void launch_typed(const BlockNormParams& p, hipStream_t s) {

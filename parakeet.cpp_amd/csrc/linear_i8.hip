@@ -183,7 +183,7 @@ template <typename YT, int CNT, bool STREAM> struct Channels {
 // block (a wave reads 1 KB of weights and 1 KB of tokens per block, straight into
 // the fragments, four blocks at a time) and the partial sums joined through LDS.
 // 64 tokens to a workgroup read the weights once instead of four times, but are fewer workgroups: 64 x 1024 x 4096
-// 9.7 us instead of 4.8.  1 x 8192 x 8192: 11.2 us, 67 MB at 6 TB/s.
+// 9.7 us instead of 4.8 (64 of them; with more channels, and so more workgroups, it was not measured).  1 x 8192 x 8192: 11.2 us, 67 MB at 6 TB/s.
 constexpr int kRowWaves = 8;
 template <typename YT>
 __device__ __forceinline__ void rows_finish(const LinearI8Params& p, int4v acc, int4v (&part)[kRowWaves][64], int nh, int m0, const float* xs) {
@@ -472,8 +472,9 @@ template <typename YT, int TM, int TN> void launch_tiles(LinearI8Params p, hipSt
 //    2000 x  4096 x 4096                   57.7       44.9       37.3        35.7                            42.1
 //   16384 x  4096 x 4096                  443        319        278         237                             245
 //    8192 x  8192 x 8192                  888        619        532         445                             450
-// Over 105 shapes of 32 to 16384 tokens, 40 of them not fitted to, the form taken is 1.2% slower than the best one on the mean, 26%
-// at most (1901 x 8099 x 426).
+// Over 63 shapes that it was fitted to the form taken is 0.4% slower than the best one on the mean (12% at most), over 40 others 2.8%
+// (26%: 1901 x 8099 x 426; 21%: 7384 x 831 x 4723).  None has weights above 18 MB, and the estimate knows neither their bytes nor that a
+// unit's second tile is a whole one: it says 13.8 us of 64 x 8192 x 8192, which takes 21.5, and 20.9 of 4223 x 1024 x 4096, 30.4.
 LinearI8Tile least_tile(int M, int N, int K) {
     const float depth = K / 1024.0f;
     const auto rounds = [&](int bm, int bn, float held) { return (float)cdiv(M, bm) * cdiv(N, bn) / held; };
