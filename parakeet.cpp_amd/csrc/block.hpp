@@ -76,7 +76,7 @@ struct RotaryPart {
     const void* src;  int64_t s_row, s_tok, s_head;
     void* dst;        int64_t d_row, d_tok, d_head;
     int heads;
-    int tok = 1;                          // tokens of a workgroup, set by the launch
+    int tok = 1, blocks = 1;              // tokens of a workgroup, workgroups of a row: set by the launch
 };
 struct RotaryParams {
     bool f32 = false;

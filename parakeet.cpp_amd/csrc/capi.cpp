@@ -1179,7 +1179,7 @@ int pkx_rotary(const pkx_rotary_args* a, void* s) {
             dst.emplace_back(x.dst, (int64_t)a->d_head * e, std::initializer_list<std::pair<int64_t, int64_t>>{{x.dst_row * e, R}, {x.dst_tok * e, n}, {x.dst_head * e, x.n_heads}});
             need(src.back().bytes() < 0x1p62 && dst.back().bytes() < 0x1p62, "rotary: strides past the address space");
             pkx::RotaryPart& o = p.part[p.parts++];
-            o = pkx::RotaryPart{x.src, x.src_row, x.src_tok, x.src_head, x.dst, x.dst_row, x.dst_tok, x.dst_head, x.n_heads, 1};
+            o = pkx::RotaryPart{x.src, x.src_row, x.src_tok, x.src_head, x.dst, x.dst_row, x.dst_tok, x.dst_head, x.n_heads};
         }
         for (size_t i = 0; i < dst.size(); ++i) {
             for (size_t j = 0; j < dst.size(); ++j) {

@@ -44,10 +44,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryParams p, int most) {
     extern __shared__ float2v turn[];        // [tok][rot / 2]
     const RotaryPart q = p.part[blockIdx.y];
     const int r = udiv_small(blockIdx.x, most), block = blockIdx.x - r * most;
+    if (block >= q.blocks) return;           // another part, of fewer tokens a block, has more; past them i0 would pass 32 bits
+    const int i0 = block * q.tok;
     int n = p.count ? p.count[r] : p.n;
     n = n > p.n ? p.n : n;
-    if ((int64_t)block * q.tok >= n) return;     // there are as many blocks as the part of the fewest tokens a block needs: past 2^31 of this one's
-    const int i0 = block * q.tok;
+    if (i0 >= n) return;
     const int toks = n - i0 < q.tok ? n - i0 : q.tok, pairs = p.rot / 2, rest = p.dk - p.rot;
     const int turned = INTER ? (p.rot + E - 1) / E : (pairs + E - 1) / E, items = turned + (rest + E - 1) / E, per = q.heads * items;
     const int all = toks * per;
@@ -134,7 +135,8 @@ template <typename ET, bool INTER, bool WHOLE, int E, int IT> void launch_typed(
         if (tok * pairs > 4096) tok = 4096 / pairs;
         tok = tok < 1 ? 1 : tok > p.n ? p.n : tok;
         p.part[z].tok = tok;
-        most = cdiv(p.n, tok) > most ? cdiv(p.n, tok) : most;
+        p.part[z].blocks = cdiv(p.n, tok);
+        most = p.part[z].blocks > most ? p.part[z].blocks : most;
         lds = tok * pairs * 8 > lds ? tok * pairs * 8 : lds;
     }
     require((double)p.R * most < (double)(1 << 22), "rotary: too many tokens for one call");
